@@ -10,7 +10,7 @@ extern "C" {
 #endif
 
 // Moves with every change of a signature or struct below; the package binds one version.
-#define NORI_OPS_VERSION 4
+#define NORI_OPS_VERSION 5
 int nori_ops_version(void);
 
 // QASS base scale of one key count (QASSMaxScaling.forward's base branch, src/synthefy_nori/model/
@@ -87,6 +87,42 @@ typedef struct {
 
 int64_t nori_dense_apply_scratch_bytes(int64_t tables, int64_t rows, int64_t groups, int32_t embed, int32_t heads, int64_t nk);
 int nori_dense_apply(const nori_dense_apply_args* args, void* stream);
+
+// LayerNorm that can be trained (layer_norm_train.hip): y = (x - mean) / sqrt(var + eps) * weight + bias over
+// rows of any width >= 1, x rows at x_row_stride elements, y rows contiguous; weight and bias (either may be
+// NULL) contiguous of their own dtypes. mean and rstd [rows] fp32 keep the statistics, or both NULL.
+int nori_layer_norm_train_forward(const void* x, int x_dtype, int64_t rows, int32_t cols, int64_t x_row_stride,
+                                  const void* weight, int w_dtype, const void* bias, int b_dtype, float eps, void* y,
+                                  int y_dtype, float* mean, float* rstd, void* stream);
+
+// Its gradients: dx (contiguous, of x's dtype), dw and db (of w_dtype and b_dtype), each NULL where it is not
+// asked for. The workspace, of nori_layer_norm_train_workspace_bytes(rows, cols), takes the partial column sums
+// of dw and db; they are joined in a fixed order, so the same inputs give the same bits. No rows: nothing is
+// written.
+int64_t nori_layer_norm_train_workspace_bytes(int64_t rows, int32_t cols);
+int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_t rows, int32_t cols, int64_t x_row_stride,
+                                   const void* dy, int dy_dtype, int64_t dy_row_stride, const void* weight, int w_dtype,
+                                   int b_dtype, const float* mean, const float* rstd, void* dx, void* dw, void* db,
+                                   void* workspace, int64_t workspace_bytes, void* stream);
+
+// Low-rank updates of many tables at once (low_rank.hip): out[i] = y[i] + (scales[id] x[i] a[id]^T) b[id]^T with
+// id the adapter of row i; rows without one take y (y NULL: zeros). x [rows, k], y and out [rows, n] of one
+// dtype at row strides, out may be y; a [adapters, rank, k] and b [adapters, n, rank] of that dtype, contiguous
+// (transposed: a [adapters, k, rank] and b [adapters, rank, n]); scales [adapters] fp32 or NULL for 1.
+// order [rows] lists the rows of group 0, then of group 1, ...: group g is order[starts[g] .. starts[g + 1]),
+// its adapter ids[g] or -1. h [rows, rank] fp32 takes scales[id] x[i] a[id]^T (rows without an adapter are left).
+#define NORI_LOW_RANK_MAX 128
+int nori_low_rank_update(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* y,
+                         int64_t y_row_stride, const void* a, const void* b, int32_t transposed, const float* scales,
+                         int32_t adapters, int32_t rank, int32_t n, const int32_t* order, const int32_t* starts,
+                         const int32_t* ids, int32_t groups, void* out, int64_t out_row_stride, float* h, void* stream);
+
+// The sum over each adapter's rows of t[i]^T h[i] as out [adapters, cols, rank] (transposed: [adapters, rank,
+// cols]) of t's dtype, t [rows, cols] at a row stride, h [rows, rank] fp32, the groups as above. Adapters without
+// a group are left as they are.
+int nori_low_rank_weight_grad(const void* t, int dtype, int64_t rows, int32_t cols, int64_t t_row_stride, const float* h,
+                              int32_t rank, int32_t adapters, const int32_t* order, const int32_t* starts,
+                              const int32_t* ids, int32_t groups, int32_t transposed, void* out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,6 +7,7 @@ calling an operator on CPU tensors, or without the built library, raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -130,7 +131,7 @@ class DenseApplyArgs(ctypes.Structure):
 
 
 # The package's own entry points beyond the C ABI (csrc/nori_ops.h), and their version.
-OPS_VERSION = 4
+OPS_VERSION = 5
 OPS: dict[str, tuple[object, list]] = {
     "nori_qass_base": (ctypes.c_int, [_f32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
     "nori_linear_f16_w32": (
@@ -148,6 +149,22 @@ OPS: dict[str, tuple[object, list]] = {
     "nori_swiglu_mlp_residual": (ctypes.c_int, [_vp, _i64, _i32, _i64, _vp, _vp, _i32, _f32, _vp, _i64, _vp]),
     "nori_dense_apply_scratch_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i64]),
     "nori_dense_apply": (ctypes.c_int, [ctypes.POINTER(DenseApplyArgs), _vp]),
+    "nori_layer_norm_train_forward": (
+        ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _vp, _i32, _f32, _vp, _i32, _vp, _vp, _vp],
+    ),
+    "nori_layer_norm_train_workspace_bytes": (_i64, [_i64, _i32]),
+    "nori_layer_norm_train_backward": (
+        ctypes.c_int,
+        [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    ),
+    "nori_low_rank_update": (
+        ctypes.c_int,
+        [_vp, _i32, _i64, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _vp,
+         _vp],
+    ),
+    "nori_low_rank_weight_grad": (
+        ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _vp],
+    ),
     "nori_rms_norm_rows": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _i32, _vp]),
 }
 
@@ -233,6 +250,16 @@ def stream_of(device: torch.device) -> int:
         raise ValueError(f"Expected a cuda device, but got: {device}")
     index = device.index if device.index is not None else torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)  # current_stream(device).cuda_stream without the Stream object
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """A context in which ``device`` is the current one: a stream takes launches from its own device only."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -1,0 +1,373 @@
+"""Low-rank adapters of many tables beside a shared projection, and the readout that is fitted with them.
+
+A batch of tables goes through one frozen model; each table's rows may take an adapter of its own,
+``out = y + s (x A^T) B^T`` with ``y`` the shared projection's output, A [rank, in] and B [out, rank].
+``low_rank_update`` is that update and its gradients for every row of the batch in one call
+(csrc/low_rank.hip), ``AdapterPlan`` says which rows take which adapter, ``LowRankAdapters`` holds the
+factors of one projection, and ``ReadoutAdapters`` those of a quantile decoder
+(``FeaturesTransformer.reg_y_decoder``): trained on the row states of the frozen model, served for many
+tables at once.
+"""
+
+from __future__ import annotations
+
+import operator
+from typing import Sequence
+
+import numpy as np
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from . import _native as nat
+from .layer import _hooked
+from .norm import _FLOATS, _rows_of, _strided_rows, trainable_layer_norm
+
+__all__ = ["AdapterPlan", "LowRankAdapters", "ReadoutAdapters", "adapted_linear", "low_rank_update"]
+
+MAX_RANK = 128  # NORI_LOW_RANK_MAX
+
+
+class AdapterPlan:
+    """Which adapter each row of a batch takes: ``adapters[i]`` (-1: none) for the ``rows[i]`` rows of table
+    i, the tables one after another along the batch's flattened rows; ``rows`` is one number where every
+    table has as many. Rows of padding are tables of their own, with -1.
+
+    Made on the host once a batch and copied to ``device``: the rows sorted by adapter, so that tables which
+    share an adapter share its tiles. It can be used by any number of calls and graphs on that device."""
+
+    def __init__(self, adapters: Sequence[int], rows: int | Sequence[int], *, device: torch.device | str):
+        ids = [operator.index(i) for i in adapters]
+        if isinstance(rows, Sequence) or hasattr(rows, "__len__"):
+            counts = [operator.index(n) for n in rows]
+        else:
+            counts = [operator.index(rows)] * len(ids)
+        if len(counts) != len(ids):
+            raise ValueError(f"{len(ids)} adapters for {len(counts)} tables")
+        if any(n < 0 for n in counts):
+            raise ValueError("a table cannot have a negative number of rows")
+        if any(i < -1 for i in ids):
+            raise ValueError("adapters are numbered from 0; -1 is none")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError(f"nori_amd kernels run on a ROCm GPU; got a plan for {self.device}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.rows = sum(counts)
+        if self.rows > 2**31 - 1:
+            raise NotImplementedError(f"a plan takes up to {2**31 - 1} rows, got {self.rows}")
+        self.most = max(ids, default=-1)  # an adapter bank has more than this many
+        if self.most > 2**31 - 2:
+            raise ValueError(f"adapter {self.most} is out of range")
+        order, starts, groups = _grouped(np.asarray(ids, dtype=np.int64), np.asarray(counts, dtype=np.int64))
+        self.adapters = tuple(int(i) for i in groups if i >= 0)  # those with rows, ascending
+        self.groups = len(groups)
+        packed = torch.from_numpy(np.concatenate([starts, groups, order]).astype(np.int32)).to(self.device)
+        self.starts, self.ids, self.order = packed.split([self.groups + 1, self.groups, self.rows])
+
+
+def _grouped(ids: np.ndarray, counts: np.ndarray) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """(the rows by ascending adapter, where each adapter's begin and the end, the adapters), tables and
+    rows of one adapter in their order, adapters without rows left out."""
+    ids, first, counts = ids[counts > 0], (np.cumsum(counts) - counts)[counts > 0], counts[counts > 0]
+    by = np.argsort(ids, kind="stable")
+    ids, first, counts = ids[by], first[by], counts[by]
+    total = int(counts.sum())
+    at = np.cumsum(counts) - counts
+    order = np.arange(total, dtype=np.int64) + np.repeat(first - at, counts)
+    groups, where = np.unique(ids, return_index=True)
+    return order, np.append(at[where], total), groups
+
+
+def _update(x, y, a, b, plan, scales, transposed, out):
+    """``out`` = y + update (y None: the update alone) by ``nori_low_rank_update``; returns h [rows, rank]."""
+    rank = int(a.shape[2 if transposed else 1])
+    k, n = int(x.shape[-1]), int(out.shape[-1])
+    x, rows, xs = _rows_of(x, k)
+    ys = 0
+    if y is not None:
+        y, _, ys = _rows_of(y, n)
+    layout = _strided_rows(out, n)
+    if layout is None:
+        raise ValueError(f"out {tuple(out.shape)} has strides {out.stride()}: its rows must be at one stride")
+    os = layout[1]
+    h = torch.empty((rows, rank), dtype=torch.float32, device=x.device)
+    with nat.on(x.device):
+        nat.check(
+            nat.lib().nori_low_rank_update(
+                x.data_ptr(), nat.dtype_code(x.dtype), rows, k, xs, nat.ptr(y), ys, a.data_ptr(), b.data_ptr(),
+                1 if transposed else 0, nat.ptr(scales), int(a.shape[0]), rank, n, plan.order.data_ptr(),
+                plan.starts.data_ptr(), plan.ids.data_ptr(), plan.groups, out.data_ptr(), os, h.data_ptr(),
+                nat.stream_of(x.device),
+            ),
+            "low_rank_update",
+        )
+    return h
+
+
+def _weight_grad(t, h, plan, like, transposed):
+    """The sum over each adapter's rows of t^T h, in ``like``'s shape, by ``nori_low_rank_weight_grad``."""
+    cols = int(t.shape[-1])
+    t, rows, ts = _rows_of(t, cols)
+    out = torch.empty_like(like) if len(plan.adapters) == like.shape[0] else torch.zeros_like(like)
+    if rows:
+        with nat.on(t.device):
+            nat.check(
+                nat.lib().nori_low_rank_weight_grad(
+                    t.data_ptr(), nat.dtype_code(t.dtype), rows, cols, ts, h.data_ptr(), int(h.shape[1]), int(like.shape[0]),
+                    plan.order.data_ptr(), plan.starts.data_ptr(), plan.ids.data_ptr(), plan.groups, 1 if transposed else 0,
+                    out.data_ptr(), nat.stream_of(t.device),
+                ),
+                "low_rank_update backward",
+            )
+    return out
+
+
+def _gradients(dy, x, a, b, h, plan, scales, needs, base=None):
+    """(dx, da, db), None where not needed; ``base`` [..., in] is what dx is added to, and overwritten."""
+    need_x, need_a, need_b = needs
+    dx = da = db = None
+    if need_x or need_a:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if base is None else base
+        if plan.rows:
+            g = _update(dy, base, b, a, plan, scales, True, dx)
+        else:
+            g = h
+        if need_a:
+            da = _weight_grad(x, g, plan, a, True)
+    if need_b:
+        db = _weight_grad(dy, h, plan, b, False)
+    return (dx if need_x else None), da, db
+
+
+class _LowRankUpdate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, a, b, plan, scales):
+        out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        h = _update(x, y, a, b, plan, scales, False, out) if plan.rows else x.new_empty((0, a.shape[1]), dtype=torch.float32)
+        ctx.save_for_backward(x, a, b, h, scales)
+        ctx.plan = plan
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, a, b, h, scales = ctx.saved_tensors
+        need_x, need_y, need_a, need_b = ctx.needs_input_grad[:4]
+        dx, da, db = _gradients(dout, x, a, b, h, ctx.plan, scales, (need_x, need_a, need_b))
+        return dx, (dout if need_y else None), da, db, None, None
+
+
+class _AdaptedLinear(torch.autograd.Function):
+    """A frozen projection and its low-rank update: the update's gradient of x is added in place to the
+    projection's."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, a, b, plan, scales):
+        with torch.autocast("cuda", enabled=False):
+            y = F.linear(x, weight, bias)
+        if _strided_rows(y, int(y.shape[-1])) is None:
+            y = y.contiguous()
+        h = _update(x, y, a, b, plan, scales, False, y) if plan.rows else x.new_empty((0, a.shape[1]), dtype=torch.float32)
+        ctx.save_for_backward(x, weight, a, b, h, scales)
+        ctx.plan = plan
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, a, b, h, scales = ctx.saved_tensors
+        need_x, _, _, need_a, need_b = ctx.needs_input_grad[:5]
+        base = None
+        if need_x:
+            with torch.autocast("cuda", enabled=False):
+                base = torch.matmul(dy.reshape(-1, dy.shape[-1]), weight).view(x.shape)
+        dx, da, db = _gradients(dy, x, a, b, h, ctx.plan, scales, (need_x, need_a, need_b), base)
+        return dx, None, None, da, db, None, None
+
+
+def _check(x, y, a, b, plan, scales):
+    """The checks of ``low_rank_update``'s arguments; (a, b, scales) as the kernels take them."""
+    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+        raise ValueError(f"factors are a [adapters, rank, in] and b [adapters, out, rank], got {tuple(a.shape)} and {tuple(b.shape)}")
+    adapters, rank, k = (int(s) for s in a.shape)
+    n = int(b.shape[1])
+    if min(adapters, rank, k, n) == 0:
+        raise ValueError(f"empty factors {tuple(a.shape)} and {tuple(b.shape)}")
+    if rank > MAX_RANK:
+        raise NotImplementedError(f"low_rank_update takes ranks up to {MAX_RANK}, got {rank}")
+    if x.dim() == 0 or int(x.shape[-1]) != k:
+        raise ValueError(f"x {tuple(x.shape)} does not end in the factors' {k} inputs")
+    if y is not None and tuple(y.shape) != (*x.shape[:-1], n):
+        raise ValueError(f"y {tuple(y.shape)} is not the projection of x {tuple(x.shape)} to {n}")
+    if x.dtype not in _FLOATS:
+        raise NotImplementedError(f"low_rank_update takes float32/float16/bfloat16, got {x.dtype}")
+    for name, t in (("y", y), ("a", a), ("b", b)):
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError(f"low_rank_update: {name} is {t.dtype}, x {x.dtype}")
+    if not isinstance(plan, AdapterPlan):
+        raise TypeError(f"plan must be an AdapterPlan, got {type(plan).__name__}")
+    device = nat.require_device(x, y, a, b, scales)
+    if plan.device != device:
+        raise RuntimeError(f"tensors on different devices: {device} and the plan's {plan.device}")
+    if x.numel() // k != plan.rows:
+        raise ValueError(f"x has {x.numel() // k} rows, the plan {plan.rows}")
+    if plan.most >= adapters:
+        raise ValueError(f"the plan names adapter {plan.most} of {adapters}")
+    if scales is not None:
+        if tuple(scales.shape) != (adapters,) or scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 [{adapters}], got {scales.dtype} {tuple(scales.shape)}")
+        if scales.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("low_rank_update has no gradient for scales")
+        scales = scales.contiguous()
+    return a.contiguous(), b.contiguous(), scales
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The bytes from t's first element to its last."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two indices of t may be one element (expanded or overlapping dimensions)."""
+    inside = 0
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda d: d[1]):
+        if stride <= inside:
+            return True
+        inside += (size - 1) * stride
+    return False
+
+
+def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether ``out`` and ``t`` may share elements. Columns side by side of one buffer's rows do not."""
+    (lo, hi), (tlo, thi) = _span(out), _span(t)
+    if out.numel() == 0 or t.numel() == 0 or hi <= tlo or thi <= lo:
+        return False
+    one, other = _strided_rows(out, int(out.shape[-1])), _strided_rows(t, int(t.shape[-1]))
+    if one is None or other is None or one[1] != other[1] or one[1] == 0:
+        return True
+    size = out.element_size()
+    row = one[1] * size
+    start, at = 0, (tlo - lo) % row
+    return not (at >= start + int(out.shape[-1]) * size and at + int(t.shape[-1]) * size <= row)
+
+
+def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: AdapterPlan,
+                    scales: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``y + scales[id] (x a[id]^T) b[id]^T`` with ``id`` the adapter ``plan`` gives each row; rows without
+    one take ``y``. x [..., in], y [..., out], a [adapters, rank, in], b [adapters, out, rank] of one
+    dtype (float32, float16 or bfloat16), ``scales`` float32 [adapters] or None for 1, rank up to 128.
+
+    Products are summed in fp32, ``x a^T`` is kept in fp32, and the sum with y is rounded once.
+    Differentiable in x, y, a and b (first derivatives; adapters no row takes get zeros). ``out``, in
+    inference, receives the result: a tensor of y's shape and dtype, y itself included, that shares no
+    element with x."""
+    a, b, scales = _check(x, y, a, b, plan, scales)
+    grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, y, a, b))
+    if out is None:
+        if grad:
+            return _LowRankUpdate.apply(x, y, a, b, plan, scales)
+        out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    elif grad or out.requires_grad:
+        raise ValueError("out is for inference: an argument asks for gradients")
+    elif tuple(out.shape) != tuple(y.shape) or out.dtype != y.dtype or out.device != y.device:
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not y's {tuple(y.shape)} {y.dtype}")
+    elif any(_overlap(out, t) for t in (x, a, b)) or (_overlap(out, y) and (out.data_ptr(), out.stride()) != (y.data_ptr(), y.stride())):
+        raise ValueError("out shares elements with an input")
+    elif _overlaps_itself(out):
+        raise ValueError(f"out has strides {out.stride()}: its elements overlap")
+    if plan.rows == 0:
+        return out
+    if _strided_rows(out, int(out.shape[-1])) is None:
+        whole = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        _update(x, y, a, b, plan, scales, False, whole)
+        return out.copy_(whole)
+    _update(x, y, a, b, plan, scales, False, out)
+    return out
+
+
+def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, a: torch.Tensor, b: torch.Tensor,
+                   plan: AdapterPlan, scales: torch.Tensor | None = None) -> torch.Tensor:
+    """``low_rank_update(x, F.linear(x, weight, bias), a, b, plan, scales)``, with x, the weights and the
+    factors in the autocast dtype where autocast is on (the factors in x's dtype elsewhere). A frozen
+    projection's output and x gradient are updated in place."""
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        x, weight, bias = x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype)
+    a, b = a.to(x.dtype), b.to(x.dtype)
+    trained = torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad))
+    if trained:
+        with torch.autocast("cuda", enabled=False):
+            return low_rank_update(x, F.linear(x, weight, bias), a, b, plan, scales)
+    nat.require_device(x, weight, bias)
+    a, b, scales = _check(x, None, a, b, plan, scales)
+    if tuple(weight.shape) != (b.shape[1], a.shape[2]):
+        raise ValueError(f"the projection's weight {tuple(weight.shape)} does not match factors {tuple(a.shape)} and {tuple(b.shape)}")
+    return _AdaptedLinear.apply(x, weight, bias, a, b, plan, scales)
+
+
+class LowRankAdapters(nn.Module):
+    """The adapters of one projection: factors ``a`` [adapters, rank, in] (normal, fan-in scale) and ``b``
+    [adapters, out, rank] (zeros: a new adapter changes nothing), and ``scales`` [adapters], alpha / rank
+    (alpha defaults to the rank)."""
+
+    def __init__(self, adapters: int, in_features: int, out_features: int, rank: int, *, alpha: float | None = None,
+                 device=None, dtype=None):
+        super().__init__()
+        if min(adapters, in_features, out_features, rank) < 1:
+            raise ValueError("adapters, in_features, out_features and rank must be positive")
+        if rank > MAX_RANK:
+            raise NotImplementedError(f"low_rank_update takes ranks up to {MAX_RANK}, got {rank}")
+        self.a = nn.Parameter(torch.randn(adapters, rank, in_features, device=device, dtype=dtype) * in_features ** -0.5)
+        self.b = nn.Parameter(torch.zeros(adapters, out_features, rank, device=device, dtype=dtype))
+        self.register_buffer("scales", torch.full((adapters,), (rank if alpha is None else alpha) / rank, device=device,
+                                                  dtype=torch.float32))
+
+    def forward(self, x: torch.Tensor, y: torch.Tensor, plan: AdapterPlan) -> torch.Tensor:
+        """``low_rank_update`` of y by these adapters, their factors in x's dtype."""
+        return low_rank_update(x, y, self.a.to(x.dtype), self.b.to(x.dtype), plan, self.scales)
+
+    def linear(self, x: torch.Tensor, projection: nn.Linear, plan: AdapterPlan) -> torch.Tensor:
+        """``adapted_linear`` of x by ``projection`` and these adapters; a projection that is hooked or of
+        another class is called."""
+        if type(projection) is not nn.Linear or _hooked(projection):
+            y = projection(x)
+            return self(x.to(y.dtype), y, plan)
+        return adapted_linear(x, projection.weight, projection.bias, self.a, self.b, plan, self.scales)
+
+
+class ReadoutAdapters(nn.Module):
+    """Adapters of a quantile decoder, ``Linear -> LayerNorm -> GELU -> Linear``
+    (``FeaturesTransformer.reg_y_decoder``): one bank beside each of its two projections.
+
+    ``readout(decoder, states, plan)`` decodes row states [..., width] of many tables, each with its own
+    adapter. The decoder itself is left as it is; freeze it (``requires_grad_(False)``) to train the adapters
+    alone, and its LayerNorm's affine trains with them where it asks for gradients."""
+
+    def __init__(self, decoder: nn.Sequential, adapters: int, rank: int, *, alpha: float | None = None):
+        super().__init__()
+        first, _, _, last = self._parts(decoder)
+        where = dict(device=first.weight.device, dtype=torch.float32)
+        self.first = LowRankAdapters(adapters, first.in_features, first.out_features, rank, alpha=alpha, **where)
+        self.last = LowRankAdapters(adapters, last.in_features, last.out_features, rank, alpha=alpha, **where)
+
+    @staticmethod
+    def _parts(decoder: nn.Sequential) -> tuple[nn.Linear, nn.LayerNorm, nn.Module, nn.Linear]:
+        parts = tuple(decoder) if isinstance(decoder, nn.Sequential) else ()
+        if len(parts) != 4 or not (isinstance(parts[0], nn.Linear) and isinstance(parts[1], nn.LayerNorm)
+                                   and isinstance(parts[3], nn.Linear)) or len(parts[1].normalized_shape) != 1:
+            raise ValueError("ReadoutAdapters takes a decoder of Linear, LayerNorm, activation, Linear")
+        return parts
+
+    def forward(self, decoder: nn.Sequential, states: torch.Tensor, plan: AdapterPlan) -> torch.Tensor:
+        first, norm, activation, last = self._parts(decoder)
+        h = self.first.linear(states, first, plan)
+        # under autocast torch's layer norm answers in float32; outside it in its input's dtype
+        wide = torch.float32 if torch.is_autocast_enabled("cuda") else h.dtype
+        if type(norm) is not nn.LayerNorm or _hooked(norm):
+            h = norm(h)
+        else:
+            h = trainable_layer_norm(h, norm.weight, norm.bias, norm.eps, out_dtype=wide)
+        h = activation(h)
+        return self.last.linear(h, last, plan)

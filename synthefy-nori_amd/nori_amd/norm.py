@@ -358,6 +358,113 @@ def layer_norm(
     return out.view(*x.shape[:-1], cols)
 
 
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _rows_of(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
+    """(t, or its contiguous copy where its rows of ``cols`` elements are not at one stride; rows; stride)."""
+    layout = _strided_rows(t, cols)
+    if layout is None:
+        t = t.contiguous()
+        layout = t.numel() // cols, cols
+    return (t, *layout)
+
+
+def _train_forward(x, weight, bias, eps, out_dtype, keep):
+    """(y, mean, rstd) by ``nori_layer_norm_train_forward``; the statistics are None unless kept."""
+    cols = int(x.shape[-1])
+    x2, rows, stride = _rows_of(x, cols)
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+    if rows:
+        with nat.on(x.device):
+            nat.check(
+                nat.lib().nori_layer_norm_train_forward(
+                    x2.data_ptr(), nat.dtype_code(x.dtype), rows, cols, stride,
+                    nat.ptr(weight), 0 if weight is None else nat.dtype_code(weight.dtype),
+                    nat.ptr(bias), 0 if bias is None else nat.dtype_code(bias.dtype), eps,
+                    y.data_ptr(), nat.dtype_code(out_dtype), stats[0].data_ptr() if keep else None,
+                    stats[1].data_ptr() if keep else None, nat.stream_of(x.device),
+                ),
+                "trainable_layer_norm",
+            )
+    return y, stats
+
+
+def _train_backward(dy, x, weight, bias, stats, need_x, need_w, need_b):
+    """(dx, dweight, dbias), None where not needed, by ``nori_layer_norm_train_backward``."""
+    cols = int(x.shape[-1])
+    x2, rows, stride = _rows_of(x, cols)
+    dy2, _, dy_stride = _rows_of(dy, cols)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+    make = torch.empty_like if rows else torch.zeros_like  # no rows: the sums over them are zero
+    dw = make(weight) if need_w else None
+    db = make(bias) if need_b else None
+    if rows and (need_x or need_w or need_b):
+        with nat.on(x.device):
+            size = nat.lib().nori_layer_norm_train_workspace_bytes(rows, cols) if need_w or need_b else 0
+            workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+            nat.check(
+                nat.lib().nori_layer_norm_train_backward(
+                    x2.data_ptr(), nat.dtype_code(x.dtype), rows, cols, stride, dy2.data_ptr(), nat.dtype_code(dy.dtype),
+                    dy_stride, nat.ptr(weight), 0 if weight is None else nat.dtype_code(weight.dtype),
+                    0 if bias is None else nat.dtype_code(bias.dtype), stats[0].data_ptr(), stats[1].data_ptr(),
+                    nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.ptr(workspace), size, nat.stream_of(x.device),
+                ),
+                "trainable_layer_norm backward",
+            )
+    return dx, dw, db
+
+
+class _TrainableLayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, out_dtype):
+        y, stats = _train_forward(x, weight, bias, eps, out_dtype, True)
+        ctx.save_for_backward(x, weight, bias, stats)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return (*_train_backward(dy, *ctx.saved_tensors, *ctx.needs_input_grad[:3]), None, None)
+
+
+def trainable_layer_norm(
+    x: torch.Tensor,
+    weight: torch.Tensor | None,
+    bias: torch.Tensor | None,
+    eps: float = 1e-5,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """``F.layer_norm`` over the last axis with its gradients: x [..., C] of any width C >= 1, ``weight``
+    and ``bias`` [C] or None, each of float32, float16 or bfloat16, the result in ``out_dtype``
+    (default x's). Statistics, affine and the sums of the gradients are fp32, every result rounded once.
+
+    Differentiable in x, weight and bias (first derivatives), the gradients in their inputs' dtypes; the
+    affine gradients are summed in a fixed order, so the same inputs give the same bits. Rows at one
+    stride are read as they lie, other layouts through a contiguous copy. ``layer_norm`` is the forward
+    pass for inference (widths a multiple of 4, an optional ReLU), without gradients."""
+    cols = int(x.shape[-1]) if x.dim() else 0
+    if cols == 0:
+        raise ValueError(f"trainable_layer_norm needs rows of at least one element, got {tuple(x.shape)}")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
+        if t is not None and t.dtype not in _FLOATS:
+            raise NotImplementedError(f"trainable_layer_norm takes float32/float16/bfloat16, got {name} {t.dtype}")
+    if out_dtype not in _FLOATS:
+        raise NotImplementedError(f"trainable_layer_norm gives float32/float16/bfloat16, not {out_dtype}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != (cols,):
+            raise ValueError(f"trainable_layer_norm: {name} {tuple(t.shape)} does not match rows of {cols}")
+    if not eps >= 0.0:
+        raise ValueError(f"trainable_layer_norm: eps must be a non-negative number, got {eps}")
+    nat.require_device(x, weight, bias)
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _TrainableLayerNorm.apply(x, weight, bias, float(eps), out_dtype)
+    return _train_forward(x, weight, bias, float(eps), out_dtype, False)[0]
+
+
 # Widths (in = out features) the fused SwiGLU kernel is built for.
 FUSED_MLP_WIDTHS = (128, 256, 352)
 

@@ -33,13 +33,14 @@ from __future__ import annotations
 import ctypes
 import math
 from dataclasses import dataclass
-from typing import Any, Callable, Literal
+from typing import Any, Callable, Literal, Sequence
 
 import torch
 import torch.nn as nn
 from torch.amp import autocast
 
 from . import _native as nat
+from .adapters import AdapterPlan, ReadoutAdapters
 from .encoders import (
     MaskEmbEncoder,
     PromptQuantilePLEEncoder,
@@ -459,6 +460,8 @@ class FeaturesTransformer(nn.Module):
         calculate_sample_attention: bool = False,
         calculate_feature_attention: bool = False,
         return_embeddings: bool = False,
+        readout_adapters: ReadoutAdapters | None = None,
+        table_adapters: Sequence[int] | None = None,
         **kwargs: Any,
     ):
         """Context rows [0, eval_pos) and query rows [eval_pos, S) through the model together
@@ -469,7 +472,8 @@ class FeaturesTransformer(nn.Module):
         positional and target-aware embeddings, passed through the cell and row layers, and
         the query rows' row states decoded into quantiles [B, S - eval_pos, Q]. With
         ``return_embeddings`` it returns the row states [B, S, width]; with ``mask_prediction``
-        the reference's dict. The dense layer stack's uncached forward is not part of this
+        the reference's dict. ``readout_adapters`` and ``table_adapters`` adapt the decoder to
+        single tables (``decode``). The dense layer stack's uncached forward is not part of this
         package: dense models run through ``forward_cached_regression``.
         """
         if self.two_phase_config is None:
@@ -505,7 +509,7 @@ class FeaturesTransformer(nn.Module):
         row_states, cell_states = self.transformer_encoder(cells, y_masked, eval_pos, inplace=True)
         if return_embeddings:
             return row_states
-        reg_output = self.reg_y_decoder(row_states[:, eval_pos:])
+        reg_output = self.decode(row_states[:, eval_pos:], readout_adapters, table_adapters)
         if not self.mask_prediction:
             return reg_output
         skip = self.feature_decoder is None or getattr(self, "_skip_feature_decoder", False)
@@ -520,6 +524,19 @@ class FeaturesTransformer(nn.Module):
                 "std_for_normalization": pre.get("_norm_std"),
             },
         }
+
+    def decode(self, states: torch.Tensor, readout_adapters: ReadoutAdapters | None = None,
+               table_adapters: Sequence[int] | None = None) -> torch.Tensor:
+        """The quantile bank of row states [B, rows, width] (``return_embeddings`` gives them), the decoder
+        adapted to table i by adapter ``table_adapters[i]`` of ``readout_adapters`` (-1: not at all)."""
+        if readout_adapters is None:
+            if table_adapters is not None:
+                raise ValueError("table_adapters without readout_adapters")
+            return self.reg_y_decoder(states)
+        if table_adapters is None or len(table_adapters) != states.shape[0]:
+            raise ValueError(f"readout_adapters need the adapter of each of the {states.shape[0]} tables")
+        plan = AdapterPlan(table_adapters, states.shape[1], device=states.device)
+        return readout_adapters(self.reg_y_decoder, states, plan)
 
     def _require_context_cache(self) -> None:
         if self.two_phase_config is not None:
@@ -767,9 +784,14 @@ class FeaturesTransformer(nn.Module):
         row_chunk_size: int | None = None,
         adaptive_query_chunk: bool = True,
         query_chunk_attempt_callback: Callable[[int, Literal["success", "oom"]], None] | None = None,
+        return_embeddings: bool = False,
+        readout_adapters: ReadoutAdapters | None = None,
+        table_adapters: Sequence[int] | None = None,
     ) -> torch.Tensor:
         """Score query rows against a prebuilt ``ContextCache``; mutates nothing on it
-        (:961-1078). Returns ``[B, Nq, num_reg_quantiles]``."""
+        (:961-1078). Returns ``[B, Nq, num_reg_quantiles]``; with ``return_embeddings`` the row states
+        ``[B, Nq, embed_dim]`` that the decoder reads. ``readout_adapters`` and ``table_adapters`` adapt
+        the decoder to single tables (``decode``)."""
         self._require_context_cache()
         if self.mask_prediction:
             raise NotImplementedError("apply_context_cache requires mask_prediction=False")
@@ -810,7 +832,8 @@ class FeaturesTransformer(nn.Module):
             out = self.transformer_encoder.forward_test_with_cache(
                 torch.cat((xq, yq.unsqueeze(2)), dim=2), context.caches, feature_atten_mask=None
             )
-            return self.reg_y_decoder(self.encoder_out_norm(out)[:, :, -1])
+            states = self.encoder_out_norm(out)[:, :, -1]
+            return states if return_embeddings else self.decode(states, readout_adapters, table_adapters)
 
         chunk = n_test if row_chunk_size is None or row_chunk_size <= 0 else row_chunk_size
         outputs = []
