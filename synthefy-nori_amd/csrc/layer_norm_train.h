@@ -1,11 +1,15 @@
 // What the forward and the backward kernels of the trainable LayerNorm share.
 //
 // Rows in registers. A group of G lanes owns a row and holds it as NV vectors of V elements a lane: vector
-// i of lane l is at column (i * G + l) * V. G is 16 (rows up to 128), 64 or 256 (a workgroup), V is 4
-// where rows, strides and pointers keep vectors whole and 1 elsewhere. Rows too wide for that are looped over.
+// i of lane l is at column (i * G + l) * V. V is 16 bytes of x, read and written at any alignment (global memory
+// takes vectors at any byte); where a row is no whole number of vectors (RAGGED) its last one is moved back to
+// end with the row, and the elements that it shares with the one before are left out of the sums (stored twice,
+// the same value). G is 16 (rows up to 128), 64 or 256 (a workgroup). Rows shorter than a vector are held an
+// element a lane, rows too wide for registers are looped over.
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "nori_common.h"
 
@@ -15,42 +19,52 @@ using namespace nori;
 
 constexpr int kThreads = 256;
 
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int DT>
+using elem = std::conditional_t<DT == NORI_F32, uint32_t, uint16_t>;
+
+// V elements as they lie in memory
+template <int DT, int V>
+struct Raw {
+    elem<DT> e[V];
+};
 
 template <int DT, int V>
-__device__ __forceinline__ void load(const void* p, int64_t i, float (&v)[V]) {
-    if constexpr (V == 1) {
-        v[0] = load_elem<DT>(p, i);
-    } else if constexpr (DT == NORI_F32) {
-        const f32x4 c = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(p) + i);
+__device__ __forceinline__ Raw<DT, V> fetch(const void* p, int64_t i) {
+    Raw<DT, V> r;
+    __builtin_memcpy(&r, reinterpret_cast<const elem<DT>*>(p) + i, sizeof r);
+    return r;
+}
+
+template <int DT, int V>
+__device__ __forceinline__ void widen(const Raw<DT, V>& r, float (&v)[V]) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = c[k];
-    } else {
-        const u32x2 c = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint16_t*>(p) + i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint16_t h = (uint16_t)(c[k >> 1] >> (16 * (k & 1)));
-            v[k] = DT == NORI_F16 ? f16_to_f32(h) : bf16_to_f32(h);
-        }
+    for (int k = 0; k < V; ++k) {
+        if constexpr (DT == NORI_F32) v[k] = __uint_as_float(r.e[k]);
+        else v[k] = DT == NORI_F16 ? f16_to_f32(r.e[k]) : bf16_to_f32(r.e[k]);
     }
 }
 
 template <int DT, int V>
 __device__ __forceinline__ void store(void* p, int64_t i, const float (&v)[V]) {
-    if constexpr (V == 1) {
-        store_elem<DT>(p, i, v[0]);
-    } else if constexpr (DT == NORI_F32) {
-        *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + i) = f32x4{v[0], v[1], v[2], v[3]};
-    } else {
-        u32x2 c;
+    Raw<DT, V> r;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t lo = DT == NORI_F16 ? f32_to_f16(v[2 * k]) : f32_to_bf16(v[2 * k]);
-            const uint32_t hi = DT == NORI_F16 ? f32_to_f16(v[2 * k + 1]) : f32_to_bf16(v[2 * k + 1]);
-            c[k] = lo | (hi << 16);
-        }
-        *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p) + i) = c;
+    for (int k = 0; k < V; ++k) {
+        if constexpr (DT == NORI_F32) r.e[k] = __float_as_uint(v[k]);
+        else r.e[k] = DT == NORI_F16 ? f32_to_f16(v[k]) : f32_to_bf16(v[k]);
     }
+    __builtin_memcpy(reinterpret_cast<elem<DT>*>(p) + i, &r, sizeof r);
+}
+
+// vector i of a lane: its column, and how many of its elements the vector before it holds too
+template <int V, int G, bool RAGGED>
+__device__ __forceinline__ int column(int i, int lane, int cols, int& shared) {
+    const int c = (i * G + lane) * V;
+    shared = 0;
+    if (RAGGED && c < cols && c + V > cols) {
+        shared = c + V - cols;
+        return cols - V;
+    }
+    return c;
 }
 
 // affine parameters, of a type known at run time; `none` where there are none
@@ -63,14 +77,16 @@ __device__ __forceinline__ float param(const void* p, int dt, int64_t i, float n
 
 template <int V>
 __device__ __forceinline__ void params(const void* p, int dt, int64_t i, float none, float (&v)[V]) {
-    if (V == 4 && p && (uintptr_t)p % (dt == NORI_F32 ? 16 : 8) == 0) {
-        if (dt == NORI_F32) load<NORI_F32, V>(p, i, v);
-        else if (dt == NORI_F16) load<NORI_F16, V>(p, i, v);
-        else load<NORI_BF16, V>(p, i, v);
-        return;
-    }
+    if (!p) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = param(p, dt, i + k, none);
+        for (int k = 0; k < V; ++k) v[k] = none;
+    } else if (dt == NORI_F32) {
+        widen<NORI_F32, V>(fetch<NORI_F32, V>(p, i), v);
+    } else if (dt == NORI_F16) {
+        widen<NORI_F16, V>(fetch<NORI_F16, V>(p, i), v);
+    } else {
+        widen<NORI_BF16, V>(fetch<NORI_BF16, V>(p, i), v);
+    }
 }
 
 // The sums of a and b over the group's lanes, in every one of them. A workgroup's partial sums pass through
@@ -93,40 +109,44 @@ __device__ __forceinline__ void group_sums(float& a, float& b, float* slots, int
     }
 }
 
-// the kernel for rows of `cols`: calls go(V, G, NV) with integral constants, or loop() past what registers hold
-template <class Go, class Loop>
-void choose(int cols, bool vectors, Go go, Loop loop) {
-#define NORI_LN_TRY(V, G, NV) \
-    if (cols <= (V) * (G) * (NV)) return go(std::integral_constant<int, V>{}, std::integral_constant<int, G>{}, std::integral_constant<int, NV>{})
-    if (vectors) {
-        NORI_LN_TRY(4, 16, 1);
-        NORI_LN_TRY(4, 16, 2);
-        NORI_LN_TRY(4, 64, 1);
-        NORI_LN_TRY(4, 64, 2);
-        NORI_LN_TRY(4, 64, 3);
-        NORI_LN_TRY(4, 64, 4);
-        NORI_LN_TRY(4, 64, 6);
-        NORI_LN_TRY(4, 64, 8);
-        NORI_LN_TRY(4, 256, 4);
-        NORI_LN_TRY(4, 256, 8);
+// The kernel for rows of `cols`: calls go(V, G, NV, RAGGED) with integral constants, or loop() past what registers
+// hold. A row goes to the fewest lanes that hold it in 32 values each, a workgroup to the ones that a wavefront
+// does not.
+template <int DT, class Go, class Loop>
+void choose(int cols, Go go, Loop loop) {
+    constexpr int VW = DT == NORI_F32 ? 4 : 8;
+#define NORI_LN_CALL(V, G, NV, R) \
+    go(std::integral_constant<int, V>{}, std::integral_constant<int, G>{}, std::integral_constant<int, NV>{}, \
+       std::integral_constant<bool, R>{})
+#define NORI_LN_TRY(G, NV) \
+    if (cols <= VW * (G) * (NV)) return cols % VW ? NORI_LN_CALL(VW, G, NV, true) : NORI_LN_CALL(VW, G, NV, false)
+    if (cols < VW) return NORI_LN_CALL(1, 16, 1, false);
+    if constexpr (VW == 8) {
+        NORI_LN_TRY(16, 1);
+        NORI_LN_TRY(64, 1);
+        NORI_LN_TRY(64, 2);
+        NORI_LN_TRY(64, 3);
+        NORI_LN_TRY(64, 4);
+        NORI_LN_TRY(256, 2);
+        NORI_LN_TRY(256, 4);
     } else {
-        NORI_LN_TRY(1, 16, 4);
-        NORI_LN_TRY(1, 64, 4);
-        NORI_LN_TRY(1, 64, 8);
-        NORI_LN_TRY(1, 64, 16);
-        NORI_LN_TRY(1, 256, 8);
-        NORI_LN_TRY(1, 256, 16);
+        NORI_LN_TRY(16, 1);
+        NORI_LN_TRY(16, 2);
+        NORI_LN_TRY(64, 1);
+        NORI_LN_TRY(64, 2);
+        NORI_LN_TRY(64, 3);
+        NORI_LN_TRY(64, 4);
+        NORI_LN_TRY(64, 6);
+        NORI_LN_TRY(64, 8);
+        NORI_LN_TRY(256, 4);
+        NORI_LN_TRY(256, 8);
     }
 #undef NORI_LN_TRY
+#undef NORI_LN_CALL
     loop();
 }
 
 inline bool is_float(int dt) { return dt == NORI_F32 || dt == NORI_F16 || dt == NORI_BF16; }
-
-// whether rows of `cols` at `stride` from p are whole vectors of 4
-inline bool whole4(const void* p, int dt, int cols, int64_t stride) {
-    return cols % 4 == 0 && stride % 4 == 0 && (uintptr_t)p % (4 * dtype_size(dt)) == 0;
-}
 
 inline int check(const char* what, int64_t rows, int32_t cols, int x_dtype, int y_dtype, int64_t xs, int64_t ys) {
     if (!is_float(x_dtype) || !is_float(y_dtype))

@@ -6,8 +6,6 @@
 //
 // HBM-bound: each row is read and written once, c (e_x + e_y) bytes. Groups walk the rows in a grid-stride
 // loop, so that the affine parameters are read once a group and not once a row.
-#include <type_traits>
-
 #include "layer_norm_train.h"
 
 namespace {
@@ -25,66 +23,67 @@ struct Forward {
     float *mean, *rstd;  // null: not kept
 };
 
-template <int XDT, int YDT, int V, int G, int NV>
+template <int XDT, int YDT, int V, int G, int NV, bool RAGGED>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const Forward a) {
     __shared__ float slots[16];
     int turn = 0;
     const int lane = threadIdx.x % G;
     const float inv_n = 1.0f / (float)a.cols;
     float w[NV][V], b[NV][V];
+    int at[NV], shared[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (i * G + lane) * V;
-        if (c < a.cols) {
-            params<V>(a.w, a.wdt, c, 1.f, w[i]);
-            params<V>(a.b, a.bdt, c, 0.f, b[i]);
+        at[i] = column<V, G, RAGGED>(i, lane, a.cols, shared[i]);
+        if (at[i] < a.cols) {
+            params<V>(a.w, a.wdt, at[i], 1.f, w[i]);
+            params<V>(a.b, a.bdt, at[i], 0.f, b[i]);
         }
     }
     const int64_t per = kThreads / G, step = (int64_t)gridDim.x * per;
+    Raw<XDT, V> next[NV];
+    auto ask = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            next[i] = {};
+            if (row < a.rows && at[i] < a.cols) next[i] = fetch<XDT, V>(a.x, row * a.xs + at[i]);
+        }
+    };
+    ask((int64_t)blockIdx.x * per + threadIdx.x / G);
     // every group of a wavefront, every wavefront of a workgroup, goes round as often: the sums stay uniform
     for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += step) {
         const int64_t row = row0 + threadIdx.x / G;
-        const bool ok = row < a.rows;
         float v[NV][V];
         float s = 0.f, none = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + lane) * V;
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[i][k] = 0.f;
-            if (ok && c < a.cols) load<XDT, V>(a.x, row * a.xs + c, v[i]);
-        }
+        for (int i = 0; i < NV; ++i) widen<XDT, V>(next[i], v[i]);
+        ask(row + step);  // the next row's loads run under this row's sums
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int k = 0; k < V; ++k) s += v[i][k];
+            for (int k = 0; k < V; ++k) s += !RAGGED || k >= shared[i] ? v[i][k] : 0.f;
         group_sums<G>(s, none, slots, turn);
         const float mean = s * inv_n;
         s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool in = (i * G + lane) * V < a.cols;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                v[i][k] = in ? v[i][k] - mean : 0.f;
-                s += v[i][k] * v[i][k];
+                v[i][k] -= mean;
+                s += at[i] < a.cols && (!RAGGED || k >= shared[i]) ? v[i][k] * v[i][k] : 0.f;
             }
-        }
         group_sums<G>(s, none, slots, turn);
         const float rstd = rsqrtf(s * inv_n + a.eps);
-        if (ok) {
+        if (row >= a.rows) continue;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (i * G + lane) * V;
-                if (c >= a.cols) continue;
+        for (int i = 0; i < NV; ++i) {
+            if (at[i] >= a.cols) continue;
 #pragma unroll
-                for (int k = 0; k < V; ++k) v[i][k] = v[i][k] * rstd * w[i][k] + b[i][k];
-                store<YDT, V>(a.y, row * a.cols + c, v[i]);
-            }
-            if (lane == 0 && a.mean) {
-                a.mean[row] = mean;
-                a.rstd[row] = rstd;
-            }
+            for (int k = 0; k < V; ++k) v[i][k] = v[i][k] * rstd * w[i][k] + b[i][k];
+            store<YDT, V>(a.y, row * a.cols + at[i], v[i]);
+        }
+        if (lane == 0 && a.mean) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
         }
     }
 }
@@ -133,16 +132,16 @@ extern "C" int nori_layer_norm_train_forward(const void* x, int x_dtype, int64_t
     if (!x || !y || !mean != !rstd) return fail(NORI_ERR_INVALID, "layer_norm_train_forward: null pointer");
     const Forward a{x, rows, x_row_stride, cols, weight, bias, w_dtype, b_dtype, eps, y, mean, rstd};
     hipStream_t stream = (hipStream_t)stream_v;
-    const bool vectors = whole4(x, x_dtype, cols, x_row_stride) && whole4(y, y_dtype, cols, cols);
     const int64_t most = (int64_t)device_cus() * 16;
     NORI_DISPATCH_FLOAT(x_dtype, XDT, {
         NORI_DISPATCH_FLOAT(y_dtype, YDT, {
-            choose(
-                cols, vectors,
-                [&](auto V_, auto G_, auto NV_) {
+            choose<XDT>(
+                cols,
+                [&](auto V_, auto G_, auto NV_, auto R_) {
                     constexpr int V = decltype(V_)::value, G = decltype(G_)::value, NV = decltype(NV_)::value;
+                    constexpr bool R = decltype(R_)::value;
                     const int64_t need = (rows + kThreads / G - 1) / (kThreads / G);
-                    hipLaunchKernelGGL((forward_kernel<XDT, YDT, V, G, NV>), dim3((unsigned)std::min(need, most)),
+                    hipLaunchKernelGGL((forward_kernel<XDT, YDT, V, G, NV, R>), dim3((unsigned)std::min(need, most)),
                                        dim3(kThreads), 0, stream, a);
                 },
                 [&] {

@@ -6,8 +6,6 @@
 // HBM-bound: x and dy are read and dx written once, c (2 e_x + e_y) bytes a row. A group holds its columns'
 // sums in registers over all of its rows; a workgroup adds its groups' in LDS and writes one partial row, and
 // a second launch adds the partial rows, in their order, so the same inputs give the same bits.
-#include <type_traits>
-
 #include "layer_norm_train.h"
 
 namespace {
@@ -31,69 +29,81 @@ __device__ __forceinline__ void store_param(void* p, int dt, int64_t i, float v)
     else reinterpret_cast<uint16_t*>(p)[i] = dt == NORI_F16 ? f32_to_f16(v) : f32_to_bf16(v);
 }
 
-template <int XDT, int YDT, int V, int G, int NV>
+template <int XDT, int YDT, int V, int G, int NV, bool RAGGED>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const Backward a) {
     __shared__ float slots[16];
     int turn = 0;
     const int lane = threadIdx.x % G;
     const float inv_n = 1.0f / (float)a.cols;
     float w[NV][V], dw[NV][V], db[NV][V];
+    int at[NV], shared[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (i * G + lane) * V;
+        at[i] = column<V, G, RAGGED>(i, lane, a.cols, shared[i]);
 #pragma unroll
         for (int k = 0; k < V; ++k) w[i][k] = dw[i][k] = db[i][k] = 0.f;
-        if (c < a.cols) params<V>(a.w, a.wdt, c, 1.f, w[i]);
+        if (at[i] < a.cols) params<V>(a.w, a.wdt, at[i], 1.f, w[i]);
     }
     const int64_t per = kThreads / G, step = (int64_t)gridDim.x * per;
+    Raw<XDT, V> next_x[NV];
+    Raw<YDT, V> next_dy[NV];
+    float next_mean, next_rstd;
+    auto ask = [&](int64_t row) {
+        next_mean = next_rstd = 0.f;
+        if (row < a.rows) next_mean = a.mean[row], next_rstd = a.rstd[row];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            next_x[i] = {};
+            next_dy[i] = {};
+            if (row < a.rows && at[i] < a.cols) {
+                next_x[i] = fetch<XDT, V>(a.x, row * a.xs + at[i]);
+                next_dy[i] = fetch<YDT, V>(a.dy, row * a.dys + at[i]);
+            }
+        }
+    };
+    ask((int64_t)blockIdx.x * per + threadIdx.x / G);
     for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < a.rows; row0 += step) {
         const int64_t row = row0 + threadIdx.x / G;
-        const bool ok = row < a.rows;
         float x[NV][V], dy[NV][V];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + lane) * V;
-#pragma unroll
-            for (int k = 0; k < V; ++k) x[i][k] = dy[i][k] = 0.f;
-            if (ok && c < a.cols) {
-                load<XDT, V>(a.x, row * a.xs + c, x[i]);
-                load<YDT, V>(a.dy, row * a.dys + c, dy[i]);
-            }
+            widen<XDT, V>(next_x[i], x[i]);
+            widen<YDT, V>(next_dy[i], dy[i]);
         }
-        const float mean = ok ? a.mean[row] : 0.f, rstd = ok ? a.rstd[row] : 0.f;
+        const float mean = next_mean, rstd = next_rstd;
+        ask(row + step);  // the next row's loads run under this row's sums
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool in = (i * G + lane) * V < a.cols;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                x[i][k] = in ? (x[i][k] - mean) * rstd : 0.f;  // xh
-                const float g = dy[i][k] * w[i][k];
+                x[i][k] = (x[i][k] - mean) * rstd;  // xh; past the row's end dy and w are zero
+                const float d = !RAGGED || k >= shared[i] ? dy[i][k] : 0.f;
+                const float g = d * w[i][k];
                 s1 += g;
                 s2 += g * x[i][k];
-                dw[i][k] += dy[i][k] * x[i][k];
-                db[i][k] += dy[i][k];
+                dw[i][k] += d * x[i][k];
+                db[i][k] += d;
             }
-        }
         if (!a.dx) continue;
         group_sums<G>(s1, s2, slots, turn);
         s1 *= inv_n;
         s2 *= inv_n;
-        if (!ok) continue;
+        if (row >= a.rows) continue;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + lane) * V;
-            if (c >= a.cols) continue;
+            if (at[i] >= a.cols) continue;
             float d[V];
 #pragma unroll
             for (int k = 0; k < V; ++k) d[k] = rstd * (dy[i][k] * w[i][k] - s1 - x[i][k] * s2);
-            store<XDT, V>(a.dx, row * a.cols + c, d);
+            store<XDT, V>(a.dx, row * a.cols + at[i], d);
         }
     }
     if (!a.partial) return;
     float* out = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
     if constexpr (G < kThreads) {
-        // the groups' sums, one after another; columns past a.cols hold zeros
+        // The groups' sums, one after another. A moved vector's shared elements, zero in its sums, are another
+        // lane's of the same instruction: they are left to it.
         constexpr int kWide = V * G * NV;
         __shared__ float sums[2][kWide];
         for (int g = 0; g < kThreads / G; ++g) {
@@ -102,7 +112,8 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Backward a) {
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
                     for (int k = 0; k < V; ++k) {
-                        const int c = (i * G + lane) * V + k;
+                        if (RAGGED && k < shared[i]) continue;
+                        const int c = at[i] + k;
                         sums[0][c] = g == 0 ? dw[i][k] : sums[0][c] + dw[i][k];
                         sums[1][c] = g == 0 ? db[i][k] : sums[1][c] + db[i][k];
                     }
@@ -118,8 +129,8 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Backward a) {
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const int c = (i * G + lane) * V + k;
-                if (c < a.cols) {
+                const int c = at[i] + k;
+                if (c < a.cols && (!RAGGED || k >= shared[i])) {
                     out[c] = dw[i][k];
                     out[a.cols + c] = db[i][k];
                 }
@@ -219,17 +230,16 @@ extern "C" int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_
     Backward a{x,    dy, rows, x_row_stride, dy_row_stride, cols, weight, w_dtype, b_dtype, mean, rstd, dx, dw, db,
                columns ? reinterpret_cast<float*>(workspace) : nullptr, parts_of(rows)};
     hipStream_t stream = (hipStream_t)stream_v;
-    const bool vectors = whole4(x, x_dtype, cols, x_row_stride) && whole4(dy, dy_dtype, cols, dy_row_stride) &&
-                         whole4(dx, x_dtype, cols, cols);
     NORI_DISPATCH_FLOAT(x_dtype, XDT, {
         NORI_DISPATCH_FLOAT(dy_dtype, YDT, {
-            choose(
-                cols, vectors,
-                [&](auto V_, auto G_, auto NV_) {
+            choose<XDT>(
+                cols,
+                [&](auto V_, auto G_, auto NV_, auto R_) {
                     constexpr int V = decltype(V_)::value, G = decltype(G_)::value, NV = decltype(NV_)::value;
+                    constexpr bool R = decltype(R_)::value;
                     // never more workgroups than the workspace has rows for
                     a.parts = (int)std::min<int64_t>((rows + kThreads / G - 1) / (kThreads / G), a.parts);
-                    hipLaunchKernelGGL((backward_kernel<XDT, YDT, V, G, NV>), dim3((unsigned)a.parts), dim3(kThreads), 0,
+                    hipLaunchKernelGGL((backward_kernel<XDT, YDT, V, G, NV, R>), dim3((unsigned)a.parts), dim3(kThreads), 0,
                                        stream, a);
                 },
                 [&] {
