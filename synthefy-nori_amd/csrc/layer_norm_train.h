@@ -4,7 +4,7 @@
 // i of lane l is at column (i * G + l) * V. V is 16 bytes of x, read and written at any alignment (global memory
 // takes vectors at any byte); where a row is no whole number of vectors (RAGGED) its last one is moved back to
 // end with the row, and the elements that it shares with the one before are left out of the sums (stored twice,
-// the same value). G is 16 (rows up to 128), 64 or 256 (a workgroup). Rows shorter than a vector are held an
+// the same value). G is 4, 8 or 16 (rows up to 128), 64 or 256 (a workgroup). Rows shorter than a vector are held an
 // element a lane, rows too wide for registers are looped over.
 #pragma once
 
@@ -120,7 +120,9 @@ void choose(int cols, Go go, Loop loop) {
        std::integral_constant<bool, R>{})
 #define NORI_LN_TRY(G, NV) \
     if (cols <= VW * (G) * (NV)) return cols % VW ? NORI_LN_CALL(VW, G, NV, true) : NORI_LN_CALL(VW, G, NV, false)
-    if (cols < VW) return NORI_LN_CALL(1, 16, 1, false);
+    if (cols < VW) return NORI_LN_CALL(1, 8, 1, false);
+    NORI_LN_TRY(4, 1);
+    NORI_LN_TRY(8, 1);
     if constexpr (VW == 8) {
         NORI_LN_TRY(16, 1);
         NORI_LN_TRY(64, 1);

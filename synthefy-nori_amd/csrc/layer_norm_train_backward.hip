@@ -102,12 +102,21 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Backward a) {
     if (!a.partial) return;
     float* out = a.partial + (int64_t)blockIdx.x * 2 * a.cols;
     if constexpr (G < kThreads) {
-        // The groups' sums, one after another. A moved vector's shared elements, zero in its sums, are another
+        // The groups' sums: a wavefront's by shuffles, the wavefronts' one after another. A moved vector's shared elements, zero in its sums, are another
         // lane's of the same instruction: they are left to it.
         constexpr int kWide = V * G * NV;
         __shared__ float sums[2][kWide];
-        for (int g = 0; g < kThreads / G; ++g) {
-            if (threadIdx.x / G == g) {
+#pragma unroll
+        for (int off = G; off < 64; off <<= 1)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    dw[i][k] += __shfl_xor(dw[i][k], off, 64);
+                    db[i][k] += __shfl_xor(db[i][k], off, 64);
+                }
+        for (int g = 0; g < kThreads / 64; ++g) {
+            if (threadIdx.x / 64 == g && threadIdx.x % 64 < G) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -202,14 +211,19 @@ __global__ void __launch_bounds__(kJoin * kJoin) join_kernel(const Backward a) {
     if (blockIdx.y == 1 && a.db) store_param(a.db, a.bdt, c, s);
 }
 
-// Workgroups of the first launch: a row a group while there are few, then as many as run at once, three a
-// compute unit (their sums cost 8 c bytes each, twice).
-int parts_of(int64_t rows) { return (int)std::min<int64_t>((rows + 3) / 4, (int64_t)device_cus() * 3); }
+// Workgroups of the first launch: four rows each while there are few, then as many as a compute unit holds, by the
+// registers of a row: `held` values a lane. Fewer idle, more wait their turn, and each costs 8 c bytes of sums,
+// twice (262144 x 1680 bf16: 577 us with one a unit, 525 with two, 552 with three; 1048576 x 128 fp16: 282, 170
+// and 152; 4096 x 8192 fp16, whose rows take all registers: 56, 68 and 81).
+int64_t parts_of(int64_t rows, int held, bool workgroup_a_row) {
+    const int per = held <= 8 ? 3 : workgroup_a_row && held > 16 ? 1 : 2;
+    return std::min<int64_t>((rows + 3) / 4, (int64_t)device_cus() * per);
+}
 
 }  // namespace
 
 extern "C" int64_t nori_layer_norm_train_workspace_bytes(int64_t rows, int32_t cols) {
-    return rows <= 0 || cols <= 0 ? 0 : (int64_t)parts_of(rows) * 2 * cols * 4;
+    return rows <= 0 || cols <= 0 ? 0 : parts_of(rows, 1, false) * 2 * cols * 4;  // the most there can be
 }
 
 extern "C" int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_t rows, int32_t cols, int64_t x_row_stride,
@@ -228,7 +242,7 @@ extern "C" int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_
         return fail(NORI_ERR_INVALID, "layer_norm_train_backward: workspace of %lld bytes, %lld needed",
                     (long long)workspace_bytes, (long long)nori_layer_norm_train_workspace_bytes(rows, cols));
     Backward a{x,    dy, rows, x_row_stride, dy_row_stride, cols, weight, w_dtype, b_dtype, mean, rstd, dx, dw, db,
-               columns ? reinterpret_cast<float*>(workspace) : nullptr, parts_of(rows)};
+               columns ? reinterpret_cast<float*>(workspace) : nullptr, (int)parts_of(rows, 1, false)};
     hipStream_t stream = (hipStream_t)stream_v;
     NORI_DISPATCH_FLOAT(x_dtype, XDT, {
         NORI_DISPATCH_FLOAT(dy_dtype, YDT, {
@@ -237,8 +251,7 @@ extern "C" int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_
                 [&](auto V_, auto G_, auto NV_, auto R_) {
                     constexpr int V = decltype(V_)::value, G = decltype(G_)::value, NV = decltype(NV_)::value;
                     constexpr bool R = decltype(R_)::value;
-                    // never more workgroups than the workspace has rows for
-                    a.parts = (int)std::min<int64_t>((rows + kThreads / G - 1) / (kThreads / G), a.parts);
+                    a.parts = (int)std::min<int64_t>((rows + kThreads / G - 1) / (kThreads / G), parts_of(rows, V * NV, G == 256));
                     hipLaunchKernelGGL((backward_kernel<XDT, YDT, V, G, NV, R>), dim3((unsigned)a.parts), dim3(kThreads), 0,
                                        stream, a);
                 },
