@@ -79,8 +79,9 @@ def _grouped(ids: np.ndarray, counts: np.ndarray) -> tuple[np.ndarray, np.ndarra
     return order, np.append(at[where], total), groups
 
 
-def _update(x, y, a, b, plan, scales, transposed, out):
-    """``out`` = y + update (y None: the update alone) by ``nori_low_rank_update``; returns h [rows, rank]."""
+def _update(x, y, a, b, plan, scales, transposed, out, keep=True):
+    """``out`` = y + update (y None: the update alone) by ``nori_low_rank_update``; returns h [rows, rank], None
+    unless kept."""
     rank = int(a.shape[2 if transposed else 1])
     k, n = int(x.shape[-1]), int(out.shape[-1])
     x, rows, xs = _rows_of(x, k)
@@ -91,14 +92,18 @@ def _update(x, y, a, b, plan, scales, transposed, out):
     if layout is None:
         raise ValueError(f"out {tuple(out.shape)} has strides {out.stride()}: its rows must be at one stride")
     os = layout[1]
-    h = torch.empty((rows, rank), dtype=torch.float32, device=x.device)
+    h = torch.empty((rows, rank), dtype=torch.float32, device=x.device) if keep else None
+    lib, dtype, adapters = nat.lib(), nat.dtype_code(x.dtype), int(a.shape[0])
+    workspace, size = None, 0
+    if transposed:
+        size = lib.nori_low_rank_workspace_bytes(dtype, k, n, rank, adapters)
+        workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
     with nat.on(x.device):
         nat.check(
-            nat.lib().nori_low_rank_update(
-                x.data_ptr(), nat.dtype_code(x.dtype), rows, k, xs, nat.ptr(y), ys, a.data_ptr(), b.data_ptr(),
-                1 if transposed else 0, nat.ptr(scales), int(a.shape[0]), rank, n, plan.order.data_ptr(),
-                plan.starts.data_ptr(), plan.ids.data_ptr(), plan.groups, out.data_ptr(), os, h.data_ptr(),
-                nat.stream_of(x.device),
+            lib.nori_low_rank_update(
+                x.data_ptr(), dtype, rows, k, xs, nat.ptr(y), ys, a.data_ptr(), b.data_ptr(), 1 if transposed else 0,
+                nat.ptr(scales), adapters, rank, n, plan.order.data_ptr(), plan.starts.data_ptr(), plan.ids.data_ptr(),
+                plan.groups, out.data_ptr(), os, nat.ptr(h), nat.ptr(workspace), size, nat.stream_of(x.device),
             ),
             "low_rank_update",
         )
@@ -281,9 +286,9 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
         return out
     if _strided_rows(out, int(out.shape[-1])) is None:
         whole = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        _update(x, y, a, b, plan, scales, False, whole)
+        _update(x, y, a, b, plan, scales, False, whole, False)
         return out.copy_(whole)
-    _update(x, y, a, b, plan, scales, False, out)
+    _update(x, y, a, b, plan, scales, False, out, False)
     return out
 
 

@@ -104,7 +104,7 @@ def test_library_refuses_bad_arguments_before_any_device_work():
     bw = [16, nat.NORI_F16, 4, 10, 10, 16, nat.NORI_F16, 10, None, 0, 0, 16, 16, None, 16, None, None, 0, None]
     assert lib.nori_layer_norm_train_backward(*bw) == nat.NORI_ERR_INVALID  # dw without a workspace
     assert b"workspace" in lib.nori_last_error()
-    up = [None, nat.NORI_F16, 4, 8, 8, None, 8, None, None, 0, None, 2, 4, 8, None, None, None, 1, None, 8, None, None]
+    up = [None, nat.NORI_F16, 4, 8, 8, None, 8, None, None, 0, None, 2, 4, 8, None, None, None, 1, None, 8, None, None, 0, None]
     assert lib.nori_low_rank_update(*up) == nat.NORI_ERR_INVALID  # null pointers
     for at, value, code in ((1, nat.NORI_I8, nat.NORI_ERR_UNSUPPORTED), (12, 129, nat.NORI_ERR_UNSUPPORTED), (12, 0, nat.NORI_ERR_INVALID),
                             (3, 0, nat.NORI_ERR_INVALID), (2, 0, nat.NORI_OK), (2, 1 << 31, nat.NORI_ERR_UNSUPPORTED)):
