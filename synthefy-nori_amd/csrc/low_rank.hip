@@ -326,28 +326,181 @@ __global__ void __launch_bounds__(kThreads) transpose_kernel(const E* from, E* t
 }
 
 struct Grad {
-    const void* t;  // [rows][cols]
-    const float* h; // [rows][rank]
+    const void* t;   // [rows][cols]
+    const float* h;  // [rows][rank]
     int64_t ts;
     int cols, rank, adapters;
     const int32_t *order, *starts, *ids;
     int groups;
-    void* out;  // [adapters][...]
+    void* out;  // [adapters][cols][rank], transposed: [adapters][rank][cols]
     int64_t o_col, o_rank;
+    int part;        // rows of one; a multiple of 128
+    float* partial;  // [parts of the groups with more than one][cols][rank]
 };
 
-// a workgroup per (group, 256 columns, rank)
-template <int DT>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const Grad g) {
-    const int c = blockIdx.y * kThreads + threadIdx.x, j = blockIdx.z;
-    const int id = g.ids[blockIdx.x];
-    if (c >= g.cols || id < 0 || id >= g.adapters) return;
-    float v = 0.f;
-    for (int p = g.starts[blockIdx.x]; p < g.starts[blockIdx.x + 1]; ++p) {
-        const int64_t row = g.order[p];
-        v += load_elem<DT>(g.t, row * g.ts + c) * g.h[row * g.rank + j];
+// Where the partial sums of a group with several parts begin: 2 starts / part is enough for the ones before it,
+// since a length above `part` has at most twice length / part, less one, rounded up.
+__device__ __forceinline__ int64_t partial_of(const Grad& q, int group) { return 2 * (int64_t)q.starts[group] / q.part; }
+
+__device__ __forceinline__ void store_grad(const Grad& q, int dt, int id, int c, int j, float v) {
+    const int64_t i = (int64_t)id * q.cols * q.rank + c * q.o_col + j * q.o_rank;
+    if (dt == NORI_F32) reinterpret_cast<float*>(q.out)[i] = v;
+    else reinterpret_cast<uint16_t*>(q.out)[i] = dt == NORI_F16 ? f32_to_f16(v) : f32_to_bf16(v);
+}
+
+// t^T h over one part of a group's rows: 128 (fp32: 64) columns by up to 64 ranks a workgroup, whose wavefronts
+// take every fourth step of rows and add their sums in LDS, in order.
+// The sum runs over rows, which t has apart. 16-bit: a lane reads 16 bytes of each of 8 rows and turns the 8 x 8
+// block in registers, so that it holds 8 rows of one column for each of 8 instructions; column t of a lane's
+// block belongs to instruction t. fp32: an instruction takes 4 rows, no turning. h, in fp32, enters in two pieces
+// of the 16-bit type as in the update; a power of two per wavefront that follows the largest element so far keeps
+// fp16's pieces in range (sums so far are brought to a new one).
+template <int DT, int RT>
+__global__ void __launch_bounds__(kThreads) grad_kernel(const Grad q) {
+    using M = Mma<DT>;
+    using E = typename M::elem;
+    using F = typename M::frag;
+    constexpr bool F32 = DT == NORI_F32;
+    constexpr int W = M::W, CT = W;            // a lane's columns, an instruction each
+    constexpr int STEP = F32 ? 4 : 32;         // rows of a step
+    constexpr int U = F32 ? 4 : 1;             // steps whose loads go together
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    int number;
+    const int group = group_of_tile(q.starts, q.groups, q.part, blockIdx.x, number);
+    const int begin = q.starts[group], last = q.starts[group + 1];
+    const int64_t first64 = (int64_t)begin + (int64_t)number * q.part;
+    const int id = q.ids[group];
+    if (first64 >= last || id < 0 || id >= q.adapters) return;
+    const int first = (int)first64, end = min(last, first + q.part);
+    const int c0 = blockIdx.y * 16 * W + W * m, j0 = blockIdx.z * 16 * RT;
+    const E* t = reinterpret_cast<const E*>(q.t) + c0;
+    const int there = q.cols - c0;
+
+    f32x4 acc[RT][CT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < CT; ++i) acc[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float up = 1.0f, down = 1.0f;
+    float reach = 0.f;  // elements below it fit the present power of two
+    constexpr int EACH = F32 ? 1 : 8;  // rows a lane holds of a step
+    for (int p0 = first + wave * STEP * U; p0 < end; p0 += STEP * U * kWaves) {
+        F raw[U][EACH];
+        float h[U][EACH][RT];
+#pragma unroll
+        for (int s = 0; s < U; ++s)
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int p = p0 + STEP * s + EACH * g + i;
+                const int64_t row = q.order[min(p, end - 1)];
+                raw[s][i] = F{};
+                if (p < end) raw[s][i] = fetch<DT>(t + row * q.ts, there);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const int j = j0 + 16 * r + m;
+                    h[s][i][r] = p < end && j < q.rank ? q.h[row * q.rank + j] : 0.f;
+                }
+            }
+        if constexpr (F32) {
+#pragma unroll
+            for (int s = 0; s < U; ++s)
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int i = 0; i < CT; ++i)
+                        acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(raw[s][0][i], h[s][0][r], acc[r][i], 0, 0, 0);
+        } else {
+            if constexpr (DT == NORI_F16) {
+                float largest = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        const float v = fabsf(h[0][i][r]);
+                        largest = v < __builtin_inff() ? fmaxf(largest, v) : largest;
+                    }
+#pragma unroll
+                for (int off = 32; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
+                if (largest > reach) {  // the same in every lane
+                    const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 8, -110), 110);
+                    const float to = __uint_as_float((uint32_t)(127 - e) << 23);
+                    const float change = reach > 0.f ? to * up : 0.f;  // no sums yet: they are zero
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int i = 0; i < CT; ++i) acc[r][i] = reach > 0.f ? acc[r][i] * change : acc[r][i];
+                    up = __uint_as_float((uint32_t)(127 + e) << 23);
+                    down = to;
+                    reach = up * 512.0f;  // scaled: below 2^9, the pieces of the smallest that counts above 2^-24
+                }
+            }
+            F high[RT], low[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = h[0][i][r] * down;
+                    high[r][i] = narrow<DT>(v);
+                    low[r][i] = fabsf(v) < __builtin_inff() ? narrow<DT>(v - widen<DT>(high[r][i])) : E(0);
+                }
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
+                F col;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) col[e] = raw[0][e][i];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    acc[r][i] = M::mul(col, high[r], acc[r][i]);
+                    acc[r][i] = M::mul(col, low[r], acc[r][i]);
+                }
+            }
+        }
     }
-    store_elem<DT>(g.out, (int64_t)id * g.cols * g.rank + c * g.o_col + j * g.o_rank, v);
+    // the wavefronts' sums, a rank tile at a time. acc[r][i][j] of lane (m, g): column W (4 g + j) + i, rank 16 r + m
+    __shared__ f32x4 sums[kWaves][CT][64];
+    const bool whole = last - begin <= q.part;
+    float* part = whole ? nullptr : q.partial + (partial_of(q, group) + number) * q.cols * q.rank;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < CT; ++i) sums[wave][i][lane] = acc[r][i] * up;
+        __syncthreads();
+        for (int i = wave; i < CT; i += kWaves) {
+            const f32x4 v = (sums[0][i][lane] + sums[1][i][lane]) + (sums[2][i][lane] + sums[3][i][lane]);
+            const int j = j0 + 16 * r + m;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = blockIdx.y * 16 * W + W * (4 * g + e) + i;
+                if (c >= q.cols || j >= q.rank) continue;
+                if (whole) store_grad(q, DT, id, c, j, v[e]);
+                else part[(int64_t)c * q.rank + j] = v[e];
+            }
+        }
+    }
+}
+
+// the parts of the groups that have several, in their order
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(const Grad q, int dt) {
+    const int group = blockIdx.y, id = q.ids[group];
+    const int length = q.starts[group + 1] - q.starts[group];
+    const int64_t size = (int64_t)q.cols * q.rank, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (length <= q.part || id < 0 || id >= q.adapters || i >= size) return;
+    const float* part = q.partial + partial_of(q, group) * size + i;
+    const int parts = (length + q.part - 1) / q.part;
+    float v = 0.f;
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) v += part[p * size];
+    store_grad(q, dt, id, (int)(i / q.rank), (int)(i % q.rank), v);
+}
+
+// Rows of a part: about four workgroups a compute unit, and no part so short that its sums cost as much as its rows
+// (8 rank bytes a column, twice, against 2 to 4 a row).
+int part_of(int64_t rows, int cols, int rank, int dtype) {
+    const int wide = dtype == NORI_F32 ? 64 : 128;
+    const int64_t chunks = (int64_t)((cols + wide - 1) / wide) * ((rank + 63) / 64);
+    const int64_t want = rows * chunks / (4 * (int64_t)device_cus());
+    return (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 256), 8192);
 }
 
 bool is_float(int dt) { return dt == NORI_F32 || dt == NORI_F16 || dt == NORI_BF16; }
@@ -432,20 +585,50 @@ extern "C" int nori_low_rank_update(const void* x, int dtype, int64_t rows, int3
     return launch_status("low_rank_update");
 }
 
+extern "C" int64_t nori_low_rank_weight_grad_workspace_bytes(int dtype, int64_t rows, int32_t cols, int32_t rank,
+                                                             int64_t longest) {
+    if (rows <= 0 || cols <= 0 || rank <= 0) return 0;
+    const int part = part_of(rows, cols, rank, dtype);
+    return longest <= part ? 0 : (2 * rows / part + 1) * cols * rank * 4;
+}
+
 extern "C" int nori_low_rank_weight_grad(const void* t, int dtype, int64_t rows, int32_t cols, int64_t t_row_stride,
                                          const float* h, int32_t rank, int32_t adapters, const int32_t* order,
-                                         const int32_t* starts, const int32_t* ids, int32_t groups, int32_t transposed,
-                                         void* out, void* stream_v) {
+                                         const int32_t* starts, const int32_t* ids, int32_t groups, int64_t longest,
+                                         int32_t transposed, void* out, void* workspace, int64_t workspace_bytes,
+                                         void* stream_v) {
     clear_error();
     if (int rc = check("low_rank_weight_grad", dtype, rows, groups, cols, 1, rank, adapters)) return rc;
     if (rows == 0) return NORI_OK;
     if (!t || !h || !order || !starts || !ids || !out || groups <= 0)
         return fail(NORI_ERR_INVALID, "low_rank_weight_grad: null pointer");
-    Grad g{t, h, t_row_stride, cols, rank, adapters, order, starts, ids, groups, out, rank, 1};
-    if (transposed) g.o_col = 1, g.o_rank = cols;
+    if (longest < 1 || longest > rows)
+        return fail(NORI_ERR_INVALID, "low_rank_weight_grad: a longest group of %lld rows of %lld", (long long)longest, (long long)rows);
+    const int64_t need = nori_low_rank_weight_grad_workspace_bytes(dtype, rows, cols, rank, longest);
+    if (need && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < need))
+        return fail(NORI_ERR_INVALID, "low_rank_weight_grad: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                    (long long)need);
+    Grad q{t, h, t_row_stride, cols, rank, adapters, order, starts, ids, groups, out, rank, 1, part_of(rows, cols, rank, dtype),
+           reinterpret_cast<float*>(workspace)};
+    if (transposed) q.o_col = 1, q.o_rank = cols;
+    hipStream_t stream = (hipStream_t)stream_v;
+    const int64_t parts = rows / q.part + groups;
+    auto go = [&](auto DT_, auto RT_) {
+        constexpr int DT = decltype(DT_)::value, RT = decltype(RT_)::value, WIDE = 16 * Mma<DT>::W;
+        hipLaunchKernelGGL((grad_kernel<DT, RT>),
+                           dim3((unsigned)parts, (unsigned)((cols + WIDE - 1) / WIDE), (unsigned)((rank + 16 * RT - 1) / (16 * RT))),
+                           dim3(kThreads), 0, stream, q);
+    };
     NORI_DISPATCH_FLOAT(dtype, DT, {
-        hipLaunchKernelGGL((grad_kernel<DT>), dim3(groups, (unsigned)((cols + kThreads - 1) / kThreads), rank), dim3(kThreads), 0,
-                           (hipStream_t)stream_v, g);
+        constexpr std::integral_constant<int, DT> DT_{};
+        if (rank <= 16) go(DT_, std::integral_constant<int, 1>{});
+        else if (rank <= 32) go(DT_, std::integral_constant<int, 2>{});
+        else go(DT_, std::integral_constant<int, 4>{});
     });
+    if (need) {
+        const int64_t size = (int64_t)cols * rank;
+        hipLaunchKernelGGL(grad_join_kernel, dim3((unsigned)((size + kThreads - 1) / kThreads), groups), dim3(kThreads), 0, stream,
+                           q, dtype);
+    }
     return launch_status("low_rank_weight_grad");
 }

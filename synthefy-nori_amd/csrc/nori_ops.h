@@ -121,11 +121,14 @@ int nori_low_rank_update(const void* x, int dtype, int64_t rows, int32_t k, int6
 int64_t nori_low_rank_workspace_bytes(int dtype, int32_t k, int32_t n, int32_t rank, int32_t adapters);
 
 // The sum over each adapter's rows of t[i]^T h[i] as out [adapters, cols, rank] (transposed: [adapters, rank,
-// cols]) of t's dtype, t [rows, cols] at a row stride, h [rows, rank] fp32, the groups as above. Adapters without
-// a group are left as they are.
+// cols]) of t's dtype, t [rows, cols] at a row stride, h [rows, rank] fp32, the groups as above, `longest` the most
+// rows of one with an adapter. Groups of many rows are summed in parts, joined in a fixed order, in the
+// workspace. Adapters without a group are left as they are.
 int nori_low_rank_weight_grad(const void* t, int dtype, int64_t rows, int32_t cols, int64_t t_row_stride, const float* h,
                               int32_t rank, int32_t adapters, const int32_t* order, const int32_t* starts,
-                              const int32_t* ids, int32_t groups, int32_t transposed, void* out, void* stream);
+                              const int32_t* ids, int32_t groups, int64_t longest, int32_t transposed, void* out,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+int64_t nori_low_rank_weight_grad_workspace_bytes(int dtype, int64_t rows, int32_t cols, int32_t rank, int64_t longest);
 
 #ifdef __cplusplus
 }

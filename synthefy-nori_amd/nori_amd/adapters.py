@@ -62,6 +62,7 @@ class AdapterPlan:
         order, starts, groups = _grouped(np.asarray(ids, dtype=np.int64), np.asarray(counts, dtype=np.int64))
         self.adapters = tuple(int(i) for i in groups if i >= 0)  # those with rows, ascending
         self.groups = len(groups)
+        self.longest = int(np.diff(starts)[groups >= 0].max(initial=0))  # the most rows of one adapter
         packed = torch.from_numpy(np.concatenate([starts, groups, order]).astype(np.int32)).to(self.device)
         self.starts, self.ids, self.order = packed.split([self.groups + 1, self.groups, self.rows])
 
@@ -115,13 +116,16 @@ def _weight_grad(t, h, plan, like, transposed):
     cols = int(t.shape[-1])
     t, rows, ts = _rows_of(t, cols)
     out = torch.empty_like(like) if len(plan.adapters) == like.shape[0] else torch.zeros_like(like)
-    if rows:
+    if plan.longest:
+        lib, dtype, rank = nat.lib(), nat.dtype_code(t.dtype), int(h.shape[1])
+        size = lib.nori_low_rank_weight_grad_workspace_bytes(dtype, rows, cols, rank, plan.longest)
+        workspace = torch.empty(size, dtype=torch.uint8, device=t.device) if size else None
         with nat.on(t.device):
             nat.check(
-                nat.lib().nori_low_rank_weight_grad(
-                    t.data_ptr(), nat.dtype_code(t.dtype), rows, cols, ts, h.data_ptr(), int(h.shape[1]), int(like.shape[0]),
-                    plan.order.data_ptr(), plan.starts.data_ptr(), plan.ids.data_ptr(), plan.groups, 1 if transposed else 0,
-                    out.data_ptr(), nat.stream_of(t.device),
+                lib.nori_low_rank_weight_grad(
+                    t.data_ptr(), dtype, rows, cols, ts, h.data_ptr(), rank, int(like.shape[0]), plan.order.data_ptr(),
+                    plan.starts.data_ptr(), plan.ids.data_ptr(), plan.groups, plan.longest, 1 if transposed else 0,
+                    out.data_ptr(), nat.ptr(workspace), size, nat.stream_of(t.device),
                 ),
                 "low_rank_update backward",
             )
