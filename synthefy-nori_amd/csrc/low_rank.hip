@@ -97,6 +97,14 @@ __device__ __forceinline__ int group_of_tile(const int32_t* starts, int groups, 
     return g;
 }
 
+// What this wavefront wrote to LDS is what its lanes read after this: LDS serves a wavefront in order, the compiler
+// has to keep it.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 struct Update {
     const void *x, *y, *a, *b;
     int64_t xs, ys, os;
@@ -107,159 +115,374 @@ struct Update {
     int columns;  // of out, a workgroup's
     void* out;
     float* h;  // [rows][rank], rows as in x; null: not kept
+    void *pa, *pb;  // the groups' factors as operands (Packed), or null: read where they lie
 };
 
-// RP: the rank rounded up to 16, 32, 64 or 128. TM rows a tile. With 64 rows each wavefront sums its own 16 rows
-// of h over all of k; with 16 rows the wavefronts share the rows and split k (few rows: the latency of k counts).
-// Both products put the factor's rows where results run along the lane's registers: h comes as 4 ranks a lane, out
-// as W consecutive columns of a row.
-// h enters the second product in two pieces of the inputs' type, high and low, which keep 22 bits of a row's
-// largest element in fp16 (after a power of two that brings the row near 1, so that nothing leaves fp16's range)
-// and 16 in bf16; in fp32 it stays as it is. The result, rounded once, holds at most 11 and 8 bits.
-template <int DT, int RP, int TM>
+// The factors in the order that the matrix instructions take them: an operand's 64 lanes side by side, ranks and ends
+// padded with zeros. The factor of the first product: [step along k][rank tile], KB elements of k (128 bytes of a row of
+// x) rounded up; of the second: [tile of 16 columns][operand along the rank], 64 columns rounded up. Read from where
+// they lie, an operand's lanes are 16 rows apart, which takes the address units four times as long.
+template <int DT, int RP>
+struct Packed {
+    using M = Mma<DT>;
+    static constexpr int W = M::W, KS = 4 * W, KB = 8 * W, RT = RP / 16;
+    static constexpr bool F32 = DT == NORI_F32;
+    static constexpr bool HALF = !F32 && RP == 16;  // a rank of 16 fills half an operand: its other half takes the low pieces
+    static constexpr int KC = F32 ? RP / 16 : (RP + 31) / 32;
+    static constexpr int PER = W / 4;  // tiles of 16 columns that make a lane's W consecutive ones
+
+    __host__ __device__ static int batches(int k) { return (k + KB - 1) / KB; }
+    __host__ __device__ static int tiles(int n) { return (n + 63) / 64 * 4; }
+    static constexpr int LANES = HALF ? 32 : 64;  // of an operand of the second product
+    // vectors of one adapter
+    __host__ __device__ static int64_t first(int k) { return (int64_t)batches(k) * 2 * RT * 64; }
+    __host__ __device__ static int64_t second(int n) { return (int64_t)tiles(n) * KC * LANES; }
+    // of tile t, the column of a lane's row m: its result then is W columns side by side, in lanes of one m 16 PER apart
+    __device__ static int column(int t, int m) { return 16 * PER * (t / PER) + W * (m >> 2) + 4 * (t % PER) + (m & 3); }
+    __device__ static int rank_of(int c, int g) { return HALF ? W * (g & 1) : KS * c + W * g; }
+};
+
+// a lane's W elements of an operand a thread
+template <int DT, int RP>
+__global__ void __launch_bounds__(kThreads) pack_kernel(const Update u, int transposed) {
+    using P = Packed<DT, RP>;
+    using E = typename Mma<DT>::elem;
+    const int group = blockIdx.y, id = u.ids[group];
+    if (id < 0 || id >= u.adapters) return;
+    const int64_t first = P::first(u.k), i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int lane = (int)(i % 64), m = lane & 15, g = lane >> 4;  // (first is a multiple of 64)
+    typename Mma<DT>::frag f = {};
+    if (i < first) {
+        const int op = (int)(i / 64), j = 16 * (op % P::RT) + m, k0 = op / P::RT * P::KS + P::W * g;
+        const E* a = reinterpret_cast<const E*>(u.a) + (int64_t)id * u.rank * u.k;
+        if (j < u.rank) {
+#pragma unroll
+            for (int e = 0; e < P::W; ++e)
+                if (k0 + e < u.k) f[e] = transposed ? a[(int64_t)(k0 + e) * u.rank + j] : a[(int64_t)j * u.k + k0 + e];
+        }
+        reinterpret_cast<typename Mma<DT>::frag*>(u.pa)[group * first + i] = f;
+        return;
+    }
+    const int64_t second = P::second(u.n), at = i - first;
+    if (at >= second) return;
+    const int op = (int)(at / P::LANES), n = P::column(op / P::KC, m), rank0 = P::rank_of(op % P::KC, g);
+    const E* b = reinterpret_cast<const E*>(u.b) + (int64_t)id * u.n * u.rank;
+    if (n < u.n) {
+#pragma unroll
+        for (int e = 0; e < P::W; ++e)
+            if (rank0 + e < u.rank) f[e] = transposed ? b[(int64_t)(rank0 + e) * u.n + n] : b[(int64_t)n * u.rank + rank0 + e];
+    }
+    reinterpret_cast<typename Mma<DT>::frag*>(u.pb)[group * second + at] = f;
+}
+
+// A lane's ranks of h, rank 16 t + 4 g + j of row m in acc[t][j], times s: kept in fp32 (`keep`, null: not), and put
+// into LDS as the second product takes them, in two pieces of the inputs' type, high and low, which keep 22 bits of a
+// row's largest element in fp16 (after a power of two that brings the row near 1, so that nothing leaves fp16's
+// range) and 16 in bf16; in fp32 h stays as it is. The result, rounded once, holds at most 11 and 8 bits.
+template <int DT, int RT, int ROWS, int PITCH, int PIECES>
+__device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float* keep, int g, int row,
+                                      typename Mma<DT>::elem (&hs)[PIECES][ROWS][PITCH], float (&factor)[ROWS]) {
+    using E = typename Mma<DT>::elem;
+    float largest = 0.f;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool in = 16 * t + 4 * g + j < rank;
+            acc[t][j] = in ? acc[t][j] * s : 0.f;
+            if (in && keep) keep[16 * t + 4 * g + j] = acc[t][j];
+            const float v = fabsf(acc[t][j]);
+            largest = v < __builtin_inff() ? fmaxf(largest, v) : largest;
+        }
+    float up = 1.0f, down = 1.0f;
+    if constexpr (DT == NORI_F16) {
+        largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
+        largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
+        // 2^e, the largest element's binade, and 2^-e; e within what both are normal for
+        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -120), 120);
+        up = __uint_as_float((uint32_t)(127 + e) << 23);
+        down = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+    if (g == 0) factor[row] = up;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float v = acc[t][j] * down;
+            const E high = narrow<DT>(v);
+            hs[0][row][16 * t + 4 * g + j] = high;
+            if constexpr (PIECES == 2)
+                hs[1][row][16 * t + 4 * g + j] = fabsf(v) < __builtin_inff() ? narrow<DT>(v - widen<DT>(high)) : E(0);
+        }
+}
+
+// Many rows. A workgroup takes 64 rows of one group: each wavefront its own 16 through the first product, then all 64
+// through the second for 64 columns at a time. x, y and out pass through LDS, a wavefront's own, between the order
+// they lie in memory (8 lanes a run of 128 bytes) and the operands' (a lane a row), and the packed factors are read
+// as operands: every access takes the address units as few cycles as its bytes do.
+// RP: the rank rounded up to 16, 32, 64 or 128.
+template <int DT, int RP>
 __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
     using M = Mma<DT>;
+    using P = Packed<DT, RP>;
     using E = typename M::elem;
     using F = typename M::frag;
-    constexpr int W = M::W, KS = 4 * W, RT = RP / 16, TILES = TM / 16;
-    constexpr bool F32 = DT == NORI_F32;
-    constexpr int PIECES = F32 ? 1 : 2;
-    constexpr int PITCH = RP + W;  // of a row of h in LDS, in elements
-    __shared__ __align__(16) E hs[PIECES][TM][PITCH];
-    __shared__ float factor[TM];
-    __shared__ f32x4 part[TM == 16 ? kWaves : 1][TM == 16 ? RT : 1][64];
+    constexpr int W = M::W, RT = P::RT, KB = P::KB, KC = P::KC, PER = P::PER;
+    constexpr int PIECES = P::F32 ? 1 : 2, PITCH = RP + W;  // of a row of h in LDS, in elements
+    constexpr int NT = 4, CB = 16 * NT, OUT = CB + 4;       // columns at a time, a row of them in LDS
+    constexpr int XROW = KB + W;                            // a row of x in LDS
+    constexpr int LC = CB / W, LR = 64 / LC, LI = 16 / LR;  // lanes along a row of out, rows at once, times a tile
+    constexpr int AHEAD = 4;  // batches of x asked for before the one in work
+    union Stage {
+        E x[2][16][XROW];
+        float out[2][16][OUT];
+    };
+    __shared__ __align__(16) Stage stage[kWaves];
+    __shared__ __align__(16) E hs[PIECES][64][PITCH];
+    __shared__ float factor[64];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     int number;
-    const int group = group_of_tile(u.starts, u.groups, TM, blockIdx.x, number);
+    const int group = group_of_tile(u.starts, u.groups, 64, blockIdx.x, number);
     const int end = u.starts[group + 1];
-    const int64_t first64 = (int64_t)u.starts[group] + (int64_t)number * TM;
+    const int64_t first64 = (int64_t)u.starts[group] + (int64_t)number * 64;
     if (first64 >= end) return;
     const int first = (int)first64;
     const int id = u.ids[group];
     const bool active = id >= 0 && id < u.adapters;
+    if (!active && u.y == u.out) return;  // the rows stay as they are
+
+    // y's and out's rows of this lane, 16 a tile, and the columns
+    const int stop = min(u.n, ((int)blockIdx.y + 1) * u.columns), lc = W * (lane % LC);
+    int row[4 * LI];
+#pragma unroll
+    for (int i = 0; i < 4 * LI; ++i) row[i] = u.order[min(first + LR * i + lane / LC, end - 1)];
+    F y[4 * LI];
+    auto ask = [&](int i, int n0) {
+        y[i] = F{};
+        if (!u.y || n0 >= stop) return;
+        const E* p = reinterpret_cast<const E*>(u.y) + (int64_t)row[i] * u.ys + n0 + lc;
+        if (n0 + CB <= u.n) y[i] = fetch<DT>(p);
+        else y[i] = fetch<DT>(p, u.n - n0 - lc);
+    };
+    int n0 = blockIdx.y * u.columns + CB * wave;
+#pragma unroll
+    for (int i = 0; i < 4 * LI; ++i) ask(i, n0);
 
     if (active) {
         // ---- h = s x A^T
-        const int mine = TM == 16 ? 0 : 16 * wave;
-        const int64_t row = u.order[min(first + mine + m, end - 1)];
-        const E* x = reinterpret_cast<const E*>(u.x) + row * u.xs + W * g;
-        const E* a = reinterpret_cast<const E*>(u.a) + (int64_t)id * u.rank * u.k + W * g;
+        const F* pa = reinterpret_cast<const F*>(u.pa) + group * P::first(u.k) + lane;
+        const int xr = lane >> 3, xc = W * (lane & 7), batches = P::batches(u.k);
+        const E* x0 = reinterpret_cast<const E*>(u.x) + (int64_t)u.order[min(first + 16 * wave + xr, end - 1)] * u.xs + xc;
+        const E* x1 = reinterpret_cast<const E*>(u.x) + (int64_t)u.order[min(first + 16 * wave + 8 + xr, end - 1)] * u.xs + xc;
+        F xf[AHEAD][2];
+        auto askx = [&](int i, F (&f)[2]) {
+            if ((i + 1) * KB <= u.k) {
+                f[0] = fetch<DT>(x0 + i * KB);
+                f[1] = fetch<DT>(x1 + i * KB);
+            } else {
+                f[0] = fetch<DT>(x0 + i * KB, u.k - i * KB - xc);
+                f[1] = fetch<DT>(x1 + i * KB, u.k - i * KB - xc);
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (j < batches) askx(j, xf[j]);
         f32x4 acc[RT];
-        const E* at[RT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            at[t] = a + (int64_t)min(16 * t + m, u.rank - 1) * u.k;  // ranks past the last are dropped below
-        }
-        const int whole = u.k / KS;
-        constexpr int kStep = TM == 16 ? kWaves : 1;
-#pragma unroll 4
-        for (int s = TM == 16 ? wave : 0; s < whole; s += kStep) {
-            const F xf = fetch<DT>(x + s * KS);
+        for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < batches; i0 += AHEAD) {
 #pragma unroll
-            for (int t = 0; t < RT; ++t) acc[t] = M::mul(fetch<DT>(at[t] + s * KS), xf, acc[t]);
-        }
-        if (u.k % KS && (TM != 16 || wave == whole % kWaves)) {
-            const int there = u.k - whole * KS - W * g;
-            const F xf = fetch<DT>(x + whole * KS, there);
+            for (int j = 0; j < AHEAD; ++j) {
+                const int i = i0 + j;
+                if (i >= batches) break;
+                F af[2][RT];
 #pragma unroll
-            for (int t = 0; t < RT; ++t) acc[t] = M::mul(fetch<DT>(at[t] + whole * KS, there), xf, acc[t]);
-        }
-        if constexpr (TM == 16) {
+                for (int q = 0; q < 2 * RT; ++q) af[q / RT][q % RT] = pa[(int64_t)(i * 2 * RT + q) * 64];
+                E(&xs)[16][XROW] = stage[wave].x[j & 1];
+                *reinterpret_cast<F*>(&xs[xr][xc]) = xf[j][0];
+                *reinterpret_cast<F*>(&xs[8 + xr][xc]) = xf[j][1];
+                if (i + AHEAD < batches) askx(i + AHEAD, xf[j]);
+                wave_sync();
 #pragma unroll
-            for (int t = 0; t < RT; ++t) part[wave][t][lane] = acc[t];
-            __syncthreads();
+                for (int q = 0; q < 2; ++q) {
+                    const F v = *reinterpret_cast<const F*>(&xs[m][q * 4 * W + W * g]);
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-                acc[t] = (part[0][t][lane] + part[1][t][lane]) + (part[2][t][lane] + part[3][t][lane]);
-        }
-        const float s = u.scales ? u.scales[id] : 1.0f;
-        float largest = 0.f;
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                acc[t][j] = 16 * t + 4 * g + j < u.rank ? acc[t][j] * s : 0.f;
-                const float v = fabsf(acc[t][j]);
-                largest = v < __builtin_inff() ? fmaxf(largest, v) : largest;
-            }
-        if (TM != 16 || wave == 0) {
-            if (u.h && blockIdx.y == 0 && first + mine + m < end) {
-                float* h = u.h + row * u.rank;
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (16 * t + 4 * g + j < u.rank) h[16 * t + 4 * g + j] = acc[t][j];
-            }
-            float up = 1.0f, down = 1.0f;
-            if constexpr (DT == NORI_F16) {
-                largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
-                largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
-                // 2^e, the largest element's binade, and 2^-e; e within what both are normal for
-                const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -120), 120);
-                up = __uint_as_float((uint32_t)(127 + e) << 23);
-                down = __uint_as_float((uint32_t)(127 - e) << 23);
-            }
-            if (g == 0) factor[mine + m] = up;
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float v = acc[t][j] * down;
-                    const E high = narrow<DT>(v);
-                    hs[0][mine + m][16 * t + 4 * g + j] = high;
-                    if constexpr (!F32) {
-                        const float rest = v - widen<DT>(high);
-                        hs[1][mine + m][16 * t + 4 * g + j] = fabsf(v) < __builtin_inff() ? narrow<DT>(rest) : E(0);
-                    }
+                    for (int t = 0; t < RT; ++t) acc[t] = M::mul(af[q][t], v, acc[t]);
                 }
+            }
+            wave_sync();
         }
+        const int p = first + 16 * wave + m;
+        float* keep = u.h && blockIdx.y == 0 && p < end ? u.h + (int64_t)u.order[min(p, end - 1)] * u.rank : nullptr;
+        put_h<DT, RT, 64, PITCH, PIECES>(acc, u.scales ? u.scales[id] : 1.0f, u.rank, keep, g, 16 * wave + m, hs, factor);
         __syncthreads();
-    } else if (u.y == u.out) {
-        return;  // the rows stay as they are
     }
 
     // ---- out = y + h B^T
-    constexpr int PER = W / 4;        // tiles of 16 columns that make a lane's W consecutive ones
-    constexpr int NT = 4, NV = NT / PER;  // tiles and vectors a step
-    constexpr int KC = F32 ? RP / 16 : (RP + 31) / 32;  // operands along the rank
-    int64_t yrow[TILES], orow[TILES];
+    const F* pb = reinterpret_cast<const F*>(u.pb) + group * P::second(u.n) + lane % P::LANES;
+    for (; n0 < stop; n0 += CB * kWaves) {
+        F bf[KC][NT];
+        if (active) {
 #pragma unroll
-    for (int r = 0; r < TILES; ++r) {
-        const int64_t row = u.order[min(first + 16 * r + m, end - 1)];
-        yrow[r] = row * u.ys;
-        orow[r] = row * u.os;
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) bf[c][t] = pb[(int64_t)((n0 / 16 + t) * KC + c) * P::LANES];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float(&os)[16][OUT] = stage[wave].out[r & 1];
+            if (active) {
+                f32x4 acc[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int p = 0; p < (P::HALF ? 1 : PIECES); ++p) {
+                        const F hf = *reinterpret_cast<const F*>(&hs[P::HALF ? g >> 1 : p][16 * r + m][P::rank_of(c, g)]);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t] = M::mul(bf[c][t], hf, acc[t]);
+                    }
+                const float f = factor[16 * r + m];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    *reinterpret_cast<f32x4*>(&os[m][16 * PER * (t / PER) + W * g + 4 * (t % PER)]) = acc[t] * f;
+                wave_sync();
+            }
+#pragma unroll
+            for (int i = 0; i < LI; ++i) {
+                const int at = LR * i + lane / LC;
+                F o = y[LI * r + i];  // rows without an adapter keep y's bits
+                ask(LI * r + i, n0 + CB * kWaves);
+                if (active) {
+                    float d[W];
+#pragma unroll
+                    for (int e = 0; e < W; e += 4)
+                        *reinterpret_cast<f32x4*>(&d[e]) = *reinterpret_cast<const f32x4*>(&os[at][lc + e]);
+#pragma unroll
+                    for (int e = 0; e < W; ++e) o[e] = narrow<DT>(widen<DT>(o[e]) + d[e]);
+                }
+                if (first + 16 * r + at >= end) continue;
+                E* to = reinterpret_cast<E*>(u.out) + (int64_t)row[LI * r + i] * u.os + n0 + lc;
+                if (n0 + CB <= u.n || n0 + lc + W <= u.n) {
+                    __builtin_memcpy(to, &o, sizeof o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < W; ++e)
+                        if (n0 + lc + e < u.n) to[e] = o[e];
+                }
+            }
+        }
+        wave_sync();
     }
+}
+
+// Few rows, where what counts is how long one tile takes: the wavefronts of a workgroup share a tile of 16 rows, split
+// k among them, and take 32 columns each at a time. The factors are read where they lie (u.pa null) or packed.
+template <int DT, int RP>
+__global__ void __launch_bounds__(kThreads) update_few_kernel(const Update u) {
+    using M = Mma<DT>;
+    using P = Packed<DT, RP>;
+    using E = typename M::elem;
+    using F = typename M::frag;
+    constexpr int W = M::W, KS = P::KS, RT = P::RT, KC = P::KC, PER = P::PER;
+    constexpr int PIECES = P::F32 ? 1 : 2, PITCH = RP + W;
+    constexpr int NT = 2, CB = 16 * NT, NV = NT / PER;
+    __shared__ __align__(16) E hs[PIECES][16][PITCH];
+    __shared__ float factor[16];
+    __shared__ f32x4 part[kWaves][RT][64];
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
+    int number;
+    const int group = group_of_tile(u.starts, u.groups, 16, blockIdx.x, number);
+    const int end = u.starts[group + 1];
+    const int64_t first64 = (int64_t)u.starts[group] + (int64_t)number * 16;
+    if (first64 >= end) return;
+    const int first = (int)first64;
+    const int id = u.ids[group];
+    const bool active = id >= 0 && id < u.adapters;
+    if (!active && u.y == u.out) return;  // the rows stay as they are
+
+    const int stop = min(u.n, ((int)blockIdx.y + 1) * u.columns);
+    const int64_t row = u.order[min(first + m, end - 1)];
+    F y[NV];
+    auto ask = [&](int n0) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = n0 + 16 * PER * v + W * g;
+            y[v] = F{};
+            if (u.y && n0 < stop) y[v] = fetch<DT>(reinterpret_cast<const E*>(u.y) + row * u.ys + c, u.n - c);
+        }
+    };
+    int n0 = blockIdx.y * u.columns + CB * wave;
+    ask(n0);
+
+    if (active) {
+        // ---- h = s x A^T
+        const E* x = reinterpret_cast<const E*>(u.x) + row * u.xs + W * g;
+        const E* a = reinterpret_cast<const E*>(u.a) + (int64_t)id * u.rank * u.k + W * g;
+        const F* pa = reinterpret_cast<const F*>(u.pa) + group * P::first(u.k) + lane;
+        f32x4 acc[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int AHEAD = RT <= 2 ? 4 : RT == 4 ? 2 : 1;  // steps whose loads go together
+        auto steps = [&](int s, auto many, auto whole) {
+            constexpr int N = decltype(many)::value;
+            F xf[N], af[N][RT];
+#pragma unroll
+            for (int p = 0; p < N; ++p) {
+                const int k0 = (s + p * kWaves) * KS;
+                const int there = decltype(whole)::value ? W : u.k - k0 - W * g;
+                xf[p] = fetch<DT>(x + k0, there);
+#pragma unroll
+                for (int t = 0; t < RT; ++t)  // ranks past the last are dropped by put_h
+                    af[p][t] = u.pa ? pa[(int64_t)((s + p * kWaves) * RT + t) * 64]
+                                    : fetch<DT>(a + (int64_t)min(16 * t + m, u.rank - 1) * u.k + k0, there);
+            }
+#pragma unroll
+            for (int p = 0; p < N; ++p)
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[t] = M::mul(af[p][t], xf[p], acc[t]);
+        };
+        int s = wave;
+        for (; (s + (AHEAD - 1) * kWaves + 1) * KS <= u.k; s += AHEAD * kWaves)
+            steps(s, std::integral_constant<int, AHEAD>{}, std::true_type{});
+        for (; s * KS < u.k; s += kWaves) steps(s, std::integral_constant<int, 1>{}, std::false_type{});
+#pragma unroll
+        for (int t = 0; t < RT; ++t) part[wave][t][lane] = acc[t];
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+                acc[t] = (part[0][t][lane] + part[1][t][lane]) + (part[2][t][lane] + part[3][t][lane]);
+            float* keep = u.h && blockIdx.y == 0 && first + m < end ? u.h + row * u.rank : nullptr;
+            put_h<DT, RT, 16, PITCH, PIECES>(acc, u.scales ? u.scales[id] : 1.0f, u.rank, keep, g, m, hs, factor);
+        }
+        __syncthreads();
+    }
+
+    // ---- out = y + h B^T
     const E* b = reinterpret_cast<const E*>(u.b) + (int64_t)(active ? id : 0) * u.n * u.rank;
     const int64_t behind = (int64_t)(u.adapters - (active ? id : 0)) * u.n * u.rank;  // elements from b to the bank's end
-    const int stop = min(u.n, ((int)blockIdx.y + 1) * u.columns);
-    for (int n0 = blockIdx.y * u.columns + 64 * wave; n0 < stop; n0 += 64 * kWaves) {
-        F yv[TILES][NV];
+    const F* pb = reinterpret_cast<const F*>(u.pb) + group * P::second(u.n) + lane % P::LANES;
+    const float f = active ? factor[m] : 0.f;
+    for (; n0 < stop; n0 += CB * kWaves) {
+        f32x4 acc[NT];
 #pragma unroll
-        for (int r = 0; r < TILES; ++r)
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int c = n0 + 16 * PER * v + W * g;
-                yv[r][v] = F{};
-                if (u.y) yv[r][v] = fetch<DT>(reinterpret_cast<const E*>(u.y) + yrow[r] + c, u.n - c);
-            }
-        f32x4 acc[TILES][NT];
-#pragma unroll
-        for (int r = 0; r < TILES; ++r)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (active) {
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                // a rank of 16 fills half an operand: its other half takes the low pieces
-                const int rank0 = (!F32 && RP == 16 ? W * (g & 1) : 4 * W * c + W * g);
+                const int rank0 = P::rank_of(c, g);
                 F bf[NT];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const int n = min(n0 + 16 * PER * (t / PER) + W * (m >> 2) + 4 * (t % PER) + (m & 3), u.n - 1);
-                    const int64_t i = (int64_t)n * u.rank + rank0;
+                    if (u.pb) {
+                        bf[t] = pb[(int64_t)((n0 / 16 + t) * KC + c) * P::LANES];
+                        continue;
+                    }
+                    const int64_t i = (int64_t)min(n0 + P::column(t, m), u.n - 1) * u.rank + rank0;
                     bf[t] = F{};
                     if (rank0 < u.rank) {
                         if (i + W <= behind) bf[t] = fetch<DT>(b + i);  // past its rank's end: dropped next
@@ -270,59 +493,37 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
                     }
                 }
 #pragma unroll
-                for (int p = 0; p < (!F32 && RP == 16 ? 1 : PIECES); ++p)
+                for (int p = 0; p < (P::HALF ? 1 : PIECES); ++p) {
+                    const F hf = *reinterpret_cast<const F*>(&hs[P::HALF ? g >> 1 : p][m][rank0]);
 #pragma unroll
-                    for (int r = 0; r < TILES; ++r) {
-                        const int piece = !F32 && RP == 16 ? g >> 1 : p;
-                        const F hf = *reinterpret_cast<const F*>(&hs[piece][16 * r + m][rank0]);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[r][t] = M::mul(bf[t], hf, acc[r][t]);
-                    }
+                    for (int t = 0; t < NT; ++t) acc[t] = M::mul(bf[t], hf, acc[t]);
+                }
             }
         }
+        F o[NV];
 #pragma unroll
-        for (int r = 0; r < TILES; ++r) {
-            if (first + 16 * r + m >= end) continue;
-            const float f = active ? factor[16 * r + m] : 0.f;
+        for (int v = 0; v < NV; ++v) {
+            o[v] = y[v];  // rows without an adapter keep y's bits
+            if (active) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int c = n0 + 16 * PER * v + W * g;
-                if (c >= stop) continue;
-                F o;
+                for (int e = 0; e < W; ++e) o[v][e] = narrow<DT>(widen<DT>(o[v][e]) + f * acc[v * PER + e / 4][e % 4]);
+            }
+        }
+        ask(n0 + CB * kWaves);
+        if (first + m >= end) continue;
 #pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    // rows without an adapter keep y's bits
-                    o[e] = active ? narrow<DT>(widen<DT>(yv[r][v][e]) + f * acc[r][v * PER + e / 4][e % 4]) : yv[r][v][e];
-                }
-                E* to = reinterpret_cast<E*>(u.out) + orow[r] + c;
-                if (c + W <= u.n) {
-                    __builtin_memcpy(to, &o, sizeof o);
-                } else {
+        for (int v = 0; v < NV; ++v) {
+            const int c = n0 + 16 * PER * v + W * g;
+            E* to = reinterpret_cast<E*>(u.out) + row * u.os + c;
+            if (c + W <= u.n) {
+                __builtin_memcpy(to, &o[v], sizeof(F));
+            } else {
 #pragma unroll
-                    for (int e = 0; e < W; ++e)
-                        if (c + e < u.n) to[e] = o[e];
-                }
+                for (int e = 0; e < W; ++e)
+                    if (c + e < u.n) to[e] = o[v][e];
             }
         }
     }
-}
-
-// [adapter][rows][cols] -> [adapter][cols][rows] of the groups' adapters, 32 x 32 elements a workgroup
-template <typename E>
-__global__ void __launch_bounds__(kThreads) transpose_kernel(const E* from, E* to, int rows, int cols, const int32_t* ids,
-                                                             int adapters) {
-    __shared__ E tile[32][33];
-    const int id = ids[blockIdx.z];
-    if (id < 0 || id >= adapters) return;
-    const int64_t base = (int64_t)id * rows * cols;
-    const int c = threadIdx.x % 32, r = threadIdx.x / 32, row0 = blockIdx.y * 32, col0 = blockIdx.x * 32;
-#pragma unroll
-    for (int i = r; i < 32; i += 8)
-        if (row0 + i < rows && col0 + c < cols) tile[i][c] = from[base + (int64_t)(row0 + i) * cols + col0 + c];
-    __syncthreads();
-#pragma unroll
-    for (int i = r; i < 32; i += 8)
-        if (col0 + i < cols && row0 + c < rows) to[base + (int64_t)(col0 + i) * rows + row0 + c] = tile[c][i];
 }
 
 struct Grad {
@@ -518,8 +719,30 @@ int check(const char* what, int dtype, int64_t rows, int32_t groups, int32_t k, 
 
 }  // namespace
 
-extern "C" int64_t nori_low_rank_workspace_bytes(int dtype, int32_t k, int32_t n, int32_t rank, int32_t adapters) {
-    return (int64_t)adapters * rank * ((int64_t)k + n) * dtype_size(dtype);
+// Whether a tile a workgroup of 64 rows leaves most compute units idle, or most of each tile empty.
+static bool few_rows(int64_t rows, int32_t groups) { return rows / 64 + groups < 2 * device_cus() || rows <= 16 * (int64_t)groups; }
+
+template <class Go>
+static int by_rank(int32_t rank, Go go) {
+    if (rank <= 16) return go(std::integral_constant<int, 16>{});
+    if (rank <= 32) return go(std::integral_constant<int, 32>{});
+    if (rank <= 64) return go(std::integral_constant<int, 64>{});
+    return go(std::integral_constant<int, 128>{});
+}
+
+extern "C" int64_t nori_low_rank_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups,
+                                                 int32_t transposed) {
+    if (!is_float(dtype) || rows <= 0 || k <= 0 || n <= 0 || rank <= 0 || groups <= 0) return 0;
+    if (!transposed && few_rows(rows, groups)) return 0;
+    int64_t bytes = 0;
+    NORI_DISPATCH_FLOAT(dtype, DT, {
+        by_rank(rank, [&](auto RP_) {
+            using P = Packed<DT, decltype(RP_)::value>;
+            bytes = groups * (P::first(k) + P::second(n)) * 16;
+            return 0;
+        });
+    });
+    return bytes;
 }
 
 extern "C" int nori_low_rank_update(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* y,
@@ -536,51 +759,38 @@ extern "C" int nori_low_rank_update(const void* x, int dtype, int64_t rows, int3
     if (out_row_stride < n && rows > 1) return fail(NORI_ERR_INVALID, "low_rank_update: rows of out overlap");
     if (out == y && out_row_stride != y_row_stride && rows > 1)
         return fail(NORI_ERR_INVALID, "low_rank_update: out is y, at another row stride");
-    if (transposed && (!workspace || workspace_bytes < nori_low_rank_workspace_bytes(dtype, k, n, rank, adapters)))
+    const int64_t need = nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, groups, transposed);
+    if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
         return fail(NORI_ERR_INVALID, "low_rank_update: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                    (long long)nori_low_rank_workspace_bytes(dtype, k, n, rank, adapters));
-    Update u{x, y, a, b, x_row_stride, y_row_stride, out_row_stride, k, n, rank, adapters, scales, order, starts, ids, groups,
-             0, out, h};
+                    (long long)need);
+    Update u{x,  y, a,   b,      x_row_stride, y_row_stride, out_row_stride, k, n, rank, adapters, scales, order, starts, ids, groups,
+             0, out, h, nullptr, nullptr};
     hipStream_t stream = (hipStream_t)stream_v;
-    if (transposed) {
-        // the factors as the products read them: rows along their sums
-        auto turn = [&](auto e) {
-            using E = decltype(e);
-            E* at = reinterpret_cast<E*>(workspace);
-            E* bt = at + (int64_t)adapters * rank * k;
-            hipLaunchKernelGGL((transpose_kernel<E>), dim3((rank + 31) / 32, (k + 31) / 32, groups), dim3(kThreads), 0, stream,
-                               reinterpret_cast<const E*>(a), at, k, rank, ids, adapters);
-            hipLaunchKernelGGL((transpose_kernel<E>), dim3((n + 31) / 32, (rank + 31) / 32, groups), dim3(kThreads), 0, stream,
-                               reinterpret_cast<const E*>(b), bt, rank, n, ids, adapters);
-            u.a = at;
-            u.b = bt;
-        };
-        if (dtype == NORI_F32) turn(float{});
-        else turn(uint16_t{});
-    }
     const int cus = device_cus();
-    auto go = [&](auto DT_, auto RP_, auto TM_) {
-        constexpr int DT = decltype(DT_)::value, RP = decltype(RP_)::value, TM = decltype(TM_)::value;
-        const int64_t tiles = rows / TM + groups;
-        // out's columns are shared among workgroups, each with an h of its own, while there are few tiles
-        const int most = (n + 64 * kWaves - 1) / (64 * kWaves);
-        const int split = (int)std::min<int64_t>(most, std::max<int64_t>(1, 2 * cus / tiles));
-        const int steps = (most + split - 1) / split;
-        u.columns = steps * 64 * kWaves;
-        // tiles in multiples of 8: a tile's workgroups stay on one XCD, whose L2 holds its x
-        const unsigned gx = (unsigned)((tiles + 7) / 8 * 8), gy = (unsigned)((most + steps - 1) / steps);
-        hipLaunchKernelGGL((update_kernel<DT, RP, TM>), dim3(gx, gy), dim3(kThreads), 0, stream, u);
-    };
-    auto by_tile = [&](auto DT_, auto RP_) {
-        if (rows <= 16 * (int64_t)groups) go(DT_, RP_, std::integral_constant<int, 16>{});
-        else go(DT_, RP_, std::integral_constant<int, 64>{});
-    };
+    const bool few = few_rows(rows, groups);
     NORI_DISPATCH_FLOAT(dtype, DT, {
-        constexpr std::integral_constant<int, DT> DT_{};
-        if (rank <= 16) by_tile(DT_, std::integral_constant<int, 16>{});
-        else if (rank <= 32) by_tile(DT_, std::integral_constant<int, 32>{});
-        else if (rank <= 64) by_tile(DT_, std::integral_constant<int, 64>{});
-        else by_tile(DT_, std::integral_constant<int, 128>{});
+        by_rank(rank, [&](auto RP_) {
+            constexpr int RP = decltype(RP_)::value;
+            using P = Packed<DT, RP>;
+            if (need) {
+                u.pa = workspace;
+                u.pb = reinterpret_cast<char*>(workspace) + groups * P::first(k) * 16;
+                const int64_t each = P::first(k) + P::second(n);
+                hipLaunchKernelGGL((pack_kernel<DT, RP>), dim3((unsigned)((each + kThreads - 1) / kThreads), groups), dim3(kThreads),
+                                   0, stream, u, transposed);
+            }
+            const int64_t tiles = rows / (few ? 16 : 64) + groups;
+            // out's columns are shared among workgroups, each with an h of its own, while there are few tiles
+            const int wide = (few ? 32 : 64) * kWaves, most = (n + wide - 1) / wide;
+            const int split = (int)std::min<int64_t>(most, std::max<int64_t>(1, 2 * cus / tiles));
+            const int steps = (most + split - 1) / split;
+            u.columns = steps * wide;
+            // tiles in multiples of 8: a tile's workgroups stay on one XCD, whose L2 holds its x
+            const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)((most + steps - 1) / steps));
+            if (few) hipLaunchKernelGGL((update_few_kernel<DT, RP>), grid, dim3(kThreads), 0, stream, u);
+            else hipLaunchKernelGGL((update_kernel<DT, RP>), grid, dim3(kThreads), 0, stream, u);
+            return 0;
+        });
     });
     return launch_status("low_rank_update");
 }

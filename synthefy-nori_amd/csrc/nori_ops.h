@@ -111,14 +111,16 @@ int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_t rows, int
 // (transposed: a [adapters, k, rank] and b [adapters, rank, n]); scales [adapters] fp32 or NULL for 1.
 // order [rows] lists the rows of group 0, then of group 1, ...: group g is order[starts[g] .. starts[g + 1]),
 // its adapter ids[g] or -1, each id once. h [rows, rank] fp32, or NULL, takes scales[id] x[i] a[id]^T (rows without
-// an adapter are left). Transposed factors are turned in the workspace, of nori_low_rank_workspace_bytes.
+// an adapter are left). The workspace, of nori_low_rank_workspace_bytes and 16-byte aligned, takes the factors in
+// the matrix instructions' order (none is needed for few rows with the factors as they are).
 #define NORI_LOW_RANK_MAX 128
 int nori_low_rank_update(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* y,
                          int64_t y_row_stride, const void* a, const void* b, int32_t transposed, const float* scales,
                          int32_t adapters, int32_t rank, int32_t n, const int32_t* order, const int32_t* starts,
                          const int32_t* ids, int32_t groups, void* out, int64_t out_row_stride, float* h, void* workspace,
                          int64_t workspace_bytes, void* stream);
-int64_t nori_low_rank_workspace_bytes(int dtype, int32_t k, int32_t n, int32_t rank, int32_t adapters);
+int64_t nori_low_rank_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups,
+                                      int32_t transposed);
 
 // The sum over each adapter's rows of t[i]^T h[i] as out [adapters, cols, rank] (transposed: [adapters, rank,
 // cols]) of t's dtype, t [rows, cols] at a row stride, h [rows, rank] fp32, the groups as above, `longest` the most

@@ -162,7 +162,7 @@ OPS: dict[str, tuple[object, list]] = {
         [_vp, _i32, _i64, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _vp,
          _vp, _i64, _vp],
     ),
-    "nori_low_rank_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "nori_low_rank_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32, _i32]),
     "nori_low_rank_weight_grad": (
         ctypes.c_int,
         [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i64, _i32, _vp, _vp, _i64, _vp],

@@ -95,10 +95,8 @@ def _update(x, y, a, b, plan, scales, transposed, out, keep=True):
     os = layout[1]
     h = torch.empty((rows, rank), dtype=torch.float32, device=x.device) if keep else None
     lib, dtype, adapters = nat.lib(), nat.dtype_code(x.dtype), int(a.shape[0])
-    workspace, size = None, 0
-    if transposed:
-        size = lib.nori_low_rank_workspace_bytes(dtype, k, n, rank, adapters)
-        workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    size = lib.nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, plan.groups, 1 if transposed else 0)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     with nat.on(x.device):
         nat.check(
             lib.nori_low_rank_update(
