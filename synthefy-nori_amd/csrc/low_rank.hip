@@ -151,15 +151,23 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Update u, int tran
     if (id < 0 || id >= u.adapters) return;
     const int64_t first = P::first(u.k), i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     const int lane = (int)(i % 64), m = lane & 15, g = lane >> 4;  // (first is a multiple of 64)
-    typename Mma<DT>::frag f = {};
+    using F = typename Mma<DT>::frag;
+    // elements i0 ... of a row of `count` at a stride, zeros behind its end; every load before the first use
+    auto gather = [](const E* p, int i0, int count, int64_t stride) {
+        if (stride == 1 && i0 + P::W <= count) return fetch<DT>(p + i0);
+        E v[P::W];
+#pragma unroll
+        for (int e = 0; e < P::W; ++e) v[e] = p[min(i0 + e, count - 1) * stride];
+        F f;
+#pragma unroll
+        for (int e = 0; e < P::W; ++e) f[e] = i0 + e < count ? v[e] : E(0);
+        return f;
+    };
+    F f = {};
     if (i < first) {
         const int op = (int)(i / 64), j = 16 * (op % P::RT) + m, k0 = op / P::RT * P::KS + P::W * g;
         const E* a = reinterpret_cast<const E*>(u.a) + (int64_t)id * u.rank * u.k;
-        if (j < u.rank) {
-#pragma unroll
-            for (int e = 0; e < P::W; ++e)
-                if (k0 + e < u.k) f[e] = transposed ? a[(int64_t)(k0 + e) * u.rank + j] : a[(int64_t)j * u.k + k0 + e];
-        }
+        if (j < u.rank) f = gather(a + (transposed ? (int64_t)j : (int64_t)j * u.k), k0, u.k, transposed ? u.rank : 1);
         reinterpret_cast<typename Mma<DT>::frag*>(u.pa)[group * first + i] = f;
         return;
     }
@@ -167,11 +175,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Update u, int tran
     if (at >= second) return;
     const int op = (int)(at / P::LANES), n = P::column(op / P::KC, m), rank0 = P::rank_of(op % P::KC, g);
     const E* b = reinterpret_cast<const E*>(u.b) + (int64_t)id * u.n * u.rank;
-    if (n < u.n) {
-#pragma unroll
-        for (int e = 0; e < P::W; ++e)
-            if (rank0 + e < u.rank) f[e] = transposed ? b[(int64_t)(rank0 + e) * u.n + n] : b[(int64_t)n * u.rank + rank0 + e];
-    }
+    if (n < u.n) f = gather(b + (transposed ? (int64_t)n : (int64_t)n * u.rank), rank0, u.rank, transposed ? u.n : 1);
     reinterpret_cast<typename Mma<DT>::frag*>(u.pb)[group * second + at] = f;
 }
 
@@ -216,12 +220,17 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
         }
 }
 
-// Many rows. A workgroup takes 64 rows of one group: each wavefront its own 16 through the first product, then all 64
-// through the second for 64 columns at a time. x, y and out pass through LDS, a wavefront's own, between the order
-// they lie in memory (8 lanes a run of 128 bytes) and the operands' (a lane a row), and the packed factors are read
-// as operands: every access takes the address units as few cycles as its bytes do.
+// Many rows. A wavefront takes 16 R rows of one group through both products by itself; the four of a workgroup share
+// the factors' cache lines only. R is 1, or 2 for ranks above 32, where reading the factors costs more than the
+// registers and the LDS of twice the rows (65536 rows 1408 -> 1408: rank 64 165 against 147 us, rank 16 132 against 173). x, y and out pass through the wavefront's LDS between the order they lie in memory
+// (8 lanes a run of 128 bytes) and the operands' (a lane a row), and the packed factors are read as operands: every
+// access takes the address units as few cycles as its bytes do.
+// y and out go in windows of 128 bytes that begin where a line of out does, each row at columns of its own: the
+// result's last two blocks of columns stay in LDS. Windows at the same columns of every row leave lines half written
+// where rows are not whole lines (65536 rows of 1680 fp16, y to out alone: 136 us against 95, of 999: 65 against 45).
+// The hot loops take whole vectors only: what is left at a row's ends has code of its own, once.
 // RP: the rank rounded up to 16, 32, 64 or 128.
-template <int DT, int RP>
+template <int DT, int RP, int R>
 __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
     using M = Mma<DT>;
     using P = Packed<DT, RP>;
@@ -229,152 +238,243 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
     using F = typename M::frag;
     constexpr int W = M::W, RT = P::RT, KB = P::KB, KC = P::KC, PER = P::PER;
     constexpr int PIECES = P::F32 ? 1 : 2, PITCH = RP + W;  // of a row of h in LDS, in elements
-    constexpr int NT = 4, CB = 16 * NT, OUT = CB + 4;       // columns at a time, a row of them in LDS
+    constexpr int CB = KB, NT = CB / 16;                    // columns of a window: 128 bytes
+    constexpr int RING = 2 * CB, OUT = RING + W + 4;        // a row of the result: two blocks, the first W columns again
     constexpr int XROW = KB + W;                            // a row of x in LDS
-    constexpr int LC = CB / W, LR = 64 / LC, LI = 16 / LR;  // lanes along a row of out, rows at once, times a tile
-    constexpr int AHEAD = 4;  // batches of x asked for before the one in work
+    constexpr int AHEAD = !P::F32 && RP == 16 ? 3 : 2;      // batches of x, windows of y asked for in advance
     union Stage {
-        E x[2][16][XROW];
-        float out[2][16][OUT];
+        E x[2][16 * R][XROW];
+        float out[16 * R][OUT];
     };
     __shared__ __align__(16) Stage stage[kWaves];
-    __shared__ __align__(16) E hs[PIECES][64][PITCH];
-    __shared__ float factor[64];
+    __shared__ __align__(16) E hs[kWaves][PIECES][16 * R][PITCH];
+    __shared__ float factor[kWaves][16 * R];
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     int number;
-    const int group = group_of_tile(u.starts, u.groups, 64, blockIdx.x, number);
+    const int group = group_of_tile(u.starts, u.groups, 64 * R, blockIdx.x, number);
     const int end = u.starts[group + 1];
-    const int64_t first64 = (int64_t)u.starts[group] + (int64_t)number * 64;
+    const int64_t first64 = (int64_t)u.starts[group] + ((int64_t)number * 64 + 16 * wave) * R;
     if (first64 >= end) return;
     const int first = (int)first64;
     const int id = u.ids[group];
     const bool active = id >= 0 && id < u.adapters;
     if (!active && u.y == u.out) return;  // the rows stay as they are
 
-    // y's and out's rows of this lane, 16 a tile, and the columns
-    const int stop = min(u.n, ((int)blockIdx.y + 1) * u.columns), lc = W * (lane % LC);
-    int row[4 * LI];
+    // this lane's two rows in memory's order, its elements of a run, and where the rows' windows begin
+    const int r0 = lane >> 3, lc = W * (lane & 7);
+    const E* yrow[2 * R];
+    E* orow[2 * R];
+    int begin[2 * R];
+    int shift = 0, any = 0;
 #pragma unroll
-    for (int i = 0; i < 4 * LI; ++i) row[i] = u.order[min(first + LR * i + lane / LC, end - 1)];
-    F y[4 * LI];
-    auto ask = [&](int i, int n0) {
-        y[i] = F{};
-        if (!u.y || n0 >= stop) return;
-        const E* p = reinterpret_cast<const E*>(u.y) + (int64_t)row[i] * u.ys + n0 + lc;
-        if (n0 + CB <= u.n) y[i] = fetch<DT>(p);
-        else y[i] = fetch<DT>(p, u.n - n0 - lc);
+    for (int i = 0; i < 2 * R; ++i) {
+        const int64_t row = u.order[min(first + 8 * i + r0, end - 1)];
+        orow[i] = reinterpret_cast<E*>(u.out) + row * u.os;
+        yrow[i] = reinterpret_cast<const E*>(u.y) + row * u.ys;
+        const int past = (int)((uintptr_t)orow[i] / sizeof(E) % CB);
+        begin[i] = lc - past;
+        shift = max(shift, past);
+        any |= begin[i];
+    }
+    const int blocks = (u.n + CB - 1) / CB;
+    const int windows = blocks + (__ballot(shift > blocks * CB - u.n) ? 1 : 0);
+    const bool vectors = !__ballot((any & 3) != 0);  // of the result in LDS
+    // Where rows begin and end with whole vectors every window is taken in vectors, some of them past the row's ends;
+    // else the first and the last are taken an element at a time.
+    const bool whole = u.n % W == 0 && !__ballot(any % W != 0);
+    const int inner0 = whole || !__ballot(shift != 0) ? 0 : 1;
+    const int inner1 = whole ? windows : max(inner0, u.n / CB);
+    const F* pb = reinterpret_cast<const F*>(u.pb) + group * P::second(u.n) + lane % P::LANES;
+    F y[AHEAD][2 * R], bf[AHEAD][KC * NT];
+    // Loads come back in the order they were asked for: a window's operands are asked for beside its y, or waiting for
+    // them would be waiting for every later y too.
+    auto ask = [&](int k, F (&f)[2 * R], F (&b)[KC * NT]) {
+        if (active && k < blocks) {
+#pragma unroll
+            for (int q = 0; q < KC * NT; ++q) b[q] = pb[(int64_t)(k * NT * KC + q) * P::LANES];
+        }
+        if (!u.y) return;
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) {
+            const int c = k * CB + begin[i];
+            if (c >= 0 && c + W <= u.n) f[i] = fetch<DT>(yrow[i] + c);
+        }
     };
-    int n0 = blockIdx.y * u.columns + CB * wave;
 #pragma unroll
-    for (int i = 0; i < 4 * LI; ++i) ask(i, n0);
+    for (int j = 0; j < AHEAD; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) y[j][i] = F{};
+        if (inner0 + j < inner1) ask(inner0 + j, y[j], bf[j]);
+    }
 
+    constexpr int HF = P::HALF ? 1 : KC * PIECES;
+    F hf[R][HF];
+    float f[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) f[r] = 0.f;
     if (active) {
         // ---- h = s x A^T
         const F* pa = reinterpret_cast<const F*>(u.pa) + group * P::first(u.k) + lane;
-        const int xr = lane >> 3, xc = W * (lane & 7), batches = P::batches(u.k);
-        const E* x0 = reinterpret_cast<const E*>(u.x) + (int64_t)u.order[min(first + 16 * wave + xr, end - 1)] * u.xs + xc;
-        const E* x1 = reinterpret_cast<const E*>(u.x) + (int64_t)u.order[min(first + 16 * wave + 8 + xr, end - 1)] * u.xs + xc;
-        F xf[AHEAD][2];
-        auto askx = [&](int i, F (&f)[2]) {
-            if ((i + 1) * KB <= u.k) {
-                f[0] = fetch<DT>(x0 + i * KB);
-                f[1] = fetch<DT>(x1 + i * KB);
-            } else {
-                f[0] = fetch<DT>(x0 + i * KB, u.k - i * KB - xc);
-                f[1] = fetch<DT>(x1 + i * KB, u.k - i * KB - xc);
+        const int batches = P::batches(u.k);
+        const bool odd = u.k % W != 0;
+        const E* x[2 * R];
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i)
+            x[i] = reinterpret_cast<const E*>(u.x) + (int64_t)u.order[min(first + 8 * i + r0, end - 1)] * u.xs + lc;
+        F xf[AHEAD][2 * R], af[AHEAD][2 * RT];
+        auto askx = [&](int i, F (&f)[2 * R], F (&a)[2 * RT]) {
+#pragma unroll
+            for (int q = 0; q < 2 * RT; ++q) a[q] = pa[(int64_t)(i * 2 * RT + q) * 64];
+#pragma unroll
+            for (int q = 0; q < 2 * R; ++q) {
+                f[q] = F{};
+                if (i * KB + lc + W <= u.k) f[q] = fetch<DT>(x[q] + i * KB);
             }
         };
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
-            if (j < batches) askx(j, xf[j]);
-        f32x4 acc[RT];
+            if (j < batches) askx(j, xf[j], af[j]);
+        f32x4 acc[R][RT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int i0 = 0; i0 < batches; i0 += AHEAD) {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int i = i0 + j;
                 if (i >= batches) break;
-                F af[2][RT];
+                E(&xs)[16 * R][XROW] = stage[wave].x[j & 1];
 #pragma unroll
-                for (int q = 0; q < 2 * RT; ++q) af[q / RT][q % RT] = pa[(int64_t)(i * 2 * RT + q) * 64];
-                E(&xs)[16][XROW] = stage[wave].x[j & 1];
-                *reinterpret_cast<F*>(&xs[xr][xc]) = xf[j][0];
-                *reinterpret_cast<F*>(&xs[8 + xr][xc]) = xf[j][1];
-                if (i + AHEAD < batches) askx(i + AHEAD, xf[j]);
+                for (int q = 0; q < 2 * R; ++q) *reinterpret_cast<F*>(&xs[8 * q + r0][lc]) = xf[j][q];
+                if (odd && i == batches - 1) {  // the elements behind the last whole vector
+                    const int c = (u.k / W * W + g) % KB, k = u.k / W * W + g;
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const E* from = reinterpret_cast<const E*>(u.x) + (int64_t)u.order[min(first + 16 * r + m, end - 1)] * u.xs;
+                        if (k < u.k) xs[16 * r + m][c] = from[k];
+                        if (k + 4 < u.k) xs[16 * r + m][c + 4] = from[k + 4];
+                    }
+                }
                 wave_sync();
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const F v = *reinterpret_cast<const F*>(&xs[m][q * 4 * W + W * g]);
+                for (int q = 0; q < 2; ++q)
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) acc[t] = M::mul(af[q][t], v, acc[t]);
-                }
+                    for (int r = 0; r < R; ++r) {
+                        const F v = *reinterpret_cast<const F*>(&xs[16 * r + m][q * 4 * W + W * g]);
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) acc[r][t] = M::mul(af[j][q * RT + t], v, acc[r][t]);
+                    }
+                if (i + AHEAD < batches) askx(i + AHEAD, xf[j], af[j]);
+                wave_sync();
             }
-            wave_sync();
         }
-        const int p = first + 16 * wave + m;
-        float* keep = u.h && blockIdx.y == 0 && p < end ? u.h + (int64_t)u.order[min(p, end - 1)] * u.rank : nullptr;
-        put_h<DT, RT, 64, PITCH, PIECES>(acc, u.scales ? u.scales[id] : 1.0f, u.rank, keep, g, 16 * wave + m, hs, factor);
-        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int p = first + 16 * r + m;
+            float* keep = u.h && p < end ? u.h + (int64_t)u.order[min(p, end - 1)] * u.rank : nullptr;
+            put_h<DT, RT, 16 * R, PITCH, PIECES>(acc[r], u.scales ? u.scales[id] : 1.0f, u.rank, keep, g, 16 * r + m, hs[wave],
+                                                 factor[wave]);
+        }
+        wave_sync();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            f[r] = factor[wave][16 * r + m];
+#pragma unroll
+            for (int q = 0; q < HF; ++q)
+                hf[r][q] = *reinterpret_cast<const F*>(&hs[wave][P::HALF ? g >> 1 : q % PIECES][16 * r + m][P::rank_of(q / PIECES, g)]);
+        }
     }
 
     // ---- out = y + h B^T
-    const F* pb = reinterpret_cast<const F*>(u.pb) + group * P::second(u.n) + lane % P::LANES;
-    for (; n0 < stop; n0 += CB * kWaves) {
-        F bf[KC][NT];
-        if (active) {
+    float(&os)[16 * R][OUT] = stage[wave].out;
+    // block k of the result, into its half of the ring
+    auto product = [&](int k, const F (&b)[KC * NT]) {
+        const int half = k % 2 * CB;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            f32x4 acc[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < KC; ++c)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) bf[c][t] = pb[(int64_t)((n0 / 16 + t) * KC + c) * P::LANES];
+                for (int q = 0; q < (P::HALF ? 1 : PIECES); ++q)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[t] = M::mul(b[t * KC + c], hf[r][P::HALF ? 0 : c * PIECES + q], acc[t]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int c = 16 * PER * (t / PER) + W * g + 4 * (t % PER);
+                const f32x4 v = acc[t] * f[r];
+                *reinterpret_cast<f32x4*>(&os[16 * r + m][half + c]) = v;
+                if (t < PER && g == 0 && half == 0) *reinterpret_cast<f32x4*>(&os[16 * r + m][RING + c]) = v;
+            }
         }
+    };
+    for (int k = 0; k < windows;) {
+        if (k < inner0 || k >= inner1) {
+            if (active && k < blocks) {
+                F b[KC * NT];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float(&os)[16][OUT] = stage[wave].out[r & 1];
-            if (active) {
-                f32x4 acc[NT];
+                for (int q = 0; q < KC * NT; ++q) b[q] = pb[(int64_t)(k * NT * KC + q) * P::LANES];
+                product(k, b);
+            }
+            wave_sync();
+            // 4 lanes a row, each every fourth element
+#pragma unroll 1
+            for (int r = 0; r < R; ++r) {
+                const int64_t row = u.order[min(first + 16 * r + m, end - 1)];
+                const E* from = reinterpret_cast<const E*>(u.y) + row * u.ys;
+                E* to = reinterpret_cast<E*>(u.out) + row * u.os;
+                const int c0 = k * CB - (int)((uintptr_t)to / sizeof(E) % CB);
+                const int stop = first + 16 * r + m < end ? min(u.n, c0 + CB) : 0;
+#pragma unroll 8
+                for (int c = c0 + g; c < stop; c += 4) {
+                    if (c < 0) continue;
+                    E o = u.y ? from[c] : E(0);
+                    if (active) o = narrow<DT>(widen<DT>(o) + os[16 * r + m][c & (RING - 1)]);
+                    to[c] = o;
+                }
+            }
+            wave_sync();
+            ++k;
+            continue;
+        }
+        for (; k < inner1; k += AHEAD) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < AHEAD; ++j) {
+                const int kk = k + j;
+                if (kk >= inner1) break;
+                if (active && kk < blocks) product(kk, bf[j]);
+                wave_sync();
+                F o[2 * R];
 #pragma unroll
-                for (int c = 0; c < KC; ++c)
+                for (int i = 0; i < 2 * R; ++i) o[i] = y[j][i];  // rows without an adapter keep y's bits
+                if (kk + AHEAD < inner1) ask(kk + AHEAD, y[j], bf[j]);
 #pragma unroll
-                    for (int p = 0; p < (P::HALF ? 1 : PIECES); ++p) {
-                        const F hf = *reinterpret_cast<const F*>(&hs[P::HALF ? g >> 1 : p][16 * r + m][P::rank_of(c, g)]);
+                for (int i = 0; i < 2 * R; ++i) {
+                    const int c = kk * CB + begin[i];
+                    if (active) {
+                        const float* from = &os[8 * i + r0][c & (RING - 1)];
+                        float d[W];
+                        if (vectors) {
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[t] = M::mul(bf[c][t], hf, acc[t]);
+                            for (int e = 0; e < W; e += 4)
+                                *reinterpret_cast<f32x4*>(&d[e]) = *reinterpret_cast<const f32x4*>(from + e);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < W; ++e) d[e] = from[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < W; ++e) o[i][e] = narrow<DT>(widen<DT>(o[i][e]) + d[e]);
                     }
-                const float f = factor[16 * r + m];
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    *reinterpret_cast<f32x4*>(&os[m][16 * PER * (t / PER) + W * g + 4 * (t % PER)]) = acc[t] * f;
+                    if (first + 8 * i + r0 < end && c >= 0 && c + W <= u.n) __builtin_memcpy(orow[i] + c, &o[i], sizeof(F));
+                }
                 wave_sync();
             }
-#pragma unroll
-            for (int i = 0; i < LI; ++i) {
-                const int at = LR * i + lane / LC;
-                F o = y[LI * r + i];  // rows without an adapter keep y's bits
-                ask(LI * r + i, n0 + CB * kWaves);
-                if (active) {
-                    float d[W];
-#pragma unroll
-                    for (int e = 0; e < W; e += 4)
-                        *reinterpret_cast<f32x4*>(&d[e]) = *reinterpret_cast<const f32x4*>(&os[at][lc + e]);
-#pragma unroll
-                    for (int e = 0; e < W; ++e) o[e] = narrow<DT>(widen<DT>(o[e]) + d[e]);
-                }
-                if (first + 16 * r + at >= end) continue;
-                E* to = reinterpret_cast<E*>(u.out) + (int64_t)row[LI * r + i] * u.os + n0 + lc;
-                if (n0 + CB <= u.n || n0 + lc + W <= u.n) {
-                    __builtin_memcpy(to, &o, sizeof o);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < W; ++e)
-                        if (n0 + lc + e < u.n) to[e] = o[e];
-                }
-            }
         }
-        wave_sync();
+        k = inner1;
     }
 }
 
@@ -780,15 +880,19 @@ extern "C" int nori_low_rank_update(const void* x, int dtype, int64_t rows, int3
                                    0, stream, u, transposed);
             }
             const int64_t tiles = rows / (few ? 16 : 64) + groups;
+            if (!few) {
+                constexpr int R = RP <= 32 ? 1 : 2;
+                hipLaunchKernelGGL((update_kernel<DT, RP, R>), dim3((unsigned)(rows / (64 * R) + groups)), dim3(kThreads), 0, stream, u);
+                return 0;
+            }
             // out's columns are shared among workgroups, each with an h of its own, while there are few tiles
-            const int wide = (few ? 32 : 64) * kWaves, most = (n + wide - 1) / wide;
+            const int wide = 32 * kWaves, most = (n + wide - 1) / wide;
             const int split = (int)std::min<int64_t>(most, std::max<int64_t>(1, 2 * cus / tiles));
             const int steps = (most + split - 1) / split;
             u.columns = steps * wide;
             // tiles in multiples of 8: a tile's workgroups stay on one XCD, whose L2 holds its x
             const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)((most + steps - 1) / steps));
-            if (few) hipLaunchKernelGGL((update_few_kernel<DT, RP>), grid, dim3(kThreads), 0, stream, u);
-            else hipLaunchKernelGGL((update_kernel<DT, RP>), grid, dim3(kThreads), 0, stream, u);
+            hipLaunchKernelGGL((update_few_kernel<DT, RP>), grid, dim3(kThreads), 0, stream, u);
             return 0;
         });
     });

@@ -122,6 +122,52 @@ def test_against_the_formulas(ids, counts, k, n, rank, adapters, dtype):
     assert torch.equal(d["y"], fresh)
 
 
+# enough rows, or adapters, that workgroups take tiles of many rows: ends of rows, ranks and groups of every kind
+MANY = [
+    ([0, -1, 1], [20000, 500, 14007], 130, 77, 5, 2),
+    ([1, 0], [33333, 1], 64, 128, 16, 2),
+    ([0], [33000], 3, 999, 16, 1),
+    ([0, 1], [16501, 16503], 97, 65, 32, 2),
+    ([0, 1, -1], [30000, 3001, 90], 560, 72, 24, 2),
+    ([0, 1], [16400, 16700], 136, 200, 64, 2),
+    ([1, 0], [32900, 200], 71, 130, 50, 2),
+    ([0, 1], [20000, 13000], 128, 63, 128, 2),
+    ([0, 1], [20000, 13011], 33, 321, 77, 2),
+    ([-1 if i % 99 == 0 else (7 * i) % 540 for i in range(540)], [(i * 13) % 50 for i in range(540)], 56, 100, 9, 540),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("ids,counts,k,n,rank,adapters", MANY)
+def test_many_rows_against_the_formulas(ids, counts, k, n, rank, adapters, dtype):
+    test_against_the_formulas(ids, counts, k, n, rank, adapters, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_many_rows_in_a_shared_buffer(dtype):
+    # x, y and out as columns of one buffer's rows, at no vector's alignment: nothing beside them moves
+    ids, counts = [1, -1, 0], [17000, 40, 16001]
+    whose = _rows(ids, counts)
+    s = _make(len(whose), 72, 85, 16, 2, dtype)
+    plan = AdapterPlan(ids, counts, device=DEV)
+    d = {n: t.to(DEV) for n, t in s.items()}
+    buffer = torch.full((len(whose), 165), float("nan"), dtype=dtype, device=DEV)
+    x, y = buffer[:, 3:75], buffer[:, 77:162]
+    x.copy_(d["x"])
+    y.copy_(d["y"])
+    _check({"y": low_rank_update(x, y, d["a"], d["b"], plan, d["scales"]).contiguous()}, s, whose, names=("y",))
+    before = buffer.clone()
+    low_rank_update(x, y, d["a"], d["b"], plan, d["scales"], out=y)
+    _check({"y": y.contiguous()}, s, whose, names=("y",))
+    mask = torch.ones(165, dtype=torch.bool, device=DEV)
+    mask[77:162] = False
+    assert torch.equal(buffer[:, mask].view(torch.uint8), before[:, mask].view(torch.uint8))
+    # non-finite rows stay in their rows
+    d["x"][5, 3], d["x"][20000, 71] = float("inf"), float("nan")
+    got = low_rank_update(d["x"], d["y"], d["a"], d["b"], plan, d["scales"])
+    assert torch.nonzero(~torch.isfinite(got).all(1)).flatten().tolist() == [5, 20000]
+
+
 def test_without_scales_and_one_gradient_at_a_time():
     ids, counts = [1, 0, -1], [30, 80, 9]
     s = _make(119, 96, 104, 8, 3, F16)  # adapter 2 has no rows: its gradients are zeros
