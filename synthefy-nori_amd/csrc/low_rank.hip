@@ -278,13 +278,13 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
         any |= begin[i];
     }
     const int blocks = (u.n + CB - 1) / CB;
-    const int windows = blocks + (__ballot(shift > blocks * CB - u.n) ? 1 : 0);
+    const int windows = u.out ? blocks + (__ballot(shift > blocks * CB - u.n) ? 1 : 0) : 0;  // null: h alone is asked for
     const bool vectors = !__ballot((any & 3) != 0);  // of the result in LDS
     // Where rows begin and end with whole vectors every window is taken in vectors, some of them past the row's ends;
     // else the first and the last are taken an element at a time.
     const bool whole = u.n % W == 0 && !__ballot(any % W != 0);
     const int inner0 = whole || !__ballot(shift != 0) ? 0 : 1;
-    const int inner1 = whole ? windows : max(inner0, u.n / CB);
+    const int inner1 = whole || !windows ? windows : max(inner0, u.n / CB);
     const F* pb = reinterpret_cast<const F*>(u.pb) + group * P::second(u.n) + lane % P::LANES;
     F y[AHEAD][2 * R], bf[AHEAD][KC * NT];
     // Loads come back in the order they were asked for: a window's operands are asked for beside its y, or waiting for
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kThreads) update_few_kernel(const Update u) {
     const bool active = id >= 0 && id < u.adapters;
     if (!active && u.y == u.out) return;  // the rows stay as they are
 
-    const int stop = min(u.n, ((int)blockIdx.y + 1) * u.columns);
+    const int stop = u.out ? min(u.n, ((int)blockIdx.y + 1) * u.columns) : 0;  // null: h alone is asked for
     const int64_t row = u.order[min(first + m, end - 1)];
     F y[NV];
     auto ask = [&](int n0) {
@@ -626,45 +626,55 @@ __global__ void __launch_bounds__(kThreads) update_few_kernel(const Update u) {
     }
 }
 
-struct Grad {
+// One of the two sums t^T h over each group's rows.
+struct Task {
     const void* t;   // [rows][cols]
     const float* h;  // [rows][rank]
     int64_t ts;
-    int cols, rank, adapters;
+    int cols;
+    int chunks;  // of its columns, a workgroup's each
+    void* out;   // [adapters][...]
+    int64_t o_col, o_rank;
+    float* partial;  // [parts of the groups with more than one][cols][rank]
+};
+
+struct Grads {
+    Task task[2];
+    int rank, adapters;
     const int32_t *order, *starts, *ids;
     int groups;
-    void* out;  // [adapters][cols][rank], transposed: [adapters][rank][cols]
-    int64_t o_col, o_rank;
-    int part;        // rows of one; a multiple of 128
-    float* partial;  // [parts of the groups with more than one][cols][rank]
+    int part;  // rows of one; a multiple of 128
 };
 
 // Where the partial sums of a group with several parts begin: 2 starts / part is enough for the ones before it,
 // since a length above `part` has at most twice length / part, less one, rounded up.
-__device__ __forceinline__ int64_t partial_of(const Grad& q, int group) { return 2 * (int64_t)q.starts[group] / q.part; }
+__device__ __forceinline__ int64_t partial_of(const Grads& q, int group) { return 2 * (int64_t)q.starts[group] / q.part; }
 
-__device__ __forceinline__ void store_grad(const Grad& q, int dt, int id, int c, int j, float v) {
-    const int64_t i = (int64_t)id * q.cols * q.rank + c * q.o_col + j * q.o_rank;
-    if (dt == NORI_F32) reinterpret_cast<float*>(q.out)[i] = v;
-    else reinterpret_cast<uint16_t*>(q.out)[i] = dt == NORI_F16 ? f32_to_f16(v) : f32_to_bf16(v);
+__device__ __forceinline__ void store_grad(const Task& k, int rank, int dt, int id, int c, int j, float v) {
+    const int64_t i = (int64_t)id * k.cols * rank + c * k.o_col + j * k.o_rank;
+    if (dt == NORI_F32) reinterpret_cast<float*>(k.out)[i] = v;
+    else reinterpret_cast<uint16_t*>(k.out)[i] = dt == NORI_F16 ? f32_to_f16(v) : f32_to_bf16(v);
 }
 
 // t^T h over one part of a group's rows: 128 (fp32: 64) columns by up to 64 ranks a workgroup, whose wavefronts
-// take every fourth step of rows and add their sums in LDS, in order.
+// take every fourth step of rows and add their sums in LDS, in order. HBM-bound: t is read once, h (4 rank bytes a
+// row) once a chunk of columns, from the L2; the next step's rows are on their way while one is summed.
 // The sum runs over rows, which t has apart. 16-bit: a lane reads 16 bytes of each of 8 rows and turns the 8 x 8
-// block in registers, so that it holds 8 rows of one column for each of 8 instructions; column t of a lane's
-// block belongs to instruction t. fp32: an instruction takes 4 rows, no turning. h, in fp32, enters in two pieces
+// block in registers, so that it holds 8 rows of one column for each of 8 instructions; column i of a lane's
+// block belongs to instruction i. fp32: an instruction takes 4 rows, no turning. h, in fp32, enters in two pieces
 // of the 16-bit type as in the update; a power of two per wavefront that follows the largest element so far keeps
 // fp16's pieces in range (sums so far are brought to a new one).
-template <int DT, int RT>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const Grad q) {
+// Where a row ends inside a lane's columns, the lane takes the last ones instead and writes them again, the same
+// values. SHORT: rows of fewer columns than a lane takes.
+template <int DT, int RT, bool SHORT>
+__global__ void __launch_bounds__(kThreads) grad_kernel(const Grads q) {
     using M = Mma<DT>;
     using E = typename M::elem;
     using F = typename M::frag;
     constexpr bool F32 = DT == NORI_F32;
-    constexpr int W = M::W, CT = W;            // a lane's columns, an instruction each
-    constexpr int STEP = F32 ? 4 : 32;         // rows of a step
-    constexpr int U = F32 ? 4 : 1;             // steps whose loads go together
+    constexpr int W = M::W, CT = W;    // a lane's columns, an instruction each
+    constexpr int EACH = 8;            // rows a lane holds of a step
+    constexpr int STEP = 32;           // rows of a step
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     int number;
     const int group = group_of_tile(q.starts, q.groups, q.part, blockIdx.x, number);
@@ -673,9 +683,36 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Grad q) {
     const int id = q.ids[group];
     if (first64 >= last || id < 0 || id >= q.adapters) return;
     const int first = (int)first64, end = min(last, first + q.part);
-    const int c0 = blockIdx.y * 16 * W + W * m, j0 = blockIdx.z * 16 * RT;
-    const E* t = reinterpret_cast<const E*>(q.t) + c0;
-    const int there = q.cols - c0;
+    const bool second = (int)blockIdx.y >= q.task[0].chunks;
+    const Task& k = q.task[second];
+    const int chunk = blockIdx.y - (second ? q.task[0].chunks : 0), j0 = blockIdx.z * 16 * RT;
+    auto column = [&](int of) { return SHORT ? 0 : min(chunk * 16 * W + W * of, k.cols - W); };
+    const E* t = reinterpret_cast<const E*>(k.t) + column(m);
+    int rank_at[RT];  // ranks past the last sum what is never written
+#pragma unroll
+    for (int r = 0; r < RT; ++r) rank_at[r] = min(j0 + 16 * r + m, q.rank - 1);
+
+    // fp32: instruction i takes rows 4 i ... 4 i + 3 of a step, so a lane's are 4 apart
+    auto place = [&](int p0, int i) { return p0 + (F32 ? 4 * i + g : EACH * g + i); };
+    F raw[EACH];
+    float h[EACH][RT];
+    int row[EACH];
+    auto ask_rows = [&](int p0) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) row[i] = q.order[min(place(p0, i), end - 1)];
+    };
+    auto ask = [&](int p0) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            raw[i] = F{};
+            if (place(p0, i) < end) {
+                if constexpr (SHORT) raw[i] = fetch<DT>(t + row[i] * k.ts, k.cols);
+                else raw[i] = fetch<DT>(t + row[i] * k.ts);
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) h[i][r] = k.h[(int64_t)row[i] * q.rank + rank_at[r]];
+        }
+    };
 
     f32x4 acc[RT][CT];
 #pragma unroll
@@ -684,52 +721,54 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Grad q) {
         for (int i = 0; i < CT; ++i) acc[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float up = 1.0f, down = 1.0f;
     float reach = 0.f;  // elements below it fit the present power of two
-    constexpr int EACH = F32 ? 1 : 8;  // rows a lane holds of a step
-    for (int p0 = first + wave * STEP * U; p0 < end; p0 += STEP * U * kWaves) {
-        F raw[U][EACH];
-        float h[U][EACH][RT];
+    const int p1 = first + wave * STEP;
+    if (p1 < end) {
+        ask_rows(p1);
+        ask(p1);
+        if (p1 + STEP * kWaves < end) ask_rows(p1 + STEP * kWaves);
+    }
+    for (int p0 = p1; p0 < end; p0 += STEP * kWaves) {
+        F now[EACH];
+        float hn[EACH][RT];
 #pragma unroll
-        for (int s = 0; s < U; ++s)
+        for (int i = 0; i < EACH; ++i) {
+            now[i] = raw[i];
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                const int p = p0 + STEP * s + EACH * g + i;
-                const int64_t row = q.order[min(p, end - 1)];
-                raw[s][i] = F{};
-                if (p < end) raw[s][i] = fetch<DT>(t + row * q.ts, there);
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const int j = j0 + 16 * r + m;
-                    h[s][i][r] = p < end && j < q.rank ? q.h[row * q.rank + j] : 0.f;
-                }
-            }
+            for (int r = 0; r < RT; ++r) hn[i][r] = place(p0, i) < end ? h[i][r] : 0.f;
+        }
+        const int p2 = p0 + STEP * kWaves;
+        if (p2 < end) ask(p2);
+        if (p2 + STEP * kWaves < end) ask_rows(p2 + STEP * kWaves);
         if constexpr (F32) {
 #pragma unroll
-            for (int s = 0; s < U; ++s)
+            for (int s = 0; s < EACH; ++s)
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
                     for (int i = 0; i < CT; ++i)
-                        acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(raw[s][0][i], h[s][0][r], acc[r][i], 0, 0, 0);
+                        acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(now[s][i], hn[s][r], acc[r][i], 0, 0, 0);
         } else {
             if constexpr (DT == NORI_F16) {
                 float largest = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < EACH; ++i)
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
-                        const float v = fabsf(h[0][i][r]);
+                        const float v = fabsf(hn[i][r]);
                         largest = v < __builtin_inff() ? fmaxf(largest, v) : largest;
                     }
+                if (__ballot(largest > reach)) {
 #pragma unroll
-                for (int off = 32; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
-                if (largest > reach) {  // the same in every lane
+                    for (int off = 32; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
                     const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 8, -110), 110);
                     const float to = __uint_as_float((uint32_t)(127 - e) << 23);
-                    const float change = reach > 0.f ? to * up : 0.f;  // no sums yet: they are zero
+                    if (reach > 0.f) {
+                        const float change = to * up;
 #pragma unroll
-                    for (int r = 0; r < RT; ++r)
+                        for (int r = 0; r < RT; ++r)
 #pragma unroll
-                        for (int i = 0; i < CT; ++i) acc[r][i] = reach > 0.f ? acc[r][i] * change : acc[r][i];
+                            for (int i = 0; i < CT; ++i) acc[r][i] = acc[r][i] * change;
+                    }
                     up = __uint_as_float((uint32_t)(127 + e) << 23);
                     down = to;
                     reach = up * 512.0f;  // scaled: below 2^9, the pieces of the smallest that counts above 2^-24
@@ -740,7 +779,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Grad q) {
             for (int r = 0; r < RT; ++r)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float v = h[0][i][r] * down;
+                    const float v = hn[i][r] * down;
                     high[r][i] = narrow<DT>(v);
                     low[r][i] = fabsf(v) < __builtin_inff() ? narrow<DT>(v - widen<DT>(high[r][i])) : E(0);
                 }
@@ -748,7 +787,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Grad q) {
             for (int i = 0; i < CT; ++i) {
                 F col;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) col[e] = raw[0][e][i];
+                for (int e = 0; e < 8; ++e) col[e] = now[e][i];
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     acc[r][i] = M::mul(col, high[r], acc[r][i]);
@@ -757,10 +796,10 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Grad q) {
             }
         }
     }
-    // the wavefronts' sums, a rank tile at a time. acc[r][i][j] of lane (m, g): column W (4 g + j) + i, rank 16 r + m
+    // the wavefronts' sums, a rank tile at a time. acc[r][i][j] of lane (m, g): column i of operand row 4 g + j, rank 16 r + m
     __shared__ f32x4 sums[kWaves][CT][64];
     const bool whole = last - begin <= q.part;
-    float* part = whole ? nullptr : q.partial + (partial_of(q, group) + number) * q.cols * q.rank;
+    float* part = whole ? nullptr : k.partial + (partial_of(q, group) + number) * k.cols * q.rank;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         __syncthreads();
@@ -772,37 +811,43 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Grad q) {
             const int j = j0 + 16 * r + m;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int c = blockIdx.y * 16 * W + W * (4 * g + e) + i;
-                if (c >= q.cols || j >= q.rank) continue;
-                if (whole) store_grad(q, DT, id, c, j, v[e]);
+                const int c = column(4 * g + e) + i;
+                if (j >= q.rank || (SHORT && (c >= k.cols || 4 * g + e > 0))) continue;
+                if (whole) store_grad(k, q.rank, DT, id, c, j, v[e]);
                 else part[(int64_t)c * q.rank + j] = v[e];
             }
         }
     }
 }
 
-// the parts of the groups that have several, in their order
-__global__ void __launch_bounds__(kThreads) grad_join_kernel(const Grad q, int dt) {
+// the parts of the groups that have several, in their order; blocks0: workgroups of the first task
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(const Grads q, int dt, int blocks0) {
+    const bool second = (int)blockIdx.x >= blocks0;
+    const Task& k = q.task[second];
     const int group = blockIdx.y, id = q.ids[group];
     const int length = q.starts[group + 1] - q.starts[group];
-    const int64_t size = (int64_t)q.cols * q.rank, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t size = (int64_t)k.cols * q.rank;
+    const int64_t i = (int64_t)(blockIdx.x - (second ? blocks0 : 0)) * kThreads + threadIdx.x;
     if (length <= q.part || id < 0 || id >= q.adapters || i >= size) return;
-    const float* part = q.partial + partial_of(q, group) * size + i;
+    const float* part = k.partial + partial_of(q, group) * size + i;
     const int parts = (length + q.part - 1) / q.part;
     float v = 0.f;
 #pragma unroll 8
     for (int p = 0; p < parts; ++p) v += part[p * size];
-    store_grad(q, dt, id, (int)(i / q.rank), (int)(i % q.rank), v);
+    store_grad(k, q.rank, dt, id, (int)(i / q.rank), (int)(i % q.rank), v);
 }
+
+int chunks_of(int cols, int dtype) { return (cols + (dtype == NORI_F32 ? 63 : 127)) / (dtype == NORI_F32 ? 64 : 128); }
 
 // Rows of a part: about four workgroups a compute unit, and no part so short that its sums cost as much as its rows
 // (8 rank bytes a column, twice, against 2 to 4 a row).
-int part_of(int64_t rows, int cols, int rank, int dtype) {
-    const int wide = dtype == NORI_F32 ? 64 : 128;
-    const int64_t chunks = (int64_t)((cols + wide - 1) / wide) * ((rank + 63) / 64);
-    const int64_t want = rows * chunks / (4 * (int64_t)device_cus());
+int part_of(int64_t rows, int chunks, int rank) {
+    const int64_t want = rows * chunks * ((rank + 63) / 64) / (4 * (int64_t)device_cus());
     return (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 256), 8192);
 }
+
+// partial sums of one task, in bytes
+int64_t partial_bytes(int64_t rows, int part, int cols, int rank) { return (2 * rows / part + 1) * cols * rank * 4; }
 
 bool is_float(int dt) { return dt == NORI_F32 || dt == NORI_F16 || dt == NORI_BF16; }
 
@@ -830,9 +875,8 @@ static int by_rank(int32_t rank, Go go) {
     return go(std::integral_constant<int, 128>{});
 }
 
-extern "C" int64_t nori_low_rank_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups,
-                                                 int32_t transposed) {
-    if (!is_float(dtype) || rows <= 0 || k <= 0 || n <= 0 || rank <= 0 || groups <= 0) return 0;
+// of the packed factors; 0 where they are read as they lie
+static int64_t packed_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups, bool transposed) {
     if (!transposed && few_rows(rows, groups)) return 0;
     int64_t bytes = 0;
     NORI_DISPATCH_FLOAT(dtype, DT, {
@@ -845,48 +889,30 @@ extern "C" int64_t nori_low_rank_workspace_bytes(int dtype, int64_t rows, int32_
     return bytes;
 }
 
-extern "C" int nori_low_rank_update(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* y,
-                                    int64_t y_row_stride, const void* a, const void* b, int32_t transposed,
-                                    const float* scales, int32_t adapters, int32_t rank, int32_t n, const int32_t* order,
-                                    const int32_t* starts, const int32_t* ids, int32_t groups, void* out,
-                                    int64_t out_row_stride, float* h, void* workspace, int64_t workspace_bytes,
-                                    void* stream_v) {
-    clear_error();
-    if (int rc = check("low_rank_update", dtype, rows, groups, k, n, rank, adapters)) return rc;
-    if (rows == 0) return NORI_OK;
-    if (!x || !a || !b || !order || !starts || !ids || !out || groups <= 0)
-        return fail(NORI_ERR_INVALID, "low_rank_update: null pointer");
-    if (out_row_stride < n && rows > 1) return fail(NORI_ERR_INVALID, "low_rank_update: rows of out overlap");
-    if (out == y && out_row_stride != y_row_stride && rows > 1)
-        return fail(NORI_ERR_INVALID, "low_rank_update: out is y, at another row stride");
-    const int64_t need = nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, groups, transposed);
-    if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
-        return fail(NORI_ERR_INVALID, "low_rank_update: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                    (long long)need);
-    Update u{x,  y, a,   b,      x_row_stride, y_row_stride, out_row_stride, k, n, rank, adapters, scales, order, starts, ids, groups,
-             0, out, h, nullptr, nullptr};
-    hipStream_t stream = (hipStream_t)stream_v;
-    const int cus = device_cus();
+// h and, where u.out is not null, out; the packed factors in `packed`, 16-byte aligned, or null
+static void launch_update(Update u, int dtype, int64_t rows, bool transposed, void* packed, hipStream_t stream) {
+    const int cus = device_cus(), groups = u.groups;
     const bool few = few_rows(rows, groups);
     NORI_DISPATCH_FLOAT(dtype, DT, {
-        by_rank(rank, [&](auto RP_) {
+        by_rank(u.rank, [&](auto RP_) {
             constexpr int RP = decltype(RP_)::value;
             using P = Packed<DT, RP>;
-            if (need) {
-                u.pa = workspace;
-                u.pb = reinterpret_cast<char*>(workspace) + groups * P::first(k) * 16;
-                const int64_t each = P::first(k) + P::second(n);
+            if (packed) {
+                u.pa = packed;
+                u.pb = reinterpret_cast<char*>(packed) + groups * P::first(u.k) * 16;
+                const int64_t each = P::first(u.k) + P::second(u.n);
                 hipLaunchKernelGGL((pack_kernel<DT, RP>), dim3((unsigned)((each + kThreads - 1) / kThreads), groups), dim3(kThreads),
-                                   0, stream, u, transposed);
+                                   0, stream, u, transposed ? 1 : 0);
             }
-            const int64_t tiles = rows / (few ? 16 : 64) + groups;
             if (!few) {
                 constexpr int R = RP <= 32 ? 1 : 2;
-                hipLaunchKernelGGL((update_kernel<DT, RP, R>), dim3((unsigned)(rows / (64 * R) + groups)), dim3(kThreads), 0, stream, u);
+                hipLaunchKernelGGL((update_kernel<DT, RP, R>), dim3((unsigned)(rows / (64 * R) + groups)), dim3(kThreads), 0, stream,
+                                   u);
                 return 0;
             }
             // out's columns are shared among workgroups, each with an h of its own, while there are few tiles
-            const int wide = 32 * kWaves, most = (n + wide - 1) / wide;
+            const int64_t tiles = rows / 16 + groups;
+            const int wide = 32 * kWaves, most = u.out ? (u.n + wide - 1) / wide : 1;
             const int split = (int)std::min<int64_t>(most, std::max<int64_t>(1, 2 * cus / tiles));
             const int steps = (most + split - 1) / split;
             u.columns = steps * wide;
@@ -896,53 +922,143 @@ extern "C" int nori_low_rank_update(const void* x, int dtype, int64_t rows, int3
             return 0;
         });
     });
+}
+
+extern "C" int64_t nori_low_rank_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups) {
+    if (!is_float(dtype) || rows <= 0 || k <= 0 || n <= 0 || rank <= 0 || groups <= 0) return 0;
+    return packed_bytes(dtype, rows, k, n, rank, groups, false);
+}
+
+extern "C" int nori_low_rank_update(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* y,
+                                    int64_t y_row_stride, const void* a, const void* b, const float* scales, int32_t adapters,
+                                    int32_t rank, int32_t n, const int32_t* order, const int32_t* starts, const int32_t* ids,
+                                    int32_t groups, void* out, int64_t out_row_stride, float* h, void* workspace,
+                                    int64_t workspace_bytes, void* stream_v) {
+    clear_error();
+    if (int rc = check("low_rank_update", dtype, rows, groups, k, n, rank, adapters)) return rc;
+    if (rows == 0) return NORI_OK;
+    if (!x || !a || !b || !order || !starts || !ids || !out || groups <= 0)
+        return fail(NORI_ERR_INVALID, "low_rank_update: null pointer");
+    if (out_row_stride < n && rows > 1) return fail(NORI_ERR_INVALID, "low_rank_update: rows of out overlap");
+    if (out == y && out_row_stride != y_row_stride && rows > 1)
+        return fail(NORI_ERR_INVALID, "low_rank_update: out is y, at another row stride");
+    const int64_t need = nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, groups);
+    if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
+        return fail(NORI_ERR_INVALID, "low_rank_update: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                    (long long)need);
+    const Update u{x,  y, a,   b,      x_row_stride, y_row_stride, out_row_stride, k, n, rank, adapters, scales, order, starts, ids,
+                   groups, 0, out, h, nullptr, nullptr};
+    launch_update(u, dtype, rows, false, need ? workspace : nullptr, (hipStream_t)stream_v);
     return launch_status("low_rank_update");
 }
 
-extern "C" int64_t nori_low_rank_weight_grad_workspace_bytes(int dtype, int64_t rows, int32_t cols, int32_t rank,
-                                                             int64_t longest) {
-    if (rows <= 0 || cols <= 0 || rank <= 0) return 0;
-    const int part = part_of(rows, cols, rank, dtype);
-    return longest <= part ? 0 : (2 * rows / part + 1) * cols * rank * 4;
+namespace {
+// the backward pass's workspace: g [rows][rank], the packed factors, the partial sums of da and of db
+struct Layout {
+    int64_t packed, da, db, end;
+    int part;
+};
+
+Layout layout_of(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups, int64_t longest, bool need_x,
+                 bool need_a, bool need_b) {
+    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    Layout l;
+    l.part = part_of(rows, (need_a ? chunks_of(k, dtype) : 0) + (need_b ? chunks_of(n, dtype) : 0), rank);
+    const bool parts = longest > l.part;
+    l.packed = up(need_x || need_a ? rows * rank * 4 : 0);
+    l.da = l.packed + up(need_x || need_a ? packed_bytes(dtype, rows, n, k, rank, groups, true) : 0);
+    l.db = l.da + up(need_a && parts ? partial_bytes(rows, l.part, k, rank) : 0);
+    l.end = l.db + up(need_b && parts ? partial_bytes(rows, l.part, n, rank) : 0);
+    return l;
+}
+}  // namespace
+
+extern "C" int64_t nori_low_rank_backward_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank,
+                                                          int32_t groups, int64_t longest, int32_t need_x, int32_t need_a,
+                                                          int32_t need_b) {
+    if (!is_float(dtype) || rows <= 0 || k <= 0 || n <= 0 || rank <= 0 || groups <= 0) return 0;
+    return layout_of(dtype, rows, k, n, rank, groups, longest, need_x, need_a, need_b).end;
 }
 
-extern "C" int nori_low_rank_weight_grad(const void* t, int dtype, int64_t rows, int32_t cols, int64_t t_row_stride,
-                                         const float* h, int32_t rank, int32_t adapters, const int32_t* order,
-                                         const int32_t* starts, const int32_t* ids, int32_t groups, int64_t longest,
-                                         int32_t transposed, void* out, void* workspace, int64_t workspace_bytes,
-                                         void* stream_v) {
+extern "C" int nori_low_rank_backward(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* dy,
+                                      int32_t n, int64_t dy_row_stride, const void* base, int64_t base_row_stride, const void* a,
+                                      const void* b, const float* scales, int32_t adapters, int32_t rank, const int32_t* order,
+                                      const int32_t* starts, const int32_t* ids, int32_t groups, int64_t longest, const float* h,
+                                      void* dx, int64_t dx_row_stride, void* da, void* db, void* workspace,
+                                      int64_t workspace_bytes, void* stream_v) {
     clear_error();
-    if (int rc = check("low_rank_weight_grad", dtype, rows, groups, cols, 1, rank, adapters)) return rc;
-    if (rows == 0) return NORI_OK;
-    if (!t || !h || !order || !starts || !ids || !out || groups <= 0)
-        return fail(NORI_ERR_INVALID, "low_rank_weight_grad: null pointer");
-    if (longest < 1 || longest > rows)
-        return fail(NORI_ERR_INVALID, "low_rank_weight_grad: a longest group of %lld rows of %lld", (long long)longest, (long long)rows);
-    const int64_t need = nori_low_rank_weight_grad_workspace_bytes(dtype, rows, cols, rank, longest);
-    if (need && (!workspace || (uintptr_t)workspace % 4 || workspace_bytes < need))
-        return fail(NORI_ERR_INVALID, "low_rank_weight_grad: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                    (long long)need);
-    Grad q{t, h, t_row_stride, cols, rank, adapters, order, starts, ids, groups, out, rank, 1, part_of(rows, cols, rank, dtype),
-           reinterpret_cast<float*>(workspace)};
-    if (transposed) q.o_col = 1, q.o_rank = cols;
+    if (int rc = check("low_rank_backward", dtype, rows, groups, k, n, rank, adapters)) return rc;
+    if (rows == 0 || (!dx && !da && !db)) return NORI_OK;
+    if (!x || !dy || !a || !b || !order || !starts || !ids || !h || groups <= 0)
+        return fail(NORI_ERR_INVALID, "low_rank_backward: null pointer");
+    if (dx && dx_row_stride < k && rows > 1) return fail(NORI_ERR_INVALID, "low_rank_backward: rows of dx overlap");
+    if (dx && dx == base && dx_row_stride != base_row_stride && rows > 1)
+        return fail(NORI_ERR_INVALID, "low_rank_backward: dx is its base, at another row stride");
+    if (longest < 0 || longest > rows)
+        return fail(NORI_ERR_INVALID, "low_rank_backward: a longest group of %lld rows of %lld", (long long)longest, (long long)rows);
+    const Layout l = layout_of(dtype, rows, k, n, rank, groups, longest, dx, da, db);
+    if (l.end && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < l.end))
+        return fail(NORI_ERR_INVALID, "low_rank_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                    (long long)l.end);
+    char* at = reinterpret_cast<char*>(workspace);
+    float* kept = reinterpret_cast<float*>(at);
     hipStream_t stream = (hipStream_t)stream_v;
-    const int64_t parts = rows / q.part + groups;
-    auto go = [&](auto DT_, auto RT_) {
-        constexpr int DT = decltype(DT_)::value, RT = decltype(RT_)::value, WIDE = 16 * Mma<DT>::W;
-        hipLaunchKernelGGL((grad_kernel<DT, RT>),
-                           dim3((unsigned)parts, (unsigned)((cols + WIDE - 1) / WIDE), (unsigned)((rank + 16 * RT - 1) / (16 * RT))),
-                           dim3(kThreads), 0, stream, q);
-    };
-    NORI_DISPATCH_FLOAT(dtype, DT, {
-        constexpr std::integral_constant<int, DT> DT_{};
-        if (rank <= 16) go(DT_, std::integral_constant<int, 1>{});
-        else if (rank <= 32) go(DT_, std::integral_constant<int, 2>{});
-        else go(DT_, std::integral_constant<int, 4>{});
-    });
-    if (need) {
-        const int64_t size = (int64_t)cols * rank;
-        hipLaunchKernelGGL(grad_join_kernel, dim3((unsigned)((size + kThreads - 1) / kThreads), groups), dim3(kThreads), 0, stream,
-                           q, dtype);
+    if (dx || da) {
+        // dx = base + (s dy B) A: the update with the factors' roles swapped, g kept for da
+        const Update u{dy, dx ? base : nullptr, b, a, dy_row_stride, base_row_stride, dx_row_stride, n, k, rank, adapters, scales, order,
+                       starts, ids, groups, 0, dx, da ? kept : nullptr, nullptr, nullptr};
+        launch_update(u, dtype, rows, true, at + l.packed, stream);
     }
-    return launch_status("low_rank_weight_grad");
+    if (!da && !db) return launch_status("low_rank_backward");
+    Grads q{};
+    q.rank = rank;
+    q.adapters = adapters;
+    q.order = order;
+    q.starts = starts;
+    q.ids = ids;
+    q.groups = groups;
+    q.part = l.part;
+    int tasks = 0;
+    if (da)  // da [adapters][rank][k]
+        q.task[tasks++] = Task{x, kept, x_row_stride, k, chunks_of(k, dtype), da, 1, k, reinterpret_cast<float*>(at + l.da)};
+    if (db)  // db [adapters][n][rank]
+        q.task[tasks++] = Task{dy, h, dy_row_stride, n, chunks_of(n, dtype), db, rank, 1, reinterpret_cast<float*>(at + l.db)};
+    const int64_t parts = rows / q.part + groups;
+    // the tasks whose rows are whole vectors together, the others by themselves
+    auto go = [&](const Grads& some, bool narrow_rows) {
+        const unsigned chunks = (unsigned)(some.task[0].chunks + some.task[1].chunks);
+        NORI_DISPATCH_FLOAT(dtype, DT, {
+            auto launch = [&](auto RT_, auto SHORT_) {
+                constexpr int RT = decltype(RT_)::value;
+                hipLaunchKernelGGL((grad_kernel<DT, RT, decltype(SHORT_)::value>),
+                                   dim3((unsigned)parts, chunks, (unsigned)((rank + 16 * RT - 1) / (16 * RT))), dim3(kThreads), 0,
+                                   stream, some);
+            };
+            if (narrow_rows) launch(std::integral_constant<int, 1>{}, std::true_type{});
+            else if (rank <= 16) launch(std::integral_constant<int, 1>{}, std::false_type{});
+            else if (rank <= 32) launch(std::integral_constant<int, 2>{}, std::false_type{});
+            else launch(std::integral_constant<int, 4>{}, std::false_type{});
+        });
+    };
+    const int vector = dtype == NORI_F32 ? 4 : 8;
+    Grads many = q, single = q;
+    many.task[0] = many.task[1] = Task{};
+    int taken = 0;
+    for (int i = 0; i < tasks; ++i) {
+        if (q.task[i].cols >= vector) {
+            many.task[taken++] = q.task[i];
+        } else {
+            single.task[0] = q.task[i];
+            single.task[1] = Task{};
+            go(single, true);
+        }
+    }
+    if (taken) go(many, false);
+    if (longest > q.part) {
+        const int blocks0 = (int)(((int64_t)q.task[0].cols * rank + kThreads - 1) / kThreads);
+        const int blocks1 = (int)(((int64_t)q.task[1].cols * rank + kThreads - 1) / kThreads);
+        hipLaunchKernelGGL(grad_join_kernel, dim3((unsigned)(blocks0 + blocks1), groups), dim3(kThreads), 0, stream, q, dtype,
+                           blocks0);
+    }
+    return launch_status("low_rank_backward");
 }

@@ -107,30 +107,32 @@ int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_t rows, int
 
 // Low-rank updates of many tables at once (low_rank.hip): out[i] = y[i] + (scales[id] x[i] a[id]^T) b[id]^T with
 // id the adapter of row i; rows without one take y (y NULL: zeros). x [rows, k], y and out [rows, n] of one
-// dtype at row strides, out may be y; a [adapters, rank, k] and b [adapters, n, rank] of that dtype, contiguous
-// (transposed: a [adapters, k, rank] and b [adapters, rank, n]); scales [adapters] fp32 or NULL for 1.
-// order [rows] lists the rows of group 0, then of group 1, ...: group g is order[starts[g] .. starts[g + 1]),
-// its adapter ids[g] or -1, each id once. h [rows, rank] fp32, or NULL, takes scales[id] x[i] a[id]^T (rows without
-// an adapter are left). The workspace, of nori_low_rank_workspace_bytes and 16-byte aligned, takes the factors in
-// the matrix instructions' order (none is needed for few rows with the factors as they are).
+// dtype at row strides, out may be y; a [adapters, rank, k] and b [adapters, n, rank] of that dtype, contiguous;
+// scales [adapters] fp32 or NULL for 1. order [rows] lists the rows of group 0, then of group 1, ...: group g is
+// order[starts[g] .. starts[g + 1]), its adapter ids[g] or -1, each id once. h [rows, rank] fp32, or NULL, takes
+// scales[id] x[i] a[id]^T (rows without an adapter are left). The workspace, of nori_low_rank_workspace_bytes and
+// 16-byte aligned, takes the factors in the matrix instructions' order (0 for few rows).
 #define NORI_LOW_RANK_MAX 128
 int nori_low_rank_update(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* y,
-                         int64_t y_row_stride, const void* a, const void* b, int32_t transposed, const float* scales,
-                         int32_t adapters, int32_t rank, int32_t n, const int32_t* order, const int32_t* starts,
-                         const int32_t* ids, int32_t groups, void* out, int64_t out_row_stride, float* h, void* workspace,
+                         int64_t y_row_stride, const void* a, const void* b, const float* scales, int32_t adapters,
+                         int32_t rank, int32_t n, const int32_t* order, const int32_t* starts, const int32_t* ids,
+                         int32_t groups, void* out, int64_t out_row_stride, float* h, void* workspace,
                          int64_t workspace_bytes, void* stream);
-int64_t nori_low_rank_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups,
-                                      int32_t transposed);
+int64_t nori_low_rank_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups);
 
-// The sum over each adapter's rows of t[i]^T h[i] as out [adapters, cols, rank] (transposed: [adapters, rank,
-// cols]) of t's dtype, t [rows, cols] at a row stride, h [rows, rank] fp32, the groups as above, `longest` the most
-// rows of one with an adapter. Groups of many rows are summed in parts, joined in a fixed order, in the
-// workspace. Adapters without a group are left as they are.
-int nori_low_rank_weight_grad(const void* t, int dtype, int64_t rows, int32_t cols, int64_t t_row_stride, const float* h,
-                              int32_t rank, int32_t adapters, const int32_t* order, const int32_t* starts,
-                              const int32_t* ids, int32_t groups, int64_t longest, int32_t transposed, void* out,
-                              void* workspace, int64_t workspace_bytes, void* stream);
-int64_t nori_low_rank_weight_grad_workspace_bytes(int dtype, int64_t rows, int32_t cols, int32_t rank, int64_t longest);
+// Its gradients, each NULL where it is not asked for: with g[i] = scales[id] dy[i] b[id],
+//     dx[i] = base[i] + g[i] a[id]   (rows without an adapter take base; base NULL: zeros; dx may be base),
+//     da[id] = sum over the adapter's rows of g[i]^T x[i],   db[id] = sum over them of dy[i]^T h[i],
+// h as the update kept it, da and db in a's and b's layout and dtype; adapters without a group are left as they
+// are. `longest` is the most rows of a group with an adapter. Rows are summed in parts that are joined in a fixed
+// order: the same inputs give the same bits.
+int nori_low_rank_backward(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* dy, int32_t n,
+                           int64_t dy_row_stride, const void* base, int64_t base_row_stride, const void* a, const void* b,
+                           const float* scales, int32_t adapters, int32_t rank, const int32_t* order, const int32_t* starts,
+                           const int32_t* ids, int32_t groups, int64_t longest, const float* h, void* dx,
+                           int64_t dx_row_stride, void* da, void* db, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t nori_low_rank_backward_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups,
+                                               int64_t longest, int32_t need_x, int32_t need_a, int32_t need_b);
 
 #ifdef __cplusplus
 }

@@ -159,15 +159,16 @@ OPS: dict[str, tuple[object, list]] = {
     ),
     "nori_low_rank_update": (
         ctypes.c_int,
-        [_vp, _i32, _i64, _i32, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _vp,
-         _vp, _i64, _vp],
+        [_vp, _i32, _i64, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _vp, _vp, _i64,
+         _vp],
     ),
-    "nori_low_rank_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32, _i32]),
-    "nori_low_rank_weight_grad": (
+    "nori_low_rank_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32]),
+    "nori_low_rank_backward": (
         ctypes.c_int,
-        [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i64, _i32, _vp, _vp, _i64, _vp],
+        [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i64, _vp, _vp,
+         _i64, _vp, _vp, _vp, _i64, _vp],
     ),
-    "nori_low_rank_weight_grad_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i64]),
+    "nori_low_rank_backward_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _i32]),
     "nori_rms_norm_rows": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _i32, _vp]),
 }
 

@@ -21,7 +21,7 @@ import torch.nn.functional as F
 
 from . import _native as nat
 from .layer import _hooked
-from .norm import _FLOATS, _rows_of, _strided_rows, trainable_layer_norm
+from .norm import _FLOATS, _first_derivative, _rows_of, _strided_rows, trainable_layer_norm
 
 __all__ = ["AdapterPlan", "LowRankAdapters", "ReadoutAdapters", "adapted_linear", "low_rank_update"]
 
@@ -65,6 +65,7 @@ class AdapterPlan:
         self.longest = int(np.diff(starts)[groups >= 0].max(initial=0))  # the most rows of one adapter
         packed = torch.from_numpy(np.concatenate([starts, groups, order]).astype(np.int32)).to(self.device)
         self.starts, self.ids, self.order = packed.split([self.groups + 1, self.groups, self.rows])
+        self.pointers = self.order.data_ptr(), self.starts.data_ptr(), self.ids.data_ptr()
 
 
 def _grouped(ids: np.ndarray, counts: np.ndarray) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
@@ -80,84 +81,72 @@ def _grouped(ids: np.ndarray, counts: np.ndarray) -> tuple[np.ndarray, np.ndarra
     return order, np.append(at[where], total), groups
 
 
-def _update(x, y, a, b, plan, scales, transposed, out, keep=True):
-    """``out`` = y + update (y None: the update alone) by ``nori_low_rank_update``; returns h [rows, rank], None
-    unless kept."""
-    rank = int(a.shape[2 if transposed else 1])
-    k, n = int(x.shape[-1]), int(out.shape[-1])
+def _update(x, y, a, b, plan, scales, out, keep):
+    """``out`` = y + update by ``nori_low_rank_update``; returns h [rows, rank] for the gradients where it is to
+    be kept, None else."""
+    k, n, rank = int(x.shape[-1]), int(out.shape[-1]), int(a.shape[1])
     x, rows, xs = _rows_of(x, k)
-    ys = 0
-    if y is not None:
-        y, _, ys = _rows_of(y, n)
+    y, _, ys = _rows_of(y, n)
     layout = _strided_rows(out, n)
     if layout is None:
         raise ValueError(f"out {tuple(out.shape)} has strides {out.stride()}: its rows must be at one stride")
-    os = layout[1]
-    h = torch.empty((rows, rank), dtype=torch.float32, device=x.device) if keep else None
-    lib, dtype, adapters = nat.lib(), nat.dtype_code(x.dtype), int(a.shape[0])
-    size = lib.nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, plan.groups, 1 if transposed else 0)
-    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    with nat.on(x.device):
+    device = x.device
+    h = torch.empty((rows, rank), dtype=torch.float32, device=device) if keep else None
+    lib, dtype = nat.lib(), nat.dtype_code(x.dtype)
+    size = lib.nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, plan.groups)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    with nat.on(device):
         nat.check(
             lib.nori_low_rank_update(
-                x.data_ptr(), dtype, rows, k, xs, nat.ptr(y), ys, a.data_ptr(), b.data_ptr(), 1 if transposed else 0,
-                nat.ptr(scales), adapters, rank, n, plan.order.data_ptr(), plan.starts.data_ptr(), plan.ids.data_ptr(),
-                plan.groups, out.data_ptr(), os, nat.ptr(h), nat.ptr(workspace), size, nat.stream_of(x.device),
+                x.data_ptr(), dtype, rows, k, xs, y.data_ptr(), ys, a.data_ptr(), b.data_ptr(), nat.ptr(scales), int(a.shape[0]),
+                rank, n, *plan.pointers, plan.groups, out.data_ptr(), layout[1], nat.ptr(h), nat.ptr(workspace), size,
+                nat.stream_of(device),
             ),
             "low_rank_update",
         )
     return h
 
 
-def _weight_grad(t, h, plan, like, transposed):
-    """The sum over each adapter's rows of t^T h, in ``like``'s shape, by ``nori_low_rank_weight_grad``."""
-    cols = int(t.shape[-1])
-    t, rows, ts = _rows_of(t, cols)
-    out = torch.empty_like(like) if len(plan.adapters) == like.shape[0] else torch.zeros_like(like)
-    if plan.longest:
-        lib, dtype, rank = nat.lib(), nat.dtype_code(t.dtype), int(h.shape[1])
-        size = lib.nori_low_rank_weight_grad_workspace_bytes(dtype, rows, cols, rank, plan.longest)
-        workspace = torch.empty(size, dtype=torch.uint8, device=t.device) if size else None
-        with nat.on(t.device):
+def _gradients(dy, x, a, b, h, plan, scales, needs, base=None):
+    """(dx, da, db), None where not needed, by ``nori_low_rank_backward``; ``base`` [..., in] is what dx is
+    added to, and overwritten."""
+    need_x, need_a, need_b = needs
+    k, n, rank = int(x.shape[-1]), int(dy.shape[-1]), int(a.shape[1])
+    device = x.device
+    x2, rows, xs = _rows_of(x, k)
+    dy2, _, ys = _rows_of(dy, n)
+    dx = (torch.empty(x.shape, dtype=x.dtype, device=device) if base is None else base) if need_x else None
+    make = torch.empty_like if len(plan.adapters) == a.shape[0] else torch.zeros_like  # adapters no row takes: zeros
+    da = make(a) if need_a else None
+    db = make(b) if need_b else None
+    if rows and any(needs):
+        lib, dtype = nat.lib(), nat.dtype_code(x.dtype)
+        size = lib.nori_low_rank_backward_workspace_bytes(dtype, rows, k, n, rank, plan.groups, plan.longest, need_x, need_a,
+                                                          need_b)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        with nat.on(device):
             nat.check(
-                lib.nori_low_rank_weight_grad(
-                    t.data_ptr(), dtype, rows, cols, ts, h.data_ptr(), rank, int(like.shape[0]), plan.order.data_ptr(),
-                    plan.starts.data_ptr(), plan.ids.data_ptr(), plan.groups, plan.longest, 1 if transposed else 0,
-                    out.data_ptr(), nat.ptr(workspace), size, nat.stream_of(t.device),
+                lib.nori_low_rank_backward(
+                    x2.data_ptr(), dtype, rows, k, xs, dy2.data_ptr(), n, ys, nat.ptr(base), k, a.data_ptr(), b.data_ptr(),
+                    nat.ptr(scales), int(a.shape[0]), rank, *plan.pointers, plan.groups, plan.longest, h.data_ptr(), nat.ptr(dx), k,
+                    nat.ptr(da), nat.ptr(db), nat.ptr(workspace), size, nat.stream_of(device),
                 ),
                 "low_rank_update backward",
             )
-    return out
-
-
-def _gradients(dy, x, a, b, h, plan, scales, needs, base=None):
-    """(dx, da, db), None where not needed; ``base`` [..., in] is what dx is added to, and overwritten."""
-    need_x, need_a, need_b = needs
-    dx = da = db = None
-    if need_x or need_a:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if base is None else base
-        if plan.rows:
-            g = _update(dy, base, b, a, plan, scales, True, dx)
-        else:
-            g = h
-        if need_a:
-            da = _weight_grad(x, g, plan, a, True)
-    if need_b:
-        db = _weight_grad(dy, h, plan, b, False)
-    return (dx if need_x else None), da, db
+    return dx, da, db
 
 
 class _LowRankUpdate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, a, b, plan, scales):
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        h = _update(x, y, a, b, plan, scales, False, out) if plan.rows else x.new_empty((0, a.shape[1]), dtype=torch.float32)
+        h = _update(x, y, a, b, plan, scales, out, True)
         ctx.save_for_backward(x, a, b, h, scales)
         ctx.plan = plan
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, dout):
         x, a, b, h, scales = ctx.saved_tensors
         need_x, need_y, need_a, need_b = ctx.needs_input_grad[:4]
@@ -175,13 +164,13 @@ class _AdaptedLinear(torch.autograd.Function):
             y = F.linear(x, weight, bias)
         if _strided_rows(y, int(y.shape[-1])) is None:
             y = y.contiguous()
-        h = _update(x, y, a, b, plan, scales, False, y) if plan.rows else x.new_empty((0, a.shape[1]), dtype=torch.float32)
+        h = _update(x, y, a, b, plan, scales, y, True)
         ctx.save_for_backward(x, weight, a, b, h, scales)
         ctx.plan = plan
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         x, weight, a, b, h, scales = ctx.saved_tensors
         need_x, _, _, need_a, need_b = ctx.needs_input_grad[:5]
@@ -288,9 +277,9 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
         return out
     if _strided_rows(out, int(out.shape[-1])) is None:
         whole = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        _update(x, y, a, b, plan, scales, False, whole, False)
+        _update(x, y, a, b, plan, scales, whole, False)
         return out.copy_(whole)
-    _update(x, y, a, b, plan, scales, False, out, False)
+    _update(x, y, a, b, plan, scales, out, False)
     return out
 
 

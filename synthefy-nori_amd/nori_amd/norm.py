@@ -371,7 +371,7 @@ def _rows_of(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
 
 
 def _train_forward(x, weight, bias, eps, out_dtype, keep):
-    """(y, mean, rstd) by ``nori_layer_norm_train_forward``; the statistics are None unless kept."""
+    """(y, [mean, rstd] of every row) by ``nori_layer_norm_train_forward``; the statistics are None unless kept."""
     cols = int(x.shape[-1])
     x2, rows, stride = _rows_of(x, cols)
     y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
@@ -383,8 +383,8 @@ def _train_forward(x, weight, bias, eps, out_dtype, keep):
                     x2.data_ptr(), nat.dtype_code(x.dtype), rows, cols, stride,
                     nat.ptr(weight), 0 if weight is None else nat.dtype_code(weight.dtype),
                     nat.ptr(bias), 0 if bias is None else nat.dtype_code(bias.dtype), eps,
-                    y.data_ptr(), nat.dtype_code(out_dtype), stats[0].data_ptr() if keep else None,
-                    stats[1].data_ptr() if keep else None, nat.stream_of(x.device),
+                    y.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(stats), stats.data_ptr() + 4 * rows if keep else None,
+                    nat.stream_of(x.device),
                 ),
                 "trainable_layer_norm",
             )
@@ -408,12 +408,22 @@ def _train_backward(dy, x, weight, bias, stats, need_x, need_w, need_b):
                 nat.lib().nori_layer_norm_train_backward(
                     x2.data_ptr(), nat.dtype_code(x.dtype), rows, cols, stride, dy2.data_ptr(), nat.dtype_code(dy.dtype),
                     dy_stride, nat.ptr(weight), 0 if weight is None else nat.dtype_code(weight.dtype),
-                    0 if bias is None else nat.dtype_code(bias.dtype), stats[0].data_ptr(), stats[1].data_ptr(),
+                    0 if bias is None else nat.dtype_code(bias.dtype), stats.data_ptr(), stats.data_ptr() + 4 * rows,
                     nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.ptr(workspace), size, nat.stream_of(x.device),
                 ),
                 "trainable_layer_norm backward",
             )
     return dx, dw, db
+
+
+def _first_derivative(backward):
+    """``once_differentiable``, without the time its checks take where no graph of the gradients is made."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 class _TrainableLayerNorm(torch.autograd.Function):
@@ -424,7 +434,7 @@ class _TrainableLayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         return (*_train_backward(dy, *ctx.saved_tensors, *ctx.needs_input_grad[:3]), None, None)
 

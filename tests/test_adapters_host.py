@@ -104,10 +104,27 @@ def test_library_refuses_bad_arguments_before_any_device_work():
     bw = [16, nat.NORI_F16, 4, 10, 10, 16, nat.NORI_F16, 10, None, 0, 0, 16, 16, None, 16, None, None, 0, None]
     assert lib.nori_layer_norm_train_backward(*bw) == nat.NORI_ERR_INVALID  # dw without a workspace
     assert b"workspace" in lib.nori_last_error()
-    up = [None, nat.NORI_F16, 4, 8, 8, None, 8, None, None, 0, None, 2, 4, 8, None, None, None, 1, None, 8, None, None, 0, None]
+    up = [None, nat.NORI_F16, 4, 8, 8, None, 8, None, None, None, 2, 4, 8, None, None, None, 1, None, 8, None, None, 0, None]
     assert lib.nori_low_rank_update(*up) == nat.NORI_ERR_INVALID  # null pointers
-    for at, value, code in ((1, nat.NORI_I8, nat.NORI_ERR_UNSUPPORTED), (12, 129, nat.NORI_ERR_UNSUPPORTED), (12, 0, nat.NORI_ERR_INVALID),
-                            (3, 0, nat.NORI_ERR_INVALID), (2, 0, nat.NORI_OK), (2, 1 << 31, nat.NORI_ERR_UNSUPPORTED)):
+    for at, value, code in ((1, nat.NORI_I8, nat.NORI_ERR_UNSUPPORTED), (11, 129, nat.NORI_ERR_UNSUPPORTED), (11, 0, nat.NORI_ERR_INVALID),
+                            (3, 0, nat.NORI_ERR_INVALID), (2, 0, nat.NORI_OK), (2, 1 << 31, nat.NORI_ERR_UNSUPPORTED),
+                            (16, 65536, nat.NORI_ERR_UNSUPPORTED)):
         bad = list(up)
         bad[at] = value
         assert lib.nori_low_rank_update(*bad) == code, at
+    full = [16, nat.NORI_F16, 100000, 8, 8, 16, 8, 16, 16, None, 2, 4, 8, 16, 16, 16, 1, 16, 8, None, None, 0, None]
+    assert lib.nori_low_rank_update(*full) == nat.NORI_ERR_INVALID and b"workspace" in lib.nori_last_error()
+    full[18] = 7
+    assert lib.nori_low_rank_update(*full) == nat.NORI_ERR_INVALID and b"overlap" in lib.nori_last_error()
+    full[5], full[17], full[18] = 16, 16, 9
+    assert lib.nori_low_rank_update(*full) == nat.NORI_ERR_INVALID and b"another row stride" in lib.nori_last_error()
+    back = [16, nat.NORI_F16, 4, 8, 8, 16, 8, 8, None, 8, 16, 16, None, 2, 4, 16, 16, 16, 1, 4, 16, 16, 8, 16, 16, None, 0, None]
+    assert lib.nori_low_rank_backward(*back) == nat.NORI_ERR_INVALID and b"workspace" in lib.nori_last_error()
+    for at, value, code in ((1, nat.NORI_I8, nat.NORI_ERR_UNSUPPORTED), (14, 129, nat.NORI_ERR_UNSUPPORTED), (19, 5, nat.NORI_ERR_INVALID),
+                            (0, None, nat.NORI_ERR_INVALID), (20, None, nat.NORI_ERR_INVALID), (22, 7, nat.NORI_ERR_INVALID),
+                            (2, 0, nat.NORI_OK)):
+        bad = list(back)
+        bad[at] = value
+        assert lib.nori_low_rank_backward(*bad) == code, at
+    back[21] = back[23] = back[24] = None
+    assert lib.nori_low_rank_backward(*back) == nat.NORI_OK  # nothing is asked for
