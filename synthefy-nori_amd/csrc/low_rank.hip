@@ -626,10 +626,16 @@ __global__ void __launch_bounds__(kThreads) update_few_kernel(const Update u) {
     }
 }
 
+// Tiles of 16 ranks a workgroup of the gradients' kernel sums, and workgroups of it that a compute unit holds.
+constexpr int grad_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : 4; }
+constexpr int grad_held(int tiles) { return tiles == 1 ? 3 : tiles == 2 ? 2 : 1; }
+
 // One of the two sums t^T h over each group's rows.
 struct Task {
     const void* t;   // [rows][cols]
     const float* h;  // [rows][rank]
+    void* ops;       // h as operands (pack_rows_kernel)
+    int* exps;       // and the power of two of each step of them
     int64_t ts;
     int cols;
     int chunks;  // of its columns, a workgroup's each
@@ -656,25 +662,99 @@ __device__ __forceinline__ void store_grad(const Task& k, int rank, int dt, int 
     else reinterpret_cast<uint16_t*>(k.out)[i] = dt == NORI_F16 ? f32_to_f16(v) : f32_to_bf16(v);
 }
 
+// h in the order that grad_kernel's instructions take it, 32 rows of a group a step: [step][tile of 16 ranks][lane],
+// a lane's 8 rows 8 g ... 8 g + 7 of rank 16 tile + m, zeros past the group's end. 16-bit: two pieces of the type, high
+// and low, as in the update, fp16's after a power of two that brings the step's largest element to 2^8 (exps[step]; no
+// piece then leaves fp16's range, the smallest bit kept is 2^-32 of the largest). fp32: as they are. Every chunk of
+// columns reads them, so they are made once (split in the sums themselves: 60 % of a wavefront's instructions).
+constexpr int kStep = 32;  // rows
+
+// steps of group g: from starts[g] / 32 + g
+__device__ __forceinline__ int64_t step_of(const int32_t* starts, int group, int in_group) {
+    return (int64_t)starts[group] / kStep + group + in_group;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) pack_rows_kernel(const Grads q) {
+    using E = typename Mma<DT>::elem;
+    const Task& k = q.task[blockIdx.y];
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int slot = blockIdx.x * kWaves + (threadIdx.x >> 6);
+    int number;
+    const int group = group_of_tile(q.starts, q.groups, kStep, slot, number);
+    const int end = q.starts[group + 1], id = q.ids[group];
+    const int64_t first = (int64_t)q.starts[group] + (int64_t)number * kStep;
+    if (first >= end || id < 0 || id >= q.adapters) return;
+    const int tiles = (q.rank + 15) / 16;
+    const float* row[8];
+    bool in[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int p = (int)first + 8 * g + i;
+        in[i] = p < end;
+        row[i] = k.h + (int64_t)q.order[min(p, end - 1)] * q.rank;
+    }
+    auto load = [&](int t, float (&v)[8]) {
+        const int j = 16 * t + m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = row[i][min(j, q.rank - 1)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = in[i] && j < q.rank ? v[i] : 0.f;
+    };
+    float down = 1.0f;
+    if constexpr (DT == NORI_F16) {
+        float largest = 0.f;
+        for (int t = 0; t < tiles; ++t) {
+            float v[8];
+            load(t, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) largest = fabsf(v[i]) < __builtin_inff() ? fmaxf(largest, fabsf(v[i])) : largest;
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
+        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 8, -110), 110);
+        down = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (lane == 0) k.exps[slot] = e;
+    }
+    for (int t = 0; t < tiles; ++t) {
+        float v[8];
+        load(t, v);
+        const int64_t at = ((int64_t)slot * tiles + t) * 64 + lane;
+        if constexpr (DT == NORI_F32) {
+            f32x4* to = reinterpret_cast<f32x4*>(k.ops) + 2 * at;
+            to[0] = f32x4{v[0], v[1], v[2], v[3]};
+            to[1] = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+            u16x8 high, low;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float s = v[i] * down;
+                high[i] = narrow<DT>(s);
+                low[i] = fabsf(s) < __builtin_inff() ? narrow<DT>(s - widen<DT>(high[i])) : E(0);
+            }
+            u16x8* to = reinterpret_cast<u16x8*>(k.ops) + 2 * at;
+            to[0] = high;
+            to[1] = low;
+        }
+    }
+}
+
 // t^T h over one part of a group's rows: 128 (fp32: 64) columns by up to 64 ranks a workgroup, whose wavefronts
-// take every fourth step of rows and add their sums in LDS, in order. HBM-bound: t is read once, h (4 rank bytes a
-// row) once a chunk of columns, from the L2; the next step's rows are on their way while one is summed.
+// take every fourth step of rows and add their sums in LDS, in order. HBM-bound: t is read once, h once a chunk of
+// columns, from the L2; the next step's rows are on their way while one is summed.
 // The sum runs over rows, which t has apart. 16-bit: a lane reads 16 bytes of each of 8 rows and turns the 8 x 8
 // block in registers, so that it holds 8 rows of one column for each of 8 instructions; column i of a lane's
-// block belongs to instruction i. fp32: an instruction takes 4 rows, no turning. h, in fp32, enters in two pieces
-// of the 16-bit type as in the update; a power of two per wavefront that follows the largest element so far keeps
-// fp16's pieces in range (sums so far are brought to a new one).
+// block belongs to instruction i. fp32: instruction i takes row 8 g + i of the lane groups g, no turning. fp16's sums
+// are kept at the largest power of two of the steps so far: a larger one rescales them, a smaller one its operands.
 // Where a row ends inside a lane's columns, the lane takes the last ones instead and writes them again, the same
 // values. SHORT: rows of fewer columns than a lane takes.
 template <int DT, int RT, bool SHORT>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const Grads q) {
+__global__ void __launch_bounds__(kThreads, grad_held(RT)) grad_kernel(const Grads q) {
     using M = Mma<DT>;
     using E = typename M::elem;
     using F = typename M::frag;
     constexpr bool F32 = DT == NORI_F32;
-    constexpr int W = M::W, CT = W;    // a lane's columns, an instruction each
-    constexpr int EACH = 8;            // rows a lane holds of a step
-    constexpr int STEP = 32;           // rows of a step
+    constexpr int W = M::W, CT = W;  // a lane's columns, an instruction each
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     int number;
     const int group = group_of_tile(q.starts, q.groups, q.part, blockIdx.x, number);
@@ -685,33 +765,37 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Grads q) {
     const int first = (int)first64, end = min(last, first + q.part);
     const bool second = (int)blockIdx.y >= q.task[0].chunks;
     const Task& k = q.task[second];
-    const int chunk = blockIdx.y - (second ? q.task[0].chunks : 0), j0 = blockIdx.z * 16 * RT;
+    const int chunk = blockIdx.y - (second ? q.task[0].chunks : 0), t0 = blockIdx.z * RT, tiles = (q.rank + 15) / 16;
     auto column = [&](int of) { return SHORT ? 0 : min(chunk * 16 * W + W * of, k.cols - W); };
     const E* t = reinterpret_cast<const E*>(k.t) + column(m);
-    int rank_at[RT];  // ranks past the last sum what is never written
-#pragma unroll
-    for (int r = 0; r < RT; ++r) rank_at[r] = min(j0 + 16 * r + m, q.rank - 1);
+    const int64_t step0 = step_of(q.starts, group, number * (q.part / kStep));
 
-    // fp32: instruction i takes rows 4 i ... 4 i + 3 of a step, so a lane's are 4 apart
-    auto place = [&](int p0, int i) { return p0 + (F32 ? 4 * i + g : EACH * g + i); };
-    F raw[EACH];
-    float h[EACH][RT];
-    int row[EACH];
-    auto ask_rows = [&](int p0) {
+    int row[8];
+    F raw[8];
+    F ops[RT][2];
+    int exp_asked = 0;
+    auto ask_rows = [&](int s) {
+        const int p = first + s * kStep + 8 * g;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) row[i] = q.order[min(place(p0, i), end - 1)];
+        for (int i = 0; i < 8; ++i) row[i] = q.order[min(p + i, end - 1)];
     };
-    auto ask = [&](int p0) {
+    auto ask = [&](int s) {
+        const int p = first + s * kStep + 8 * g;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
+        for (int i = 0; i < 8; ++i) {
             raw[i] = F{};
-            if (place(p0, i) < end) {
+            if (p + i < end) {
                 if constexpr (SHORT) raw[i] = fetch<DT>(t + row[i] * k.ts, k.cols);
                 else raw[i] = fetch<DT>(t + row[i] * k.ts);
             }
-#pragma unroll
-            for (int r = 0; r < RT; ++r) h[i][r] = k.h[(int64_t)row[i] * q.rank + rank_at[r]];
         }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {  // tiles past the last sum what is never written
+            const F* from = reinterpret_cast<const F*>(k.ops) + (((step0 + s) * tiles + min(t0 + r, tiles - 1)) * 64 + lane) * 2;
+            ops[r][0] = from[0];
+            ops[r][1] = from[1];
+        }
+        if constexpr (DT == NORI_F16) exp_asked = k.exps[step0 + s];
     };
 
     f32x4 acc[RT][CT];
@@ -719,96 +803,77 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(const Grads q) {
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int i = 0; i < CT; ++i) acc[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float up = 1.0f, down = 1.0f;
-    float reach = 0.f;  // elements below it fit the present power of two
-    const int p1 = first + wave * STEP;
-    if (p1 < end) {
-        ask_rows(p1);
-        ask(p1);
-        if (p1 + STEP * kWaves < end) ask_rows(p1 + STEP * kWaves);
+    int scale = -1000;  // the sums' power of two; none yet
+    const int steps = (end - first + kStep - 1) / kStep;
+    if (wave < steps) {
+        ask_rows(wave);
+        ask(wave);
+        if (wave + kWaves < steps) ask_rows(wave + kWaves);
     }
-    for (int p0 = p1; p0 < end; p0 += STEP * kWaves) {
-        F now[EACH];
-        float hn[EACH][RT];
+    for (int s = wave; s < steps; s += kWaves) {
+        F now[8], hn[RT][2];
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            now[i] = raw[i];
+        for (int i = 0; i < 8; ++i) now[i] = raw[i];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) hn[i][r] = place(p0, i) < end ? h[i][r] : 0.f;
-        }
-        const int p2 = p0 + STEP * kWaves;
-        if (p2 < end) ask(p2);
-        if (p2 + STEP * kWaves < end) ask_rows(p2 + STEP * kWaves);
+        for (int r = 0; r < RT; ++r) hn[r][0] = ops[r][0], hn[r][1] = ops[r][1];
+        const int e = exp_asked;
+        if (s + kWaves < steps) ask(s + kWaves);
+        if (s + 2 * kWaves < steps) ask_rows(s + 2 * kWaves);
         if constexpr (F32) {
 #pragma unroll
-            for (int s = 0; s < EACH; ++s)
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int i = 0; i < CT; ++i)
-                        acc[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(now[s][i], hn[s][r], acc[r][i], 0, 0, 0);
+                    for (int c = 0; c < CT; ++c)
+                        acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(now[i][c], hn[r][i / 4][i % 4], acc[r][c], 0, 0, 0);
         } else {
             if constexpr (DT == NORI_F16) {
-                float largest = 0.f;
-#pragma unroll
-                for (int i = 0; i < EACH; ++i)
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        const float v = fabsf(hn[i][r]);
-                        largest = v < __builtin_inff() ? fmaxf(largest, v) : largest;
-                    }
-                if (__ballot(largest > reach)) {
-#pragma unroll
-                    for (int off = 32; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
-                    const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 8, -110), 110);
-                    const float to = __uint_as_float((uint32_t)(127 - e) << 23);
-                    if (reach > 0.f) {
-                        const float change = to * up;
+                if (e > scale) {  // the same in every lane
+                    const float change = __uint_as_float((uint32_t)max(127 + scale - e, 0) << 23);
+                    if (scale > -1000) {
 #pragma unroll
                         for (int r = 0; r < RT; ++r)
 #pragma unroll
-                            for (int i = 0; i < CT; ++i) acc[r][i] = acc[r][i] * change;
+                            for (int c = 0; c < CT; ++c) acc[r][c] = acc[r][c] * change;
                     }
-                    up = __uint_as_float((uint32_t)(127 + e) << 23);
-                    down = to;
-                    reach = up * 512.0f;  // scaled: below 2^9, the pieces of the smallest that counts above 2^-24
+                    scale = e;
+                } else if (e < scale) {
+                    // 2^(e - scale), in fp16: below 2^-24 nothing is left of them beside what the sums hold
+                    const _Float16 f = (_Float16)__uint_as_float((uint32_t)max(127 + e - scale, 1) << 23);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) hn[r][p] = __builtin_bit_cast(F, __builtin_bit_cast(f16x8, hn[r][p]) * f);
                 }
             }
-            F high[RT], low[RT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = hn[i][r] * down;
-                    high[r][i] = narrow<DT>(v);
-                    low[r][i] = fabsf(v) < __builtin_inff() ? narrow<DT>(v - widen<DT>(high[r][i])) : E(0);
-                }
-#pragma unroll
-            for (int i = 0; i < CT; ++i) {
+            for (int c = 0; c < CT; ++c) {
                 F col;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) col[e] = now[e][i];
+                for (int i = 0; i < 8; ++i) col[i] = now[i][c];
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    acc[r][i] = M::mul(col, high[r], acc[r][i]);
-                    acc[r][i] = M::mul(col, low[r], acc[r][i]);
+                    acc[r][c] = M::mul(col, hn[r][0], acc[r][c]);
+                    acc[r][c] = M::mul(col, hn[r][1], acc[r][c]);
                 }
             }
         }
     }
-    // the wavefronts' sums, a rank tile at a time. acc[r][i][j] of lane (m, g): column i of operand row 4 g + j, rank 16 r + m
+    // the wavefronts' sums, a rank tile at a time. acc[r][c][j] of lane (m, g): column c of operand row 4 g + j, rank 16 r + m
     __shared__ f32x4 sums[kWaves][CT][64];
+    const float up = DT == NORI_F16 && scale > -1000 ? __uint_as_float((uint32_t)(127 + scale) << 23) : 1.0f;
     const bool whole = last - begin <= q.part;
     float* part = whole ? nullptr : k.partial + (partial_of(q, group) + number) * k.cols * q.rank;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < CT; ++i) sums[wave][i][lane] = acc[r][i] * up;
+        for (int c = 0; c < CT; ++c) sums[wave][c][lane] = acc[r][c] * up;
         __syncthreads();
         for (int i = wave; i < CT; i += kWaves) {
             const f32x4 v = (sums[0][i][lane] + sums[1][i][lane]) + (sums[2][i][lane] + sums[3][i][lane]);
-            const int j = j0 + 16 * r + m;
+            const int j = 16 * (t0 + r) + m;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int c = column(4 * g + e) + i;
@@ -839,12 +904,28 @@ __global__ void __launch_bounds__(kThreads) grad_join_kernel(const Grads q, int 
 
 int chunks_of(int cols, int dtype) { return (cols + (dtype == NORI_F32 ? 63 : 127)) / (dtype == NORI_F32 ? 64 : 128); }
 
-// Rows of a part: about four workgroups a compute unit, and no part so short that its sums cost as much as its rows
-// (8 rank bytes a column, twice, against 2 to 4 a row).
-int part_of(int64_t rows, int chunks, int rank) {
-    const int64_t want = rows * chunks * ((rank + 63) / 64) / (4 * (int64_t)device_cus());
-    return (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 256), 8192);
+// Rows of a part: the longest group is cut into the number of parts that costs a compute unit the fewest rows. A
+// workgroup costs its rows, 64 for its start, and for its sums, written and joined, 64 a tile of ranks (128 columns of
+// 16 ranks, twice, against 256 bytes a row); where all of a unit's workgroups run at once, their starts and ends fall
+// together and cost a quarter more. (65536 rows of 32 adapters, 1680 columns, rank 16 fp16: 70 us in 448 workgroups
+// of 2048 rows, 57 in 896 of 1024; 64 adapters, 1408 columns: 54 in 704 of 1024, 44 in 1408 of 512; 65536 rows of one
+// adapter, 1408 columns, rank 64, where a unit holds one workgroup: 85 in 253 of 2816, 113 in 473 of 1536.)
+int part_of(int64_t rows, int64_t longest, int groups, int chunks, int rank) {
+    const int tiles = grad_tiles(rank), held = grad_held(tiles), cus = device_cus();
+    const int64_t slices = (int64_t)chunks * ((rank + 16 * tiles - 1) / (16 * tiles)), mean = (rows + groups - 1) / groups;
+    int64_t best = 0, least = 0;
+    for (int64_t p = 1; p <= 64; ++p) {
+        const int64_t part = std::max<int64_t>((longest + p - 1) / p + 127, 256) / 128 * 128;
+        const int64_t each = (groups * ((mean + part - 1) / part) * slices + cus - 1) / cus;  // workgroups of a unit
+        const int64_t cost = each * (part + 64 * (tiles + 1)) * (held > 1 && each <= held ? 5 : 4);
+        if (!best || cost < least) best = part, least = cost;
+        if (part == 256) break;
+    }
+    return (int)best;
 }
+
+// h or g as operands, in bytes
+int64_t operand_bytes(int64_t rows, int groups, int rank) { return (rows / kStep + groups) * ((rank + 15) / 16) * 64 * 32; }
 
 // partial sums of one task, in bytes
 int64_t partial_bytes(int64_t rows, int part, int cols, int rank) { return (2 * rows / part + 1) * cols * rank * 4; }
@@ -953,9 +1034,10 @@ extern "C" int nori_low_rank_update(const void* x, int dtype, int64_t rows, int3
 }
 
 namespace {
-// the backward pass's workspace: g [rows][rank], the packed factors, the partial sums of da and of db
+// the backward pass's workspace: g [rows][rank], the packed factors, g and h as operands and their steps' powers of
+// two, the partial sums of da and of db
 struct Layout {
-    int64_t packed, da, db, end;
+    int64_t packed, ops_a, ops_b, da, db, end;
     int part;
 };
 
@@ -963,10 +1045,13 @@ Layout layout_of(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, in
                  bool need_a, bool need_b) {
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
     Layout l;
-    l.part = part_of(rows, (need_a ? chunks_of(k, dtype) : 0) + (need_b ? chunks_of(n, dtype) : 0), rank);
+    l.part = part_of(rows, longest, groups, (need_a ? chunks_of(k, dtype) : 0) + (need_b ? chunks_of(n, dtype) : 0), rank);
     const bool parts = longest > l.part;
     l.packed = up(need_x || need_a ? rows * rank * 4 : 0);
-    l.da = l.packed + up(need_x || need_a ? packed_bytes(dtype, rows, n, k, rank, groups, true) : 0);
+    l.ops_a = l.packed + up(need_x || need_a ? packed_bytes(dtype, rows, n, k, rank, groups, true) : 0);
+    const int64_t ops = up(operand_bytes(rows, groups, rank)) + up((rows / kStep + groups) * 4);
+    l.ops_b = l.ops_a + (need_a ? ops : 0);
+    l.da = l.ops_b + (need_b ? ops : 0);
     l.db = l.da + up(need_a && parts ? partial_bytes(rows, l.part, k, rank) : 0);
     l.end = l.db + up(need_b && parts ? partial_bytes(rows, l.part, n, rank) : 0);
     return l;
@@ -1019,10 +1104,18 @@ extern "C" int nori_low_rank_backward(const void* x, int dtype, int64_t rows, in
     q.groups = groups;
     q.part = l.part;
     int tasks = 0;
-    if (da)  // da [adapters][rank][k]
-        q.task[tasks++] = Task{x, kept, x_row_stride, k, chunks_of(k, dtype), da, 1, k, reinterpret_cast<float*>(at + l.da)};
-    if (db)  // db [adapters][n][rank]
-        q.task[tasks++] = Task{dy, h, dy_row_stride, n, chunks_of(n, dtype), db, rank, 1, reinterpret_cast<float*>(at + l.db)};
+    const int64_t exps = (operand_bytes(rows, groups, rank) + 255) / 256 * 256;
+    auto task = [&](const void* t, const float* h, int64_t ops, int64_t ts, int cols, void* out, int64_t o_col, int64_t o_rank,
+                    int64_t partial) {
+        q.task[tasks++] = Task{t, h, at + ops, reinterpret_cast<int*>(at + ops + exps), ts, cols, chunks_of(cols, dtype), out, o_col,
+                               o_rank, reinterpret_cast<float*>(at + partial)};
+    };
+    if (da) task(x, kept, l.ops_a, x_row_stride, k, da, 1, k, l.da);          // [adapters][rank][k]
+    if (db) task(dy, h, l.ops_b, dy_row_stride, n, db, rank, 1, l.db);        // [adapters][n][rank]
+    const unsigned slots = (unsigned)((rows / kStep + groups + kWaves - 1) / kWaves);
+    NORI_DISPATCH_FLOAT(dtype, DT, {
+        hipLaunchKernelGGL((pack_rows_kernel<DT>), dim3(slots, (unsigned)tasks), dim3(kThreads), 0, stream, q);
+    });
     const int64_t parts = rows / q.part + groups;
     // the tasks whose rows are whole vectors together, the others by themselves
     auto go = [&](const Grads& some, bool narrow_rows) {
@@ -1035,8 +1128,8 @@ extern "C" int nori_low_rank_backward(const void* x, int dtype, int64_t rows, in
                                    stream, some);
             };
             if (narrow_rows) launch(std::integral_constant<int, 1>{}, std::true_type{});
-            else if (rank <= 16) launch(std::integral_constant<int, 1>{}, std::false_type{});
-            else if (rank <= 32) launch(std::integral_constant<int, 2>{}, std::false_type{});
+            else if (grad_tiles(rank) == 1) launch(std::integral_constant<int, 1>{}, std::false_type{});
+            else if (grad_tiles(rank) == 2) launch(std::integral_constant<int, 2>{}, std::false_type{});
             else launch(std::integral_constant<int, 4>{}, std::false_type{});
         });
     };
