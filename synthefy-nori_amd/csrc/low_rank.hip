@@ -945,8 +945,12 @@ int check(const char* what, int dtype, int64_t rows, int32_t groups, int32_t k, 
 
 }  // namespace
 
-// Whether a tile a workgroup of 64 rows leaves most compute units idle, or most of each tile empty.
-static bool few_rows(int64_t rows, int32_t groups) { return rows / 64 + groups < 2 * device_cus() || rows <= 16 * (int64_t)groups; }
+// Whether tiles of 64 rows leave compute units idle, or are mostly empty. Packing the factors costs a launch, and 64 rows
+// an adapter read lower ranks' as fast where they lie (512 tables x 64 rows 256 -> 384 rank 16: 34 us packed, 25 not;
+// 65536 rows of 32 adapters 560 -> 1680: 119 and 160).
+static bool few_rows(int64_t rows, int32_t groups, int32_t rank) {
+    return rows / 64 + groups < 2 * device_cus() || rows <= (rank <= 32 ? 64 : 16) * (int64_t)groups;
+}
 
 template <class Go>
 static int by_rank(int32_t rank, Go go) {
@@ -958,7 +962,7 @@ static int by_rank(int32_t rank, Go go) {
 
 // of the packed factors; 0 where they are read as they lie
 static int64_t packed_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups, bool transposed) {
-    if (!transposed && few_rows(rows, groups)) return 0;
+    if (!transposed && few_rows(rows, groups, rank)) return 0;
     int64_t bytes = 0;
     NORI_DISPATCH_FLOAT(dtype, DT, {
         by_rank(rank, [&](auto RP_) {
@@ -973,7 +977,7 @@ static int64_t packed_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32
 // h and, where u.out is not null, out; the packed factors in `packed`, 16-byte aligned, or null
 static void launch_update(Update u, int dtype, int64_t rows, bool transposed, void* packed, hipStream_t stream) {
     const int cus = device_cus(), groups = u.groups;
-    const bool few = few_rows(rows, groups);
+    const bool few = few_rows(rows, groups, u.rank);
     NORI_DISPATCH_FLOAT(dtype, DT, {
         by_rank(u.rank, [&](auto RP_) {
             constexpr int RP = decltype(RP_)::value;
@@ -991,11 +995,18 @@ static void launch_update(Update u, int dtype, int64_t rows, bool transposed, vo
                                    u);
                 return 0;
             }
-            // out's columns are shared among workgroups, each with an h of its own, while there are few tiles
+            // out's columns are shared among as many workgroups, each with an h of its own, as take the least time: about
+            // 1 us of latency for every 512 of k and every round of columns, and the cycles of a compute unit's address
+            // units, twice the elements that its workgroups read (64 tables x 16 rows 1408 -> 999: 14 us at 4, 18 at
+            // 8; 32 x 128 560 -> 1680: 22 us at 1, 15 at 3)
             const int64_t tiles = rows / 16 + groups;
             const int wide = 32 * kWaves, most = u.out ? (u.n + wide - 1) / wide : 1;
-            const int split = (int)std::min<int64_t>(most, std::max<int64_t>(1, 2 * cus / tiles));
-            const int steps = (most + split - 1) / split;
+            int steps = most;
+            for (int64_t split = 1, least = 0; split <= most; ++split) {
+                const int64_t round = (most + split - 1) / split, each = (tiles * split + cus - 1) / cus;
+                const int64_t cost = 2400 * (u.k / 512 + round) + each * 2 * (u.k * (P::RT + 1) + round * wide * (P::RT + 2));
+                if (!least || cost < least) least = cost, steps = (int)round;
+            }
             u.columns = steps * wide;
             // tiles in multiples of 8: a tile's workgroups stay on one XCD, whose L2 holds its x
             const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)((most + steps - 1) / steps));
