@@ -228,7 +228,6 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
 // y and out go in windows of 128 bytes that begin where a line of out does, each row at columns of its own: the
 // result's last two blocks of columns stay in LDS. Windows at the same columns of every row leave lines half written
 // where rows are not whole lines (65536 rows of 1680 fp16, y to out alone: 136 us against 95, of 999: 65 against 45).
-// The hot loops take whole vectors only: what is left at a row's ends has code of its own, once.
 // RP: the rank rounded up to 16, 32, 64 or 128.
 template <int DT, int RP, int R>
 __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
@@ -279,12 +278,13 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
     }
     const int blocks = (u.n + CB - 1) / CB;
     const int windows = u.out ? blocks + (__ballot(shift > blocks * CB - u.n) ? 1 : 0) : 0;  // null: h alone is asked for
-    const bool vectors = !__ballot((any & 3) != 0);  // of the result in LDS
-    // Where rows begin and end with whole vectors every window is taken in vectors, some of them past the row's ends;
-    // else the first and the last are taken an element at a time.
-    const bool whole = u.n % W == 0 && !__ballot(any % W != 0);
-    const int inner0 = whole || !__ballot(shift != 0) ? 0 : 1;
-    const int inner1 = whole || !windows ? windows : max(inner0, u.n / CB);
+    const bool vectors = !__ballot((any & 3) != 0) && u.n % 4 == 0;  // of the result in LDS
+    // A lane's W columns of a window. Where a row ends, or begins, inside them it takes the row's last, or first, W
+    // instead and writes those it shares with its neighbour again, the same values: both have read their y before either
+    // writes, also where out is y, since a window's y is asked for before the window before it is written.
+    auto column = [&](int k, int i) { return min(max(k * CB + begin[i], 0), u.n - W); };
+    auto inside = [&](int k, int i) { return k * CB + begin[i] > -W && k * CB + begin[i] < u.n; };
+    const int vector_windows = u.n >= W ? windows : 0;  // shorter rows are taken an element at a time
     const F* pb = reinterpret_cast<const F*>(u.pb) + group * P::second(u.n) + lane % P::LANES;
     F y[AHEAD][2 * R], bf[AHEAD][KC * NT];
     // Loads come back in the order they were asked for: a window's operands are asked for beside its y, or waiting for
@@ -297,15 +297,14 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
         if (!u.y) return;
 #pragma unroll
         for (int i = 0; i < 2 * R; ++i) {
-            const int c = k * CB + begin[i];
-            if (c >= 0 && c + W <= u.n) f[i] = fetch<DT>(yrow[i] + c);
+            if (inside(k, i)) f[i] = fetch<DT>(yrow[i] + column(k, i));
         }
     };
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
 #pragma unroll
         for (int i = 0; i < 2 * R; ++i) y[j][i] = F{};
-        if (inner0 + j < inner1) ask(inner0 + j, y[j], bf[j]);
+        if (j < vector_windows) ask(j, y[j], bf[j]);
     }
 
     constexpr int HF = P::HALF ? 1 : KC * PIECES;
@@ -412,69 +411,59 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
             }
         }
     };
-    for (int k = 0; k < windows;) {
-        if (k < inner0 || k >= inner1) {
-            if (active && k < blocks) {
-                F b[KC * NT];
+    for (int k0 = 0; k0 < vector_windows; k0 += AHEAD) {
 #pragma unroll
-                for (int q = 0; q < KC * NT; ++q) b[q] = pb[(int64_t)(k * NT * KC + q) * P::LANES];
-                product(k, b);
-            }
+        for (int j = 0; j < AHEAD; ++j) {
+            const int k = k0 + j;
+            if (k >= vector_windows) break;
+            if (active && k < blocks) product(k, bf[j]);
             wave_sync();
-            // 4 lanes a row, each every fourth element
-#pragma unroll 1
-            for (int r = 0; r < R; ++r) {
-                const int64_t row = u.order[min(first + 16 * r + m, end - 1)];
-                const E* from = reinterpret_cast<const E*>(u.y) + row * u.ys;
-                E* to = reinterpret_cast<E*>(u.out) + row * u.os;
-                const int c0 = k * CB - (int)((uintptr_t)to / sizeof(E) % CB);
-                const int stop = first + 16 * r + m < end ? min(u.n, c0 + CB) : 0;
-#pragma unroll 8
-                for (int c = c0 + g; c < stop; c += 4) {
-                    if (c < 0) continue;
-                    E o = u.y ? from[c] : E(0);
-                    if (active) o = narrow<DT>(widen<DT>(o) + os[16 * r + m][c & (RING - 1)]);
-                    to[c] = o;
-                }
-            }
-            wave_sync();
-            ++k;
-            continue;
-        }
-        for (; k < inner1; k += AHEAD) {
+            F o[2 * R];
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                const int kk = k + j;
-                if (kk >= inner1) break;
-                if (active && kk < blocks) product(kk, bf[j]);
-                wave_sync();
-                F o[2 * R];
+            for (int i = 0; i < 2 * R; ++i) o[i] = y[j][i];  // rows without an adapter keep y's bits
+            if (k + AHEAD < vector_windows) ask(k + AHEAD, y[j], bf[j]);
 #pragma unroll
-                for (int i = 0; i < 2 * R; ++i) o[i] = y[j][i];  // rows without an adapter keep y's bits
-                if (kk + AHEAD < inner1) ask(kk + AHEAD, y[j], bf[j]);
+            for (int i = 0; i < 2 * R; ++i) {
+                const int c = column(k, i);
+                if (active) {
+                    const float* from = &os[8 * i + r0][c & (RING - 1)];
+                    float d[W];
+                    if (vectors) {
 #pragma unroll
-                for (int i = 0; i < 2 * R; ++i) {
-                    const int c = kk * CB + begin[i];
-                    if (active) {
-                        const float* from = &os[8 * i + r0][c & (RING - 1)];
-                        float d[W];
-                        if (vectors) {
+                        for (int e = 0; e < W; e += 4)
+                            *reinterpret_cast<f32x4*>(&d[e]) = *reinterpret_cast<const f32x4*>(from + e);
+                    } else {
 #pragma unroll
-                            for (int e = 0; e < W; e += 4)
-                                *reinterpret_cast<f32x4*>(&d[e]) = *reinterpret_cast<const f32x4*>(from + e);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < W; ++e) d[e] = from[e];
-                        }
-#pragma unroll
-                        for (int e = 0; e < W; ++e) o[i][e] = narrow<DT>(widen<DT>(o[i][e]) + d[e]);
+                        for (int e = 0; e < W; ++e) d[e] = from[e];
                     }
-                    if (first + 8 * i + r0 < end && c >= 0 && c + W <= u.n) __builtin_memcpy(orow[i] + c, &o[i], sizeof(F));
+#pragma unroll
+                    for (int e = 0; e < W; ++e) o[i][e] = narrow<DT>(widen<DT>(o[i][e]) + d[e]);
                 }
-                wave_sync();
+                if (first + 8 * i + r0 < end && inside(k, i)) __builtin_memcpy(orow[i] + c, &o[i], sizeof(F));
             }
+            wave_sync();
         }
-        k = inner1;
+    }
+    if (u.n >= W) return;
+    // one block of fewer than W columns: 4 lanes a row, each every fourth element
+    if (windows && active) {
+        F b[KC * NT];
+#pragma unroll
+        for (int q = 0; q < KC * NT; ++q) b[q] = pb[(int64_t)q * P::LANES];
+        product(0, b);
+    }
+    wave_sync();
+#pragma unroll 1
+    for (int r = 0; r < R; ++r) {
+        const int64_t row = u.order[min(first + 16 * r + m, end - 1)];
+        const E* from = reinterpret_cast<const E*>(u.y) + row * u.ys;
+        E* to = reinterpret_cast<E*>(u.out) + row * u.os;
+        for (int c = g; c < u.n; c += 4) {
+            if (!windows || first + 16 * r + m >= end) continue;
+            E o = u.y ? from[c] : E(0);
+            if (active) o = narrow<DT>(widen<DT>(o) + os[16 * r + m][c]);
+            to[c] = o;
+        }
     }
 }
 
