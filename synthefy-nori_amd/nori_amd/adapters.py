@@ -11,7 +11,6 @@ tables at once.
 
 from __future__ import annotations
 
-import operator
 from typing import Sequence
 
 import numpy as np
@@ -37,35 +36,43 @@ class AdapterPlan:
     share an adapter share its tiles. It can be used by any number of calls and graphs on that device."""
 
     def __init__(self, adapters: Sequence[int], rows: int | Sequence[int], *, device: torch.device | str):
-        ids = [operator.index(i) for i in adapters]
-        if isinstance(rows, Sequence) or hasattr(rows, "__len__"):
-            counts = [operator.index(n) for n in rows]
-        else:
-            counts = [operator.index(rows)] * len(ids)
+        ids = _whole_numbers(adapters)
+        counts = _whole_numbers(rows)
+        if ids.ndim != 1 or counts.ndim > 1:
+            raise ValueError(f"adapters and rows are sequences of numbers, got shapes {ids.shape} and {counts.shape}")
+        if counts.ndim == 0:
+            counts = np.full(ids.shape, counts)
         if len(counts) != len(ids):
             raise ValueError(f"{len(ids)} adapters for {len(counts)} tables")
-        if any(n < 0 for n in counts):
+        if (counts < 0).any():
             raise ValueError("a table cannot have a negative number of rows")
-        if any(i < -1 for i in ids):
+        if (ids < -1).any():
             raise ValueError("adapters are numbered from 0; -1 is none")
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise RuntimeError(f"nori_amd kernels run on a ROCm GPU; got a plan for {self.device}")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self.rows = sum(counts)
-        if self.rows > 2**31 - 1:
-            raise NotImplementedError(f"a plan takes up to {2**31 - 1} rows, got {self.rows}")
-        self.most = max(ids, default=-1)  # an adapter bank has more than this many
+        self.rows = int(counts.sum())
+        if self.rows > 2**29:
+            raise NotImplementedError(f"a plan takes up to {2**29} rows, got {self.rows}")
+        self.most = int(ids.max(initial=-1))  # an adapter bank has more than this many
         if self.most > 2**31 - 2:
             raise ValueError(f"adapter {self.most} is out of range")
-        order, starts, groups = _grouped(np.asarray(ids, dtype=np.int64), np.asarray(counts, dtype=np.int64))
-        self.adapters = tuple(int(i) for i in groups if i >= 0)  # those with rows, ascending
+        order, starts, groups = _grouped(ids, counts)
+        self.adapters = tuple(groups[groups >= 0].tolist())  # those with rows, ascending
         self.groups = len(groups)
         self.longest = int(np.diff(starts)[groups >= 0].max(initial=0))  # the most rows of one adapter
-        packed = torch.from_numpy(np.concatenate([starts, groups, order]).astype(np.int32)).to(self.device)
+        packed = torch.from_numpy(np.concatenate([starts, groups, order], dtype=np.int32, casting="unsafe")).to(self.device)
         self.starts, self.ids, self.order = packed.split([self.groups + 1, self.groups, self.rows])
         self.pointers = self.order.data_ptr(), self.starts.data_ptr(), self.ids.data_ptr()
+
+
+def _whole_numbers(values) -> np.ndarray:
+    values = np.asarray(values)
+    if values.size and values.dtype.kind not in "iu":
+        raise TypeError(f"whole numbers are wanted, got {values.dtype}")
+    return values.astype(np.int64)
 
 
 def _grouped(ids: np.ndarray, counts: np.ndarray) -> tuple[np.ndarray, np.ndarray, np.ndarray]:

@@ -363,10 +363,11 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 def _rows_of(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
     """(t, or its contiguous copy where its rows of ``cols`` elements are not at one stride; rows; stride)."""
+    if t.is_contiguous():
+        return t, t.numel() // cols, cols
     layout = _strided_rows(t, cols)
     if layout is None:
-        t = t.contiguous()
-        layout = t.numel() // cols, cols
+        return t.contiguous(), t.numel() // cols, cols
     return (t, *layout)
 
 

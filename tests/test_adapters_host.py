@@ -32,6 +32,12 @@ def test_plans_refuse_what_they_cannot_mean():
         make([-2], 4)
     with pytest.raises(TypeError):
         make([0.5], 4)
+    with pytest.raises(TypeError):
+        make([0], [4.0])
+    with pytest.raises(ValueError, match="sequences"):
+        make([[0, 1]], 4)
+    with pytest.raises(ValueError, match="sequences"):
+        make(0, 4)
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         nori_amd.AdapterPlan([0], 4, device="cpu")
 
