@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "nori_hip.h"
 #include "nori_ops.h"
 
@@ -27,11 +29,16 @@ inline int dtype_size(int dt) {
     }
 }
 
-// Compute units of the current device (256 on MI355X; that when the query fails).
+// Compute units of the current device (256 on MI355X; that when the query fails), asked for once a device: the query
+// takes longer than a launch's other checks together.
 inline int device_cus() {
+    static std::atomic<int> known[64];
     int dev = 0, cus = 0;
     if (hipGetDevice(&dev) != hipSuccess) return 256;
+    const bool kept = dev >= 0 && dev < 64;
+    if (kept && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
     if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+    if (kept) known[dev].store(cus, std::memory_order_relaxed);
     return cus;
 }
 
