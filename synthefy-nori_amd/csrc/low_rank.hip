@@ -7,9 +7,8 @@
 // Rows are taken by adapter: order[] lists the rows of group 0, then of group 1, ..., a group being
 // every row of the batch with one adapter id (-1: the rows without one), starts[] where each begins.
 //
-// HBM-bound at the ranks this is used with: e (k + 2 n) bytes against 2 r (k + n) FLOP a row. A workgroup
-// therefore takes a tile of one group's rows through both products, h staying in LDS; x, the factors and y come
-// straight to the registers that the matrix instructions read, h is the only thing exchanged between lanes.
+// HBM-bound at the ranks this is used with: e (k + 2 n) bytes against 2 r (k + n) FLOP a row. A tile of one
+// group's rows therefore goes through both products in one kernel, h staying in LDS.
 #include <algorithm>
 #include <type_traits>
 
@@ -222,9 +221,11 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
 
 // Many rows. A wavefront takes 16 R rows of one group through both products by itself; the four of a workgroup share
 // the factors' cache lines only. R is 1, or 2 for ranks above 32, where reading the factors costs more than the
-// registers and the LDS of twice the rows (65536 rows 1408 -> 1408: rank 64 165 against 147 us, rank 16 132 against 173). x, y and out pass through the wavefront's LDS between the order they lie in memory
-// (8 lanes a run of 128 bytes) and the operands' (a lane a row), and the packed factors are read as operands: every
-// access takes the address units as few cycles as its bytes do.
+// registers and the LDS of twice the rows (65536 rows 1408 -> 1408 rank 64 fp16: 165 us with 1, 147 with 2; 560 -> 1680
+// rank 16: 132 and 173).
+// x, y and out pass through the wavefront's LDS between the order they lie in memory (8 lanes a run of 128 bytes) and
+// the operands' (a lane a row), and the packed factors are read as operands: every access takes the address units as few
+// cycles as its bytes do.
 // y and out go in windows of 128 bytes that begin where a line of out does, each row at columns of its own: the
 // result's last two blocks of columns stay in LDS. Windows at the same columns of every row leave lines half written
 // where rows are not whole lines (65536 rows of 1680 fp16, y to out alone: 136 us against 95, of 999: 65 against 45).
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
     const bool active = id >= 0 && id < u.adapters;
     if (!active && u.y == u.out) return;  // the rows stay as they are
 
-    // this lane's two rows in memory's order, its elements of a run, and where the rows' windows begin
+    // this lane's 2 R rows in memory's order, its elements of a run, and where the rows' windows begin
     const int r0 = lane >> 3, lc = W * (lane & 7);
     const E* yrow[2 * R];
     E* orow[2 * R];

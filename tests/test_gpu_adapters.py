@@ -133,6 +133,8 @@ MANY = [
     ([1, 0], [32900, 200], 71, 130, 50, 2),
     ([0, 1], [20000, 13000], 128, 63, 128, 2),
     ([0, 1], [20000, 13011], 33, 321, 77, 2),
+    ([1, -1, 0], [15000, 30, 18001], 40, 5, 8, 2),
+    ([0], [33001], 1, 1, 40, 1),
     ([-1 if i % 99 == 0 else (7 * i) % 540 for i in range(540)], [(i * 13) % 50 for i in range(540)], 56, 100, 9, 540),
 ]
 
