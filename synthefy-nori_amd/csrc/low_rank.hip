@@ -222,7 +222,7 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
 // Many rows. A wavefront takes 16 R rows of one group through both products by itself; the four of a workgroup share
 // the factors' cache lines only. R is 1, or 2 for ranks above 32, where reading the factors costs more than the
 // registers and the LDS of twice the rows (65536 rows 1408 -> 1408 rank 64 fp16: 165 us with 1, 147 with 2; 560 -> 1680
-// rank 16: 132 and 173).
+// rank 16: 132 and 173), unless compute units would stay idle (16384 rows 560 -> 1680 rank 128: 51 and 72).
 // x, y and out pass through the wavefront's LDS between the order they lie in memory (8 lanes a run of 128 bytes) and
 // the operands' (a lane a row), and the packed factors are read as operands: every access takes the address units as few
 // cycles as its bytes do.
@@ -937,9 +937,11 @@ int check(const char* what, int dtype, int64_t rows, int32_t groups, int32_t k, 
 
 // Whether tiles of 64 rows leave compute units idle, or are mostly empty. Packing the factors costs a launch, and 64 rows
 // an adapter read lower ranks' as fast where they lie (512 tables x 64 rows 256 -> 384 rank 16: 34 us packed, 25 not;
-// 65536 rows of 32 adapters 560 -> 1680: 119 and 160).
+// 65536 rows of 32 adapters 560 -> 1680: 119 and 160). Factors of more than 64 columns are worth packing from one tile
+// a compute unit on (4 tables x 4096 rows 560 -> 1680 bf16, out and h, then dx: rank 128 51 + 42 us packed, 113 + 56
+// not; 1408 -> 1408 rank 64 50 + 47 and 58 + 37).
 static bool few_rows(int64_t rows, int32_t groups, int32_t rank) {
-    return rows / 64 + groups < 2 * device_cus() || rows <= (rank <= 32 ? 64 : 16) * (int64_t)groups;
+    return rows / 64 + groups < (rank <= 64 ? 2 : 1) * device_cus() || rows <= (rank <= 32 ? 64 : 16) * (int64_t)groups;
 }
 
 template <class Go>
@@ -980,9 +982,19 @@ static void launch_update(Update u, int dtype, int64_t rows, bool transposed, vo
                                    0, stream, u, transposed ? 1 : 0);
             }
             if (!few) {
-                constexpr int R = RP <= 32 ? 1 : 2;
-                hipLaunchKernelGGL((update_kernel<DT, RP, R>), dim3((unsigned)(rows / (64 * R) + groups)), dim3(kThreads), 0, stream,
-                                   u);
+                const auto launch = [&](auto R_) {
+                    constexpr int R = decltype(R_)::value;
+                    hipLaunchKernelGGL((update_kernel<DT, RP, R>), dim3((unsigned)(rows / (64 * R) + groups)), dim3(kThreads), 0,
+                                       stream, u);
+                };
+                if constexpr (RP <= 32) {
+                    launch(std::integral_constant<int, 1>{});
+                } else {
+                    if constexpr (RP > 64) {
+                        if (rows / 64 + groups < 2 * cus) return launch(std::integral_constant<int, 1>{}), 0;
+                    }
+                    launch(std::integral_constant<int, 2>{});
+                }
                 return 0;
             }
             // out's columns are shared among as many workgroups, each with an h of its own, as take the least time: about

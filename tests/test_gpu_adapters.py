@@ -135,6 +135,8 @@ MANY = [
     ([0, 1], [20000, 13011], 33, 321, 77, 2),
     ([1, -1, 0], [15000, 30, 18001], 40, 5, 8, 2),
     ([0], [33001], 1, 1, 40, 1),
+    ([0, -1, 1], [9000, 100, 8009], 135, 203, 128, 2),
+    ([1, 0], [17, 17003], 63, 64, 65, 2),
     ([-1 if i % 99 == 0 else (7 * i) % 540 for i in range(540)], [(i * 13) % 50 for i in range(540)], 56, 100, 9, 540),
 ]
 
