@@ -154,6 +154,8 @@ inline int check(const char* what, int64_t rows, int32_t cols, int x_dtype, int 
     if (!is_float(x_dtype) || !is_float(y_dtype))
         return fail(NORI_ERR_UNSUPPORTED, "%s: unsupported dtypes %s and %s", what, dtype_name(x_dtype), dtype_name(y_dtype));
     if (rows < 0 || cols <= 0) return fail(NORI_ERR_INVALID, "%s: bad shape (%lld rows of %d)", what, (long long)rows, cols);
+    if (cols > NORI_LAYER_NORM_MAX)
+        return fail(NORI_ERR_UNSUPPORTED, "%s: rows of %d columns (up to %d)", what, cols, NORI_LAYER_NORM_MAX);
     if (xs < 0 || ys < 0) return fail(NORI_ERR_INVALID, "%s: negative row strides", what);
     return NORI_OK;
 }

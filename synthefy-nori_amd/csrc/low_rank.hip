@@ -928,6 +928,8 @@ int check(const char* what, int dtype, int64_t rows, int32_t groups, int32_t k, 
         return fail(NORI_ERR_INVALID, "%s: bad shape (%lld rows, %d -> %d, %d adapters)", what, (long long)rows, k, n, adapters);
     if (rank <= 0 || rank > NORI_LOW_RANK_MAX)
         return fail(rank <= 0 ? NORI_ERR_INVALID : NORI_ERR_UNSUPPORTED, "%s: rank %d (1 to %d)", what, rank, NORI_LOW_RANK_MAX);
+    if (k > NORI_LOW_RANK_COLUMNS || n > NORI_LOW_RANK_COLUMNS)  // offsets in one adapter's factors, and the grids, stay in range
+        return fail(NORI_ERR_UNSUPPORTED, "%s: %d -> %d columns (up to %d)", what, k, n, NORI_LOW_RANK_COLUMNS);
     if (rows > (int64_t)1 << 29) return fail(NORI_ERR_UNSUPPORTED, "%s: too many rows", what);
     if (groups > 65535) return fail(NORI_ERR_UNSUPPORTED, "%s: %d adapters in one call (65535 at most)", what, groups);
     return NORI_OK;

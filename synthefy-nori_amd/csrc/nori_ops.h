@@ -89,8 +89,9 @@ int64_t nori_dense_apply_scratch_bytes(int64_t tables, int64_t rows, int64_t gro
 int nori_dense_apply(const nori_dense_apply_args* args, void* stream);
 
 // LayerNorm that can be trained (layer_norm_train.hip): y = (x - mean) / sqrt(var + eps) * weight + bias over
-// rows of any width >= 1, x rows at x_row_stride elements, y rows contiguous; weight and bias (either may be
+// rows of 1 to NORI_LAYER_NORM_MAX columns, x rows at x_row_stride elements, y rows contiguous; weight and bias (either may be
 // NULL) contiguous of their own dtypes. mean and rstd [rows] fp32 keep the statistics, or both NULL.
+#define NORI_LAYER_NORM_MAX (1 << 30)
 int nori_layer_norm_train_forward(const void* x, int x_dtype, int64_t rows, int32_t cols, int64_t x_row_stride,
                                   const void* weight, int w_dtype, const void* bias, int b_dtype, float eps, void* y,
                                   int y_dtype, float* mean, float* rstd, void* stream);
@@ -111,8 +112,10 @@ int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_t rows, int
 // scales [adapters] fp32 or NULL for 1. order [rows] lists the rows of group 0, then of group 1, ...: group g is
 // order[starts[g] .. starts[g + 1]), its adapter ids[g] or -1, each id once. h [rows, rank] fp32, or NULL, takes
 // scales[id] x[i] a[id]^T (rows without an adapter are left). The workspace, of nori_low_rank_workspace_bytes and
-// 16-byte aligned, takes the factors in the matrix instructions' order (0 for few rows).
+// 16-byte aligned, takes the factors in the matrix instructions' order (0 for few rows). Ranks up to NORI_LOW_RANK_MAX, k
+// and n up to NORI_LOW_RANK_COLUMNS.
 #define NORI_LOW_RANK_MAX 128
+#define NORI_LOW_RANK_COLUMNS (1 << 20)
 int nori_low_rank_update(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* y,
                          int64_t y_row_stride, const void* a, const void* b, const float* scales, int32_t adapters,
                          int32_t rank, int32_t n, const int32_t* order, const int32_t* starts, const int32_t* ids,

@@ -25,6 +25,7 @@ from .norm import _FLOATS, _first_derivative, _rows_of, _strided_rows, trainable
 __all__ = ["AdapterPlan", "LowRankAdapters", "ReadoutAdapters", "adapted_linear", "low_rank_update"]
 
 MAX_RANK = 128  # NORI_LOW_RANK_MAX
+MAX_COLUMNS = 2**20  # NORI_LOW_RANK_COLUMNS
 
 
 class AdapterPlan:
@@ -199,6 +200,8 @@ def _check(x, y, a, b, plan, scales):
         raise ValueError(f"empty factors {tuple(a.shape)} and {tuple(b.shape)}")
     if rank > MAX_RANK:
         raise NotImplementedError(f"low_rank_update takes ranks up to {MAX_RANK}, got {rank}")
+    if max(k, n) > MAX_COLUMNS or adapters >= 2**31:
+        raise NotImplementedError(f"low_rank_update takes up to {MAX_COLUMNS} columns and 2^31 - 1 adapters, got {adapters} of {k} -> {n}")
     if x.dim() == 0 or int(x.shape[-1]) != k:
         raise ValueError(f"x {tuple(x.shape)} does not end in the factors' {k} inputs")
     if y is not None and tuple(y.shape) != (*x.shape[:-1], n):
@@ -260,7 +263,8 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
                     scales: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """``y + scales[id] (x a[id]^T) b[id]^T`` with ``id`` the adapter ``plan`` gives each row; rows without
     one take ``y``. x [..., in], y [..., out], a [adapters, rank, in], b [adapters, out, rank] of one
-    dtype (float32, float16 or bfloat16), ``scales`` float32 [adapters] or None for 1, rank up to 128.
+    dtype (float32, float16 or bfloat16), ``scales`` float32 [adapters] or None for 1, rank up to 128, in and
+    out up to 2^20.
 
     Products are summed in fp32, ``x a^T`` is kept in fp32, and the sum with y is rounded once.
     Differentiable in x, y, a and b (first derivatives; adapters no row takes get zeros). ``out``, in

@@ -359,6 +359,7 @@ def layer_norm(
 
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+MAX_TRAIN_WIDTH = 2**30  # NORI_LAYER_NORM_MAX
 
 
 def _rows_of(t: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
@@ -447,7 +448,7 @@ def trainable_layer_norm(
     eps: float = 1e-5,
     out_dtype: torch.dtype | None = None,
 ) -> torch.Tensor:
-    """``F.layer_norm`` over the last axis with its gradients: x [..., C] of any width C >= 1, ``weight``
+    """``F.layer_norm`` over the last axis with its gradients: x [..., C], 1 <= C <= 2^30, ``weight``
     and ``bias`` [C] or None, each of float32, float16 or bfloat16, the result in ``out_dtype``
     (default x's). Statistics, affine and the sums of the gradients are fp32, every result rounded once.
 
@@ -458,6 +459,8 @@ def trainable_layer_norm(
     cols = int(x.shape[-1]) if x.dim() else 0
     if cols == 0:
         raise ValueError(f"trainable_layer_norm needs rows of at least one element, got {tuple(x.shape)}")
+    if cols > MAX_TRAIN_WIDTH:
+        raise NotImplementedError(f"trainable_layer_norm takes rows of up to {MAX_TRAIN_WIDTH} elements, got {cols}")
     out_dtype = x.dtype if out_dtype is None else out_dtype
     for name, t in (("x", x), ("weight", weight), ("bias", bias)):
         if t is not None and t.dtype not in _FLOATS:

@@ -62,6 +62,15 @@ def test_updates_refuse_mismatched_arguments():
         call(x, y, torch.randn(2, 129, 8), torch.randn(2, 6, 129), plan)
     with pytest.raises(ValueError, match="empty"):
         call(x, y, torch.randn(2, 0, 8), torch.randn(2, 6, 0), plan)
+    wide = torch.zeros(1)
+    with pytest.raises(NotImplementedError, match="1048576 columns"):
+        call(wide.expand(5, 2**20 + 1), y, wide.expand(2, 4, 2**20 + 1), b, plan)
+    with pytest.raises(NotImplementedError, match="1048576 columns"):
+        call(x, wide.expand(5, 2**20 + 1), a, wide.expand(2, 2**20 + 1, 4), plan)
+    with pytest.raises(NotImplementedError, match="2147483648 of 8 -> 6"):
+        call(x, y, wide.expand(2**31, 4, 8), wide.expand(2**31, 6, 4), plan)
+    with pytest.raises(NotImplementedError, match="1073741824 elements"):
+        nori_amd.trainable_layer_norm(wide.expand(2, 2**32 + 8), None, None)
     with pytest.raises(TypeError, match="AdapterPlan"):
         call(x, y, a, b, [0])
     with pytest.raises(RuntimeError, match="ROCm GPU"):
@@ -107,6 +116,8 @@ def test_library_refuses_bad_arguments_before_any_device_work():
         bad = list(fw)
         bad[at] = value
         assert lib.nori_layer_norm_train_forward(*bad) == code, at
+    fw[3] = fw[4] = 2**30 + 1
+    assert lib.nori_layer_norm_train_forward(*fw) == nat.NORI_ERR_UNSUPPORTED
     bw = [16, nat.NORI_F16, 4, 10, 10, 16, nat.NORI_F16, 10, None, 0, 0, 16, 16, None, 16, None, None, 0, None]
     assert lib.nori_layer_norm_train_backward(*bw) == nat.NORI_ERR_INVALID  # dw without a workspace
     assert b"workspace" in lib.nori_last_error()
@@ -114,7 +125,8 @@ def test_library_refuses_bad_arguments_before_any_device_work():
     assert lib.nori_low_rank_update(*up) == nat.NORI_ERR_INVALID  # null pointers
     for at, value, code in ((1, nat.NORI_I8, nat.NORI_ERR_UNSUPPORTED), (11, 129, nat.NORI_ERR_UNSUPPORTED), (11, 0, nat.NORI_ERR_INVALID),
                             (3, 0, nat.NORI_ERR_INVALID), (2, 0, nat.NORI_OK), (2, 1 << 31, nat.NORI_ERR_UNSUPPORTED),
-                            (16, 65536, nat.NORI_ERR_UNSUPPORTED)):
+                            (16, 65536, nat.NORI_ERR_UNSUPPORTED), (3, 2**20 + 1, nat.NORI_ERR_UNSUPPORTED),
+                            (12, 2**20 + 1, nat.NORI_ERR_UNSUPPORTED)):
         bad = list(up)
         bad[at] = value
         assert lib.nori_low_rank_update(*bad) == code, at
