@@ -162,17 +162,22 @@ class _LowRankUpdate(torch.autograd.Function):
         return dx, (dout if need_y else None), da, db, None, None
 
 
+def _projected(x, weight, bias, a, b, plan, scales, keep):
+    """(F.linear(x, weight, bias), updated in place; h where it is to be kept, None else)."""
+    with torch.autocast("cuda", enabled=False):
+        y = F.linear(x, weight, bias)
+    if _strided_rows(y, int(y.shape[-1])) is None:
+        y = y.contiguous()
+    return y, _update(x, y, a, b, plan, scales, y, keep)
+
+
 class _AdaptedLinear(torch.autograd.Function):
     """A frozen projection and its low-rank update: the update's gradient of x is added in place to the
     projection's."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, a, b, plan, scales):
-        with torch.autocast("cuda", enabled=False):
-            y = F.linear(x, weight, bias)
-        if _strided_rows(y, int(y.shape[-1])) is None:
-            y = y.contiguous()
-        h = _update(x, y, a, b, plan, scales, y, True)
+        y, h = _projected(x, weight, bias, a, b, plan, scales, True)
         ctx.save_for_backward(x, weight, a, b, h, scales)
         ctx.plan = plan
         return y
@@ -311,7 +316,9 @@ def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     a, b, scales = _check(x, None, a, b, plan, scales)
     if tuple(weight.shape) != (b.shape[1], a.shape[2]):
         raise ValueError(f"the projection's weight {tuple(weight.shape)} does not match factors {tuple(a.shape)} and {tuple(b.shape)}")
-    return _AdaptedLinear.apply(x, weight, bias, a, b, plan, scales)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, a, b)):
+        return _AdaptedLinear.apply(x, weight, bias, a, b, plan, scales)
+    return _projected(x, weight, bias, a, b, plan, scales, False)[0]
 
 
 class LowRankAdapters(nn.Module):

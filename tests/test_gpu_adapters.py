@@ -400,6 +400,9 @@ def test_adapted_linear_and_its_gradients(frozen):
     host = {"x": s["x"], "a": s["a"], "b": s["b"], "weight": weight, "bias": bias}
     d = {n: t.to(DEV).requires_grad_(n in names) for n, t in host.items()}
     y = adapted_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], plan, s["scales"].to(DEV))
+    with torch.no_grad():
+        served = adapted_linear(d["x"], d["weight"], d["bias"], d["a"], d["b"], plan, s["scales"].to(DEV))
+    assert not served.requires_grad and torch.equal(served, y)
     got = torch.autograd.grad(y, [d[n] for n in names], s["dy"].to(DEV))
     e = {n: t.double().requires_grad_(True) for n, t in host.items()}
     want_y = _adapted_formula(e["x"], e["weight"], e["bias"], e["a"], e["b"], whose, s["scales"].double())
