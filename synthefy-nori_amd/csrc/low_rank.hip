@@ -222,7 +222,7 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
 // Many rows. A wavefront takes 16 R rows of one group through both products by itself; the four of a workgroup share
 // the factors' cache lines only. R is 1, or 2 for ranks above 32, where reading the factors costs more than the
 // registers and the LDS of twice the rows (65536 rows 1408 -> 1408 rank 64 fp16: 165 us with 1, 147 with 2; 560 -> 1680
-// rank 16: 132 and 173), unless compute units would stay idle (16384 rows 560 -> 1680 rank 128: 51 and 72).
+// rank 16: 132 and 173), unless that leaves too many compute units idle (short_round).
 // x, y and out pass through the wavefront's LDS between the order they lie in memory (8 lanes a run of 128 bytes) and
 // the operands' (a lane a row), and the packed factors are read as operands: every access takes the address units as few
 // cycles as its bytes do.
@@ -946,6 +946,16 @@ static bool few_rows(int64_t rows, int32_t groups, int32_t rank) {
     return rows / 64 + groups < (rank <= 64 ? 2 : 1) * device_cus() || rows <= (rank <= 32 ? 64 : 16) * (int64_t)groups;
 }
 
+// Whether tiles of 128 rows, of which a compute unit holds one, leave too many units idle: fewer tiles than units, or, at
+// ranks to 64, whose tiles of 64 rows take little more than half the time, a last round of less than half of them
+// (1408 -> 1408 rank 64 fp16, out, then dx, tiles of 64 rows against 128: 40000 rows 133 + 83 us and 133 + 103, 33000
+// 106 + 80 and 122 + 104, but 64000 159 + 133 and 144 + 126; 560 -> 1680 rank 128: 50000 216 + 140 and 167 + 106).
+static bool short_round(int64_t rows, int32_t groups, int ranks) {
+    const int cus = device_cus();
+    if (ranks > 64) return rows / 64 + groups < 2 * cus;
+    return rows / 128 < 3 * cus && (rows / 128 + cus - 1) % cus < cus / 2;
+}
+
 template <class Go>
 static int by_rank(int32_t rank, Go go) {
     if (rank <= 16) return go(std::integral_constant<int, 16>{});
@@ -991,10 +1001,9 @@ static void launch_update(Update u, int dtype, int64_t rows, bool transposed, vo
                 };
                 if constexpr (RP <= 32) {
                     launch(std::integral_constant<int, 1>{});
+                } else if (short_round(rows, groups, RP)) {
+                    launch(std::integral_constant<int, 1>{});
                 } else {
-                    if constexpr (RP > 64) {
-                        if (rows / 64 + groups < 2 * cus) return launch(std::integral_constant<int, 1>{}), 0;
-                    }
                     launch(std::integral_constant<int, 2>{});
                 }
                 return 0;

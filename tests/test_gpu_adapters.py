@@ -137,6 +137,9 @@ MANY = [
     ([0], [33001], 1, 1, 40, 1),
     ([0, -1, 1], [9000, 100, 8009], 135, 203, 128, 2),
     ([1, 0], [17, 17003], 63, 64, 65, 2),
+    ([0, -1, 1], [30000, 90, 28011], 136, 199, 64, 2),
+    ([1, 0], [50001, 7003], 71, 130, 50, 2),
+    ([0], [57001], 5, 3, 40, 1),
     ([-1 if i % 99 == 0 else (7 * i) % 540 for i in range(540)], [(i * 13) % 50 for i in range(540)], 56, 100, 9, 540),
 ]
 
