@@ -219,6 +219,26 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
         }
 }
 
+// A workgroup's LDS in update_kernel, sizes in elements.
+template <int DT, int RP, int R>
+struct UpdateLds {
+    using P = Packed<DT, RP>;
+    using E = typename Mma<DT>::elem;
+    static constexpr int PIECES = P::F32 ? 1 : 2, PITCH = RP + P::W;  // of a row of h
+    static constexpr int CB = P::KB;                                  // columns of a window: 128 bytes
+    static constexpr int RING = 2 * CB, OUT = RING + P::W + 4;        // a row of the result: two blocks, the first W columns again
+    static constexpr int XROW = P::KB + P::W;                         // a row of x
+    union Stage {
+        E x[2][16 * R][XROW];
+        float out[16 * R][OUT];
+    };
+    alignas(16) Stage stage[kWaves];
+    alignas(16) E hs[kWaves][PIECES][16 * R][PITCH];
+    float factor[kWaves][16 * R];
+    // workgroups that a compute unit's registers hold, where that is more than one or two
+    static constexpr int HELD = RP > 32 ? 0 : P::F32 ? 4 : 3;
+};
+
 // Many rows. A wavefront takes 16 R rows of one group through both products by itself; the four of a workgroup share
 // the factors' cache lines only. R is 1, or 2 for ranks above 32, where reading the factors costs more than the
 // registers and the LDS of twice the rows (65536 rows 1408 -> 1408 rank 64 fp16: 165 us with 1, 147 with 2; 560 -> 1680
@@ -231,24 +251,16 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
 // where rows are not whole lines (65536 rows of 1680 fp16, y to out alone: 136 us against 95, of 999: 65 against 45).
 // RP: the rank rounded up to 16, 32, 64 or 128.
 template <int DT, int RP, int R>
-__global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
+__global__ void __launch_bounds__(kThreads, RP <= 32 ? 3 : 1) update_kernel(const Update u) {
     using M = Mma<DT>;
     using P = Packed<DT, RP>;
     using E = typename M::elem;
     using F = typename M::frag;
+    using L = UpdateLds<DT, RP, R>;
     constexpr int W = M::W, RT = P::RT, KB = P::KB, KC = P::KC, PER = P::PER;
-    constexpr int PIECES = P::F32 ? 1 : 2, PITCH = RP + W;  // of a row of h in LDS, in elements
-    constexpr int CB = KB, NT = CB / 16;                    // columns of a window: 128 bytes
-    constexpr int RING = 2 * CB, OUT = RING + W + 4;        // a row of the result: two blocks, the first W columns again
-    constexpr int XROW = KB + W;                            // a row of x in LDS
-    constexpr int AHEAD = !P::F32 && RP == 16 ? 3 : 2;      // batches of x, windows of y asked for in advance
-    union Stage {
-        E x[2][16 * R][XROW];
-        float out[16 * R][OUT];
-    };
-    __shared__ __align__(16) Stage stage[kWaves];
-    __shared__ __align__(16) E hs[kWaves][PIECES][16 * R][PITCH];
-    __shared__ float factor[kWaves][16 * R];
+    constexpr int PIECES = L::PIECES, PITCH = L::PITCH, CB = L::CB, NT = CB / 16, RING = L::RING, OUT = L::OUT, XROW = L::XROW;
+    constexpr int AHEAD = !P::F32 && RP == 16 ? 3 : 2;  // batches of x, windows of y asked for in advance
+    __shared__ L lds;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4;
     int number;
@@ -289,12 +301,14 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
     const F* pb = reinterpret_cast<const F*>(u.pb) + group * P::second(u.n) + lane % P::LANES;
     F y[AHEAD][2 * R], bf[AHEAD][KC * NT];
     // Loads come back in the order they were asked for: a window's operands are asked for beside its y, or waiting for
-    // them would be waiting for every later y too.
-    auto ask = [&](int k, F (&f)[2 * R], F (&b)[KC * NT]) {
-        if (active && k < blocks) {
+    // them would be waiting for every later y too. The first windows' wait for h: beside A's they would take the registers
+    // of a third wavefront (40000 rows 1408 -> 1408 rank 32 fp16: 101 us so, 93 with three, 108 with them held).
+    auto ask_operands = [&](int k, F (&b)[KC * NT]) {
+        if (!active || k >= blocks) return;
 #pragma unroll
-            for (int q = 0; q < KC * NT; ++q) b[q] = pb[(int64_t)(k * NT * KC + q) * P::LANES];
-        }
+        for (int q = 0; q < KC * NT; ++q) b[q] = pb[(int64_t)(k * NT * KC + q) * P::LANES];
+    };
+    auto ask = [&](int k, F (&f)[2 * R]) {
         if (!u.y) return;
 #pragma unroll
         for (int i = 0; i < 2 * R; ++i) {
@@ -305,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
     for (int j = 0; j < AHEAD; ++j) {
 #pragma unroll
         for (int i = 0; i < 2 * R; ++i) y[j][i] = F{};
-        if (j < vector_windows) ask(j, y[j], bf[j]);
+        if (j < vector_windows) ask(j, y[j]);
     }
 
     constexpr int HF = P::HALF ? 1 : KC * PIECES;
@@ -345,7 +359,7 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
             for (int j = 0; j < AHEAD; ++j) {
                 const int i = i0 + j;
                 if (i >= batches) break;
-                E(&xs)[16 * R][XROW] = stage[wave].x[j & 1];
+                E(&xs)[16 * R][XROW] = lds.stage[wave].x[j & 1];
 #pragma unroll
                 for (int q = 0; q < 2 * R; ++q) *reinterpret_cast<F*>(&xs[8 * q + r0][lc]) = xf[j][q];
                 if (odd && i == batches - 1) {  // the elements behind the last whole vector
@@ -374,21 +388,24 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
         for (int r = 0; r < R; ++r) {
             const int p = first + 16 * r + m;
             float* keep = u.h && p < end ? u.h + (int64_t)u.order[min(p, end - 1)] * u.rank : nullptr;
-            put_h<DT, RT, 16 * R, PITCH, PIECES>(acc[r], u.scales ? u.scales[id] : 1.0f, u.rank, keep, g, 16 * r + m, hs[wave],
-                                                 factor[wave]);
+            put_h<DT, RT, 16 * R, PITCH, PIECES>(acc[r], u.scales ? u.scales[id] : 1.0f, u.rank, keep, g, 16 * r + m,
+                                                 lds.hs[wave], lds.factor[wave]);
         }
         wave_sync();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            f[r] = factor[wave][16 * r + m];
+            f[r] = lds.factor[wave][16 * r + m];
 #pragma unroll
             for (int q = 0; q < HF; ++q)
-                hf[r][q] = *reinterpret_cast<const F*>(&hs[wave][P::HALF ? g >> 1 : q % PIECES][16 * r + m][P::rank_of(q / PIECES, g)]);
+                hf[r][q] = *reinterpret_cast<const F*>(&lds.hs[wave][P::HALF ? g >> 1 : q % PIECES][16 * r + m][P::rank_of(q / PIECES, g)]);
         }
     }
 
     // ---- out = y + h B^T
-    float(&os)[16 * R][OUT] = stage[wave].out;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+        if (j < vector_windows) ask_operands(j, bf[j]);
+    float(&os)[16 * R][OUT] = lds.stage[wave].out;
     // block k of the result, into its half of the ring
     auto product = [&](int k, const F (&b)[KC * NT]) {
         const int half = k % 2 * CB;
@@ -422,7 +439,10 @@ __global__ void __launch_bounds__(kThreads) update_kernel(const Update u) {
             F o[2 * R];
 #pragma unroll
             for (int i = 0; i < 2 * R; ++i) o[i] = y[j][i];  // rows without an adapter keep y's bits
-            if (k + AHEAD < vector_windows) ask(k + AHEAD, y[j], bf[j]);
+            if (k + AHEAD < vector_windows) {
+                ask_operands(k + AHEAD, bf[j]);
+                ask(k + AHEAD, y[j]);
+            }
 #pragma unroll
             for (int i = 0; i < 2 * R; ++i) {
                 const int c = column(k, i);
@@ -937,23 +957,43 @@ int check(const char* what, int dtype, int64_t rows, int32_t groups, int32_t k, 
 
 }  // namespace
 
-// Whether tiles of 64 rows leave compute units idle, or are mostly empty. Packing the factors costs a launch, and 64 rows
-// an adapter read lower ranks' as fast where they lie (512 tables x 64 rows 256 -> 384 rank 16: 34 us packed, 25 not;
-// 65536 rows of 32 adapters 560 -> 1680: 119 and 160). Factors of more than 64 columns are worth packing from one tile
-// a compute unit on (4 tables x 4096 rows 560 -> 1680 bf16, out and h, then dx: rank 128 51 + 42 us packed, 113 + 56
-// not; 1408 -> 1408 rank 64 50 + 47 and 58 + 37).
+// Whether there are few tiles of 16 rows a compute unit, or tiles of 64 are mostly empty. Packing the factors costs a launch, and
+// 64 rows an adapter read lower ranks' as fast where they lie (512 tables x 64 rows 256 -> 384 rank 16: 34 us packed, 25
+// not; 65536 rows of 32 adapters 560 -> 1680: 119 and 160). The time of a tile is the latency of its passes over k and n,
+// which few rows' kernel shares among its wavefronts; the more ranks, the sooner reading the factors costs it more. Out,
+// then dx, in us, packed against not: 1408 -> 1408 rank 32 fp16 17000 rows 41 + 37 and 45 + 33, 24000 42 + 39 and
+// 62 + 40; rank 64 bf16 8000 44 + 42 and 41 + 32, 14000 44 + 42 and 58 + 38; 560 -> 1680 rank 128 fp16 4000 54 + 43
+// and 40 + 32, 11000 54 + 44 and 111 + 55.
 static bool few_rows(int64_t rows, int32_t groups, int32_t rank) {
-    return rows / 64 + groups < (rank <= 64 ? 2 : 1) * device_cus() || rows <= (rank <= 32 ? 64 : 16) * (int64_t)groups;
+    const int held = rank <= 32 ? 5 : rank <= 64 ? 3 : 2;
+    return rows / 16 + groups < held * device_cus() || rows <= (rank <= 32 ? 64 : 16) * (int64_t)groups;
 }
 
-// Whether tiles of 128 rows, of which a compute unit holds one, leave too many units idle: fewer tiles than units, or, at
-// ranks to 64, whose tiles of 64 rows take little more than half the time, a last round of less than half of them
-// (1408 -> 1408 rank 64 fp16, out, then dx, tiles of 64 rows against 128: 40000 rows 133 + 83 us and 133 + 103, 33000
-// 106 + 80 and 122 + 104, but 64000 159 + 133 and 144 + 126; 560 -> 1680 rank 128: 50000 216 + 140 and 167 + 106).
-static bool short_round(int64_t rows, int32_t groups, int ranks) {
+// Whether tiles of 128 rows, of which a compute unit holds one, leave too many units idle: while tiles of 64 rows fit the
+// units, two each to rank 64 and one above, and, to rank 64, where the last of few rounds is less than half full.
+// Out, then dx, in us, tiles of 64 rows against 128: 1408 -> 1408 rank 64, 20000 rows 53 + 50 and 59 + 56, 40000 133 + 83
+// and 133 + 103, but 64000 159 + 133 and 144 + 126; 560 -> 1680 rank 128, 14000 54 + 45 and 75 + 58, but 20000
+// 92 + 74 and 75 + 58.
+static bool short_round(int64_t rows, int ranks) {
     const int cus = device_cus();
-    if (ranks > 64) return rows / 64 + groups < 2 * cus;
-    return rows / 128 < 3 * cus && (rows / 128 + cus - 1) % cus < cus / 2;
+    if (ranks > 64) return rows / 64 <= cus;
+    return rows / 64 <= 2 * cus || (rows / 128 < 3 * cus && (rows / 128 + cus - 1) % cus < cus / 2);
+}
+
+// LDS that a workgroup of update_kernel asks for beside its own, so that a compute unit takes `c` of them at a time and not
+// all `held`: the c whose rounds, c as long each, end first. (16-bit types hold 3: 40000 rows 1408 -> 1408 rank 32 fp16,
+// out, then dx: 93 + 50 us with 3 and 101 + 62 with 2, one round or two; 65536: 135 + 109 and 124 + 97, two rounds each.)
+static unsigned unused_lds(int64_t tiles, int held, int own) {
+    const int64_t cus = device_cus();
+    int64_t least = 0;
+    int take = 0;
+    for (int c = 2; c <= held; ++c) {
+        const int64_t rounds = (tiles + c * cus - 1) / (c * cus);
+        if (!take || rounds * c <= least) least = rounds * c, take = c;
+        if (rounds == 1) break;  // no unit then takes more than its share (8 x 4096 352 -> 1408 rank 32: 47 us with 3, 42 with 2)
+    }
+    const int whole = take == held ? 0 : take == 2 ? 60 * 1024 : 52 * 1024;  // of 160 KB
+    return (unsigned)std::max(0, whole - own);
 }
 
 template <class Go>
@@ -996,12 +1036,13 @@ static void launch_update(Update u, int dtype, int64_t rows, bool transposed, vo
             if (!few) {
                 const auto launch = [&](auto R_) {
                     constexpr int R = decltype(R_)::value;
-                    hipLaunchKernelGGL((update_kernel<DT, RP, R>), dim3((unsigned)(rows / (64 * R) + groups)), dim3(kThreads), 0,
-                                       stream, u);
+                    const int64_t tiles = rows / (64 * R) + groups;
+                    hipLaunchKernelGGL((update_kernel<DT, RP, R>), dim3((unsigned)tiles), dim3(kThreads),
+                                       unused_lds(rows / (64 * R), UpdateLds<DT, RP, R>::HELD, sizeof(UpdateLds<DT, RP, R>)), stream, u);
                 };
                 if constexpr (RP <= 32) {
                     launch(std::integral_constant<int, 1>{});
-                } else if (short_round(rows, groups, RP)) {
+                } else if (short_round(rows, RP)) {
                     launch(std::integral_constant<int, 1>{});
                 } else {
                     launch(std::integral_constant<int, 2>{});

@@ -140,6 +140,10 @@ MANY = [
     ([0, -1, 1], [30000, 90, 28011], 136, 199, 64, 2),
     ([1, 0], [50001, 7003], 71, 130, 50, 2),
     ([0], [57001], 5, 3, 40, 1),
+    ([0, 1, -1], [20000, 13, 1007], 72, 139, 30, 2),
+    ([-1, 0, 1], [100, 22007, 28000], 64, 96, 12, 2),
+    ([0, -1, 1], [17000, 100, 4009], 135, 203, 128, 2),
+    ([1, 0], [13, 8500], 63, 264, 90, 2),
     ([-1 if i % 99 == 0 else (7 * i) % 540 for i in range(540)], [(i * 13) % 50 for i in range(540)], 56, 100, 9, 540),
 ]
 
