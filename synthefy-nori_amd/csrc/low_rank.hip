@@ -235,8 +235,10 @@ struct UpdateLds {
     alignas(16) Stage stage[kWaves];
     alignas(16) E hs[kWaves][PIECES][16 * R][PITCH];
     float factor[kWaves][16 * R];
-    // workgroups that a compute unit's registers hold, where that is more than one or two
+    // workgroups that a compute unit's registers hold, where that is more than one or two, and whether more are better where
+    // fewer would end as soon
     static constexpr int HELD = RP > 32 ? 0 : P::F32 ? 4 : 3;
+    static constexpr bool MORE = P::F32 || RP == 16;
 };
 
 // Many rows. A wavefront takes 16 R rows of one group through both products by itself; the four of a workgroup share
@@ -982,14 +984,16 @@ static bool short_round(int64_t rows, int ranks) {
 
 // LDS that a workgroup of update_kernel asks for beside its own, so that a compute unit takes `c` of them at a time and not
 // all `held`: the c whose rounds, c as long each, end first. (16-bit types hold 3: 40000 rows 1408 -> 1408 rank 32 fp16,
-// out, then dx: 93 + 50 us with 3 and 101 + 62 with 2, one round or two; 65536: 135 + 109 and 124 + 97, two rounds each.)
-static unsigned unused_lds(int64_t tiles, int held, int own) {
+// out, then dx: 93 + 50 us with 3 and 101 + 62 with 2, one round or two; 65536: 135 + 109 and 124 + 97, two rounds each.
+// Where two of 3 end with three of 2, 75000 rows 352 -> 999 rank 16: 91 + 48 and 93 + 51; fp32 560 -> 1680 rank 32: 324 + 227
+// and 347 + 228; rank 32 bf16, 89324 rows of 48 tables 1408 -> 999, a sixth of them not adapted: 149 and 142 forward.)
+static unsigned unused_lds(int64_t tiles, int held, bool more, int own) {
     const int64_t cus = device_cus();
     int64_t least = 0;
     int take = 0;
     for (int c = 2; c <= held; ++c) {
         const int64_t rounds = (tiles + c * cus - 1) / (c * cus);
-        if (!take || rounds * c <= least) least = rounds * c, take = c;
+        if (!take || rounds * c < least + more) least = rounds * c, take = c;
         if (rounds == 1) break;  // no unit then takes more than its share (8 x 4096 352 -> 1408 rank 32: 47 us with 3, 42 with 2)
     }
     const int whole = take == held ? 0 : take == 2 ? 60 * 1024 : 52 * 1024;  // of 160 KB
@@ -1036,9 +1040,10 @@ static void launch_update(Update u, int dtype, int64_t rows, bool transposed, vo
             if (!few) {
                 const auto launch = [&](auto R_) {
                     constexpr int R = decltype(R_)::value;
+                    using L = UpdateLds<DT, RP, R>;
                     const int64_t tiles = rows / (64 * R) + groups;
                     hipLaunchKernelGGL((update_kernel<DT, RP, R>), dim3((unsigned)tiles), dim3(kThreads),
-                                       unused_lds(rows / (64 * R), UpdateLds<DT, RP, R>::HELD, sizeof(UpdateLds<DT, RP, R>)), stream, u);
+                                       unused_lds(rows / (64 * R), L::HELD, L::MORE, sizeof(L)), stream, u);
                 };
                 if constexpr (RP <= 32) {
                     launch(std::integral_constant<int, 1>{});
