@@ -49,11 +49,11 @@ class AdapterPlan:
             raise ValueError("a table cannot have a negative number of rows")
         if (ids < -1).any():
             raise ValueError("adapters are numbered from 0; -1 is none")
-        self.device = torch.device(device)
-        if self.device.type != "cuda":
-            raise RuntimeError(f"nori_amd kernels run on a ROCm GPU; got a plan for {self.device}")
-        if self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError(f"nori_amd kernels run on a ROCm GPU; got a plan for {device}")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         self.rows = int(counts.sum())
         if self.rows > 2**29:
             raise NotImplementedError(f"a plan takes up to {2**29} rows, got {self.rows}")
@@ -64,9 +64,30 @@ class AdapterPlan:
         self.adapters = tuple(groups[groups >= 0].tolist())  # those with rows, ascending
         self.groups = len(groups)
         self.longest = int(np.diff(starts)[groups >= 0].max(initial=0))  # the most rows of one adapter
-        packed = torch.from_numpy(np.concatenate([starts, groups, order], dtype=np.int32, casting="unsafe")).to(self.device)
-        self.starts, self.ids, self.order = packed.split([self.groups + 1, self.groups, self.rows])
-        self.pointers = self.order.data_ptr(), self.starts.data_ptr(), self.ids.data_ptr()
+        self._packed = torch.from_numpy(np.concatenate([starts, groups, order], dtype=np.int32, casting="unsafe")).to(device)
+
+    # Taken from the tensor on each call: a copy of the plan, or one loaded elsewhere, has memory of its own.
+    @property
+    def device(self) -> torch.device:
+        return self._packed.device
+
+    @property
+    def starts(self) -> torch.Tensor:
+        return self._packed[: self.groups + 1]
+
+    @property
+    def ids(self) -> torch.Tensor:
+        return self._packed[self.groups + 1 : 2 * self.groups + 1]
+
+    @property
+    def order(self) -> torch.Tensor:
+        return self._packed[2 * self.groups + 1 :]
+
+    @property
+    def pointers(self) -> tuple[int, int, int]:
+        """Of ``order``, ``starts`` and ``ids``."""
+        at = self._packed.data_ptr()
+        return at + 4 * (2 * self.groups + 1), at, at + 4 * (self.groups + 1)
 
 
 def _whole_numbers(values) -> np.ndarray:
