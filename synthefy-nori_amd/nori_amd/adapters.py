@@ -20,7 +20,7 @@ import torch.nn.functional as F
 
 from . import _native as nat
 from .layer import _hooked
-from .norm import _FLOATS, _first_derivative, _rows_of, _strided_rows, trainable_layer_norm
+from .norm import _FLOATS, _first_derivative, _refuse_tangents, _rows_of, _strided_rows, trainable_layer_norm
 
 __all__ = ["AdapterPlan", "LowRankAdapters", "ReadoutAdapters", "adapted_linear", "low_rank_update"]
 
@@ -239,6 +239,7 @@ def _check(x, y, a, b, plan, scales):
             raise ValueError(f"low_rank_update: {name} is {t.dtype}, x {x.dtype}")
     if not isinstance(plan, AdapterPlan):
         raise TypeError(f"plan must be an AdapterPlan, got {type(plan).__name__}")
+    _refuse_tangents("low_rank_update", x, y, a, b, scales)
     device = nat.require_device(x, y, a, b, scales)
     if plan.device != device:
         raise RuntimeError(f"tensors on different devices: {device} and the plan's {plan.device}")
@@ -293,9 +294,10 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
     out up to 2^20.
 
     Products are summed in fp32, ``x a^T`` is kept in fp32, and the sum with y is rounded once.
-    Differentiable in x, y, a and b (first derivatives; adapters no row takes get zeros). ``out``, in
+    Differentiable in x, y, a and b (first derivatives, in reverse mode; adapters no row takes get zeros). ``out``, in
     inference, receives the result: a tensor of y's shape and dtype, y itself included, that shares no
     element with x."""
+    _refuse_tangents("low_rank_update", out)
     a, b, scales = _check(x, y, a, b, plan, scales)
     grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, y, a, b))
     if out is None:
@@ -333,6 +335,7 @@ def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     if trained:
         with torch.autocast("cuda", enabled=False):
             return low_rank_update(x, F.linear(x, weight, bias), a, b, plan, scales)
+    _refuse_tangents("adapted_linear", weight, bias)
     nat.require_device(x, weight, bias)
     a, b, scales = _check(x, None, a, b, plan, scales)
     if tuple(weight.shape) != (b.shape[1], a.shape[2]):

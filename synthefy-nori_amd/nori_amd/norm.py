@@ -7,6 +7,7 @@ import ctypes
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -418,6 +419,14 @@ def _train_backward(dy, x, weight, bias, stats, need_x, need_w, need_b):
     return dx, dw, db
 
 
+def _refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """A dual tensor does not ask for gradients: without this its tangent would be left out without a word."""
+    if forward_ad._current_level < 0:  # no level, no tangents: the usual case, asked without a call a tensor
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivatives")
+
+
 def _first_derivative(backward):
     """``once_differentiable``, without the time its checks take where no graph of the gradients is made."""
     guarded = torch.autograd.function.once_differentiable(backward)
@@ -452,7 +461,7 @@ def trainable_layer_norm(
     and ``bias`` [C] or None, each of float32, float16 or bfloat16, the result in ``out_dtype``
     (default x's). Statistics, affine and the sums of the gradients are fp32, every result rounded once.
 
-    Differentiable in x, weight and bias (first derivatives), the gradients in their inputs' dtypes; the
+    Differentiable in x, weight and bias (first derivatives, in reverse mode), the gradients in their inputs' dtypes; the
     affine gradients are summed in a fixed order, so the same inputs give the same bits. Rows at one
     stride are read as they lie, other layouts through a contiguous copy. ``layer_norm`` is the forward
     pass for inference (widths a multiple of 4, an optional ReLU), without gradients."""
@@ -472,6 +481,7 @@ def trainable_layer_norm(
             raise ValueError(f"trainable_layer_norm: {name} {tuple(t.shape)} does not match rows of {cols}")
     if not eps >= 0.0:
         raise ValueError(f"trainable_layer_norm: eps must be a non-negative number, got {eps}")
+    _refuse_tangents("trainable_layer_norm", x, weight, bias)
     nat.require_device(x, weight, bias)
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
