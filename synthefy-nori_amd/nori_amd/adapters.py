@@ -319,6 +319,8 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
         _update(x, y, a, b, plan, scales, whole, False)
         return out.copy_(whole)
     _update(x, y, a, b, plan, scales, out, False)
+    if not out.is_inference():  # (which have no versions)
+        torch.autograd.graph.increment_version(out)  # for graphs that saved it: the kernel wrote behind torch's back
     return out
 
 

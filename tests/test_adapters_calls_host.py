@@ -1,0 +1,59 @@
+"""What a call of the adapters does to torch's own records, with the kernels left out (CPU)."""
+import types
+
+import pytest
+import torch
+
+import nori_amd
+from nori_amd import _native as nat
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Calls of the library by name and arguments; each is a success of no effect."""
+    made = []
+
+    class Library:
+        def __getattr__(self, name):
+            def call(*args):
+                made.append((name, args))
+                return 0
+
+            return call
+
+    monkeypatch.setattr(nat, "require_device", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(nat, "stream_of", lambda device: 0)
+    monkeypatch.setattr(nat, "lib", lambda: library)
+    library = Library()
+    return made
+
+
+def _plan(rows):
+    plan = object.__new__(nori_amd.AdapterPlan)
+    plan._packed = torch.tensor([0, rows, 0, *range(rows)], dtype=torch.int32)
+    plan.rows, plan.most, plan.groups, plan.longest, plan.adapters = rows, 0, 1, rows, (0,)
+    return plan
+
+
+def _args(rows=5):
+    return types.SimpleNamespace(x=torch.randn(rows, 8), y=torch.randn(rows, 6), a=torch.randn(1, 4, 8), b=torch.randn(1, 6, 4))
+
+
+@pytest.mark.parametrize("place", ["y", "columns", "turned"])
+def test_out_is_seen_to_change(calls, place):
+    # another graph saved the tensor: its backward pass has to notice that the values are gone, as after torch's own calls
+    t = _args()
+    out = {"y": t.y, "columns": torch.randn(5, 9)[:, 2:8], "turned": torch.randn(6, 5).t()}[place]
+    w = torch.randn(5, 6, requires_grad=True)
+    loss = (w * out).sum()
+    with torch.no_grad():
+        nori_amd.low_rank_update(t.x, t.y, t.a, t.b, _plan(5), out=out)
+    assert any(name == "nori_low_rank_update" for name, _ in calls)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_out_in_inference_mode(calls):
+    with torch.inference_mode():
+        t = _args()
+        assert nori_amd.low_rank_update(t.x, t.y, t.a, t.b, _plan(5), out=t.y) is t.y
