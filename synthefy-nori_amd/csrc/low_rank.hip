@@ -179,9 +179,10 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Update u, int tran
 }
 
 // A lane's ranks of h, rank 16 t + 4 g + j of row m in acc[t][j], times s: kept in fp32 (`keep`, null: not), and put
-// into LDS as the second product takes them, in two pieces of the inputs' type, high and low, which keep 22 bits of a
-// row's largest element in fp16 (after a power of two that brings the row near 1, so that nothing leaves fp16's
-// range) and 16 in bf16; in fp32 h stays as it is. The result, rounded once, holds at most 11 and 8 bits.
+// into LDS as the second product takes them, in two pieces of the inputs' type, high and low, which keep an
+// element to 2^-22 of itself in fp16 and to 2^-16 in bf16; in fp32 h stays as it is. The result, rounded once, is kept to 2^-11 and 2^-8. fp16's
+// are taken after a power of two that brings the row's largest element to 2^14, the top of its range: what is lost below
+// its subnormal numbers is 2^-38 of that element, and a second product sums 2^15 2^16 128 at most.
 template <int DT, int RT, int ROWS, int PITCH, int PIECES>
 __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float* keep, int g, int row,
                                       typename Mma<DT>::elem (&hs)[PIECES][ROWS][PITCH], float (&factor)[ROWS]) {
@@ -201,8 +202,8 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
     if constexpr (DT == NORI_F16) {
         largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
         largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
-        // 2^e, the largest element's binade, and 2^-e; e within what both are normal for
-        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -120), 120);
+        // e: the largest element's binade less 14; within what 2^e and 2^-e are normal for
+        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -112), 127) - 14;
         up = __uint_as_float((uint32_t)(127 + e) << 23);
         down = __uint_as_float((uint32_t)(127 - e) << 23);
     }
@@ -676,8 +677,8 @@ __device__ __forceinline__ void store_grad(const Task& k, int rank, int dt, int 
 
 // h in the order that grad_kernel's instructions take it, 32 rows of a group a step: [step][tile of 16 ranks][lane],
 // a lane's 8 rows 8 g ... 8 g + 7 of rank 16 tile + m, zeros past the group's end. 16-bit: two pieces of the type, high
-// and low, as in the update, fp16's after a power of two that brings the step's largest element to 2^8 (exps[step]; no
-// piece then leaves fp16's range, the smallest bit kept is 2^-32 of the largest). fp32: as they are. Every chunk of
+// and low, as in the update, fp16's after a power of two that brings the step's largest element to 2^14 (exps[step]; no
+// piece then leaves fp16's range, the smallest bit kept is 2^-38 of the largest). fp32: as they are. Every chunk of
 // columns reads them, so they are made once (split in the sums themselves: 60 % of a wavefront's instructions).
 constexpr int kStep = 32;  // rows
 
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(const Grads q) {
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
-        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 8, -110), 110);
+        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127 - 14, -113), 113);
         down = __uint_as_float((uint32_t)(127 - e) << 23);
         if (lane == 0) k.exps[slot] = e;
     }
@@ -851,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, grad_held(RT)) grad_kernel(const Gra
                     }
                     scale = e;
                 } else if (e < scale) {
-                    // 2^(e - scale), in fp16: below 2^-24 nothing is left of them beside what the sums hold
+                    // 2^(e - scale), in fp16: of operands below 2^-38 of the largest so far nothing is left
                     const _Float16 f = (_Float16)__uint_as_float((uint32_t)max(127 + e - scale, 1) << 23);
 #pragma unroll
                     for (int r = 0; r < RT; ++r)
