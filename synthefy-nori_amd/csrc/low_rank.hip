@@ -61,6 +61,18 @@ __device__ __forceinline__ typename Mma<DT>::elem narrow(float v) {
     else return DT == NORI_F16 ? f32_to_f16(v) : f32_to_bf16(v);
 }
 
+// v as two numbers of a 16-bit type, high and low: v cut to the type's bits, and what that leaves, rounded (2^-22 of v in
+// fp16, 2^-16 in bf16). Both have v's sign, and low is zero only where v is: times an infinity each gives the infinity that v
+// gives. The smallest low that stands for zero is fp16's smallest number and bf16's smallest normal one.
+template <int DT>
+__device__ __forceinline__ void split(float v, uint16_t& high, uint16_t& low) {
+    if constexpr (DT == NORI_F16) high = __builtin_bit_cast(uint16_t, __builtin_amdgcn_cvt_pkrtz(v, 0.f)[0]);
+    else high = (uint16_t)(__float_as_uint(v) >> 16);
+    low = fabsf(v) < __builtin_inff() ? narrow<DT>(v - widen<DT>(high)) : high;
+    constexpr uint16_t kLeast = DT == NORI_F16 ? 0x0001 : 0x0080;
+    if (v != 0.f && (low & 0x7fff) < kLeast) low = (uint16_t)(kLeast | (__float_as_uint(v) >> 16 & 0x8000));
+}
+
 // W elements at p, at any alignment; of fewer than W (`there`), zeros behind them
 template <int DT>
 __device__ __forceinline__ typename Mma<DT>::frag fetch(const typename Mma<DT>::elem* p) {
@@ -186,7 +198,6 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Update u, int tran
 template <int DT, int RT, int ROWS, int PITCH, int PIECES>
 __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float* keep, int g, int row,
                                       typename Mma<DT>::elem (&hs)[PIECES][ROWS][PITCH], float (&factor)[ROWS]) {
-    using E = typename Mma<DT>::elem;
     float largest = 0.f;
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -213,10 +224,8 @@ __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float v = acc[t][j] * down;
-            const E high = narrow<DT>(v);
-            hs[0][row][16 * t + 4 * g + j] = high;
-            if constexpr (PIECES == 2)
-                hs[1][row][16 * t + 4 * g + j] = fabsf(v) < __builtin_inff() ? narrow<DT>(v - widen<DT>(high)) : E(0);
+            if constexpr (PIECES == 2) split<DT>(v, hs[0][row][16 * t + 4 * g + j], hs[1][row][16 * t + 4 * g + j]);
+            else hs[0][row][16 * t + 4 * g + j] = v;
         }
 }
 
@@ -741,9 +750,10 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(const Grads q) {
             u16x8 high, low;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float s = v[i] * down;
-                high[i] = narrow<DT>(s);
-                low[i] = fabsf(s) < __builtin_inff() ? narrow<DT>(s - widen<DT>(high[i])) : E(0);
+                E h, l;
+                split<DT>(v[i] * down, h, l);
+                high[i] = h;
+                low[i] = l;
             }
             u16x8* to = reinterpret_cast<u16x8*>(k.ops) + 2 * at;
             to[0] = high;
@@ -758,7 +768,7 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(const Grads q) {
 // The sum runs over rows, which t has apart. 16-bit: a lane reads 16 bytes of each of 8 rows and turns the 8 x 8
 // block in registers, so that it holds 8 rows of one column for each of 8 instructions; column i of a lane's
 // block belongs to instruction i. fp32: instruction i takes row 8 g + i of the lane groups g, no turning. fp16's sums
-// are kept at the largest power of two of the steps so far: a larger one rescales them, a smaller one its operands.
+// are kept at the largest power of two of the steps so far: a larger one rescales them, a smaller one its own sums.
 // Where a row ends inside a lane's columns, the lane takes the last ones instead and writes them again, the same
 // values. SHORT: rows of fewer columns than a lane takes.
 template <int DT, int RT, bool SHORT>
@@ -841,36 +851,41 @@ __global__ void __launch_bounds__(kThreads, grad_held(RT)) grad_kernel(const Gra
                     for (int c = 0; c < CT; ++c)
                         acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(now[i][c], hn[r][i / 4][i % 4], acc[r][c], 0, 0, 0);
         } else {
+            float step = 1.0f;  // of this step's sums
             if constexpr (DT == NORI_F16) {
-                if (e > scale) {  // the same in every lane
-                    const float change = __uint_as_float((uint32_t)max(127 + scale - e, 0) << 23);
+                // (the same in every lane; 2^-126 stands for less, beside a 2^-38 that the pieces leave out)
+                if (e > scale) {
                     if (scale > -1000) {
+                        const float change = __uint_as_float((uint32_t)max(127 + scale - e, 1) << 23);
 #pragma unroll
                         for (int r = 0; r < RT; ++r)
 #pragma unroll
                             for (int c = 0; c < CT; ++c) acc[r][c] = acc[r][c] * change;
                     }
                     scale = e;
-                } else if (e < scale) {
-                    // 2^(e - scale), in fp16: of operands below 2^-38 of the largest so far nothing is left
-                    const _Float16 f = (_Float16)__uint_as_float((uint32_t)max(127 + e - scale, 1) << 23);
-#pragma unroll
-                    for (int r = 0; r < RT; ++r)
-#pragma unroll
-                        for (int p = 0; p < 2; ++p) hn[r][p] = __builtin_bit_cast(F, __builtin_bit_cast(f16x8, hn[r][p]) * f);
                 }
+                step = __uint_as_float((uint32_t)max(127 + e - scale, 1) << 23);
             }
+            auto sum = [&](auto apart) {
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                F col;
+                for (int c = 0; c < CT; ++c) {
+                    F col;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) col[i] = now[i][c];
+                    for (int i = 0; i < 8; ++i) col[i] = now[i][c];
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    acc[r][c] = M::mul(col, hn[r][0], acc[r][c]);
-                    acc[r][c] = M::mul(col, hn[r][1], acc[r][c]);
+                    for (int r = 0; r < RT; ++r) {
+                        if constexpr (decltype(apart)::value) {
+                            const f32x4 d = M::mul(col, hn[r][1], M::mul(col, hn[r][0], f32x4{0.f, 0.f, 0.f, 0.f}));
+                            acc[r][c] = acc[r][c] + d * step;
+                        } else {
+                            acc[r][c] = M::mul(col, hn[r][0], acc[r][c]);
+                            acc[r][c] = M::mul(col, hn[r][1], acc[r][c]);
+                        }
+                    }
                 }
-            }
+            };
+            if (DT == NORI_F16 && step != 1.0f) sum(std::true_type{});
+            else sum(std::false_type{});
         }
     }
     // the wavefronts' sums, a rank tile at a time. acc[r][c][j] of lane (m, g): column c of operand row 4 g + j, rank 16 r + m

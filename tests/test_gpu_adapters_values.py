@@ -72,3 +72,64 @@ def test_small_beside_large_in_an_adapters_rows(rows, rank, dtype):
     _near(db[0, 0, 0], torch.tensor(half * 1.25 * 4.0, dtype=torch.float64), dtype)
     _near(db[0, 1, 0], (rows - half) * x[1, 1].double() * 2.0**-12, dtype, (rows - half) * 1.25 * 2.0**12)
     assert not bool(db[0, 2:].any()) and not bool(db[0, :, 1:].any())
+
+
+def _same_kind(got, want):
+    """Infinities and NaN where ``want`` (float64) has them."""
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isposinf(got), torch.isposinf(want)) and torch.equal(torch.isneginf(got), torch.isneginf(want))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,rank", SIZES)
+def test_infinities_come_out_as_the_formulas_have_them(rows, rank, dtype):
+    print(f"{rows} rows rank {rank} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(rows * 3 + rank)
+    inf = float("inf")
+    k, n = 24, 75
+    # eighths of small integers: sums are exact, and half of the x a^T are what the type holds in one piece
+    draw = lambda *s: torch.randint(-4, 5, s, generator=g).double() / 8  # noqa: E731
+    x, a, b, dy = draw(rows, k), draw(1, rank, k), draw(1, n, rank), draw(rows, n)
+    x[rows // 2, 3], x[0, 5], dy[rows // 3, 7] = inf, -inf, inf
+    b[0, 11, 0], b[0, 12, rank - 1], b[0, 74, rank // 2], b[0, 13] = inf, -inf, inf, 0.0
+    a[0, 1, 9] = inf
+    y = draw(rows, n)
+    d = [t.to(DEV, dtype) for t in (x, y, a, b)]
+    for i in (0, 2, 3):
+        d[i].requires_grad_(True)
+    plan = AdapterPlan([0], rows, device=DEV)
+    out = low_rank_update(*d, plan)
+    dx, da, db = torch.autograd.grad(out, (d[0], d[2], d[3]), dy.to(DEV, dtype))
+    h, gr = x @ a[0].T, dy @ b[0]
+    for got, want in ((out, y + h @ b[0].T), (dx, gr @ a[0]), (da[0], gr.T @ x), (db[0], dy.T @ h)):
+        _same_kind(got.detach(), want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,rank", SIZES)
+def test_one_infinite_factor(rows, rank, dtype):
+    # every other value finite: the infinity's column, and no other, is infinite, with the sign of x a^T and of dy b
+    print(f"{rows} rows rank {rank} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(rows * 5 + rank)
+    draw = lambda *s: (torch.randint(1, 9, s, generator=g) * (2 * torch.randint(0, 2, s, generator=g) - 1)).double() / 8  # noqa: E731
+    k, n = 24, 75
+    x, a, b, y = draw(rows, k), torch.zeros(1, rank, k).double(), draw(1, n, rank), draw(rows, n)
+    a[0, 0, 0], a[0, rank - 1, 1] = 1.0, 1.0  # x a^T: columns of x, exact in one piece
+    b[0, 40, rank - 1] = float("inf")
+    plan = AdapterPlan([0], rows, device=DEV)
+    out = low_rank_update(*(t.to(DEV, dtype) for t in (x, y, a, b)), plan).double().cpu()
+    assert torch.equal(torch.nonzero(~torch.isfinite(out)).unique(dim=0)[:, 1].unique(), torch.tensor([40]))
+    want = x[:, 1 if rank > 1 else 0].sign() * float("inf")
+    assert torch.equal(out[:, 40], want)
+    # in the gradients, an infinite value of one row
+    dy = draw(rows, n)
+    x[rows // 2, 0] = float("inf")
+    b[0, 40, rank - 1] = 1.0
+    d = [t.to(DEV, dtype) for t in (x, y, a, b)]
+    d[2].requires_grad_(True)
+    (da,) = torch.autograd.grad(low_rank_update(*d, plan), d[2], dy.to(DEV, dtype))
+    gr = dy[rows // 2] @ b[0]
+    some = gr != 0
+    assert torch.equal(da[0, some.to(DEV), 0].double().cpu(), gr[some].sign() * float("inf"))
+    assert bool(torch.isnan(da[0, ~some.to(DEV), 0]).all()) and bool(torch.isfinite(da[0, :, 1:]).all())
