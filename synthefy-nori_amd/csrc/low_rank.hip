@@ -672,6 +672,7 @@ struct Grads {
     const int32_t *order, *starts, *ids;
     int groups;
     int part;  // rows of one; a multiple of 128
+    int dt;    // of what is written: the inputs' type or fp32
 };
 
 // Where the partial sums of a group with several parts begin: 2 starts / part is enough for the ones before it,
@@ -906,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, grad_held(RT)) grad_kernel(const Gra
             for (int e = 0; e < 4; ++e) {
                 const int c = column(4 * g + e) + i;
                 if (j >= q.rank || (SHORT && (c >= k.cols || 4 * g + e > 0))) continue;
-                if (whole) store_grad(k, q.rank, DT, id, c, j, v[e]);
+                if (whole) store_grad(k, q.rank, q.dt, id, c, j, v[e]);
                 else part[(int64_t)c * q.rank + j] = v[e];
             }
         }
@@ -914,7 +915,7 @@ __global__ void __launch_bounds__(kThreads, grad_held(RT)) grad_kernel(const Gra
 }
 
 // the parts of the groups that have several, in their order; blocks0: workgroups of the first task
-__global__ void __launch_bounds__(kThreads) grad_join_kernel(const Grads q, int dt, int blocks0) {
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(const Grads q, int blocks0) {
     const bool second = (int)blockIdx.x >= blocks0;
     const Task& k = q.task[second];
     const int group = blockIdx.y, id = q.ids[group];
@@ -927,7 +928,7 @@ __global__ void __launch_bounds__(kThreads) grad_join_kernel(const Grads q, int 
     float v = 0.f;
 #pragma unroll 8
     for (int p = 0; p < parts; ++p) v += part[p * size];
-    store_grad(k, q.rank, dt, id, (int)(i / q.rank), (int)(i % q.rank), v);
+    store_grad(k, q.rank, q.dt, id, (int)(i / q.rank), (int)(i % q.rank), v);
 }
 
 int chunks_of(int cols, int dtype) { return (cols + (dtype == NORI_F32 ? 63 : 127)) / (dtype == NORI_F32 ? 64 : 128); }
@@ -1151,12 +1152,12 @@ extern "C" int64_t nori_low_rank_backward_workspace_bytes(int dtype, int64_t row
     return layout_of(dtype, rows, k, n, rank, groups, longest, need_x, need_a, need_b).end;
 }
 
-extern "C" int nori_low_rank_backward(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* dy,
-                                      int32_t n, int64_t dy_row_stride, const void* base, int64_t base_row_stride, const void* a,
-                                      const void* b, const float* scales, int32_t adapters, int32_t rank, const int32_t* order,
-                                      const int32_t* starts, const int32_t* ids, int32_t groups, int64_t longest, const float* h,
-                                      void* dx, int64_t dx_row_stride, void* da, void* db, void* workspace,
-                                      int64_t workspace_bytes, void* stream_v) {
+// grad_dtype: of da and db
+static int backward(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* dy, int32_t n,
+                    int64_t dy_row_stride, const void* base, int64_t base_row_stride, const void* a, const void* b,
+                    const float* scales, int32_t adapters, int32_t rank, const int32_t* order, const int32_t* starts,
+                    const int32_t* ids, int32_t groups, int64_t longest, const float* h, void* dx, int64_t dx_row_stride, void* da,
+                    void* db, int grad_dtype, void* workspace, int64_t workspace_bytes, void* stream_v) {
     clear_error();
     if (int rc = check("low_rank_backward", dtype, rows, groups, k, n, rank, adapters)) return rc;
     if (rows == 0 || (!dx && !da && !db)) return NORI_OK;
@@ -1189,6 +1190,7 @@ extern "C" int nori_low_rank_backward(const void* x, int dtype, int64_t rows, in
     q.ids = ids;
     q.groups = groups;
     q.part = l.part;
+    q.dt = grad_dtype;
     int tasks = 0;
     const int64_t exps = (operand_bytes(rows, groups, rank) + 255) / 256 * 256;
     auto task = [&](const void* t, const float* h, int64_t ops, int64_t ts, int cols, void* out, int64_t o_col, int64_t o_rank,
@@ -1236,8 +1238,27 @@ extern "C" int nori_low_rank_backward(const void* x, int dtype, int64_t rows, in
     if (longest > q.part) {
         const int blocks0 = (int)(((int64_t)q.task[0].cols * rank + kThreads - 1) / kThreads);
         const int blocks1 = (int)(((int64_t)q.task[1].cols * rank + kThreads - 1) / kThreads);
-        hipLaunchKernelGGL(grad_join_kernel, dim3((unsigned)(blocks0 + blocks1), groups), dim3(kThreads), 0, stream, q, dtype,
-                           blocks0);
+        hipLaunchKernelGGL(grad_join_kernel, dim3((unsigned)(blocks0 + blocks1), groups), dim3(kThreads), 0, stream, q, blocks0);
     }
     return launch_status("low_rank_backward");
+}
+
+extern "C" int nori_low_rank_backward(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* dy,
+                                      int32_t n, int64_t dy_row_stride, const void* base, int64_t base_row_stride, const void* a,
+                                      const void* b, const float* scales, int32_t adapters, int32_t rank, const int32_t* order,
+                                      const int32_t* starts, const int32_t* ids, int32_t groups, int64_t longest, const float* h,
+                                      void* dx, int64_t dx_row_stride, void* da, void* db, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+    return backward(x, dtype, rows, k, x_row_stride, dy, n, dy_row_stride, base, base_row_stride, a, b, scales, adapters, rank, order,
+                    starts, ids, groups, longest, h, dx, dx_row_stride, da, db, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int nori_low_rank_backward_f32(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* dy,
+                                          int32_t n, int64_t dy_row_stride, const void* base, int64_t base_row_stride,
+                                          const void* a, const void* b, const float* scales, int32_t adapters, int32_t rank,
+                                          const int32_t* order, const int32_t* starts, const int32_t* ids, int32_t groups,
+                                          int64_t longest, const float* h, void* dx, int64_t dx_row_stride, void* da, void* db,
+                                          void* workspace, int64_t workspace_bytes, void* stream) {
+    return backward(x, dtype, rows, k, x_row_stride, dy, n, dy_row_stride, base, base_row_stride, a, b, scales, adapters, rank, order,
+                    starts, ids, groups, longest, h, dx, dx_row_stride, da, db, NORI_F32, workspace, workspace_bytes, stream);
 }

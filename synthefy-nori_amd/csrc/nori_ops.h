@@ -10,7 +10,7 @@ extern "C" {
 #endif
 
 // Moves with every change of a signature or struct below; the package binds one version.
-#define NORI_OPS_VERSION 5
+#define NORI_OPS_VERSION 6
 int nori_ops_version(void);
 
 // QASS base scale of one key count (QASSMaxScaling.forward's base branch, src/synthefy_nori/model/
@@ -134,6 +134,12 @@ int nori_low_rank_backward(const void* x, int dtype, int64_t rows, int32_t k, in
                            const float* scales, int32_t adapters, int32_t rank, const int32_t* order, const int32_t* starts,
                            const int32_t* ids, int32_t groups, int64_t longest, const float* h, void* dx,
                            int64_t dx_row_stride, void* da, void* db, void* workspace, int64_t workspace_bytes, void* stream);
+// the same with da and db in fp32, for factors kept in fp32 beside 16-bit rows: their sums are not rounded
+int nori_low_rank_backward_f32(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* dy, int32_t n,
+                               int64_t dy_row_stride, const void* base, int64_t base_row_stride, const void* a, const void* b,
+                               const float* scales, int32_t adapters, int32_t rank, const int32_t* order, const int32_t* starts,
+                               const int32_t* ids, int32_t groups, int64_t longest, const float* h, void* dx,
+                               int64_t dx_row_stride, void* da, void* db, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t nori_low_rank_backward_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups,
                                                int64_t longest, int32_t need_x, int32_t need_a, int32_t need_b);
 

@@ -131,7 +131,7 @@ class DenseApplyArgs(ctypes.Structure):
 
 
 # The package's own entry points beyond the C ABI (csrc/nori_ops.h), and their version.
-OPS_VERSION = 5
+OPS_VERSION = 6
 OPS: dict[str, tuple[object, list]] = {
     "nori_qass_base": (ctypes.c_int, [_f32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
     "nori_linear_f16_w32": (
@@ -164,6 +164,11 @@ OPS: dict[str, tuple[object, list]] = {
     ),
     "nori_low_rank_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32]),
     "nori_low_rank_backward": (
+        ctypes.c_int,
+        [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i64, _vp, _vp,
+         _i64, _vp, _vp, _vp, _i64, _vp],
+    ),
+    "nori_low_rank_backward_f32": (
         ctypes.c_int,
         [_vp, _i32, _i64, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i64, _vp, _vp,
          _i64, _vp, _vp, _vp, _i64, _vp],

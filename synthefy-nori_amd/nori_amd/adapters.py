@@ -136,9 +136,9 @@ def _update(x, y, a, b, plan, scales, out, keep):
     return h
 
 
-def _gradients(dy, x, a, b, h, plan, scales, needs, base=None):
-    """(dx, da, db), None where not needed, by ``nori_low_rank_backward``; ``base`` [..., in] is what dx is
-    added to, and overwritten."""
+def _gradients(dy, x, a, b, h, plan, scales, needs, base=None, grad_dtype=None):
+    """(dx, da, db), None where not needed, by ``nori_low_rank_backward``, da and db of ``grad_dtype``, x's (the
+    default) or float32; ``base`` [..., in] is what dx is added to, and overwritten."""
     need_x, need_a, need_b = needs
     k, n, rank = int(x.shape[-1]), int(dy.shape[-1]), int(a.shape[1])
     device = x.device
@@ -146,16 +146,17 @@ def _gradients(dy, x, a, b, h, plan, scales, needs, base=None):
     dy2, _, ys = _rows_of(dy, n)
     dx = (torch.empty(x.shape, dtype=x.dtype, device=device) if base is None else base) if need_x else None
     make = torch.empty_like if len(plan.adapters) == a.shape[0] else torch.zeros_like  # adapters no row takes: zeros
-    da = make(a) if need_a else None
-    db = make(b) if need_b else None
+    da = make(a, dtype=grad_dtype) if need_a else None
+    db = make(b, dtype=grad_dtype) if need_b else None
     if rows and any(needs):
         lib, dtype = nat.lib(), nat.dtype_code(x.dtype)
         size = lib.nori_low_rank_backward_workspace_bytes(dtype, rows, k, n, rank, plan.groups, plan.longest, need_x, need_a,
                                                           need_b)
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        call = lib.nori_low_rank_backward if grad_dtype in (None, x.dtype) else lib.nori_low_rank_backward_f32
         with nat.on(device):
             nat.check(
-                lib.nori_low_rank_backward(
+                call(
                     x2.data_ptr(), dtype, rows, k, xs, dy2.data_ptr(), n, ys, nat.ptr(base), k, a.data_ptr(), b.data_ptr(),
                     nat.ptr(scales), int(a.shape[0]), rank, *plan.pointers, plan.groups, plan.longest, h.data_ptr(), nat.ptr(dx), k,
                     nat.ptr(da), nat.ptr(db), nat.ptr(workspace), size, nat.stream_of(device),
@@ -168,6 +169,7 @@ def _gradients(dy, x, a, b, h, plan, scales, needs, base=None):
 class _LowRankUpdate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, a, b, plan, scales):
+        ctx.grad_dtype, a, b = a.dtype, a.to(x.dtype), b.to(x.dtype)
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
         h = _update(x, y, a, b, plan, scales, out, True)
         ctx.save_for_backward(x, a, b, h, scales)
@@ -179,7 +181,7 @@ class _LowRankUpdate(torch.autograd.Function):
     def backward(ctx, dout):
         x, a, b, h, scales = ctx.saved_tensors
         need_x, need_y, need_a, need_b = ctx.needs_input_grad[:4]
-        dx, da, db = _gradients(dout, x, a, b, h, ctx.plan, scales, (need_x, need_a, need_b))
+        dx, da, db = _gradients(dout, x, a, b, h, ctx.plan, scales, (need_x, need_a, need_b), None, ctx.grad_dtype)
         return dx, (dout if need_y else None), da, db, None, None
 
 
@@ -198,6 +200,7 @@ class _AdaptedLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, a, b, plan, scales):
+        ctx.grad_dtype, a, b = a.dtype, a.to(x.dtype), b.to(x.dtype)
         y, h = _projected(x, weight, bias, a, b, plan, scales, True)
         ctx.save_for_backward(x, weight, a, b, h, scales)
         ctx.plan = plan
@@ -212,7 +215,7 @@ class _AdaptedLinear(torch.autograd.Function):
         if need_x:
             with torch.autocast("cuda", enabled=False):
                 base = torch.matmul(dy.reshape(-1, dy.shape[-1]), weight).view(x.shape)
-        dx, da, db = _gradients(dy, x, a, b, h, ctx.plan, scales, (need_x, need_a, need_b), base)
+        dx, da, db = _gradients(dy, x, a, b, h, ctx.plan, scales, (need_x, need_a, need_b), base, ctx.grad_dtype)
         return dx, None, None, da, db, None, None
 
 
@@ -234,9 +237,10 @@ def _check(x, y, a, b, plan, scales):
         raise ValueError(f"y {tuple(y.shape)} is not the projection of x {tuple(x.shape)} to {n}")
     if x.dtype not in _FLOATS:
         raise NotImplementedError(f"low_rank_update takes float32/float16/bfloat16, got {x.dtype}")
-    for name, t in (("y", y), ("a", a), ("b", b)):
-        if t is not None and t.dtype != x.dtype:
-            raise ValueError(f"low_rank_update: {name} is {t.dtype}, x {x.dtype}")
+    if y is not None and y.dtype != x.dtype:
+        raise ValueError(f"low_rank_update: y is {y.dtype}, x {x.dtype}")
+    if a.dtype != b.dtype or a.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"low_rank_update: a is {a.dtype}, b is {b.dtype}, x {x.dtype}")
     if not isinstance(plan, AdapterPlan):
         raise TypeError(f"plan must be an AdapterPlan, got {type(plan).__name__}")
     _refuse_tangents("low_rank_update", x, y, a, b, scales)
@@ -291,7 +295,8 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
     """``y + scales[id] (x a[id]^T) b[id]^T`` with ``id`` the adapter ``plan`` gives each row; rows without
     one take ``y``. x [..., in], y [..., out], a [adapters, rank, in], b [adapters, out, rank] of one
     dtype (float32, float16 or bfloat16), ``scales`` float32 [adapters] or None for 1, rank up to 128, in and
-    out up to 2^20.
+    out up to 2^20. a and b may be float32 beside 16-bit x and y: they are rounded to x's dtype, their gradients, summed
+    in fp32, are not.
 
     Products are summed in fp32, ``x a^T`` is kept in fp32, and the sum with y is rounded once.
     Differentiable in x, y, a and b (first derivatives, in reverse mode; adapters no row takes get zeros). ``out``, in
@@ -314,6 +319,7 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
         raise ValueError(f"out has strides {out.stride()}: its elements overlap")
     if plan.rows == 0:
         return out
+    a, b = a.to(x.dtype), b.to(x.dtype)
     if _strided_rows(out, int(out.shape[-1])) is None:
         whole = torch.empty(y.shape, dtype=y.dtype, device=y.device)
         _update(x, y, a, b, plan, scales, whole, False)
@@ -324,15 +330,23 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
     return out
 
 
+def _factors(a: torch.Tensor, b: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """a and b as ``low_rank_update`` takes them beside rows of ``dtype``: float32 ones as they are, so that their
+    gradients are not rounded on the way back."""
+    if a.dtype == b.dtype == torch.float32:
+        return a, b
+    return a.to(dtype), b.to(dtype)
+
+
 def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, a: torch.Tensor, b: torch.Tensor,
                    plan: AdapterPlan, scales: torch.Tensor | None = None) -> torch.Tensor:
     """``low_rank_update(x, F.linear(x, weight, bias), a, b, plan, scales)``, with x, the weights and the
-    factors in the autocast dtype where autocast is on (the factors in x's dtype elsewhere). A frozen
-    projection's output and x gradient are updated in place."""
+    factors in the autocast dtype where autocast is on (the factors in x's dtype elsewhere; float32 factors keep
+    float32 gradients). A frozen projection's output and x gradient are updated in place."""
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
         x, weight, bias = x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype)
-    a, b = a.to(x.dtype), b.to(x.dtype)
+    a, b = _factors(a, b, x.dtype)
     trained = torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad))
     if trained:
         with torch.autocast("cuda", enabled=False):
@@ -344,7 +358,7 @@ def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         raise ValueError(f"the projection's weight {tuple(weight.shape)} does not match factors {tuple(a.shape)} and {tuple(b.shape)}")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, a, b)):
         return _AdaptedLinear.apply(x, weight, bias, a, b, plan, scales)
-    return _projected(x, weight, bias, a, b, plan, scales, False)[0]
+    return _projected(x, weight, bias, a.to(x.dtype), b.to(x.dtype), plan, scales, False)[0]
 
 
 class LowRankAdapters(nn.Module):
@@ -366,7 +380,7 @@ class LowRankAdapters(nn.Module):
 
     def forward(self, x: torch.Tensor, y: torch.Tensor, plan: AdapterPlan) -> torch.Tensor:
         """``low_rank_update`` of y by these adapters, their factors in x's dtype."""
-        return low_rank_update(x, y, self.a.to(x.dtype), self.b.to(x.dtype), plan, self.scales)
+        return low_rank_update(x, y, *_factors(self.a, self.b, x.dtype), plan, self.scales)
 
     def linear(self, x: torch.Tensor, projection: nn.Linear, plan: AdapterPlan) -> torch.Tensor:
         """``adapted_linear`` of x by ``projection`` and these adapters; a projection that is hooked or of
