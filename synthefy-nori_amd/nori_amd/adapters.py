@@ -364,7 +364,7 @@ def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
 class LowRankAdapters(nn.Module):
     """The adapters of one projection: factors ``a`` [adapters, rank, in] (normal, fan-in scale) and ``b``
     [adapters, out, rank] (zeros: a new adapter changes nothing), and ``scales`` [adapters], alpha / rank
-    (alpha defaults to the rank)."""
+    (alpha defaults to the rank), float32 through casts of the module."""
 
     def __init__(self, adapters: int, in_features: int, out_features: int, rank: int, *, alpha: float | None = None,
                  device=None, dtype=None):
@@ -377,6 +377,13 @@ class LowRankAdapters(nn.Module):
         self.b = nn.Parameter(torch.zeros(adapters, out_features, rank, device=device, dtype=dtype))
         self.register_buffer("scales", torch.full((adapters,), (rank if alpha is None else alpha) / rank, device=device,
                                                   dtype=torch.float32))
+
+    def _apply(self, fn, recurse=True):
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != torch.float32:  # a cast of the module is the factors': the kernels take float32 scales
+            self.scales = scales.to(self.scales.device)
+        return self
 
     def forward(self, x: torch.Tensor, y: torch.Tensor, plan: AdapterPlan) -> torch.Tensor:
         """``low_rank_update`` of y by these adapters, their factors in x's dtype."""
