@@ -493,6 +493,7 @@ class FeaturesTransformer(nn.Module):
             raise ValueError("the two-phase encoder (Model v3) supports regression only; pass task_type='reg'")
         if calculate_sample_attention or calculate_feature_attention:
             raise NotImplementedError("attention-score diagnostics are not computed by the HIP attention path")
+        self._require_readout(readout_adapters, table_adapters, x.shape[0], return_embeddings)
         seq_len = x.shape[1]
         x_dict, n_pad = self._build_x_preprocess_inputs(x, eval_pos)
         pre = self.process_4_x(self.x_preprocess(x_dict))
@@ -529,14 +530,21 @@ class FeaturesTransformer(nn.Module):
                table_adapters: Sequence[int] | None = None) -> torch.Tensor:
         """The quantile bank of row states [B, rows, width] (``return_embeddings`` gives them), the decoder
         adapted to table i by adapter ``table_adapters[i]`` of ``readout_adapters`` (-1: not at all)."""
+        self._require_readout(readout_adapters, table_adapters, states.shape[0])
+        if readout_adapters is None:
+            return self.reg_y_decoder(states)
+        plan = AdapterPlan(table_adapters, states.shape[1], device=states.device)
+        return readout_adapters(self.reg_y_decoder, states, plan)
+
+    @staticmethod
+    def _require_readout(readout_adapters, table_adapters, tables: int, return_embeddings: bool = False) -> None:
         if readout_adapters is None:
             if table_adapters is not None:
                 raise ValueError("table_adapters without readout_adapters")
-            return self.reg_y_decoder(states)
-        if table_adapters is None or len(table_adapters) != states.shape[0]:
-            raise ValueError(f"readout_adapters need the adapter of each of the {states.shape[0]} tables")
-        plan = AdapterPlan(table_adapters, states.shape[1], device=states.device)
-        return readout_adapters(self.reg_y_decoder, states, plan)
+        elif table_adapters is None or len(table_adapters) != tables:
+            raise ValueError(f"readout_adapters need the adapter of each of the {tables} tables")
+        elif return_embeddings:
+            raise ValueError("return_embeddings gives the row states, which no readout_adapters decode; pass them to decode")
 
     def _require_context_cache(self) -> None:
         if self.two_phase_config is not None:
@@ -797,6 +805,7 @@ class FeaturesTransformer(nn.Module):
             raise NotImplementedError("apply_context_cache requires mask_prediction=False")
         if len(x_test.shape) != 3:
             raise AssertionError("x_test must be [Batch, seq, Feature]")
+        self._require_readout(readout_adapters, table_adapters, x_test.shape[0], return_embeddings)
         eval_pos = context.eval_pos
         n_test = x_test.shape[1]
         if n_test <= 0:

@@ -32,3 +32,28 @@ def test_scales_move_and_load_with_the_bank():
     assert bank.to("meta").first.scales.device.type == "meta" and bank.first.scales.dtype == torch.float32
     empty = nori_amd.LowRankAdapters(2, 8, 12, 3, device="meta").to_empty(device="cpu")
     assert empty.scales.device.type == "cpu" and empty.scales.dtype == torch.float32
+
+
+@pytest.fixture(scope="module")
+def models():
+    from nori_amd.api import NORI_6M_CONFIG, build_model
+
+    two_phase = dict(NORI_6M_CONFIG, nlayers=1, two_phase_config=dict(target_tokens=1, row_layers=1, row_heads=2, row_hidden_dim=64))
+    return build_model(dict(NORI_6M_CONFIG, nlayers=1)), build_model(two_phase)
+
+
+@pytest.mark.parametrize("ids,match", [([0, 1, -1], "return_embeddings gives the row states"), (None, "each of the 3 tables"),
+                                       ([0, 1], "each of the 3 tables")])
+def test_adapters_are_not_left_out_of_row_states(models, ids, match):
+    # row states are not decoded: adapters asked for beside them would do nothing; refused before the layers run
+    dense, two_phase = models
+    bank = nori_amd.ReadoutAdapters(dense.reg_y_decoder, 2, 4)
+    x, y = torch.randn(3, 10, 6), torch.randn(3, 8)
+    with pytest.raises(ValueError, match=match):
+        dense.apply_context_cache(x, None, return_embeddings=True, readout_adapters=bank, table_adapters=ids)
+    with pytest.raises(ValueError, match=match):
+        two_phase(x, y, 8, task_type="reg", return_embeddings=True, readout_adapters=bank, table_adapters=ids)
+    with pytest.raises(ValueError, match="without readout_adapters"):
+        dense.apply_context_cache(x, None, return_embeddings=True, table_adapters=[0, 0, 0])
+    with pytest.raises(ValueError, match="without readout_adapters"):
+        two_phase(x, y, 8, task_type="reg", return_embeddings=True, table_adapters=[0, 0, 0])
