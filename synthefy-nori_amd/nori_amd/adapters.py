@@ -54,7 +54,8 @@ class AdapterPlan:
             raise RuntimeError(f"nori_amd kernels run on a ROCm GPU; got a plan for {device}")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        self.rows = int(counts.sum())
+        longest = int(counts.max(initial=0))  # (a sum of longer ones may pass 64 bits)
+        self.rows = longest if longest > 2**29 else int(counts.sum())
         if self.rows > 2**29:
             raise NotImplementedError(f"a plan takes up to {2**29} rows, got {self.rows}")
         self.most = int(ids.max(initial=-1))  # an adapter bank has more than this many
@@ -94,6 +95,8 @@ def _whole_numbers(values) -> np.ndarray:
     values = np.asarray(values)
     if values.size and values.dtype.kind not in "iu":
         raise TypeError(f"whole numbers are wanted, got {values.dtype}")
+    if values.dtype == np.uint64:
+        values = np.minimum(values, np.uint64(2**63 - 1))  # stays out of range, where a cast would wrap to -1
     return values.astype(np.int64)
 
 

@@ -4,6 +4,7 @@ import copy
 import io
 import pickle
 
+import numpy as np
 import pytest
 import torch
 
@@ -42,3 +43,17 @@ def test_a_plan_is_where_its_rows_are(plan, monkeypatch):
     x, y, a, b = torch.randn(10, 8), torch.randn(10, 6), torch.randn(3, 4, 8), torch.randn(3, 6, 4)
     with pytest.raises(RuntimeError, match="different devices"):
         ad._check(x, y, a, b, plan, None)
+
+
+@pytest.mark.parametrize("ids,rows,error,match", [
+    ([0, 1], [2**62, 2**62], NotImplementedError, "rows"),  # whose sum passes 64 bits
+    ([0] * 3, 2**29, NotImplementedError, "rows"),
+    ([0], 2**63 - 1, NotImplementedError, "rows"),
+    (np.array([2**64 - 1], dtype=np.uint64), [1], ValueError, "out of range"),  # -1 where 64 bits wrap
+    ([0], np.array([2**64 - 3], dtype=np.uint64), NotImplementedError, "rows"),
+    ([2**63 - 1], [1], ValueError, "out of range"),
+    ([2**31 - 1], [0], ValueError, "out of range"),
+])
+def test_numbers_past_their_range_are_refused(ids, rows, error, match):
+    with pytest.raises(error, match=match):
+        nori_amd.AdapterPlan(ids, rows, device="cuda:0")
