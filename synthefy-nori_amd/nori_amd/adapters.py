@@ -17,6 +17,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules import module as _module_base
 
 from . import _native as nat
 from .layer import _hooked
@@ -341,6 +342,12 @@ def _factors(a: torch.Tensor, b: torch.Tensor, dtype: torch.dtype) -> tuple[torc
     return a.to(dtype), b.to(dtype)
 
 
+def _watched(module: nn.Module) -> bool:
+    """Whether a call of the module would run a hook, in its backward pass or forward."""
+    return bool(_hooked(module) or module._backward_hooks or module._backward_pre_hooks
+                or _module_base._global_backward_hooks or _module_base._global_backward_pre_hooks)
+
+
 def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, a: torch.Tensor, b: torch.Tensor,
                    plan: AdapterPlan, scales: torch.Tensor | None = None) -> torch.Tensor:
     """``low_rank_update(x, F.linear(x, weight, bias), a, b, plan, scales)``, with x, the weights and the
@@ -395,7 +402,7 @@ class LowRankAdapters(nn.Module):
     def linear(self, x: torch.Tensor, projection: nn.Linear, plan: AdapterPlan) -> torch.Tensor:
         """``adapted_linear`` of x by ``projection`` and these adapters; a projection that is hooked or of
         another class is called."""
-        if type(projection) is not nn.Linear or _hooked(projection):
+        if type(projection) is not nn.Linear or _watched(projection):
             y = projection(x)
             return self(x.to(y.dtype), y, plan)
         return adapted_linear(x, projection.weight, projection.bias, self.a, self.b, plan, self.scales)
@@ -429,7 +436,7 @@ class ReadoutAdapters(nn.Module):
         h = self.first.linear(states, first, plan)
         # under autocast torch's layer norm answers in float32; outside it in its input's dtype
         wide = torch.float32 if torch.is_autocast_enabled("cuda") else h.dtype
-        if type(norm) is not nn.LayerNorm or _hooked(norm):
+        if type(norm) is not nn.LayerNorm or _watched(norm):
             h = norm(h)
         else:
             h = trainable_layer_norm(h, norm.weight, norm.bias, norm.eps, out_dtype=wide)

@@ -57,3 +57,18 @@ def test_out_in_inference_mode(calls):
     with torch.inference_mode():
         t = _args()
         assert nori_amd.low_rank_update(t.x, t.y, t.a, t.b, _plan(5), out=t.y) is t.y
+
+
+def _decoder():
+    return torch.nn.Sequential(torch.nn.Linear(8, 12), torch.nn.LayerNorm(12), torch.nn.GELU(), torch.nn.Linear(12, 6))
+
+
+@pytest.mark.parametrize("watch", ["register_full_backward_hook", "register_full_backward_pre_hook", "register_forward_hook"])
+@pytest.mark.parametrize("part", [0, 1, 3])
+def test_watched_parts_of_a_decoder_are_called(calls, watch, part):
+    decoder = _decoder().requires_grad_(False)
+    bank = nori_amd.ReadoutAdapters(decoder, 1, 4)
+    seen = []
+    getattr(decoder[part], watch)(lambda m, *rest: seen.append(m))
+    bank(decoder, torch.randn(5, 8, requires_grad=True), _plan(5)).sum().backward()
+    assert seen == [decoder[part]]
