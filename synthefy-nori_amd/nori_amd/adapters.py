@@ -425,7 +425,8 @@ class ReadoutAdapters(nn.Module):
 
     @staticmethod
     def _parts(decoder: nn.Sequential) -> tuple[nn.Linear, nn.LayerNorm, nn.Module, nn.Linear]:
-        parts = tuple(decoder) if isinstance(decoder, nn.Sequential) else ()
+        whole = isinstance(decoder, nn.Sequential) and type(decoder).forward is nn.Sequential.forward
+        parts = tuple(decoder) if whole else ()
         if len(parts) != 4 or not (isinstance(parts[0], nn.Linear) and isinstance(parts[1], nn.LayerNorm)
                                    and isinstance(parts[3], nn.Linear)) or len(parts[1].normalized_shape) != 1:
             raise ValueError("ReadoutAdapters takes a decoder of Linear, LayerNorm, activation, Linear")
@@ -433,6 +434,8 @@ class ReadoutAdapters(nn.Module):
 
     def forward(self, decoder: nn.Sequential, states: torch.Tensor, plan: AdapterPlan) -> torch.Tensor:
         first, norm, activation, last = self._parts(decoder)
+        if decoder._forward_hooks or decoder._forward_pre_hooks or decoder._backward_hooks or decoder._backward_pre_hooks:
+            raise NotImplementedError("the decoder's parts are called one by one, which hooks of the whole would not see")
         h = self.first.linear(states, first, plan)
         # under autocast torch's layer norm answers in float32; outside it in its input's dtype
         wide = torch.float32 if torch.is_autocast_enabled("cuda") else h.dtype

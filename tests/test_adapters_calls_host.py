@@ -72,3 +72,33 @@ def test_watched_parts_of_a_decoder_are_called(calls, watch, part):
     getattr(decoder[part], watch)(lambda m, *rest: seen.append(m))
     bank(decoder, torch.randn(5, 8, requires_grad=True), _plan(5)).sum().backward()
     assert seen == [decoder[part]]
+
+
+@pytest.mark.parametrize("watch", ["register_full_backward_hook", "register_full_backward_pre_hook", "register_forward_hook",
+                                   "register_forward_pre_hook"])
+def test_watched_decoders_are_refused(calls, watch):
+    # the decoder's parts are called one by one: a hook of the whole would not see them
+    decoder = _decoder()
+    bank = nori_amd.ReadoutAdapters(decoder, 1, 4)
+    handle = getattr(decoder, watch)(lambda m, *rest: None)
+    with pytest.raises(NotImplementedError, match="hooks"):
+        bank(decoder, torch.randn(5, 8), _plan(5))
+    handle.remove()
+    assert bank(decoder, torch.randn(5, 8), _plan(5)).shape == (5, 6)
+
+
+def test_decoders_with_a_forward_of_their_own_are_refused(calls):
+    class Doubled(torch.nn.Sequential):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Named(torch.nn.Sequential):
+        pass
+
+    with pytest.raises(ValueError, match="decoder"):
+        nori_amd.ReadoutAdapters(Doubled(*_decoder()), 1, 4)
+    decoder = _decoder()
+    bank = nori_amd.ReadoutAdapters(decoder, 1, 4)
+    with pytest.raises(ValueError, match="decoder"):
+        bank(Doubled(*decoder), torch.randn(5, 8), _plan(5))
+    assert bank(Named(*decoder), torch.randn(5, 8), _plan(5)).shape == (5, 6)
