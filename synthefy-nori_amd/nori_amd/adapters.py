@@ -305,7 +305,7 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
     Products are summed in fp32, ``x a^T`` is kept in fp32, and the sum with y is rounded once.
     Differentiable in x, y, a and b (first derivatives, in reverse mode; adapters no row takes get zeros). ``out``, in
     inference, receives the result: a tensor of y's shape and dtype, y itself included, that shares no
-    element with x."""
+    element with x, the factors or the scales."""
     _refuse_tangents("low_rank_update", out)
     a, b, scales = _check(x, y, a, b, plan, scales)
     grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, y, a, b))
@@ -317,7 +317,8 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
         raise ValueError("out is for inference: an argument asks for gradients")
     elif tuple(out.shape) != tuple(y.shape) or out.dtype != y.dtype or out.device != y.device:
         raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not y's {tuple(y.shape)} {y.dtype}")
-    elif any(_overlap(out, t) for t in (x, a, b)) or (_overlap(out, y) and (out.data_ptr(), out.stride()) != (y.data_ptr(), y.stride())):
+    elif any(_overlap(out, t) for t in (x, a, b, scales) if t is not None) or (
+            _overlap(out, y) and (out.data_ptr(), out.stride()) != (y.data_ptr(), y.stride())):
         raise ValueError("out shares elements with an input")
     elif _overlaps_itself(out):
         raise ValueError(f"out has strides {out.stride()}: its elements overlap")

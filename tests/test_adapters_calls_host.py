@@ -102,3 +102,13 @@ def test_decoders_with_a_forward_of_their_own_are_refused(calls):
     with pytest.raises(ValueError, match="decoder"):
         bank(Doubled(*decoder), torch.randn(5, 8), _plan(5))
     assert bank(Named(*decoder), torch.randn(5, 8), _plan(5)).shape == (5, 6)
+
+
+def test_out_shares_nothing_with_scales(calls):
+    # the scales are read while out is written
+    t = _args()
+    memory = torch.randn(40)
+    y, scales = memory[:30].view(5, 6), memory[3:4]
+    with pytest.raises(ValueError, match="shares elements"):
+        nori_amd.low_rank_update(t.x, y, t.a, t.b, _plan(5), scales, out=y)
+    assert nori_amd.low_rank_update(t.x, y, t.a, t.b, _plan(5), memory[30:31], out=y) is y
