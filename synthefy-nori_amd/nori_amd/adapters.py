@@ -126,9 +126,9 @@ def _update(x, y, a, b, plan, scales, out, keep):
     device = x.device
     h = torch.empty((rows, rank), dtype=torch.float32, device=device) if keep else None
     lib, dtype = nat.lib(), nat.dtype_code(x.dtype)
-    size = lib.nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, plan.groups)
-    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     with nat.on(device):
+        size = lib.nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, plan.groups)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         nat.check(
             lib.nori_low_rank_update(
                 x.data_ptr(), dtype, rows, k, xs, y.data_ptr(), ys, a.data_ptr(), b.data_ptr(), nat.ptr(scales), int(a.shape[0]),
@@ -154,11 +154,11 @@ def _gradients(dy, x, a, b, h, plan, scales, needs, base=None, grad_dtype=None):
     db = make(b, dtype=grad_dtype) if need_b else None
     if rows and any(needs):
         lib, dtype = nat.lib(), nat.dtype_code(x.dtype)
-        size = lib.nori_low_rank_backward_workspace_bytes(dtype, rows, k, n, rank, plan.groups, plan.longest, need_x, need_a,
-                                                          need_b)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         call = lib.nori_low_rank_backward if grad_dtype in (None, x.dtype) else lib.nori_low_rank_backward_f32
         with nat.on(device):
+            size = lib.nori_low_rank_backward_workspace_bytes(dtype, rows, k, n, rank, plan.groups, plan.longest, need_x, need_a,
+                                                              need_b)
+            workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
             nat.check(
                 call(
                     x2.data_ptr(), dtype, rows, k, xs, dy2.data_ptr(), n, ys, nat.ptr(base), k, a.data_ptr(), b.data_ptr(),

@@ -112,3 +112,36 @@ def test_out_shares_nothing_with_scales(calls):
     with pytest.raises(ValueError, match="shares elements"):
         nori_amd.low_rank_update(t.x, y, t.a, t.b, _plan(5), scales, out=y)
     assert nori_amd.low_rank_update(t.x, y, t.a, t.b, _plan(5), memory[30:31], out=y) is y
+
+
+def test_sizes_are_asked_for_on_the_tensors_device(calls, monkeypatch):
+    # workspaces go by the compute units of the current device, as the launch does: both have to be asked in its context
+    import contextlib
+
+    inside, asked = [], []
+
+    @contextlib.contextmanager
+    def on(device):
+        inside.append(device)
+        yield
+        inside.pop()
+
+    class Library:
+        def __getattr__(self, name):
+            def call(*args):
+                asked.append((name, bool(inside)))
+                return 0
+
+            return call
+
+    monkeypatch.setattr(nat, "on", on)
+    monkeypatch.setattr(nat, "lib", Library)
+    t = _args()
+    for leaf in (t.x, t.a, t.b):
+        leaf.requires_grad_(True)
+    nori_amd.low_rank_update(t.x, t.y, t.a, t.b, _plan(5)).sum().backward()
+    x = torch.randn(5, 8, requires_grad=True)
+    nori_amd.trainable_layer_norm(x, torch.ones(8, requires_grad=True), None).sum().backward()
+    names = [n for n, _ in asked if n.startswith("nori_low_rank") or n.startswith("nori_layer_norm")]
+    assert {"nori_low_rank_workspace_bytes", "nori_low_rank_backward_workspace_bytes", "nori_layer_norm_train_workspace_bytes"} <= set(names)
+    assert all(ok for n, ok in asked if n in names), asked
