@@ -67,6 +67,17 @@ class AdapterPlan:
         self.groups = len(groups)
         self.longest = int(np.diff(starts)[groups >= 0].max(initial=0))  # the most rows of one adapter
         self._packed = torch.from_numpy(np.concatenate([starts, groups, order], dtype=np.int32, casting="unsafe")).to(device)
+        self._streams: set[int] = set()
+
+    def used_on(self, stream: int) -> None:
+        """Keeps the plan's memory, once the plan is gone, from what other streams do before ``stream``, the device's
+        current one, is through with it: no caller has the tensor to tell the allocator so."""
+        if stream not in self._streams:
+            self._packed.record_stream(torch.cuda.current_stream(self.device))
+            self._streams.add(stream)
+
+    def __getstate__(self):
+        return {**self.__dict__, "_streams": set()}  # a copy's memory is its own
 
     # Taken from the tensor on each call: a copy of the plan, or one loaded elsewhere, has memory of its own.
     @property
@@ -129,11 +140,13 @@ def _update(x, y, a, b, plan, scales, out, keep):
     with nat.on(device):
         size = lib.nori_low_rank_workspace_bytes(dtype, rows, k, n, rank, plan.groups)
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        stream = nat.stream_of(device)
+        plan.used_on(stream)
         nat.check(
             lib.nori_low_rank_update(
                 x.data_ptr(), dtype, rows, k, xs, y.data_ptr(), ys, a.data_ptr(), b.data_ptr(), nat.ptr(scales), int(a.shape[0]),
                 rank, n, *plan.pointers, plan.groups, out.data_ptr(), layout[1], nat.ptr(h), nat.ptr(workspace), size,
-                nat.stream_of(device),
+                stream,
             ),
             "low_rank_update",
         )
@@ -159,21 +172,27 @@ def _gradients(dy, x, a, b, h, plan, scales, needs, base=None, grad_dtype=None):
             size = lib.nori_low_rank_backward_workspace_bytes(dtype, rows, k, n, rank, plan.groups, plan.longest, need_x, need_a,
                                                               need_b)
             workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+            stream = nat.stream_of(device)
+            plan.used_on(stream)
             nat.check(
                 call(
                     x2.data_ptr(), dtype, rows, k, xs, dy2.data_ptr(), n, ys, nat.ptr(base), k, a.data_ptr(), b.data_ptr(),
                     nat.ptr(scales), int(a.shape[0]), rank, *plan.pointers, plan.groups, plan.longest, h.data_ptr(), nat.ptr(dx), k,
-                    nat.ptr(da), nat.ptr(db), nat.ptr(workspace), size, nat.stream_of(device),
+                    nat.ptr(da), nat.ptr(db), nat.ptr(workspace), size, stream,
                 ),
                 "low_rank_update backward",
             )
     return dx, da, db
 
 
+def _cast(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return t if t.dtype == dtype else t.to(dtype)
+
+
 class _LowRankUpdate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, a, b, plan, scales):
-        ctx.grad_dtype, a, b = a.dtype, a.to(x.dtype), b.to(x.dtype)
+        ctx.grad_dtype, a, b = a.dtype, _cast(a, x.dtype), _cast(b, x.dtype)
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
         h = _update(x, y, a, b, plan, scales, out, True)
         ctx.save_for_backward(x, a, b, h, scales)
@@ -204,7 +223,7 @@ class _AdaptedLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, a, b, plan, scales):
-        ctx.grad_dtype, a, b = a.dtype, a.to(x.dtype), b.to(x.dtype)
+        ctx.grad_dtype, a, b = a.dtype, _cast(a, x.dtype), _cast(b, x.dtype)
         y, h = _projected(x, weight, bias, a, b, plan, scales, True)
         ctx.save_for_backward(x, weight, a, b, h, scales)
         ctx.plan = plan
@@ -309,7 +328,8 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
     _refuse_tangents("low_rank_update", out)
     a, b, scales = _check(x, y, a, b, plan, scales)
     grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, y, a, b))
-    if out is None:
+    given = out is not None
+    if not given:
         if grad:
             return _LowRankUpdate.apply(x, y, a, b, plan, scales)
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
@@ -324,13 +344,13 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
         raise ValueError(f"out has strides {out.stride()}: its elements overlap")
     if plan.rows == 0:
         return out
-    a, b = a.to(x.dtype), b.to(x.dtype)
+    a, b = _cast(a, x.dtype), _cast(b, x.dtype)
     if _strided_rows(out, int(out.shape[-1])) is None:
         whole = torch.empty(y.shape, dtype=y.dtype, device=y.device)
         _update(x, y, a, b, plan, scales, whole, False)
         return out.copy_(whole)
     _update(x, y, a, b, plan, scales, out, False)
-    if not out.is_inference():  # (which have no versions)
+    if given and not out.is_inference():  # (which have no versions)
         torch.autograd.graph.increment_version(out)  # for graphs that saved it: the kernel wrote behind torch's back
     return out
 
@@ -369,7 +389,7 @@ def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         raise ValueError(f"the projection's weight {tuple(weight.shape)} does not match factors {tuple(a.shape)} and {tuple(b.shape)}")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, a, b)):
         return _AdaptedLinear.apply(x, weight, bias, a, b, plan, scales)
-    return _projected(x, weight, bias, a.to(x.dtype), b.to(x.dtype), plan, scales, False)[0]
+    return _projected(x, weight, bias, _cast(a, x.dtype), _cast(b, x.dtype), plan, scales, False)[0]
 
 
 class LowRankAdapters(nn.Module):

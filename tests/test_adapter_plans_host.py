@@ -57,3 +57,15 @@ def test_a_plan_is_where_its_rows_are(plan, monkeypatch):
 def test_numbers_past_their_range_are_refused(ids, rows, error, match):
     with pytest.raises(error, match=match):
         nori_amd.AdapterPlan(ids, rows, device="cuda:0")
+
+
+def test_a_stream_is_recorded_once(plan, monkeypatch):
+    recorded = []
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: "stream")
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, stream: recorded.append((self.data_ptr(), stream)))
+    for stream in (7, 0, 7, 0):
+        plan.used_on(stream)
+    assert recorded == [(plan.starts.data_ptr(), "stream")] * 2
+    other = copy.deepcopy(plan)
+    other.used_on(7)
+    assert recorded[2:] == [(other.starts.data_ptr(), "stream")]

@@ -24,6 +24,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(nat, "require_device", lambda *t: torch.device("cpu"))
     monkeypatch.setattr(nat, "stream_of", lambda device: 0)
     monkeypatch.setattr(nat, "lib", lambda: library)
+    monkeypatch.setattr(nori_amd.AdapterPlan, "used_on", lambda plan, stream: made.append(("used_on", (plan, stream))), raising=False)
     library = Library()
     return made
 
@@ -145,3 +146,13 @@ def test_sizes_are_asked_for_on_the_tensors_device(calls, monkeypatch):
     names = [n for n, _ in asked if n.startswith("nori_low_rank") or n.startswith("nori_layer_norm")]
     assert {"nori_low_rank_workspace_bytes", "nori_low_rank_backward_workspace_bytes", "nori_layer_norm_train_workspace_bytes"} <= set(names)
     assert all(ok for n, ok in asked if n in names), asked
+
+
+def test_plans_are_told_of_the_streams_that_read_them(calls):
+    t = _args()
+    plan = _plan(5)
+    x = t.x.requires_grad_(True)
+    nori_amd.low_rank_update(x, t.y, t.a, t.b, plan).sum().backward()
+    at = [i for i, (name, _) in enumerate(calls) if name == "used_on"]
+    assert [calls[i + 1][0] for i in at] == ["nori_low_rank_update", "nori_low_rank_backward"]  # just before each launch
+    assert all(calls[i][1][0] is plan for i in at)

@@ -29,3 +29,24 @@ def test_copies_of_a_plan_outlive_it():
     for other in copies:
         assert other.device == DEV and torch.equal(low_rank_update(x, y, a, b, other), want)
     assert len(taken) == 8
+
+
+def test_a_plan_may_go_while_another_stream_still_reads_it():
+    # made on one stream, used on another behind other work, and dropped at once: its memory is not handed out meanwhile
+    x, y, a, b = _make(4000, 24, 40, 4, 2)
+    ids = [1, 0, -1, 1]
+    want = low_rank_update(x, y, a, b, AdapterPlan(ids, 1000, device=DEV))
+    side = torch.cuda.Stream(DEV)
+    busy = torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    plan = AdapterPlan(ids, 1000, device=DEV)
+    at, size = plan._packed.data_ptr(), plan._packed.numel()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy = busy @ busy * 1e-4
+        got = low_rank_update(x, y, a, b, plan)
+    del plan
+    taken = [torch.zeros(size, dtype=torch.int32, device=DEV) for _ in range(4)]
+    assert all(t.data_ptr() != at for t in taken)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
