@@ -1134,7 +1134,7 @@ Layout layout_of(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, in
     Layout l;
     l.part = part_of(rows, longest, groups, (need_a ? chunks_of(k, dtype) : 0) + (need_b ? chunks_of(n, dtype) : 0), rank);
     const bool parts = longest > l.part;
-    l.packed = up(need_x || need_a ? rows * rank * 4 : 0);
+    l.packed = up(need_a ? rows * rank * 4 : 0);
     l.ops_a = l.packed + up(need_x || need_a ? packed_bytes(dtype, rows, n, k, rank, groups, true) : 0);
     const int64_t ops = up(operand_bytes(rows, groups, rank)) + up((rows / kStep + groups) * 4);
     l.ops_b = l.ops_a + (need_a ? ops : 0);
@@ -1161,7 +1161,7 @@ static int backward(const void* x, int dtype, int64_t rows, int32_t k, int64_t x
     clear_error();
     if (int rc = check("low_rank_backward", dtype, rows, groups, k, n, rank, adapters)) return rc;
     if (rows == 0 || (!dx && !da && !db)) return NORI_OK;
-    if (!x || !dy || !a || !b || !order || !starts || !ids || !h || groups <= 0)
+    if (!x || !dy || !a || !b || !order || !starts || !ids || (db && !h) || groups <= 0)
         return fail(NORI_ERR_INVALID, "low_rank_backward: null pointer");
     if (dx && dx_row_stride < k && rows > 1) return fail(NORI_ERR_INVALID, "low_rank_backward: rows of dx overlap");
     if (dx && dx == base && dx_row_stride != base_row_stride && rows > 1)

@@ -177,7 +177,7 @@ def _gradients(dy, x, a, b, h, plan, scales, needs, base=None, grad_dtype=None):
             nat.check(
                 call(
                     x2.data_ptr(), dtype, rows, k, xs, dy2.data_ptr(), n, ys, nat.ptr(base), k, a.data_ptr(), b.data_ptr(),
-                    nat.ptr(scales), int(a.shape[0]), rank, *plan.pointers, plan.groups, plan.longest, h.data_ptr(), nat.ptr(dx), k,
+                    nat.ptr(scales), int(a.shape[0]), rank, *plan.pointers, plan.groups, plan.longest, nat.ptr(h), nat.ptr(dx), k,
                     nat.ptr(da), nat.ptr(db), nat.ptr(workspace), size, stream,
                 ),
                 "low_rank_update backward",
@@ -194,7 +194,7 @@ class _LowRankUpdate(torch.autograd.Function):
     def forward(ctx, x, y, a, b, plan, scales):
         ctx.grad_dtype, a, b = a.dtype, _cast(a, x.dtype), _cast(b, x.dtype)
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-        h = _update(x, y, a, b, plan, scales, out, True)
+        h = _update(x, y, a, b, plan, scales, out, ctx.needs_input_grad[3])  # b's gradient alone reads it
         ctx.save_for_backward(x, a, b, h, scales)
         ctx.plan = plan
         return out
@@ -224,7 +224,7 @@ class _AdaptedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, a, b, plan, scales):
         ctx.grad_dtype, a, b = a.dtype, _cast(a, x.dtype), _cast(b, x.dtype)
-        y, h = _projected(x, weight, bias, a, b, plan, scales, True)
+        y, h = _projected(x, weight, bias, a, b, plan, scales, ctx.needs_input_grad[4])
         ctx.save_for_backward(x, weight, a, b, h, scales)
         ctx.plan = plan
         return y

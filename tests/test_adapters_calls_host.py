@@ -156,3 +156,32 @@ def test_plans_are_told_of_the_streams_that_read_them(calls):
     at = [i for i, (name, _) in enumerate(calls) if name == "used_on"]
     assert [calls[i + 1][0] for i in at] == ["nori_low_rank_update", "nori_low_rank_backward"]  # just before each launch
     assert all(calls[i][1][0] is plan for i in at)
+
+
+@pytest.mark.parametrize("leaf", ["x", "y", "a", "b"])
+@pytest.mark.parametrize("frozen", [True, False])
+def test_x_times_a_is_kept_for_b_alone(calls, leaf, frozen):
+    # no other gradient reads it
+    t = _args()
+    getattr(t, leaf).requires_grad_(True)
+    if frozen:
+        if leaf == "y":
+            return
+        out = nori_amd.adapted_linear(t.x, torch.randn(6, 8), None, t.a, t.b, _plan(5))
+    else:
+        out = nori_amd.low_rank_update(t.x, t.y, t.a, t.b, _plan(5))
+    out.sum().backward()
+    sent = {name: args for name, args in calls}
+    assert (sent["nori_low_rank_update"][19] is not None) == (leaf == "b")
+    if leaf != "y":
+        assert (sent["nori_low_rank_backward"][20] is not None) == (leaf == "b")
+
+
+def test_the_library_wants_x_times_a_for_db_alone():
+    lib = nat.lib()
+    back = [16, nat.NORI_F32, 4, 8, 8, 16, 8, 8, None, 8, 16, 16, None, 2, 4, 16, 16, 16, 1, 4, None, 16, 8, 16, 16, None, 0, None]
+    assert lib.nori_low_rank_backward(*back) == nat.NORI_ERR_INVALID and b"null pointer" in lib.nori_last_error()
+    back[24] = None  # dx and da: refused for the workspace, before any device work
+    assert lib.nori_low_rank_backward(*back) == nat.NORI_ERR_INVALID and b"workspace" in lib.nori_last_error()
+    needs = [lib.nori_low_rank_backward_workspace_bytes(nat.NORI_F32, 100000, 8, 8, 4, 1, 100000, *n) for n in ((1, 0, 0), (1, 1, 0))]
+    assert needs[0] < 100000 * 4 * 4 <= needs[1]  # dy b is kept for da alone
