@@ -194,21 +194,26 @@ constexpr int kJoin = 32;
 
 __global__ void __launch_bounds__(kJoin * kJoin) join_kernel(const Backward a) {
     __shared__ float sums[kJoin][kJoin + 1];
-    const int c = blockIdx.x * kJoin + threadIdx.x % kJoin, first = threadIdx.x / kJoin;
-    float s = 0.f;
-    if (c < a.cols) {
-        const float* p = a.partial + (int64_t)blockIdx.y * a.cols + c;
+    const int first = threadIdx.x / kJoin, lane = threadIdx.x % kJoin;
+    for (int c0 = blockIdx.x * kJoin; c0 < a.cols; c0 += gridDim.x * kJoin) {
+        const int c = c0 + lane;
+        float s = 0.f;
+        if (c < a.cols) {
+            const float* p = a.partial + (int64_t)blockIdx.y * a.cols + c;
 #pragma unroll 8
-        for (int i = first; i < a.parts; i += kJoin) s += p[(int64_t)i * 2 * a.cols];
-    }
-    sums[first][threadIdx.x % kJoin] = s;
-    __syncthreads();
-    if (first != 0 || c >= a.cols) return;
-    s = 0.f;
+            for (int i = first; i < a.parts; i += kJoin) s += p[(int64_t)i * 2 * a.cols];
+        }
+        sums[first][lane] = s;
+        __syncthreads();
+        if (first == 0 && c < a.cols) {
+            s = 0.f;
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i) s += sums[i][threadIdx.x];
-    if (blockIdx.y == 0 && a.dw) store_param(a.dw, a.wdt, c, s);
-    if (blockIdx.y == 1 && a.db) store_param(a.db, a.bdt, c, s);
+            for (int i = 0; i < kJoin; ++i) s += sums[i][lane];
+            if (blockIdx.y == 0 && a.dw) store_param(a.dw, a.wdt, c, s);
+            if (blockIdx.y == 1 && a.db) store_param(a.db, a.bdt, c, s);
+        }
+        __syncthreads();
+    }
 }
 
 // Workgroups of the first launch: four rows each while there are few, then as many as a compute unit holds, by the
@@ -268,6 +273,8 @@ extern "C" int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_
         });
     });
     if (columns)
-        hipLaunchKernelGGL(join_kernel, dim3((unsigned)((cols + kJoin - 1) / kJoin), 2), dim3(kJoin * kJoin), 0, stream, a);
+        // a grid holds fewer than 2^32 threads, which is no error but cut: at most 2^31, a workgroup goes round beyond them
+        hipLaunchKernelGGL(join_kernel, dim3((unsigned)std::min((cols + kJoin - 1) / kJoin, 1 << 21), 2), dim3(kJoin * kJoin), 0,
+                           stream, a);
     return launch_status("layer_norm_train_backward");
 }
