@@ -460,7 +460,7 @@ class ReadoutAdapters(nn.Module):
         h = self.first.linear(states, first, plan)
         # under autocast torch's layer norm answers in float32; outside it in its input's dtype
         wide = torch.float32 if torch.is_autocast_enabled("cuda") else h.dtype
-        if type(norm) is not nn.LayerNorm or _watched(norm):
+        if type(norm) is not nn.LayerNorm or _watched(norm) or tuple(norm.normalized_shape) != (h.shape[-1],):
             h = norm(h)
         else:
             h = trainable_layer_norm(h, norm.weight, norm.bias, norm.eps, out_dtype=wide)

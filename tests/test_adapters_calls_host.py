@@ -185,3 +185,12 @@ def test_the_library_wants_x_times_a_for_db_alone():
     assert lib.nori_low_rank_backward(*back) == nat.NORI_ERR_INVALID and b"workspace" in lib.nori_last_error()
     needs = [lib.nori_low_rank_backward_workspace_bytes(nat.NORI_F32, 100000, 8, 8, 4, 1, 100000, *n) for n in ((1, 0, 0), (1, 1, 0))]
     assert needs[0] < 100000 * 4 * 4 <= needs[1]  # dy b is kept for da alone
+
+
+def test_a_norm_of_another_width_is_refused(calls):
+    # without an affine nothing else names the width; torch's own layer norm raises
+    decoder = torch.nn.Sequential(torch.nn.Linear(8, 12), torch.nn.LayerNorm(10, elementwise_affine=False), torch.nn.GELU(),
+                                  torch.nn.Linear(12, 6))
+    bank = nori_amd.ReadoutAdapters(decoder, 1, 4)
+    with pytest.raises(RuntimeError, match="normalized_shape"):
+        bank(decoder, torch.randn(5, 8), _plan(5))
