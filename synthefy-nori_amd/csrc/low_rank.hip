@@ -63,14 +63,14 @@ __device__ __forceinline__ typename Mma<DT>::elem narrow(float v) {
 
 // v as two numbers of a 16-bit type, high and low: v cut to the type's bits, and what that leaves, rounded (2^-22 of v in
 // fp16, 2^-16 in bf16). Both have v's sign, and low is zero only where v is: times an infinity each gives the infinity that v
-// gives. The smallest low that stands for zero is fp16's smallest number and bf16's smallest normal one.
+// gives. The low that stands for zero is fp16's smallest number, and bf16's smallest normal one where that is 2^-16 of v or less.
 template <int DT>
 __device__ __forceinline__ void split(float v, uint16_t& high, uint16_t& low) {
     if constexpr (DT == NORI_F16) high = __builtin_bit_cast(uint16_t, __builtin_amdgcn_cvt_pkrtz(v, 0.f)[0]);
     else high = (uint16_t)(__float_as_uint(v) >> 16);
     low = fabsf(v) < __builtin_inff() ? narrow<DT>(v - widen<DT>(high)) : high;
-    constexpr uint16_t kLeast = DT == NORI_F16 ? 0x0001 : 0x0080;
-    if (v != 0.f && (low & 0x7fff) < kLeast) low = (uint16_t)(kLeast | (__float_as_uint(v) >> 16 & 0x8000));
+    const uint16_t least = DT == NORI_F16 || fabsf(v) < 0x1p-110f ? 0x0001 : 0x0080;
+    if (v != 0.f && (low & 0x7fff) < least) low = (uint16_t)(least | (__float_as_uint(v) >> 16 & 0x8000));
 }
 
 // W elements at p, at any alignment; of fewer than W (`there`), zeros behind them

@@ -133,3 +133,28 @@ def test_one_infinite_factor(rows, rank, dtype):
     some = gr != 0
     assert torch.equal(da[0, some.to(DEV), 0].double().cpu(), gr[some].sign() * float("inf"))
     assert bool(torch.isnan(da[0, ~some.to(DEV), 0]).all()) and bool(torch.isfinite(da[0, :, 1:]).all())
+
+
+@pytest.mark.parametrize("power", [-100, -112, -120, -125])
+@pytest.mark.parametrize("rows,rank", SIZES)
+def test_bfloat16_keeps_values_near_its_smallest(rows, rank, power):
+    # x a^T = 2^power u with u of 8 bits, b brings it back to size: 2^-16 of it is left out at most, or 2^-133 below 2^-117
+    print(f"{rows} rows rank {rank} 2^{power}", flush=True)
+    g = torch.Generator().manual_seed(rows + rank)
+    x = (1 + torch.randint(0, 128, (rows, 1), generator=g).double() / 128) * 2.0 ** (power // 2)
+    a, b = torch.zeros(1, rank, 1).double(), torch.zeros(1, 70, rank).double()
+    a[0, rank - 1], b[0, ::3, rank - 1] = 2.0 ** (power - power // 2), 2.0 ** (-power - 10)
+    y = torch.zeros(rows, 70, dtype=BF16)
+    d = [t.to(DEV, BF16) for t in (x, y, a, b)]
+    leaf = d[3].float().requires_grad_(True)
+    plan = AdapterPlan([0], rows, device=DEV)
+    got = low_rank_update(*d, plan).double().cpu()
+    want = (x * 2.0 ** (power - power // 2)) * b[0, :, rank - 1]
+    kept = want.abs() * 2.0**-16 + 2.0**-133 * b[0, :, rank - 1]
+    assert bool(((got - want).abs() <= kept + (want.abs() + kept) * 2.0**-8).all()), float(((got - want).abs() / want.abs().clamp_min(1e-30)).max())
+    # and in the sums over rows: the same value in each of two rows, 2^k times it
+    dy = torch.zeros(rows, 70, dtype=BF16)
+    dy[0, 4] = dy[-1, 4] = 2.0 ** (-power - 10)
+    (db,) = torch.autograd.grad(low_rank_update(d[0], d[1], d[2].float(), leaf, plan), leaf, dy.to(DEV))
+    want = (x[0] + x[-1] if rows > 1 else x[0]) * 2.0 ** (power - power // 2) * 2.0 ** (-power - 10)
+    assert float((db[0, 4, rank - 1].double().cpu() - want).abs()) <= float(want) * (2.0**-16 + 2.0**-22) + 2 * 2.0**-133 * 2.0 ** (-power - 10)
