@@ -130,6 +130,8 @@ def _update(x, y, a, b, plan, scales, out, keep):
     be kept, None else."""
     k, n, rank = int(x.shape[-1]), int(out.shape[-1]), int(a.shape[1])
     x, rows, xs = _rows_of(x, k)
+    if rows == 0:
+        return torch.empty((0, rank), dtype=torch.float32, device=x.device) if keep else None
     y, _, ys = _rows_of(y, n)
     layout = _strided_rows(out, n)
     if layout is None:
@@ -291,6 +293,8 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 
 def _overlaps_itself(t: torch.Tensor) -> bool:
     """Whether two indices of t may be one element (expanded or overlapping dimensions)."""
+    if t.numel() == 0:
+        return False
     inside = 0
     for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda d: d[1]):
         if stride <= inside:

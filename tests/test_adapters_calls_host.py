@@ -194,3 +194,25 @@ def test_a_norm_of_another_width_is_refused(calls):
     bank = nori_amd.ReadoutAdapters(decoder, 1, 4)
     with pytest.raises(RuntimeError, match="normalized_shape"):
         bank(decoder, torch.randn(5, 8), _plan(5))
+
+
+@pytest.mark.parametrize("shape", [(0,), (2, 0), (0, 3), (2, 0, 3)])
+def test_batches_without_rows(calls, shape):
+    # of any number of dimensions: an empty one has no stride to go by
+    plan = _plan(0)
+    plan.groups, plan.adapters, plan._packed = 0, (), torch.zeros(1, dtype=torch.int32)
+    a, b = (t.requires_grad_(True) for t in (torch.randn(2, 4, 8), torch.randn(2, 6, 4)))
+    x, weight, bias = torch.randn(*shape, 8, requires_grad=True), torch.randn(6, 8), torch.randn(6)
+    for call in (lambda: nori_amd.low_rank_update(x, torch.randn(*shape, 6), a, b, plan),
+                 lambda: nori_amd.adapted_linear(x, weight, bias, a, b, plan)):
+        out = call()
+        grads = torch.autograd.grad(out.sum(), (x, a, b))
+        assert out.shape == (*shape, 6) and [g.shape for g in grads] == [x.shape, a.shape, b.shape]
+        assert not any(bool(g.any()) for g in grads)
+        with torch.no_grad():
+            assert call().shape == (*shape, 6)
+    y = nori_amd.trainable_layer_norm(x, torch.ones(8, requires_grad=True), None)
+    assert torch.autograd.grad(y.sum(), x)[0].shape == x.shape
+    out = torch.empty(*shape, 6)
+    with torch.no_grad():
+        assert nori_amd.low_rank_update(x, torch.randn(*shape, 6), a, b, plan, out=out) is out
