@@ -191,10 +191,10 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Update u, int tran
 }
 
 // A lane's ranks of h, rank 16 t + 4 g + j of row m in acc[t][j], times s: kept in fp32 (`keep`, null: not), and put
-// into LDS as the second product takes them, in two pieces of the inputs' type, high and low, which keep an
-// element to 2^-22 of itself in fp16 and to 2^-16 in bf16; in fp32 h stays as it is. The result, rounded once, is kept to 2^-11 and 2^-8. fp16's
-// are taken after a power of two that brings the row's largest element to 2^14, the top of its range: what is lost below
-// its subnormal numbers is 2^-38 of that element, and a second product sums 2^15 2^16 128 at most.
+// into LDS as the second product takes them, in two pieces of the inputs' type, high and low, which keep an element to
+// 2^-22 of itself in fp16 and to 2^-16 in bf16; in fp32 h stays as it is. The result, rounded once, is kept to 2^-11 and
+// 2^-8. fp16's are taken after a power of two that brings the row's largest element to 2^14, the top of its range: what
+// is lost below its subnormal numbers is 2^-38 of that element, and a second product sums 2^15 2^16 128 at most.
 template <int DT, int RT, int ROWS, int PITCH, int PIECES>
 __device__ __forceinline__ void put_h(f32x4 (&acc)[RT], float s, int rank, float* keep, int g, int row,
                                       typename Mma<DT>::elem (&hs)[PIECES][ROWS][PITCH], float (&factor)[ROWS]) {
@@ -764,8 +764,8 @@ __global__ void __launch_bounds__(kThreads) pack_rows_kernel(const Grads q) {
 }
 
 // t^T h over one part of a group's rows: 128 (fp32: 64) columns by up to 64 ranks a workgroup, whose wavefronts
-// take every fourth step of rows and add their sums in LDS, in order. HBM-bound: t is read once, h once a chunk of
-// columns, from the L2; the next step's rows are on their way while one is summed.
+// take every fourth step of rows and add their sums in LDS, in order. HBM-bound: t is read once for every 64
+// ranks, h once a chunk of columns, from the L2; the next step's rows are on their way while one is summed.
 // The sum runs over rows, which t has apart. 16-bit: a lane reads 16 bytes of each of 8 rows and turns the 8 x 8
 // block in registers, so that it holds 8 rows of one column for each of 8 instructions; column i of a lane's
 // block belongs to instruction i. fp32: instruction i takes row 8 g + i of the lane groups g, no turning. fp16's sums
@@ -1000,10 +1000,11 @@ static bool short_round(int64_t rows, int ranks) {
 }
 
 // LDS that a workgroup of update_kernel asks for beside its own, so that a compute unit takes `c` of them at a time and not
-// all `held`: the c whose rounds, c as long each, end first. (16-bit types hold 3: 40000 rows 1408 -> 1408 rank 32 fp16,
-// out, then dx: 93 + 50 us with 3 and 101 + 62 with 2, one round or two; 65536: 135 + 109 and 124 + 97, two rounds each.
-// Where two of 3 end with three of 2, 75000 rows 352 -> 999 rank 16: 91 + 48 and 93 + 51; fp32 560 -> 1680 rank 32: 324 + 227
-// and 347 + 228; rank 32 bf16, 89324 rows of 48 tables 1408 -> 999, a sixth of them not adapted: 149 and 142 forward.)
+// all `held`: the c whose rounds, c as long each, end first. In us, out with h, then dx with g: 16-bit types hold 3; 40000
+// rows 1408 -> 1408 rank 32 fp16, one round or two: 88 + 76 with 3 and 98 + 81 with 2; 65536, two rounds each: 144 + 112 and
+// 125 + 108. Where rounds tie (`more`): 75000 rows 352 -> 999 rank 16 fp16: 82 + 69 with 3, 89 + 71 with 2; 560 -> 1680 rank
+// 32 fp32, which holds 4: 65536 rows 253 + 191 with 4, 277 + 182 with 2, and 98304 rows 354 + 264 with 3, 385 + 261
+// with 2; but rank 32 bf16, 89324 rows of 48 tables 1408 -> 999, a sixth of them not adapted: 150 + 134 and 147 + 133.
 static unsigned unused_lds(int64_t tiles, int held, bool more, int own) {
     const int64_t cus = device_cus();
     int64_t least = 0;

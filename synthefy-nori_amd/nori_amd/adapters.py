@@ -325,7 +325,8 @@ def low_rank_update(x: torch.Tensor, y: torch.Tensor, a: torch.Tensor, b: torch.
     out up to 2^20. a and b may be float32 beside 16-bit x and y: they are rounded to x's dtype, their gradients, summed
     in fp32, are not.
 
-    Products are summed in fp32, ``x a^T`` is kept in fp32, and the sum with y is rounded once.
+    Products are summed in fp32 and the sum with y is rounded once. In float16 ``x a^T`` enters the second product to 2^-22
+    of itself and 2^-38 of the largest in its row, in bfloat16 to 2^-16 of itself, in float32 whole.
     Differentiable in x, y, a and b (first derivatives, in reverse mode; adapters no row takes get zeros). ``out``, in
     inference, receives the result: a tensor of y's shape and dtype, y itself included, that shares no
     element with x, the factors or the scales."""
