@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(kThreads) icl_attention_rows_kernel(const Args
 // 40,000 rows 25 / 46 / 87 / 90 there, 37 / 37 / 38 / 40 here.
 bool takes_rows(const Args& a, int64_t groups, int64_t qb) {
     return (a.d > 32 || (a.d > 16 && qb > 1)) && a.q_dtype == NORI_F16 && (a.flags & kQVec8) && (a.flags & kOutVec4) && a.d % 8 == 0 && a.d <= 64 &&
-           (uintptr_t)a.kv % 16 == 0 && a.kv_bg % 8 == 0 && a.kv_row % 8 == 0 && a.kv_half % 8 == 0 && groups < 0x7fffffffLL;
+           (uintptr_t)a.kv % 16 == 0 && a.kv_bg % 8 == 0 && a.kv_row % 8 == 0 && a.kv_half % 8 == 0 &&
+           one_launch((groups + kThreads / 8 - 1) / (kThreads / 8), kThreads);
 }
 
 int launch_rows(const Args& a, uint32_t groups, uint32_t nqb, int qb, const Prologue& pro, hipStream_t stream) {
@@ -415,7 +416,7 @@ int launch_chunked(const Args& a, const Prologue& pro, hipStream_t stream) {
     int g = 1;
     while (g < quads) g *= 2;
     const int64_t threads = rows * g;
-    if ((threads + kThreads - 1) / kThreads > 0x7fffffffLL)
+    if (!one_launch((threads + kThreads - 1) / kThreads, kThreads))
         return fail(NORI_ERR_UNSUPPORTED, "icl_attention: %lld query rows exceed one launch", (long long)rows);
     const dim3 grid((unsigned)((threads + kThreads - 1) / kThreads)), block(kThreads);
     switch (g) {

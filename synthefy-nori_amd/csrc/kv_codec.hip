@@ -484,6 +484,7 @@ extern "C" int nori_kv_quantize_int8(const void* src, int src_dtype, int64_t n_o
     if (tiled) {
         const int64_t tiles_per_outer = (n_inner + kTileThreads - 1) / kTileThreads;
         const int64_t grid = tiles_per_outer * n_outer;
+        if (!one_launch(grid, kTileThreads)) return fail(NORI_ERR_UNSUPPORTED, "quantize_int8: cache too large for one launch");
         const size_t lds = ((size_t)kTileThreads * d * es + 15) / 16 * 16 + (size_t)kTileThreads * d;
         NORI_DISPATCH_FLOAT(src_dtype, DT,
             hipLaunchKernelGGL(quantize_tile_kernel<DT>, dim3((unsigned)grid), dim3(kTileThreads), lds, stream,
@@ -492,6 +493,7 @@ extern "C" int nori_kv_quantize_int8(const void* src, int src_dtype, int64_t n_o
     } else {
         const int64_t total = n_outer * n_inner;
         const int64_t grid = (total + kTileThreads - 1) / kTileThreads;
+        if (!one_launch(grid, kTileThreads)) return fail(NORI_ERR_UNSUPPORTED, "quantize_int8: cache too large for one launch");
         NORI_DISPATCH_FLOAT(src_dtype, DT,
             hipLaunchKernelGGL(quantize_direct_kernel<DT>, dim3((unsigned)grid), dim3(kTileThreads), 0, stream, src,
                                n_outer, n_inner, d, src_outer_stride, src_inner_stride, codes, codes_outer_stride,
@@ -520,7 +522,8 @@ extern "C" int nori_kv_dequantize_int8(const int8_t* codes, const float* scales,
     if (flat) {
         const int64_t chunks_per_outer = (n_inner * d + 15) / 16;
         const int64_t blocks = (chunks_per_outer * n_outer + kTileThreads - 1) / kTileThreads;
-        if (blocks > 0x7fffffffLL) return fail(NORI_ERR_UNSUPPORTED, "dequantize_int8: cache too large for one launch");
+        if (!one_launch(blocks, kTileThreads))
+            return fail(NORI_ERR_UNSUPPORTED, "dequantize_int8: cache too large for one launch");
         NORI_DISPATCH_FLOAT(dst_dtype, DT,
             hipLaunchKernelGGL(dequant_flat_kernel<DT>, dim3((unsigned)blocks), dim3(kTileThreads), 0, stream, codes,
                                n_outer, n_inner, d, codes_outer_stride, scales, scales_outer_stride, (uint8_t*)dst,
@@ -531,6 +534,7 @@ extern "C" int nori_kv_dequantize_int8(const int8_t* codes, const float* scales,
     if (tiled) {
         const int64_t tiles_per_outer = (n_inner + kTileThreads - 1) / kTileThreads;
         const int64_t grid = tiles_per_outer * n_outer;
+        if (!one_launch(grid, kTileThreads)) return fail(NORI_ERR_UNSUPPORTED, "dequantize_int8: cache too large for one launch");
         const size_t lds = ((size_t)kTileThreads * d + 15) / 16 * 16 + (size_t)kTileThreads * d * es;
         NORI_DISPATCH_FLOAT(dst_dtype, DT,
             hipLaunchKernelGGL(dequant_tile_kernel<DT>, dim3((unsigned)grid), dim3(kTileThreads), lds, stream, codes,
@@ -539,6 +543,7 @@ extern "C" int nori_kv_dequantize_int8(const int8_t* codes, const float* scales,
     } else {
         const int64_t total = n_outer * n_inner;
         const int64_t grid = (total + kTileThreads - 1) / kTileThreads;
+        if (!one_launch(grid, kTileThreads)) return fail(NORI_ERR_UNSUPPORTED, "dequantize_int8: cache too large for one launch");
         NORI_DISPATCH_FLOAT(dst_dtype, DT,
             hipLaunchKernelGGL(dequant_direct_kernel<DT>, dim3((unsigned)grid), dim3(kTileThreads), 0, stream, codes,
                                n_outer, n_inner, d, codes_outer_stride, codes_inner_stride, scales,

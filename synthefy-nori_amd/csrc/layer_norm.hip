@@ -263,7 +263,9 @@ extern "C" int nori_layer_norm(const void* x, int x_dtype, int64_t rows, int32_t
     if (!x || !y) return fail(NORI_ERR_INVALID, "layer_norm: null pointer");
     if ((uintptr_t)x % (4 * dtype_size(x_dtype)) || (uintptr_t)y % (4 * dtype_size(y_dtype)))
         return fail(NORI_ERR_INVALID, "layer_norm: x and y must be aligned to 4 elements");
-    if (rows > (int64_t)0x7fffffff * kThreads / 64) return fail(NORI_ERR_UNSUPPORTED, "layer_norm: too many rows");
+    const int g = cols / 4, lanes = g <= 64 && (g & (g - 1)) == 0 ? g : 64;  // of a row
+    if (rows > 0xffffffffLL || !one_launch((rows * lanes + kThreads - 1) / kThreads, kThreads))
+        return fail(NORI_ERR_UNSUPPORTED, "layer_norm: too many rows");
     hipStream_t stream = (hipStream_t)stream_v;
     NORI_DISPATCH_FLOAT(x_dtype, XDT, {
         NORI_DISPATCH_FLOAT(y_dtype, YDT, {

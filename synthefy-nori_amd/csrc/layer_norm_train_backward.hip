@@ -273,7 +273,7 @@ extern "C" int nori_layer_norm_train_backward(const void* x, int x_dtype, int64_
         });
     });
     if (columns)
-        // a grid holds fewer than 2^32 threads, which is no error but cut: at most 2^31, a workgroup goes round beyond them
+        // at most 2^31 threads (one_launch): past 2^26 columns a workgroup goes round
         hipLaunchKernelGGL(join_kernel, dim3((unsigned)std::min((cols + kJoin - 1) / kJoin, 1 << 21), 2), dim3(kJoin * kJoin), 0,
                            stream, a);
     return launch_status("layer_norm_train_backward");

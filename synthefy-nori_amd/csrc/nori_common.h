@@ -42,6 +42,9 @@ inline int device_cus() {
     return cus;
 }
 
+// Whether so many workgroups of `threads` are one launch: a grid of 2^32 threads or more is cut without an error.
+inline bool one_launch(int64_t blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
+
 inline const char* dtype_name(int dt) {
     switch (dt) {
         case NORI_F32: return "float32";

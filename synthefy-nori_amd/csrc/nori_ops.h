@@ -126,9 +126,9 @@ int64_t nori_low_rank_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_
 // Its gradients, each NULL where it is not asked for: with g[i] = scales[id] dy[i] b[id],
 //     dx[i] = base[i] + g[i] a[id]   (rows without an adapter take base; base NULL: zeros; dx may be base),
 //     da[id] = sum over the adapter's rows of g[i]^T x[i],   db[id] = sum over them of dy[i]^T h[i],
-// h as the update kept it (db alone reads it), da and db in a's and b's layout and dtype; adapters without a group are left as they
-// are. `longest` is the most rows of a group with an adapter. Rows are summed in parts that are joined in a fixed
-// order: the same inputs give the same bits.
+// h as the update kept it (db alone reads it), da and db in a's and b's layout and dtype; adapters without a group are
+// left as they are. `longest` is the most rows of a group with an adapter. Rows are summed in parts that are joined in a
+// fixed order: the same inputs give the same bits.
 int nori_low_rank_backward(const void* x, int dtype, int64_t rows, int32_t k, int64_t x_row_stride, const void* dy, int32_t n,
                            int64_t dy_row_stride, const void* base, int64_t base_row_stride, const void* a, const void* b,
                            const float* scales, int32_t adapters, int32_t rank, const int32_t* order, const int32_t* starts,

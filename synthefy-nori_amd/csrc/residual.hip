@@ -61,7 +61,7 @@ int launch(const float* x, const void* u, float alpha, int64_t n, float* out, hi
     const bool vec = n % 4 == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)u % (4 * us) == 0;
     const int64_t items = vec ? n / 4 : n;
     const int64_t blocks = (items + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffffLL) return fail(NORI_ERR_UNSUPPORTED, "residual_add: %lld elements exceed one launch", (long long)n);
+    if (!one_launch(blocks, kThreads)) return fail(NORI_ERR_UNSUPPORTED, "residual_add: %lld elements exceed one launch", (long long)n);
     if (vec)
         hipLaunchKernelGGL((residual_add_vec_kernel<UT>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, x, u, alpha, items, out);
     else

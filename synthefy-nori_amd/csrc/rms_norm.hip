@@ -283,7 +283,9 @@ int launch(const void* x, int64_t rows, int cols, int64_t xs, const void* w, flo
         int g = 1;
         while (g < nchunks && g < 64) g <<= 1;
         const int rows_per_block = kThreads / g;
-        const unsigned grid = (unsigned)((rows + rows_per_block - 1) / rows_per_block);
+        const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
+        if (!one_launch(blocks, kThreads)) return fail(NORI_ERR_UNSUPPORTED, "rms_norm: %lld rows exceed one launch", (long long)rows);
+        const unsigned grid = (unsigned)blocks;
 #define NORI_RMS_CASE(GV)                                                                                     \
     case GV:                                                                                                   \
         hipLaunchKernelGGL((rms_norm_chunked_kernel<DT, WDT, OT, GV>), dim3(grid), dim3(kThreads), 0, stream,   \
@@ -295,7 +297,9 @@ int launch(const void* x, int64_t rows, int cols, int64_t xs, const void* w, flo
         }
 #undef NORI_RMS_CASE
     } else {
-        const unsigned grid = (unsigned)((rows + (kThreads / 64) - 1) / (kThreads / 64));
+        const int64_t blocks = (rows + (kThreads / 64) - 1) / (kThreads / 64);
+        if (!one_launch(blocks, kThreads)) return fail(NORI_ERR_UNSUPPORTED, "rms_norm: %lld rows exceed one launch", (long long)rows);
+        const unsigned grid = (unsigned)blocks;
         hipLaunchKernelGGL((rms_norm_elementwise_kernel<DT, WDT, OT>), dim3(grid), dim3(kThreads), 0, stream, x, rows,
                            cols, xs, w, eps, y, ys);
     }
@@ -351,7 +355,10 @@ int launch_residual(const float* x, const void* u, const UpdateRows& ur, float a
     int g = 1;
     while (g < nchunks && g < 64) g <<= 1;
     const int rows_per_block = kThreads / g;
-    const unsigned grid = (unsigned)((rows + rows_per_block - 1) / rows_per_block);
+    const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
+    if (!one_launch(blocks, kThreads))
+        return fail(NORI_ERR_UNSUPPORTED, "residual_add_rms_norm: %lld rows exceed one launch", (long long)rows);
+    const unsigned grid = (unsigned)blocks;
 #define NORI_RES_CASE(GV)                                                                                         \
     case GV:                                                                                                       \
         hipLaunchKernelGGL((residual_rms_norm_kernel<UT, OT, GV>), dim3(grid), dim3(kThreads), 0, stream, x, u, ur, \
@@ -424,6 +431,7 @@ int launch_rows(const float* x, uint32_t rows, int cols, uint32_t d1, uint32_t d
     while (g < nchunks && g < 64) g <<= 1;
     const int rows_per_block = kThreads / g;
     const unsigned grid = (rows + rows_per_block - 1) / rows_per_block;
+    if (!one_launch(grid, kThreads)) return fail(NORI_ERR_UNSUPPORTED, "rms_norm_rows: %u rows exceed one launch", rows);
 #define NORI_ROWS_CASE(GV)                                                                                          \
     case GV:                                                                                                         \
         hipLaunchKernelGGL((rms_norm_rows_kernel<OT, GV>), dim3(grid), dim3(kThreads), 0, stream, x, rows, cols, d1, \

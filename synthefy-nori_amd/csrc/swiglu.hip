@@ -93,7 +93,7 @@ extern "C" int nori_silu_mul(const void* gu, int dtype, int64_t rows, int32_t hi
     const int w = dtype == NORI_F32 ? 4 : 8;
     const bool vec = hidden % w == 0 && row_stride % w == 0 && out_row_stride % w == 0 && (uintptr_t)gu % 16 == 0 &&
                      (uintptr_t)out % 16 == 0 && rows * (hidden / w) < 0x7fffffffLL;
-    if (!vec && rows > 0x7fffffffLL) return fail(NORI_ERR_UNSUPPORTED, "silu_mul: too many rows");
+    if (!vec && !one_launch(rows, kThreads)) return fail(NORI_ERR_UNSUPPORTED, "silu_mul: too many rows");
     const dim3 grid(vec ? (unsigned)((rows * (hidden / w) + kThreads - 1) / kThreads) : (unsigned)rows);
     NORI_DISPATCH_FLOAT(dtype, DT, {
         if (vec) hipLaunchKernelGGL(silu_mul_vec_kernel<DT>, grid, dim3(kThreads), 0, stream, gu, rows, hidden, row_stride, out, out_row_stride);
