@@ -120,3 +120,35 @@ def test_a_loss_over_many_rows_under_a_scaler():
     assert float((bank.last.b.grad[2] - want).abs().max()) <= 2.0**-18 * float(want.abs().max())
     scaler.step(optimizer)
     scaler.update()
+
+
+def test_a_captured_step_of_fp32_factors():
+    ids, counts = [1, 0, -1, 1], [300, 40, 9, 700]
+    g = torch.Generator().manual_seed(3)
+    rows = sum(counts)
+    x, y, dy = (torch.randn(rows, c, generator=g).to(DEV, F16) for c in (96, 130, 130))
+    a, b = (torch.randn(*s, generator=g).to(DEV) * 0.1 for s in ((2, 16, 96), (2, 130, 16)))
+    plan = AdapterPlan(ids, counts, device=DEV)
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (x, a, b)]
+        out = low_rank_update(leaves[0], y, leaves[1], leaves[2], plan)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dy)]
+
+    want = [t.clone() for t in step()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for turn in range(4):
+        for t in outs:
+            t.fill_(float("nan"))
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(h, w) and torch.equal(e, w) for h, e, w in zip(outs, eager, want)), turn
+    # the factors are read, and rounded, on each replay
+    a.mul_(2.0)
+    graph.replay()
+    eager = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(h, e) for h, e in zip(outs, eager)) and not torch.equal(outs[0], want[0])
