@@ -1,0 +1,209 @@
+// Attention with gradients: checks, launch plans and the kernels that join split axes (attention_train.h has the
+// mathematics, attention_train_kernel.h the kernels).
+#include <math.h>
+
+#include <algorithm>
+
+#include "attention_train.h"
+
+using namespace nori;
+using namespace nori::attn_train;
+
+namespace {
+
+constexpr int64_t kTileRows = 64;      // a multiple of every type's tile
+constexpr int64_t kLeastRows = 256;    // of a part: below it, joining costs more than the idle units
+
+// out rows of a unit's rows from their parts: each part's result is normalised over its own keys.
+template <int DT>
+__global__ __launch_bounds__(256) void join_forward_kernel(const Args p) {
+    const auto& a = p.a;
+    const int64_t n = a.bg * a.kv_heads * p.rows, quads = a.d / 4;
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < n * quads; i += gridDim.x * 256LL) {
+        const int64_t at = i / quads, col = 4 * (i % quads);
+        float top = -INFINITY;
+        for (int64_t s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[s * n + at]);
+        f32x4 sum = {};
+        float total = 0.f;
+        const float base = top == -INFINITY ? 0.f : top;
+        for (int64_t s = 0; s < p.splits; ++s) {
+            const float l = p.part_lse[s * n + at];
+            if (l == -INFINITY) continue;  // no keys (or none that counts) in this part
+            const float w = __builtin_amdgcn_exp2f(l - base);
+            total += w;
+            sum += w * *reinterpret_cast<const f32x4*>(p.part + (s * n + at) * a.d + col);
+        }
+        const int64_t unit = at / p.rows, r = at % p.rows, b = unit / a.kv_heads;
+        if (total != 0.f) sum *= 1.f / total;
+        else if (length_of(a, b) > 0) sum = f32x4{} + NAN;  // every logit at -inf
+        const int64_t head = unit % a.kv_heads * p.group + r / a.nq, query = r % a.nq;
+        const int64_t to = ((b * a.nq + query) * a.heads + head) * a.d + col;
+        for (int j = 0; j < 4; ++j) store_elem<DT>(a.out, to + j, sum[j]);
+        if (col == 0 && a.lse) a.lse[at] = (base + __builtin_amdgcn_logf(total)) * kLn2;
+    }
+}
+
+// The sums of dq's parts, or of dk's and dv's.
+template <int DT, bool KV>
+__global__ __launch_bounds__(256) void join_sums_kernel(const Args p) {
+    const auto& a = p.a;
+    const int64_t n = a.bg * a.kv_heads * (KV ? 2 * a.nk : p.rows), quads = a.d / 4;
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < n * quads; i += gridDim.x * 256LL) {
+        const int64_t at = i / quads, col = 4 * (i % quads);
+        f32x4 sum = {};
+        for (int64_t s = 0; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4*>(p.part + (s * n + at) * a.d + col);
+        int64_t to;
+        if constexpr (KV) {
+            const int64_t unit = at / (2 * a.nk), row = at % (2 * a.nk);  // row: key, then K or V
+            to = ((unit / a.kv_heads * 2 * a.nk + row) * a.kv_heads + unit % a.kv_heads) * a.d + col;
+        } else {
+            const int64_t unit = at / p.rows, r = at % p.rows;
+            const int64_t head = unit % a.kv_heads * p.group + r / a.nq;
+            to = ((unit / a.kv_heads * a.nq + r % a.nq) * a.heads + head) * a.d + col;
+        }
+        for (int j = 0; j < 4; ++j) store_elem<DT>(KV ? a.dkv : a.dq, to + j, sum[j]);
+    }
+}
+
+int64_t part_rows(const Args& p, Kind kind) { return p.a.bg * p.a.kv_heads * (kind == kDkv ? 2 * p.a.nk : p.rows); }
+
+// Tiles of the side that stays, and parts of the side that passes where the tiles alone leave compute units idle.
+Args plan(const nori_attention_train_args& a, Kind kind) {
+    Args p{};
+    p.a = a;
+    p.group = a.heads / a.kv_heads;
+    p.rows = (int64_t)p.group * a.nq;
+    p.c = a.scale * kLog2e;
+    const int64_t stay = kind == kDkv ? a.nk : p.rows, pass = kind == kDkv ? p.rows : a.nk;
+    p.tiles = (stay + kOwn - 1) / kOwn;
+    const int64_t blocks = a.bg * a.kv_heads * p.tiles, want = 2 * device_cus();
+    int64_t splits = blocks > 0 && blocks < want ? (want + blocks - 1) / blocks : 1;
+    splits = std::max<int64_t>(1, std::min(splits, pass / kLeastRows));
+    p.per_split = std::max<int64_t>(kTileRows, ((pass + splits - 1) / splits + kTileRows - 1) / kTileRows * kTileRows);
+    p.splits = std::max<int64_t>(1, (pass + p.per_split - 1) / p.per_split);
+    return p;
+}
+
+int64_t part_bytes(const Args& p, Kind kind) { return p.splits > 1 ? p.splits * part_rows(p, kind) * p.a.d * 4 : 0; }
+int64_t aligned16(int64_t n) { return (n + 15) / 16 * 16; }
+
+int launch_typed(Kind kind, const Args& p, hipStream_t stream) {
+    const int64_t blocks = p.a.bg * p.a.kv_heads * p.tiles * p.splits;
+    switch (p.a.dtype) {
+        case NORI_F16: return launch_f16(kind, p, blocks, stream);
+        case NORI_BF16: return launch_bf16(kind, p, blocks, stream);
+        default: return launch_f32(kind, p, blocks, stream);
+    }
+}
+
+int join(Kind kind, const Args& p, hipStream_t stream) {
+    const int64_t items = part_rows(p, kind) * (p.a.d / 4);
+    const dim3 grid((unsigned)std::min<int64_t>((items + 255) / 256, 32 * device_cus())), threads(256);
+    NORI_DISPATCH_FLOAT(p.a.dtype, DT, {
+        if (kind == kForward) hipLaunchKernelGGL((join_forward_kernel<DT>), grid, threads, 0, stream, p);
+        else if (kind == kDq) hipLaunchKernelGGL((join_sums_kernel<DT, false>), grid, threads, 0, stream, p);
+        else hipLaunchKernelGGL((join_sums_kernel<DT, true>), grid, threads, 0, stream, p);
+    });
+    return launch_status("attention_train join");
+}
+
+// A pointer and the strides of its rows, in elements: loads take 4 at once.
+bool loads(const void* p, int size, std::initializer_list<int64_t> strides) {
+    if (reinterpret_cast<uintptr_t>(p) % (4 * size)) return false;
+    return std::all_of(strides.begin(), strides.end(), [](int64_t s) { return s % 4 == 0; });
+}
+
+int check(const nori_attention_train_args* a, bool backward) {
+    const char* what = backward ? "attention_train_backward" : "attention_train_forward";
+    if (!a) return fail(NORI_ERR_INVALID, "%s: null arguments", what);
+    if (a->dtype != NORI_F32 && a->dtype != NORI_F16 && a->dtype != NORI_BF16)
+        return fail(NORI_ERR_UNSUPPORTED, "%s: unsupported dtype %s", what, dtype_name(a->dtype));
+    if (a->bg < 0 || a->nq < 0 || a->nk < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads)
+        return fail(NORI_ERR_INVALID, "%s: %lld x %lld queries of %d heads over %lld keys of %d", what, (long long)a->bg, (long long)a->nq,
+                    a->heads, (long long)a->nk, a->kv_heads);
+    if (a->d < 4 || a->d > NORI_ATTENTION_TRAIN_WIDTH || a->d % 4)
+        return fail(NORI_ERR_UNSUPPORTED, "%s: heads of %d; a multiple of 4 up to %d is taken", what, a->d, NORI_ATTENTION_TRAIN_WIDTH);
+    constexpr int64_t most = 1LL << 30;
+    if (a->nq > most || a->nk > most || a->nq * (a->heads / a->kv_heads) > most)
+        return fail(NORI_ERR_UNSUPPORTED, "%s: up to 2^30 keys, and queries of heads that share one, are taken", what);
+    if (a->bg > (1LL << 40) / ((int64_t)a->heads * std::max<int64_t>(1, std::max(a->nq, a->nk))))
+        return fail(NORI_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (!(a->scale - a->scale == 0.f)) return fail(NORI_ERR_INVALID, "%s: the scale must be finite", what);
+    if (a->lengths && (a->length_group < 1)) return fail(NORI_ERR_INVALID, "%s: lengths of %lld entries each", what, (long long)a->length_group);
+    const int size = dtype_size(a->dtype);
+    if (a->bg * a->nq > 0) {
+        if (!a->q || !a->out || (backward && (!a->lse || !a->dout))) return fail(NORI_ERR_INVALID, "%s: null pointer", what);
+        if (!loads(a->q, size, {a->q_bg, a->q_row, a->q_head}) || !loads(a->out, size, {}) ||
+            (backward && (!loads(a->dout, size, {a->do_bg, a->do_row, a->do_head}) || !loads(a->dq, size, {}))))
+            return fail(NORI_ERR_UNSUPPORTED, "%s: query rows not aligned to 4 elements", what);
+    }
+    if (a->bg * a->nk > 0) {
+        if (!a->kv) return fail(NORI_ERR_INVALID, "%s: null pointer", what);
+        if (!loads(a->kv, size, {a->kv_bg, a->kv_row, a->kv_half, a->kv_head}) || (backward && !loads(a->dkv, size, {})))
+            return fail(NORI_ERR_UNSUPPORTED, "%s: key rows not aligned to 4 elements", what);
+    }
+    const Kind kinds[3] = {kForward, kDq, kDkv};
+    for (Kind k : kinds) {
+        const Args p = plan(*a, k);
+        if (!one_launch(a->bg * a->kv_heads * p.tiles * p.splits, kThreads))
+            return fail(NORI_ERR_UNSUPPORTED, "%s: more workgroups than one launch has", what);
+    }
+    return NORI_OK;
+}
+
+int check_workspace(const nori_attention_train_args* a, bool backward) {
+    const int64_t need = nori_attention_train_workspace_bytes(a, backward);
+    if (need == 0) return NORI_OK;
+    if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)
+        return fail(NORI_ERR_INVALID, "attention_train: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
+    return NORI_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t nori_attention_train_workspace_bytes(const nori_attention_train_args* a, int32_t backward) {
+    if (!a || a->heads < 1 || a->kv_heads < 1 || a->bg < 0 || a->nq < 0 || a->nk < 0) return 0;
+    if (!backward) {
+        const Args p = plan(*a, kForward);
+        return p.splits > 1 ? aligned16(part_bytes(p, kForward)) + aligned16(p.splits * part_rows(p, kForward) * 4) : 0;
+    }
+    const Args q = plan(*a, kDq), kv = plan(*a, kDkv);
+    return aligned16(part_rows(q, kDq) * 4) + std::max(a->dq ? part_bytes(q, kDq) : 0, a->dkv ? part_bytes(kv, kDkv) : 0);
+}
+
+extern "C" int nori_attention_train_forward(const nori_attention_train_args* a, void* stream_v) {
+    clear_error();
+    if (int rc = check(a, false)) return rc;
+    if (a->bg * a->nq == 0) return NORI_OK;
+    if (int rc = check_workspace(a, false)) return rc;
+    hipStream_t stream = (hipStream_t)stream_v;
+    Args p = plan(*a, kForward);
+    p.part = reinterpret_cast<float*>(a->workspace);
+    p.part_lse = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + aligned16(part_bytes(p, kForward)));
+    if (int rc = launch_typed(kForward, p, stream)) return rc;
+    return p.splits > 1 ? join(kForward, p, stream) : NORI_OK;
+}
+
+extern "C" int nori_attention_train_backward(const nori_attention_train_args* a, void* stream_v) {
+    clear_error();
+    if (int rc = check(a, true)) return rc;
+    if (a->bg == 0 || (!a->dq && !a->dkv)) return NORI_OK;
+    if (int rc = check_workspace(a, true)) return rc;
+    hipStream_t stream = (hipStream_t)stream_v;
+    float* delta = reinterpret_cast<float*>(a->workspace);
+    Args q = plan(*a, kDq);
+    if (a->nq > 0) {
+        if (!a->dq) q.splits = 1;  // the rows' sums alone
+        q.delta = delta;
+        q.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + aligned16(part_rows(q, kDq) * 4));
+        if (int rc = launch_typed(kDq, q, stream)) return rc;
+        if (q.splits > 1)
+            if (int rc = join(kDq, q, stream)) return rc;
+    }
+    if (!a->dkv || a->nk == 0) return NORI_OK;
+    Args kv = plan(*a, kDkv);
+    kv.delta = delta;
+    kv.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + aligned16(part_rows(q, kDq) * 4));
+    if (int rc = launch_typed(kDkv, kv, stream)) return rc;
+    return kv.splits > 1 ? join(kDkv, kv, stream) : NORI_OK;
+}

@@ -1,0 +1,10 @@
+// Attention with gradients over float16 rows (attention_train_kernel.h).
+#include "attention_train_kernel.h"
+
+namespace nori {
+namespace attn_train {
+
+int launch_f16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) { return launch_width<NORI_F16>(kind, p, blocks, stream); }
+
+}  // namespace attn_train
+}  // namespace nori

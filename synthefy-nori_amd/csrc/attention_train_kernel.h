@@ -1,0 +1,572 @@
+// The kernels of attention with gradients, instantiated by attention_train_<type>.hip (attention_train.h has the
+// mathematics and the layout).
+#pragma once
+
+#include "attention_train.h"
+
+namespace nori {
+namespace attn_train {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// An operand of 16 steps of a contraction: 8 elements a lane. Chunk: 4 elements, the unit of loads (head widths are
+// multiples of 4). kRows: rows of a tile that passes. kBias: the power of two on p in its 16-bit form.
+template <int DT> struct El;
+template <> struct El<NORI_F16> {
+    using T = uint16_t;
+    using Frag = f16x8;
+    using Chunk = u32x2;
+    static constexpr int kRows = 64, kPad = 8;
+    // p is below 2^-14, where float16 loses bits, for most keys of a long context: times 2^15 it keeps them to 2^-29
+    static constexpr float kBias = 15.f;
+    static constexpr bool kScaled = true;
+};
+template <> struct El<NORI_BF16> {
+    using T = uint16_t;
+    using Frag = bf16x8;
+    using Chunk = u32x2;
+    static constexpr int kRows = 64, kPad = 8;
+    static constexpr float kBias = 0.f;
+    static constexpr bool kScaled = false;
+};
+template <> struct El<NORI_F32> {
+    using T = float;
+    struct Frag { float v[8]; };
+    using Chunk = u32x4;
+    static constexpr int kRows = 32, kPad = 4;
+    static constexpr float kBias = 0.f;
+    static constexpr bool kScaled = false;
+};
+
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(const El<NORI_F32>::Frag& a, const El<NORI_F32>::Frag& b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
+}
+
+// Value of lane l ^ 32.
+__device__ __forceinline__ float other_half(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), true, false);
+    return __uint_as_float((__lane_id() < 32) ? r[1] : r[0]);
+}
+
+// Geometry of a head width padded to DK (a multiple of 16): DP is DK in whole products of 32 columns.
+template <int DT, int DK> struct Geo {
+    using E = El<DT>;
+    using T = typename E::T;
+    static constexpr int DP = (DK + 31) / 32 * 32;
+    static constexpr int LS = DP + E::kPad;      // elements from one row of a tile to the next
+    static constexpr int KS = DK / 16, MS = DP / 32;
+    static constexpr int CH = DK / 4;            // chunks a row
+    static constexpr int N = (E::kRows * CH + kThreads - 1) / kThreads;  // chunks a thread, a tile
+};
+
+// Left operand: row `row` (lane % 32 of a step's 32) of a tile, its columns 16 k + 8 h .. + 7.
+template <int DT, int DK>
+__device__ __forceinline__ typename El<DT>::Frag direct(const typename El<DT>::T* tile, int row, int k, int half) {
+    const auto* p = tile + row * Geo<DT, DK>::LS + 16 * k + 8 * half;
+    return *reinterpret_cast<const typename El<DT>::Frag*>(p);
+}
+
+// Left operand transposed: column 32 m + lane % 32 of a tile, its rows first + 4 h .. + 3 and first + 8 + 4 h .. + 3, the
+// order in which a product leaves its rows. ds_read_b64_tr_b16 gives lane i of 16 element i % 4 of the 8 bytes that lanes
+// i / 4 + 4 j point at, j = 0 .. 3: lanes 4 j .. 4 j + 3 point along row j.
+template <int DT, int DK>
+__device__ __forceinline__ typename El<DT>::Frag transposed(const typename El<DT>::T* tile, int first, int m, int lane) {
+    constexpr int LS = Geo<DT, DK>::LS;
+    if constexpr (DT == NORI_F32) {
+        typename El<DT>::Frag f;
+        const float* p = tile + (first + 4 * (lane >> 5)) * LS + 32 * m + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f.v[j] = p[((j & 3) + 8 * (j >> 2)) * LS];
+        return f;
+    } else {
+        const uint16_t* p = tile + (first + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LS + 32 * m + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * LS));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(typename El<DT>::Frag, both);
+    }
+}
+
+// Right operand of the contraction over a result's rows: registers 8 t .. 8 t + 7, rounded to the type (to nearest even).
+template <int DT>
+__device__ __forceinline__ typename El<DT>::Frag rounded(const float (&x)[16], int t) {
+    typename El<DT>::Frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (DT == NORI_F32) f.v[j] = x[8 * t + j];
+        else if constexpr (DT == NORI_F16) f[j] = (_Float16)x[8 * t + j];
+        else f[j] = (__bf16)x[8 * t + j];
+    }
+    return f;
+}
+
+// The operands that stay: columns 16 k + 8 h .. + 7 of the row at p, zeros past d or where the row is not there.
+template <int DT, int DK>
+__device__ __forceinline__ void load_own(typename El<DT>::Frag (&f)[DK / 16], const typename El<DT>::T* p, bool there, int d, int half) {
+    using E = El<DT>;
+#pragma unroll
+    for (int k = 0; k < DK / 16; ++k) {
+        typename E::Chunk c[2] = {};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int at = 16 * k + 8 * half + 4 * j;
+            if (there && at < d) c[j] = *reinterpret_cast<const typename E::Chunk*>(p + at);
+        }
+        f[k] = __builtin_bit_cast(typename E::Frag, c);
+    }
+}
+
+// Writes 4 results, columns at .. at + 3 of a row.
+template <int DT>
+__device__ __forceinline__ void store4(typename El<DT>::T* p, const float (&x)[4]) {
+    if constexpr (DT == NORI_F32) {
+        *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = DT == NORI_F16 ? f32_to_f16(x[j]) : f32_to_bf16(x[j]);
+        *reinterpret_cast<u32x2*>(p) = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
+    }
+}
+
+// Query row r of a unit: head and query.
+struct Row { int64_t head, query; };
+__device__ __forceinline__ Row row_of(const Args& p, int64_t unit_head, int r) {
+    if (p.group == 1) return {unit_head, r};
+    const int h = r / (int)p.a.nq;
+    return {unit_head * p.group + h, r - h * (int)p.a.nq};
+}
+
+struct Block { int64_t tile, split, unit, b, hk; };
+__device__ __forceinline__ Block block_of(const Args& p) {
+    int64_t i = work_index(blockIdx.x, gridDim.x);
+    Block w;
+    w.tile = i % p.tiles;
+    i /= p.tiles;
+    w.split = i % p.splits;
+    w.unit = i / p.splits;
+    w.b = w.unit / p.a.kv_heads;
+    w.hk = w.unit % p.a.kv_heads;
+    return w;
+}
+
+// A tile of two tensors on its way to LDS: chunks in registers, asked for while the tile before is worked on.
+template <int DT, int DK> struct Stage {
+    using G = Geo<DT, DK>;
+    using E = El<DT>;
+    using T = typename E::T;
+    typename E::Chunk x[G::N], y[G::N];
+
+    // at(row, two pointers): the row's first elements
+    template <class At>
+    __device__ __forceinline__ void load(int first, int end, int d, At at) {
+#pragma unroll
+        for (int i = 0; i < G::N; ++i) {
+            const int idx = threadIdx.x + i * kThreads, row = first + idx / G::CH, col = 4 * (idx % G::CH);
+            x[i] = {};
+            y[i] = {};
+            if (idx < E::kRows * G::CH && row < end && col < d) {
+                const T *px, *py;
+                at(row, px, py);
+                x[i] = *reinterpret_cast<const typename E::Chunk*>(px + col);
+                y[i] = *reinterpret_cast<const typename E::Chunk*>(py + col);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* tx, T* ty) const {
+#pragma unroll
+        for (int i = 0; i < G::N; ++i) {
+            const int idx = threadIdx.x + i * kThreads, to = idx / G::CH * G::LS + 4 * (idx % G::CH);
+            if (idx < E::kRows * G::CH) {
+                *reinterpret_cast<typename E::Chunk*>(tx + to) = x[i];
+                *reinterpret_cast<typename E::Chunk*>(ty + to) = y[i];
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------- forward
+template <int DT, int DK>
+__global__ __launch_bounds__(kThreads) void forward_kernel(const Args p) {
+    using E = El<DT>;
+    using G = Geo<DT, DK>;
+    using T = typename E::T;
+    __shared__ __attribute__((aligned(16))) T ks[E::kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T vs[E::kRows * G::LS];
+    const auto& a = p.a;
+    const Block w = block_of(p);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int64_t r64 = w.tile * kOwn + wave * 32 + (lane & 31);
+    const bool there = r64 < p.rows;
+    const int r = (int)r64;
+    const Row row = there ? row_of(p, w.hk, r) : Row{w.hk * p.group, 0};
+    const int length = length_of(a, w.b);
+    const int begin = (int)(w.split * p.per_split);
+    const int end = (int)min((int64_t)length, w.split * p.per_split + p.per_split);
+
+    typename E::Frag qf[G::KS];
+    load_own<DT, DK>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
+    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head;
+    const auto at = [&](int key, const T*& x, const T*& y) { x = kv + key * a.kv_row; y = x + a.kv_half; };
+    // the running maximum wants a positive factor: a negative one changes signs before, one of 0 makes the logits 0
+    const float c = p.c == 0.f ? 1.f : fabsf(p.c);
+    const float sign = p.c < 0.f ? -1.f : (p.c == 0.f ? 0.f : 1.f);
+
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[G::MS] = {};
+    Stage<DT, DK> stage;
+    if (begin < end) stage.load(begin, end, a.d, at);
+    for (int first = begin; first < end; first += E::kRows) {
+        __syncthreads();
+        stage.store(ks, vs);
+        __syncthreads();
+        if (first + E::kRows < end) stage.load(first + E::kRows, end, a.d, at);
+#pragma unroll
+        for (int sub = 0; sub < E::kRows / 32; ++sub) {
+            if (first + sub * 32 >= end) break;
+            f32x16 acc = {};
+#pragma unroll
+            for (int k = 0; k < G::KS; ++k) acc = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], acc);
+            float s[16];
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = sign * acc[i];
+            if (first + sub * 32 + 32 > end) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) s[i] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+            top = fmaxf(m, fmaxf(top, other_half(top)));
+            const float base = top == -INFINITY ? 0.f : top;  // (all keys so far at -inf: their p is 0)
+            const float shrink = __builtin_amdgcn_exp2f((m - base) * c);
+            m = top;
+            const float off = E::kBias - 1.f - base * c;  // p up to 2^(kBias - 1): inside float16's range
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, off));
+                sum += s[i];
+            }
+            l = l * shrink + sum;
+#pragma unroll
+            for (int j = 0; j < G::MS; ++j) o[j] *= shrink;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const auto pf = rounded<DT>(s, t);
+#pragma unroll
+                for (int j = 0; j < G::MS; ++j) o[j] = mma(transposed<DT, DK>(vs, sub * 32 + 16 * t, j, lane), pf, o[j]);
+            }
+        }
+    }
+    if (!there) return;
+    l += other_half(l);
+    const float inv = begin < end ? 1.f / l : 0.f;
+    const float lse2 = begin < end ? __builtin_amdgcn_logf(l) - (E::kBias - 1.f) + m * c : -INFINITY;
+    if (p.splits > 1) {
+        const int64_t units = a.bg * a.kv_heads;
+        const int64_t to = (w.split * units + w.unit) * p.rows + r;
+        if (half == 0) p.part_lse[to] = lse2;
+#pragma unroll
+        for (int j = 0; j < G::MS; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int col = 32 * j + 2 * i + 4 * half;
+                if (col < a.d) *reinterpret_cast<f32x4*>(p.part + to * a.d + col) = f32x4{o[j][i] * inv, o[j][i + 1] * inv, o[j][i + 2] * inv, o[j][i + 3] * inv};
+            }
+        return;
+    }
+    if (half == 0 && a.lse) a.lse[w.unit * p.rows + r] = lse2 * kLn2;
+    T* out = reinterpret_cast<T*>(a.out) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d;
+#pragma unroll
+    for (int j = 0; j < G::MS; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int col = 32 * j + 2 * i + 4 * half;
+            const float x[4] = {o[j][i] * inv, o[j][i + 1] * inv, o[j][i + 2] * inv, o[j][i + 3] * inv};
+            if (col < a.d) store4<DT>(out + col, x);
+        }
+}
+
+// ds in float16 carries a power of two a column (a query of dq, a key of dk): gradients of a mean over many rows lie below
+// float16's range, those under a loss scale above it. The power brings the first values to 2^8 and falls where a later
+// one would pass 2^15; what is summed so far is brought along. Exact, so the result does not go by it but for values
+// 2^-22 of the column's largest.
+struct Scale {
+    float f = 0.f;  // 0: nothing but zeros so far
+
+    // the values of this step with the factor on; acc takes a change of it
+    template <int MS>
+    __device__ __forceinline__ void apply(float (&x)[16], f32x16 (&acc)[MS]) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+        top = fmaxf(top, other_half(top));
+        const bool change = f == 0.f ? top > 0.f : top * f > 32768.f;
+        if (__any(change)) {
+            float next = f;
+            if (change) {
+                int e = 8 + 127 - (int)(__float_as_uint(top) >> 23);  // top * 2^e in [2^8, 2^9)
+                e = e > 120 ? 120 : (e < -100 ? -100 : e);
+                next = __uint_as_float((uint32_t)(e + 127) << 23);
+            }
+            const float by = f == 0.f ? 1.f : next / f;  // (nothing is summed while f is 0)
+#pragma unroll
+            for (int j = 0; j < MS; ++j) acc[j] *= by;
+            f = next;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= f;
+    }
+    __device__ __forceinline__ float inverse() const { return f == 0.f ? 1.f : 1.f / f; }
+};
+
+// ---------------------------------------------------------------- dq, and delta for dk and dv
+template <int DT, int DK>
+__global__ __launch_bounds__(kThreads) void dq_kernel(const Args p) {
+    using E = El<DT>;
+    using G = Geo<DT, DK>;
+    using T = typename E::T;
+    __shared__ __attribute__((aligned(16))) T ks[E::kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T vs[E::kRows * G::LS];
+    const auto& a = p.a;
+    const Block w = block_of(p);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int64_t r64 = w.tile * kOwn + wave * 32 + (lane & 31);
+    const bool there = r64 < p.rows;
+    const int r = (int)r64;
+    const Row row = there ? row_of(p, w.hk, r) : Row{w.hk * p.group, 0};
+    const int64_t unit_row = w.unit * p.rows + r;
+    const int length = length_of(a, w.b);
+    const int begin = (int)(w.split * p.per_split);
+    const int end = a.dq ? (int)min((int64_t)length, w.split * p.per_split + p.per_split) : begin;
+
+    typename E::Frag dof[G::KS], qf[G::KS];
+    load_own<DT, DK>(dof, reinterpret_cast<const T*>(a.dout) + w.b * a.do_bg + row.query * a.do_row + row.head * a.do_head, there, a.d, half);
+    load_own<DT, DK>(qf, reinterpret_cast<const T*>(a.out) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d, there, a.d, half);
+    float delta = 0.f;
+#pragma unroll
+    for (int k = 0; k < G::KS; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (DT == NORI_F32) delta = fmaf(dof[k].v[j], qf[k].v[j], delta);
+            else delta = fmaf((float)dof[k][j], (float)qf[k][j], delta);
+        }
+    }
+    delta += other_half(delta);
+    if (there && half == 0 && w.split == 0) p.delta[unit_row] = delta;
+    if (!a.dq) return;
+    load_own<DT, DK>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
+    const float lse2 = there ? a.lse[unit_row] * kLog2e : 0.f;
+    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head;
+    const auto at = [&](int key, const T*& x, const T*& y) { x = kv + key * a.kv_row; y = x + a.kv_half; };
+
+    f32x16 dq[G::MS] = {};
+    Scale scale;
+    Stage<DT, DK> stage;
+    if (begin < end) stage.load(begin, end, a.d, at);
+    for (int first = begin; first < end; first += E::kRows) {
+        __syncthreads();
+        stage.store(ks, vs);
+        __syncthreads();
+        if (first + E::kRows < end) stage.load(first + E::kRows, end, a.d, at);
+#pragma unroll
+        for (int sub = 0; sub < E::kRows / 32; ++sub) {
+            if (first + sub * 32 >= end) break;
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int k = 0; k < G::KS; ++k) {
+                s = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s);
+                dp = mma(direct<DT, DK>(vs, sub * 32 + (lane & 31), k, half), dof[k], dp);
+            }
+            float ds[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse2)) * (dp[i] - delta);
+            if (first + sub * 32 + 32 > end) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) ds[i] = 0.f;
+            }
+            if constexpr (E::kScaled) scale.apply(ds, dq);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const auto f = rounded<DT>(ds, t);
+#pragma unroll
+                for (int j = 0; j < G::MS; ++j) dq[j] = mma(transposed<DT, DK>(ks, sub * 32 + 16 * t, j, lane), f, dq[j]);
+            }
+        }
+    }
+    if (!there) return;
+    const float by = a.scale * (E::kScaled ? scale.inverse() : 1.f);
+    T* out = reinterpret_cast<T*>(a.dq) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d;
+    float* part = p.part + (w.split * a.bg * a.kv_heads * p.rows + unit_row) * a.d;
+#pragma unroll
+    for (int j = 0; j < G::MS; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int col = 32 * j + 2 * i + 4 * half;
+            const float x[4] = {dq[j][i] * by, dq[j][i + 1] * by, dq[j][i + 2] * by, dq[j][i + 3] * by};
+            if (col >= a.d) continue;
+            if (p.splits > 1) *reinterpret_cast<f32x4*>(part + col) = f32x4{x[0], x[1], x[2], x[3]};
+            else store4<DT>(out + col, x);
+        }
+}
+
+// ---------------------------------------------------------------- dk and dv
+template <int DT, int DK>
+__global__ __launch_bounds__(kThreads) void dkv_kernel(const Args p) {
+    using E = El<DT>;
+    using G = Geo<DT, DK>;
+    using T = typename E::T;
+    __shared__ __attribute__((aligned(16))) T qs[E::kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T dos[E::kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) float off[E::kRows];    // kBias - log2 of the row's sum
+    __shared__ __attribute__((aligned(16))) float deltas[E::kRows];
+    const auto& a = p.a;
+    const Block w = block_of(p);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
+    const int64_t key64 = w.tile * kOwn + wave * 32 + (lane & 31);
+    const int length = length_of(a, w.b);
+    const bool there = key64 < length;
+    const int key = (int)key64;
+    const int begin = (int)(w.split * p.per_split);
+    // (a tile behind the length has no products, its gradients are zeros)
+    const int end = w.tile * kOwn < length ? (int)min(p.rows, w.split * p.per_split + p.per_split) : begin;
+
+    typename E::Frag kf[G::KS], vf[G::KS];
+    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + (there ? key * a.kv_row : 0);
+    load_own<DT, DK>(kf, kv, there, a.d, half);
+    load_own<DT, DK>(vf, kv + a.kv_half, there, a.d, half);
+    const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.q_bg;
+    const T* dout = reinterpret_cast<const T*>(a.dout) + w.b * a.do_bg;
+    const auto at = [&](int r, const T*& x, const T*& y) {
+        const Row row = row_of(p, w.hk, r);
+        x = q + row.query * a.q_row + row.head * a.q_head;
+        y = dout + row.query * a.do_row + row.head * a.do_head;
+    };
+
+    f32x16 dk[G::MS] = {}, dv[G::MS] = {};
+    Scale scale;
+    Stage<DT, DK> stage;
+    float next_off = 0.f, next_delta = 0.f;
+    const auto statistics = [&](int first) {
+        const int r = first + threadIdx.x;
+        if (threadIdx.x < E::kRows) {
+            const bool in = r < end;
+            next_off = in ? E::kBias - a.lse[w.unit * p.rows + r] * kLog2e : 0.f;
+            next_delta = in ? p.delta[w.unit * p.rows + r] : 0.f;
+        }
+    };
+    if (begin < end) {
+        stage.load(begin, end, a.d, at);
+        statistics(begin);
+    }
+    for (int first = begin; first < end; first += E::kRows) {
+        __syncthreads();
+        stage.store(qs, dos);
+        if (threadIdx.x < E::kRows) {
+            off[threadIdx.x] = next_off;
+            deltas[threadIdx.x] = next_delta;
+        }
+        __syncthreads();
+        if (first + E::kRows < end) {
+            stage.load(first + E::kRows, end, a.d, at);
+            statistics(first + E::kRows);
+        }
+#pragma unroll
+        for (int sub = 0; sub < E::kRows / 32; ++sub) {
+            if (first + sub * 32 >= end) break;
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int k = 0; k < G::KS; ++k) {
+                s = mma(direct<DT, DK>(qs, sub * 32 + (lane & 31), k, half), kf[k], s);
+                dp = mma(direct<DT, DK>(dos, sub * 32 + (lane & 31), k, half), vf[k], dp);
+            }
+            float pr[16], ds[16];
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 o4 = *reinterpret_cast<const f32x4*>(&off[sub * 32 + 2 * i + 4 * half]);
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(&deltas[sub * 32 + 2 * i + 4 * half]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    pr[i + j] = __builtin_amdgcn_exp2f(fmaf(s[i + j], p.c, o4[j]));
+                    ds[i + j] = pr[i + j] * (dp[i + j] - d4[j]);
+                }
+            }
+            if (first + sub * 32 + 32 > end) {  // rows that are not there: 0, also beside keys that are not finite
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) pr[i] = ds[i] = 0.f;
+            }
+            if constexpr (E::kScaled) scale.apply(ds, dk);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const auto pf = rounded<DT>(pr, t), f = rounded<DT>(ds, t);
+#pragma unroll
+                for (int j = 0; j < G::MS; ++j) {
+                    dv[j] = mma(transposed<DT, DK>(dos, sub * 32 + 16 * t, j, lane), pf, dv[j]);
+                    dk[j] = mma(transposed<DT, DK>(qs, sub * 32 + 16 * t, j, lane), f, dk[j]);
+                }
+            }
+        }
+    }
+    if (key64 >= a.nk) return;
+    constexpr float unbias = DT == NORI_F16 ? 0x1p-15f : 1.f;
+    const float byk = there ? a.scale * unbias * (E::kScaled ? scale.inverse() : 1.f) : 0.f, byv = unbias;
+    T* out = reinterpret_cast<T*>(a.dkv) + (((w.b * a.nk + key) * 2) * a.kv_heads + w.hk) * a.d;
+    float* part = p.part + ((w.split * a.bg * a.kv_heads + w.unit) * a.nk + key) * 2 * a.d;
+#pragma unroll
+    for (int j = 0; j < G::MS; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int col = 32 * j + 2 * i + 4 * half;
+            float x[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = there ? dk[j][i + e] * byk : 0.f;
+                y[e] = there ? dv[j][i + e] * byv : 0.f;
+            }
+            if (col >= a.d) continue;
+            if (p.splits > 1) {
+                *reinterpret_cast<f32x4*>(part + col) = f32x4{x[0], x[1], x[2], x[3]};
+                *reinterpret_cast<f32x4*>(part + a.d + col) = f32x4{y[0], y[1], y[2], y[3]};
+            } else {
+                store4<DT>(out + col, x);
+                store4<DT>(out + (int64_t)a.kv_heads * a.d + col, y);
+            }
+        }
+}
+
+template <int DT, int DK>
+int launch(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
+    const dim3 grid((unsigned)blocks), threads(kThreads);
+    switch (kind) {
+        case kForward: hipLaunchKernelGGL((forward_kernel<DT, DK>), grid, threads, 0, stream, p); break;
+        case kDq: hipLaunchKernelGGL((dq_kernel<DT, DK>), grid, threads, 0, stream, p); break;
+        case kDkv: hipLaunchKernelGGL((dkv_kernel<DT, DK>), grid, threads, 0, stream, p); break;
+    }
+    return launch_status("attention_train");
+}
+
+template <int DT>
+int launch_width(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
+    const int d = p.a.d;
+    if (d <= 32) return launch<DT, 32>(kind, p, blocks, stream);
+    if (d <= 48) return launch<DT, 48>(kind, p, blocks, stream);
+    if (d <= 64) return launch<DT, 64>(kind, p, blocks, stream);
+    if (d <= 96) return launch<DT, 96>(kind, p, blocks, stream);
+    return launch<DT, 128>(kind, p, blocks, stream);
+}
+
+}  // namespace attn_train
+}  // namespace nori

@@ -10,7 +10,7 @@ extern "C" {
 #endif
 
 // Moves with every change of a signature or struct below; the package binds one version.
-#define NORI_OPS_VERSION 6
+#define NORI_OPS_VERSION 7
 int nori_ops_version(void);
 
 // QASS base scale of one key count (QASSMaxScaling.forward's base branch, src/synthefy_nori/model/
@@ -142,6 +142,41 @@ int nori_low_rank_backward_f32(const void* x, int dtype, int64_t rows, int32_t k
                                int64_t dx_row_stride, void* da, void* db, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t nori_low_rank_backward_workspace_bytes(int dtype, int64_t rows, int32_t k, int32_t n, int32_t rank, int32_t groups,
                                                int64_t longest, int32_t need_x, int32_t need_a, int32_t need_b);
+
+// Attention with gradients (attention_train.hip): out[b, i, h] = softmax_j(scale q[b, i, h] . k[b, j, hk]) v[b, j, hk] over the
+// first lengths[b / length_group] of nk keys (NULL: all; int32 or int64, taken between 0 and nk; none: zeros), hk = h /
+// (heads / kv_heads). q [bg, nq, heads, d] and kv [bg, nk, 2, kv_heads, d] of one dtype at element strides, d a multiple of
+// 4 up to NORI_ATTENTION_TRAIN_WIDTH with its elements side by side, strides multiples of 4, pointers aligned to 4 elements;
+// out [bg, nq, heads, d] and lse [bg, heads, nq] fp32 (natural log, -inf without keys; NULL where it is not kept) contiguous.
+// Backward: dout at its strides, out and lse as the forward call left them; dq and dkv contiguous in q's and kv's shapes,
+// each NULL where it is not asked for; gradients of keys past the length are zeros. Keys and values past the length are
+// not looked at. The workspaces, of nori_attention_train_workspace_bytes and 16-byte aligned, take the partial results of
+// long axes that few workgroups would walk, joined in order, and the backward pass's row sums: the same inputs give the
+// same bits. No rows: nothing is written; rows without keys: zeros.
+#define NORI_ATTENTION_TRAIN_WIDTH 128
+typedef struct {
+    int64_t bg, nq, nk;
+    int32_t dtype, heads, kv_heads, d;
+    const void* q;
+    int64_t q_bg, q_row, q_head;
+    const void* kv;
+    int64_t kv_bg, kv_row, kv_half, kv_head;
+    const void* lengths;
+    int64_t length_group;
+    int32_t lengths_i64;
+    float scale;
+    void* out;
+    float* lse;
+    const void* dout;
+    int64_t do_bg, do_row, do_head;
+    void *dq, *dkv;
+    void* workspace;
+    int64_t workspace_bytes;
+} nori_attention_train_args;
+
+int64_t nori_attention_train_workspace_bytes(const nori_attention_train_args* args, int32_t backward);
+int nori_attention_train_forward(const nori_attention_train_args* args, void* stream);
+int nori_attention_train_backward(const nori_attention_train_args* args, void* stream);
 
 #ifdef __cplusplus
 }

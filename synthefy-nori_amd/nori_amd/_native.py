@@ -130,8 +130,21 @@ class DenseApplyArgs(ctypes.Structure):
     )
 
 
+class AttentionTrainArgs(ctypes.Structure):
+    """``nori_attention_train_args``."""
+
+    _fields_ = (
+        [(n, _i64) for n in ("bg", "nq", "nk")] + [(n, _i32) for n in ("dtype", "heads", "kv_heads", "d")]
+        + [("q", _vp)] + [(n, _i64) for n in ("q_bg", "q_row", "q_head")]
+        + [("kv", _vp)] + [(n, _i64) for n in ("kv_bg", "kv_row", "kv_half", "kv_head")]
+        + [("lengths", _vp), ("length_group", _i64), ("lengths_i64", _i32), ("scale", _f32), ("out", _vp), ("lse", _vp)]
+        + [("dout", _vp)] + [(n, _i64) for n in ("do_bg", "do_row", "do_head")]
+        + [("dq", _vp), ("dkv", _vp), ("workspace", _vp), ("workspace_bytes", _i64)]
+    )
+
+
 # The package's own entry points beyond the C ABI (csrc/nori_ops.h), and their version.
-OPS_VERSION = 6
+OPS_VERSION = 7
 OPS: dict[str, tuple[object, list]] = {
     "nori_qass_base": (ctypes.c_int, [_f32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
     "nori_linear_f16_w32": (
@@ -174,6 +187,9 @@ OPS: dict[str, tuple[object, list]] = {
          _i64, _vp, _vp, _vp, _i64, _vp],
     ),
     "nori_low_rank_backward_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32, _i64, _i32, _i32, _i32]),
+    "nori_attention_train_workspace_bytes": (_i64, [ctypes.POINTER(AttentionTrainArgs), _i32]),
+    "nori_attention_train_forward": (ctypes.c_int, [ctypes.POINTER(AttentionTrainArgs), _vp]),
+    "nori_attention_train_backward": (ctypes.c_int, [ctypes.POINTER(AttentionTrainArgs), _vp]),
     "nori_rms_norm_rows": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _i32, _vp]),
 }
 

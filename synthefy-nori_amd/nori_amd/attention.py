@@ -12,6 +12,9 @@ Mirrors the cached-attention half of ``MultiheadAttention`` in the reference
 Queries are ``[BG, Q, H, D]`` (the layout ``forward_with_kv_cache`` builds at
 layer.py:703-706) and caches ``[BG, N, 2, Hkv, D]``. The default logit scale is
 1/sqrt(D), as SDPA and the blockwise paths use (layer.py:798, 857).
+
+``trainable_attention`` is the attention over full-precision K/V with its gradients, for contexts of any
+lengths in one padded batch; the paths above are for inference.
 """
 
 from __future__ import annotations
@@ -23,6 +26,7 @@ import torch
 
 from . import _native as nat
 from .kv_cache_scaling import BlockwiseSeqKV, ScalableSeqKV
+from .norm import _FLOATS, _first_derivative, _refuse_tangents
 
 
 def _kv_strides(kv: torch.Tensor) -> tuple[int, int, int]:
@@ -256,3 +260,120 @@ def _streamed_scan(q, kv_cache: BlockwiseSeqKV, scale: float, running_output, ru
         done = torch.cuda.Event()
         done.record(compute)
         released[j] = done
+
+
+MAX_TRAIN_HEAD = 128  # NORI_ATTENTION_TRAIN_WIDTH
+
+
+def _in_fours(t: torch.Tensor) -> torch.Tensor:
+    """t as the training kernels load it, 4 elements of a head at once: itself, or a contiguous copy."""
+    if (t.stride(-1) == 1 and t.data_ptr() % (4 * t.element_size()) == 0
+            and all(n == 1 or s % 4 == 0 for n, s in zip(t.shape[:-1], t.stride()))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _steps(t: torch.Tensor, *dims: int) -> tuple[int, ...]:
+    return tuple(t.stride(i) if t.shape[i] != 1 else 0 for i in dims)
+
+
+def _train_args(q, kv, lengths, scale, out, lse) -> nat.AttentionTrainArgs:
+    bg, nq, heads, d = q.shape
+    args = nat.AttentionTrainArgs(bg=bg, nq=nq, nk=kv.shape[1], dtype=nat.dtype_code(q.dtype), heads=heads, kv_heads=kv.shape[3], d=d,
+                                  q=q.data_ptr(), kv=kv.data_ptr(), scale=scale, out=out.data_ptr(), lse=nat.ptr(lse))
+    args.q_bg, args.q_row, args.q_head = _steps(q, 0, 1, 2)
+    args.kv_bg, args.kv_row, args.kv_half, args.kv_head = _steps(kv, 0, 1, 2, 3)
+    if lengths is not None:
+        args.lengths, args.length_group, args.lengths_i64 = lengths.data_ptr(), bg // lengths.shape[0], lengths.dtype == torch.int64
+    return args
+
+
+def _train_call(name: str, args: nat.AttentionTrainArgs, backward: bool, device: torch.device) -> None:
+    lib = nat.lib()
+    with nat.on(device):
+        size = lib.nori_attention_train_workspace_bytes(args, backward)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        args.workspace, args.workspace_bytes = nat.ptr(workspace), size
+        nat.check(getattr(lib, name)(args, nat.stream_of(device)), "trainable_attention backward" if backward else "trainable_attention")
+
+
+def _train_attend(q, kv, lengths, scale, keep):
+    """(out, the rows' log-sum-exp where it is to be kept, None else)."""
+    bg, nq, heads, _ = q.shape
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((bg, heads, nq), dtype=torch.float32, device=q.device) if keep else None
+    if out.numel():
+        _train_call("nori_attention_train_forward", _train_args(_in_fours(q), _in_fours(kv), lengths, scale, out, lse), False, q.device)
+    return out, lse
+
+
+class _TrainableAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, kv, lengths, scale):
+        out, lse = _train_attend(q, kv, lengths, scale, True)
+        ctx.save_for_backward(q, kv, lengths, out, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @_first_derivative
+    def backward(ctx, dout):
+        q, kv, lengths, out, lse = ctx.saved_tensors
+        need_q, need_kv = ctx.needs_input_grad[:2]
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
+        dkv = torch.empty(kv.shape, dtype=kv.dtype, device=kv.device) if need_kv else None
+        if (need_q and q.numel()) or (need_kv and kv.numel()):
+            q, kv, dout = _in_fours(q), _in_fours(kv), _in_fours(dout)
+            args = _train_args(q, kv, lengths, ctx.scale, out, lse)
+            args.dout, args.dq, args.dkv = dout.data_ptr(), nat.ptr(dq), nat.ptr(dkv)
+            args.do_bg, args.do_row, args.do_head = _steps(dout, 0, 1, 2)
+            _train_call("nori_attention_train_backward", args, True, q.device)
+        return dq, dkv, None, None
+
+
+def trainable_attention(q: torch.Tensor, kv: torch.Tensor, key_lengths: torch.Tensor | None = None, *,
+                        scale: float | None = None) -> torch.Tensor:
+    """``icl_attention`` over a full-precision cache with its gradients: softmax(scale * q k^T) v for every (bg, query,
+    head) of q [BG, Q, H, D] over kv [BG, N, 2, Hkv, D], both float32, float16 or bfloat16, H a multiple of Hkv, D a multiple of
+    4 up to 128; ``scale`` defaults to 1/sqrt(D). Returns [BG, Q, H, D] in q's dtype.
+
+    ``key_lengths``: int32 or int64 [tables] on q's device, BG a multiple of the tables (a table's groups follow one another): the
+    keys of each table that count, taken between 0 and N; the rest of kv is not looked at and its gradients are zeros. Queries
+    without keys give zeros and take no gradient. None: every key.
+
+    Differentiable in q and kv (first derivatives, in reverse mode). The backward pass keeps q, kv, the result and a float32
+    log-sum-exp a row, and recomputes the probabilities. Products are summed in fp32, statistics are fp32; probabilities and
+    their gradients enter the second products rounded to the inputs' dtype, in float16 under powers of two that keep
+    small ones their bits. Sums have a fixed order: the same inputs give the same bits. Strides are taken as they
+    are where 4 elements of a head are aligned together, else through a contiguous copy."""
+    if q.dim() != 4:
+        raise ValueError(f"query must be [BG, Q, H, D], got {tuple(q.shape)}")
+    if kv.dim() != 5 or kv.shape[2] != 2:
+        raise ValueError(f"K/V must be [BG, N, 2, Hkv, D], got {tuple(kv.shape)}")
+    bg, _, heads, d = q.shape
+    if kv.shape[0] != bg:
+        raise ValueError(f"K/V batch {kv.shape[0]} does not match query batch {bg}")
+    if kv.shape[-1] != d:
+        raise ValueError(f"K/V head width must match query head width {d}, got {kv.shape[-1]}")
+    if heads == 0 or kv.shape[3] == 0 or heads % kv.shape[3]:
+        raise ValueError(f"query heads {heads} cannot attend to {kv.shape[3]} K/V heads")
+    if q.dtype not in _FLOATS:
+        raise NotImplementedError(f"trainable_attention takes float32/float16/bfloat16, got {q.dtype}")
+    if kv.dtype != q.dtype:
+        raise ValueError(f"trainable_attention: K/V are {kv.dtype}, queries {q.dtype}")
+    if d == 0 or d % 4 or d > MAX_TRAIN_HEAD:
+        raise NotImplementedError(f"trainable_attention takes head widths that are multiples of 4 up to {MAX_TRAIN_HEAD}, got {d}")
+    scale = 1.0 / math.sqrt(float(d)) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"trainable_attention: the scale must be finite, got {scale}")
+    if key_lengths is not None:
+        if not isinstance(key_lengths, torch.Tensor) or key_lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError("key_lengths must be an int32 or int64 tensor")
+        if key_lengths.dim() != 1 or (bg and (key_lengths.shape[0] == 0 or bg % key_lengths.shape[0])):
+            raise ValueError(f"key_lengths {tuple(key_lengths.shape)} do not divide a batch of {bg}")
+        key_lengths = key_lengths.contiguous()
+    _refuse_tangents("trainable_attention", q, kv)
+    nat.require_device(q, kv, key_lengths)
+    if torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad):
+        return _TrainableAttention.apply(q, kv, key_lengths, scale)
+    return _train_attend(q, kv, key_lengths, scale, False)[0]
