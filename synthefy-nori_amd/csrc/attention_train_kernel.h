@@ -3,58 +3,12 @@
 #pragma once
 
 #include "attention_train.h"
+#include "train_matrix.h"
 
 namespace nori {
 namespace attn_train {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-// An operand of 16 steps of a contraction: 8 elements a lane. Chunk: 4 elements, the unit of loads (head widths are
-// multiples of 4). kRows: rows of a tile that passes. kBias: the power of two on p in its 16-bit form.
-template <int DT> struct El;
-template <> struct El<NORI_F16> {
-    using T = uint16_t;
-    using Frag = f16x8;
-    using Chunk = u32x2;
-    static constexpr int kRows = 64, kPad = 8;
-    // p is below 2^-14, where float16 loses bits, for most keys of a long context: times 2^15 it keeps them to 2^-29
-    static constexpr float kBias = 15.f;
-    static constexpr bool kScaled = true;
-};
-template <> struct El<NORI_BF16> {
-    using T = uint16_t;
-    using Frag = bf16x8;
-    using Chunk = u32x2;
-    static constexpr int kRows = 64, kPad = 8;
-    static constexpr float kBias = 0.f;
-    static constexpr bool kScaled = false;
-};
-template <> struct El<NORI_F32> {
-    using T = float;
-    struct Frag { float v[8]; };
-    using Chunk = u32x4;
-    static constexpr int kRows = 32, kPad = 4;
-    static constexpr float kBias = 0.f;
-    static constexpr bool kScaled = false;
-};
-
-__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma(const El<NORI_F32>::Frag& a, const El<NORI_F32>::Frag& b, f32x16 c) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[i], b.v[i], c, 0, 0, 0);
-    return c;
-}
-
-// Value of lane l ^ 32.
-__device__ __forceinline__ float other_half(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), true, false);
-    return __uint_as_float((__lane_id() < 32) ? r[1] : r[0]);
-}
+using namespace train;
 
 // Geometry of a head width padded to DK (a multiple of 16): DP is DK in whole products of 32 columns.
 template <int DT, int DK> struct Geo {
@@ -72,41 +26,6 @@ template <int DT, int DK>
 __device__ __forceinline__ typename El<DT>::Frag direct(const typename El<DT>::T* tile, int row, int k, int half) {
     const auto* p = tile + row * Geo<DT, DK>::LS + 16 * k + 8 * half;
     return *reinterpret_cast<const typename El<DT>::Frag*>(p);
-}
-
-// Left operand transposed: column 32 m + lane % 32 of a tile, its rows first + 4 h .. + 3 and first + 8 + 4 h .. + 3, the
-// order in which a product leaves its rows. ds_read_b64_tr_b16 gives lane i of 16 element i % 4 of the 8 bytes that lanes
-// i / 4 + 4 j point at, j = 0 .. 3: lanes 4 j .. 4 j + 3 point along row j.
-template <int DT, int DK>
-__device__ __forceinline__ typename El<DT>::Frag transposed(const typename El<DT>::T* tile, int first, int m, int lane) {
-    constexpr int LS = Geo<DT, DK>::LS;
-    if constexpr (DT == NORI_F32) {
-        typename El<DT>::Frag f;
-        const float* p = tile + (first + 4 * (lane >> 5)) * LS + 32 * m + (lane & 31);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f.v[j] = p[((j & 3) + 8 * (j >> 2)) * LS];
-        return f;
-    } else {
-        const uint16_t* p = tile + (first + 4 * (lane >> 5) + ((lane & 15) >> 2)) * LS + 32 * m + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * LS));
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_bit_cast(typename El<DT>::Frag, both);
-    }
-}
-
-// Right operand of the contraction over a result's rows: registers 8 t .. 8 t + 7, rounded to the type (to nearest even).
-template <int DT>
-__device__ __forceinline__ typename El<DT>::Frag rounded(const float (&x)[16], int t) {
-    typename El<DT>::Frag f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        if constexpr (DT == NORI_F32) f.v[j] = x[8 * t + j];
-        else if constexpr (DT == NORI_F16) f[j] = (_Float16)x[8 * t + j];
-        else f[j] = (__bf16)x[8 * t + j];
-    }
-    return f;
 }
 
 // The operands that stay: columns 16 k + 8 h .. + 7 of the row at p, zeros past d or where the row is not there.
@@ -265,7 +184,7 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(const Args p) {
             for (int t = 0; t < 2; ++t) {
                 const auto pf = rounded<DT>(s, t);
 #pragma unroll
-                for (int j = 0; j < G::MS; ++j) o[j] = mma(transposed<DT, DK>(vs, sub * 32 + 16 * t, j, lane), pf, o[j]);
+                for (int j = 0; j < G::MS; ++j) o[j] = mma(transposed<DT, G::LS>(vs, sub * 32 + 16 * t, 32 * j, lane), pf, o[j]);
             }
         }
     }
@@ -402,7 +321,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Args p) {
             for (int t = 0; t < 2; ++t) {
                 const auto f = rounded<DT>(ds, t);
 #pragma unroll
-                for (int j = 0; j < G::MS; ++j) dq[j] = mma(transposed<DT, DK>(ks, sub * 32 + 16 * t, j, lane), f, dq[j]);
+                for (int j = 0; j < G::MS; ++j) dq[j] = mma(transposed<DT, G::LS>(ks, sub * 32 + 16 * t, 32 * j, lane), f, dq[j]);
             }
         }
     }
@@ -514,8 +433,8 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Args p) {
                 const auto pf = rounded<DT>(pr, t), f = rounded<DT>(ds, t);
 #pragma unroll
                 for (int j = 0; j < G::MS; ++j) {
-                    dv[j] = mma(transposed<DT, DK>(dos, sub * 32 + 16 * t, j, lane), pf, dv[j]);
-                    dk[j] = mma(transposed<DT, DK>(qs, sub * 32 + 16 * t, j, lane), f, dk[j]);
+                    dv[j] = mma(transposed<DT, G::LS>(dos, sub * 32 + 16 * t, 32 * j, lane), pf, dv[j]);
+                    dk[j] = mma(transposed<DT, G::LS>(qs, sub * 32 + 16 * t, 32 * j, lane), f, dk[j]);
                 }
             }
         }

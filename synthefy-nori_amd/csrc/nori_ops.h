@@ -10,7 +10,7 @@ extern "C" {
 #endif
 
 // Moves with every change of a signature or struct below; the package binds one version.
-#define NORI_OPS_VERSION 7
+#define NORI_OPS_VERSION 8
 int nori_ops_version(void);
 
 // QASS base scale of one key count (QASSMaxScaling.forward's base branch, src/synthefy_nori/model/
@@ -177,6 +177,32 @@ typedef struct {
 int64_t nori_attention_train_workspace_bytes(const nori_attention_train_args* args, int32_t backward);
 int nori_attention_train_forward(const nori_attention_train_args* args, void* stream);
 int nori_attention_train_backward(const nori_attention_train_args* args, void* stream);
+
+// Activations kept in 8 bits (checkpoint.hip). Of every NORI_CHECKPOINT_GROUP columns of a row (the last group may be shorter): a
+// scale, fp32(amax / 127), and int8 codes, the nearest whole number to x / scale (ties to even, -127 .. 127; 0 where the
+// scale is 0); a code stands for code * scale. A group with an infinity or NaN stands for NaN throughout. codes
+// [rows, code_stride] with code_stride cols rounded up to 16, the columns past cols 0; scales [rows, groups]; codes 16-byte
+// aligned. x rows at x_row_stride, any alignment.
+#define NORI_CHECKPOINT_GROUP 128
+int nori_checkpoint_quantize(const void* x, int dtype, int64_t rows, int32_t cols, int64_t x_row_stride, void* codes, float* scales,
+                             void* stream);
+
+// The SwiGLU gate y = silu(g) u (fp32, rounded once) of gu [rows, 2 hidden], gate columns first; codes and scales (both NULL
+// in inference) keep g and then u, each as nori_checkpoint_quantize lays out [rows, hidden]. Its backward pass: dgu [rows, 2 hidden]
+// contiguous from the values that the codes stand for, dg = dy u sigma(g) (1 + g (1 - sigma(g))), du = dy g sigma(g).
+int nori_checkpoint_silu_mul(const void* gu, int dtype, int64_t rows, int32_t hidden, int64_t gu_row_stride, void* y, void* codes,
+                             float* scales, void* stream);
+int nori_checkpoint_silu_mul_backward(const void* codes, const float* scales, int dtype, int64_t rows, int32_t hidden, const void* dy,
+                                      int64_t dy_row_stride, void* dgu, void* stream);
+
+// The gradients of a projection's weight and bias over rows kept in 8 bits (checkpoint_grad.hip): dw [n, k] = sum over rows of
+// dy^T x, x what the codes stand for rounded to dy's dtype, db [n] = sum of dy; each NULL where it is not asked for, of its own
+// dtype (dy's or fp32), contiguous. The workspace, of nori_checkpoint_grad_workspace_bytes and 16-byte aligned, takes the sums
+// of parts of the rows, which are joined in order. Sums are fp32. No rows: zeros.
+int64_t nori_checkpoint_grad_workspace_bytes(int dtype, int64_t rows, int32_t n, int32_t k);
+int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int32_t n, int64_t dy_row_stride, const void* codes,
+                         const float* scales, int32_t k, void* dw, int dw_dtype, void* db, int db_dtype, void* workspace,
+                         int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

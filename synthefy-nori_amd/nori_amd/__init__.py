@@ -15,6 +15,7 @@ low-rank adapters beside its projections (``adapters``).
 from . import _native, encoders, layer, transformer
 from .adapters import AdapterPlan, LowRankAdapters, ReadoutAdapters, adapted_linear, low_rank_update
 from .attention import attend_dense, compute_attention_blockwise, icl_attention, trainable_attention
+from .checkpoint import checkpointed_linear, checkpointed_silu_mul
 from .kv_cache_scaling import BlockwiseSeqKV, ScalableSeqKV, dequantize_int8, quantize_int8, scale_caches
 from .kv_project import project_quantize_kv
 from .api import NoriRegressor
@@ -27,6 +28,8 @@ __all__ = [
     "LowRankAdapters",
     "ReadoutAdapters",
     "adapted_linear",
+    "checkpointed_linear",
+    "checkpointed_silu_mul",
     "low_rank_update",
     "trainable_attention",
     "trainable_layer_norm",

@@ -144,7 +144,7 @@ class AttentionTrainArgs(ctypes.Structure):
 
 
 # The package's own entry points beyond the C ABI (csrc/nori_ops.h), and their version.
-OPS_VERSION = 7
+OPS_VERSION = 8
 OPS: dict[str, tuple[object, list]] = {
     "nori_qass_base": (ctypes.c_int, [_f32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
     "nori_linear_f16_w32": (
@@ -190,6 +190,13 @@ OPS: dict[str, tuple[object, list]] = {
     "nori_attention_train_workspace_bytes": (_i64, [ctypes.POINTER(AttentionTrainArgs), _i32]),
     "nori_attention_train_forward": (ctypes.c_int, [ctypes.POINTER(AttentionTrainArgs), _vp]),
     "nori_attention_train_backward": (ctypes.c_int, [ctypes.POINTER(AttentionTrainArgs), _vp]),
+    "nori_checkpoint_quantize": (ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _vp]),
+    "nori_checkpoint_silu_mul": (ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _vp, _vp]),
+    "nori_checkpoint_silu_mul_backward": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _i64, _vp, _vp]),
+    "nori_checkpoint_grad_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32]),
+    "nori_checkpoint_grad": (
+        ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i64, _vp],
+    ),
     "nori_rms_norm_rows": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _vp, _i32, _vp]),
 }
 
