@@ -37,6 +37,7 @@ struct Args {
     float* part_lse;
     float* delta;
     float c;              // scale * log2(e)
+    bool wide;            // 16-byte chunks of the 16-bit types
 };
 
 // Keys of batch entry b.

@@ -107,10 +107,17 @@ int join(Kind kind, const Args& p, hipStream_t stream) {
     return launch_status("attention_train join");
 }
 
-// A pointer and the strides of its rows, in elements: loads take 4 at once.
-bool loads(const void* p, int size, std::initializer_list<int64_t> strides) {
-    if (reinterpret_cast<uintptr_t>(p) % (4 * size)) return false;
-    return std::all_of(strides.begin(), strides.end(), [](int64_t s) { return s % 4 == 0; });
+// A pointer and its strides, in elements: loads take n at once.
+bool loads(const void* p, int size, std::initializer_list<int64_t> strides, int n = 4) {
+    if (reinterpret_cast<uintptr_t>(p) % (n * size)) return false;
+    return std::all_of(strides.begin(), strides.end(), [n](int64_t s) { return s % n == 0; });
+}
+
+// Whether everything that is read lies in 16-byte chunks of a 16-bit type.
+bool wide(const nori_attention_train_args& a, bool backward) {
+    return a.dtype != NORI_F32 && a.d % 8 == 0 && loads(a.q, 2, {a.q_bg, a.q_row, a.q_head}, 8) &&
+           loads(a.kv, 2, {a.kv_bg, a.kv_row, a.kv_half, a.kv_head}, 8) && loads(a.out, 2, {}, 8) &&
+           (!backward || loads(a.dout, 2, {a.do_bg, a.do_row, a.do_head}, 8));
 }
 
 int check(const nori_attention_train_args* a, bool backward) {
@@ -142,6 +149,10 @@ int check(const nori_attention_train_args* a, bool backward) {
         if (!loads(a->kv, size, {a->kv_bg, a->kv_row, a->kv_half, a->kv_head}) || (backward && !loads(a->dkv, size, {})))
             return fail(NORI_ERR_UNSUPPORTED, "%s: key rows not aligned to 4 elements", what);
     }
+    // a tile's rows are at 32-bit byte offsets from its first
+    constexpr int64_t far = 1LL << 24;
+    for (int64_t s : {a->q_row, a->kv_row, backward ? a->do_row : 0})
+        if (s < 0 || s > far) return fail(NORI_ERR_UNSUPPORTED, "%s: a row stride of %lld; up to 2^24 is taken", what, (long long)s);
     const Kind kinds[3] = {kForward, kDq, kDkv};
     for (Kind k : kinds) {
         const Args p = plan(*a, k);
@@ -178,6 +189,7 @@ extern "C" int nori_attention_train_forward(const nori_attention_train_args* a, 
     if (int rc = check_workspace(a, false)) return rc;
     hipStream_t stream = (hipStream_t)stream_v;
     Args p = plan(*a, kForward);
+    p.wide = wide(*a, false);
     p.part = reinterpret_cast<float*>(a->workspace);
     p.part_lse = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + aligned16(part_bytes(p, kForward)));
     if (int rc = launch_typed(kForward, p, stream)) return rc;
@@ -192,6 +204,7 @@ extern "C" int nori_attention_train_backward(const nori_attention_train_args* a,
     hipStream_t stream = (hipStream_t)stream_v;
     float* delta = reinterpret_cast<float*>(a->workspace);
     Args q = plan(*a, kDq);
+    q.wide = wide(*a, true);
     if (a->nq > 0) {
         if (!a->dq) q.splits = 1;  // the rows' sums alone
         q.delta = delta;
@@ -202,6 +215,7 @@ extern "C" int nori_attention_train_backward(const nori_attention_train_args* a,
     }
     if (!a->dkv || a->nk == 0) return NORI_OK;
     Args kv = plan(*a, kDkv);
+    kv.wide = q.wide;
     kv.delta = delta;
     kv.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + aligned16(part_rows(q, kDq) * 4));
     if (int rc = launch_typed(kDkv, kv, stream)) return rc;

@@ -4,7 +4,7 @@
 namespace nori {
 namespace attn_train {
 
-int launch_bf16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) { return launch_width<NORI_BF16>(kind, p, blocks, stream); }
+int launch_bf16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) { return launch_chunks<NORI_BF16>(kind, p, blocks, stream); }
 
 }  // namespace attn_train
 }  // namespace nori

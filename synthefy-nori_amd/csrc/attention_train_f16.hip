@@ -4,7 +4,7 @@
 namespace nori {
 namespace attn_train {
 
-int launch_f16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) { return launch_width<NORI_F16>(kind, p, blocks, stream); }
+int launch_f16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) { return launch_chunks<NORI_F16>(kind, p, blocks, stream); }
 
 }  // namespace attn_train
 }  // namespace nori

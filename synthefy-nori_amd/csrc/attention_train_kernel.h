@@ -16,9 +16,7 @@ template <int DT, int DK> struct Geo {
     using T = typename E::T;
     static constexpr int DP = (DK + 31) / 32 * 32;
     static constexpr int LS = DP + E::kPad;      // elements from one row of a tile to the next
-    static constexpr int KS = DK / 16, MS = DP / 32;
-    static constexpr int CH = DK / 4;            // chunks a row
-    static constexpr int N = (E::kRows * CH + kThreads - 1) / kThreads;  // chunks a thread, a tile
+    static constexpr int KS = DK / 16, MS = DP / 32, NS = E::kRows / 32;
 };
 
 // Left operand: row `row` (lane % 32 of a step's 32) of a tile, its columns 16 k + 8 h .. + 7.
@@ -29,16 +27,17 @@ __device__ __forceinline__ typename El<DT>::Frag direct(const typename El<DT>::T
 }
 
 // The operands that stay: columns 16 k + 8 h .. + 7 of the row at p, zeros past d or where the row is not there.
-template <int DT, int DK>
+template <int DT, int DK, int W>
 __device__ __forceinline__ void load_own(typename El<DT>::Frag (&f)[DK / 16], const typename El<DT>::T* p, bool there, int d, int half) {
     using E = El<DT>;
+    typedef uint32_t Chunk __attribute__((ext_vector_type(W * sizeof(typename E::T) / 4)));
 #pragma unroll
     for (int k = 0; k < DK / 16; ++k) {
-        typename E::Chunk c[2] = {};
+        Chunk c[8 / W] = {};
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int at = 16 * k + 8 * half + 4 * j;
-            if (there && at < d) c[j] = *reinterpret_cast<const typename E::Chunk*>(p + at);
+        for (int j = 0; j < 8 / W; ++j) {
+            const int at = 16 * k + 8 * half + W * j;
+            if (there && at < d) c[j] = *reinterpret_cast<const Chunk*>(p + at);
         }
         f[k] = __builtin_bit_cast(typename E::Frag, c);
     }
@@ -78,44 +77,85 @@ __device__ __forceinline__ Block block_of(const Args& p) {
     return w;
 }
 
-// A tile of two tensors on its way to LDS: chunks in registers, asked for while the tile before is worked on.
-template <int DT, int DK> struct Stage {
+// A tile of two tensors on its way to LDS: chunks of W elements in registers, asked for while the tile before is worked on.
+// A thread's chunks are at the same places of every tile: 32-bit byte offsets from the tile's first row, which moves on
+// uniformly (the host keeps strides to what that takes).
+template <int DT, int DK, int W> struct Stage {
     using G = Geo<DT, DK>;
     using E = El<DT>;
     using T = typename E::T;
-    typename E::Chunk x[G::N], y[G::N];
+    typedef uint32_t Chunk __attribute__((ext_vector_type(W * sizeof(T) / 4)));
+    static constexpr int CH = DK / W;                                       // chunks a row
+    static constexpr int N = (E::kRows * CH + kThreads - 1) / kThreads;     // chunks a thread, a tile
+    Chunk x[N], y[N];
+    uint32_t ox[N], oy[N];
+    int row[N];  // past every tile for chunks that no row has: they stay zero
 
-    // at(row, two pointers): the row's first elements
-    template <class At>
-    __device__ __forceinline__ void load(int first, int end, int d, At at) {
+    __device__ __forceinline__ void place(int d, int64_t x_stride, int64_t y_stride) {
 #pragma unroll
-        for (int i = 0; i < G::N; ++i) {
-            const int idx = threadIdx.x + i * kThreads, row = first + idx / G::CH, col = 4 * (idx % G::CH);
-            x[i] = {};
-            y[i] = {};
-            if (idx < E::kRows * G::CH && row < end && col < d) {
+        for (int i = 0; i < N; ++i) {
+            const int idx = threadIdx.x + i * kThreads, r = idx / CH, col = W * (idx % CH);
+            row[i] = r < E::kRows && col < d ? r : 1 << 30;
+            ox[i] = (uint32_t)(r * (uint32_t)x_stride + col) * sizeof(T);
+            oy[i] = (uint32_t)(r * (uint32_t)y_stride + col) * sizeof(T);
+        }
+    }
+    // `left` rows from px and py on
+    __device__ __forceinline__ void load(const T* px, const T* py, int left) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] = Chunk{};
+            y[i] = Chunk{};
+            if (row[i] < left) {
+                x[i] = *reinterpret_cast<const Chunk*>(reinterpret_cast<const char*>(px) + ox[i]);
+                y[i] = *reinterpret_cast<const Chunk*>(reinterpret_cast<const char*>(py) + oy[i]);
+            }
+        }
+    }
+    // the same where rows from `over` on lie wx and wy bytes further (the next head's)
+    __device__ __forceinline__ void load_over(const T* px, const T* py, int left, int over, int64_t wx, int64_t wy) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] = Chunk{};
+            y[i] = Chunk{};
+            if (row[i] < left) {
+                const bool next = row[i] >= over;
+                x[i] = *reinterpret_cast<const Chunk*>(reinterpret_cast<const char*>(px) + ox[i] + (next ? wx : 0));
+                y[i] = *reinterpret_cast<const Chunk*>(reinterpret_cast<const char*>(py) + oy[i] + (next ? wy : 0));
+            }
+        }
+    }
+    // rows anywhere
+    template <class At>
+    __device__ __forceinline__ void load_each(int left, At at) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] = Chunk{};
+            y[i] = Chunk{};
+            if (row[i] < left) {
                 const T *px, *py;
-                at(row, px, py);
-                x[i] = *reinterpret_cast<const typename E::Chunk*>(px + col);
-                y[i] = *reinterpret_cast<const typename E::Chunk*>(py + col);
+                at(row[i], px, py);
+                const int col = W * ((threadIdx.x + i * kThreads) % CH);
+                x[i] = *reinterpret_cast<const Chunk*>(px + col);
+                y[i] = *reinterpret_cast<const Chunk*>(py + col);
             }
         }
     }
     __device__ __forceinline__ void store(T* tx, T* ty) const {
 #pragma unroll
-        for (int i = 0; i < G::N; ++i) {
-            const int idx = threadIdx.x + i * kThreads, to = idx / G::CH * G::LS + 4 * (idx % G::CH);
-            if (idx < E::kRows * G::CH) {
-                *reinterpret_cast<typename E::Chunk*>(tx + to) = x[i];
-                *reinterpret_cast<typename E::Chunk*>(ty + to) = y[i];
+        for (int i = 0; i < N; ++i) {
+            const int idx = threadIdx.x + i * kThreads, to = idx / CH * G::LS + W * (idx % CH);
+            if (E::kRows * CH % kThreads == 0 || idx < E::kRows * CH) {
+                *reinterpret_cast<Chunk*>(tx + to) = x[i];
+                *reinterpret_cast<Chunk*>(ty + to) = y[i];
             }
         }
     }
 };
 
 // ---------------------------------------------------------------- forward
-template <int DT, int DK>
-__global__ __launch_bounds__(kThreads) void forward_kernel(const Args p) {
+template <int DT, int DK, int W>
+__global__ __launch_bounds__(kThreads, DK <= 64 ? 3 : 2) void forward_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
@@ -133,56 +173,68 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(const Args p) {
     const int end = (int)min((int64_t)length, w.split * p.per_split + p.per_split);
 
     typename E::Frag qf[G::KS];
-    load_own<DT, DK>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
-    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head;
-    const auto at = [&](int key, const T*& x, const T*& y) { x = kv + key * a.kv_row; y = x + a.kv_half; };
-    // the running maximum wants a positive factor: a negative one changes signs before, one of 0 makes the logits 0
+    load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
+    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + begin * a.kv_row;
+    // the running maximum wants a positive factor: a negative one changes signs first, one of 0 makes the logits 0
     const float c = p.c == 0.f ? 1.f : fabsf(p.c);
-    const float sign = p.c < 0.f ? -1.f : (p.c == 0.f ? 0.f : 1.f);
+    if (p.c <= 0.f) {
+        const float sign = p.c < 0.f ? -1.f : 0.f;
+#pragma unroll
+        for (int k = 0; k < G::KS; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) at(qf[k], j) = at(qf[k], j) * sign;
+    }
 
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;  // of this half-wave's keys
     f32x16 o[G::MS] = {};
-    Stage<DT, DK> stage;
-    if (begin < end) stage.load(begin, end, a.d, at);
+    Stage<DT, DK, W> stage;
+    stage.place(a.d, a.kv_row, a.kv_row);
+    if (begin < end) stage.load(kv, kv + a.kv_half, end - begin);
     for (int first = begin; first < end; first += E::kRows) {
         __syncthreads();
         stage.store(ks, vs);
         __syncthreads();
-        if (first + E::kRows < end) stage.load(first + E::kRows, end, a.d, at);
+        kv += E::kRows * a.kv_row;
+        if (first + E::kRows < end) stage.load(kv, kv + a.kv_half, end - first - E::kRows);
+        f32x16 s[G::NS];
 #pragma unroll
-        for (int sub = 0; sub < E::kRows / 32; ++sub) {
-            if (first + sub * 32 >= end) break;
-            f32x16 acc = {};
+        for (int sub = 0; sub < G::NS; ++sub) {
+            s[sub] = f32x16{};
 #pragma unroll
-            for (int k = 0; k < G::KS; ++k) acc = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], acc);
-            float s[16];
-            float top = -INFINITY;
+            for (int k = 0; k < G::KS; ++k) s[sub] = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s[sub]);
+        }
+        if (first + E::kRows > end) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = sign * acc[i];
-            if (first + sub * 32 + 32 > end) {
+            for (int sub = 0; sub < G::NS; ++sub)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) s[i] = -INFINITY;
-            }
+                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) s[sub][i] = -INFINITY;
+        }
+        float top = s[0][0];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
-            top = fmaxf(m, fmaxf(top, other_half(top)));
-            const float base = top == -INFINITY ? 0.f : top;  // (all keys so far at -inf: their p is 0)
-            const float shrink = __builtin_amdgcn_exp2f((m - base) * c);
-            m = top;
-            const float off = E::kBias - 1.f - base * c;  // p up to 2^(kBias - 1): inside float16's range
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, off));
-                sum += s[i];
-            }
-            l = l * shrink + sum;
+        for (int i = 1; i < 16 * G::NS; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+        top = fmaxf(top, other_half(top));
+        // the maximum that p is taken against moves when one passes it by 2^kSlack: rarely, after the first tiles
+        if (__any((top - m) * c > E::kSlack)) {
+            const float next = fmaxf(m, top);
+            const float shrink = next == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
+            m = next;
+            l *= shrink;
 #pragma unroll
             for (int j = 0; j < G::MS; ++j) o[j] *= shrink;
+        }
+        const float off = E::kTop - (m == -INFINITY ? 0.f : m * c);  // (all keys so far at -inf: their p is 0)
+#pragma unroll
+        for (int sub = 0; sub < G::NS; ++sub) {
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(fmaf(s[sub][i], c, off));
+                l += x[i];
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const auto pf = rounded<DT>(s, t);
+                const auto pf = rounded<DT>(x, t);
 #pragma unroll
                 for (int j = 0; j < G::MS; ++j) o[j] = mma(transposed<DT, G::LS>(vs, sub * 32 + 16 * t, 32 * j, lane), pf, o[j]);
             }
@@ -191,7 +243,7 @@ __global__ __launch_bounds__(kThreads) void forward_kernel(const Args p) {
     if (!there) return;
     l += other_half(l);
     const float inv = begin < end ? 1.f / l : 0.f;
-    const float lse2 = begin < end ? __builtin_amdgcn_logf(l) - (E::kBias - 1.f) + m * c : -INFINITY;
+    const float lse2 = begin < end ? __builtin_amdgcn_logf(l) - E::kTop + m * c : -INFINITY;
     if (p.splits > 1) {
         const int64_t units = a.bg * a.kv_heads;
         const int64_t to = (w.split * units + w.unit) * p.rows + r;
@@ -225,11 +277,11 @@ struct Scale {
     float f = 0.f;  // 0: nothing but zeros so far
 
     // the values of this step with the factor on; acc takes a change of it
-    template <int MS>
-    __device__ __forceinline__ void apply(float (&x)[16], f32x16 (&acc)[MS]) {
+    template <int NS, int MS>
+    __device__ __forceinline__ void apply(float (&x)[NS][16], f32x16 (&acc)[MS]) {
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+        for (int i = 0; i < 16 * NS; ++i) top = fmaxf(top, fabsf(x[i / 16][i % 16]));
         top = fmaxf(top, other_half(top));
         const bool change = f == 0.f ? top > 0.f : top * f > 32768.f;
         if (__any(change)) {
@@ -245,14 +297,14 @@ struct Scale {
             f = next;
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= f;
+        for (int i = 0; i < 16 * NS; ++i) x[i / 16][i % 16] *= f;
     }
     __device__ __forceinline__ float inverse() const { return f == 0.f ? 1.f : 1.f / f; }
 };
 
 // ---------------------------------------------------------------- dq, and delta for dk and dv
-template <int DT, int DK>
-__global__ __launch_bounds__(kThreads) void dq_kernel(const Args p) {
+template <int DT, int DK, int W>
+__global__ __launch_bounds__(kThreads, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
@@ -271,8 +323,8 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Args p) {
     const int end = a.dq ? (int)min((int64_t)length, w.split * p.per_split + p.per_split) : begin;
 
     typename E::Frag dof[G::KS], qf[G::KS];
-    load_own<DT, DK>(dof, reinterpret_cast<const T*>(a.dout) + w.b * a.do_bg + row.query * a.do_row + row.head * a.do_head, there, a.d, half);
-    load_own<DT, DK>(qf, reinterpret_cast<const T*>(a.out) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d, there, a.d, half);
+    load_own<DT, DK, W>(dof, reinterpret_cast<const T*>(a.dout) + w.b * a.do_bg + row.query * a.do_row + row.head * a.do_head, there, a.d, half);
+    load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.out) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d, there, a.d, half);
     float delta = 0.f;
 #pragma unroll
     for (int k = 0; k < G::KS; ++k) {
@@ -285,45 +337,51 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Args p) {
     delta += other_half(delta);
     if (there && half == 0 && w.split == 0) p.delta[unit_row] = delta;
     if (!a.dq) return;
-    load_own<DT, DK>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
+    load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
     const float lse2 = there ? a.lse[unit_row] * kLog2e : 0.f;
-    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head;
-    const auto at = [&](int key, const T*& x, const T*& y) { x = kv + key * a.kv_row; y = x + a.kv_half; };
+    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + begin * a.kv_row;
 
     f32x16 dq[G::MS] = {};
     Scale scale;
-    Stage<DT, DK> stage;
-    if (begin < end) stage.load(begin, end, a.d, at);
+    Stage<DT, DK, W> stage;
+    stage.place(a.d, a.kv_row, a.kv_row);
+    if (begin < end) stage.load(kv, kv + a.kv_half, end - begin);
     for (int first = begin; first < end; first += E::kRows) {
         __syncthreads();
         stage.store(ks, vs);
         __syncthreads();
-        if (first + E::kRows < end) stage.load(first + E::kRows, end, a.d, at);
+        kv += E::kRows * a.kv_row;
+        if (first + E::kRows < end) stage.load(kv, kv + a.kv_half, end - first - E::kRows);
+        float ds[G::NS][16];
 #pragma unroll
-        for (int sub = 0; sub < E::kRows / 32; ++sub) {
-            if (first + sub * 32 >= end) break;
-            f32x16 s = {}, dp = {};
+        for (int sub = 0; sub < G::NS; ++sub) {
+            f32x16 s = {}, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] = -delta;
 #pragma unroll
             for (int k = 0; k < G::KS; ++k) {
                 s = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s);
                 dp = mma(direct<DT, DK>(vs, sub * 32 + (lane & 31), k, half), dof[k], dp);
             }
-            float ds[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse2)) * (dp[i] - delta);
-            if (first + sub * 32 + 32 > end) {
+            for (int i = 0; i < 16; ++i) ds[sub][i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse2)) * dp[i];
+        }
+        if (first + E::kRows > end) {
+#pragma unroll
+            for (int sub = 0; sub < G::NS; ++sub)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) ds[i] = 0.f;
-            }
-            if constexpr (E::kScaled) scale.apply(ds, dq);
+                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) ds[sub][i] = 0.f;
+        }
+        if constexpr (E::kScaled) scale.apply(ds, dq);
+#pragma unroll
+        for (int sub = 0; sub < G::NS; ++sub)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const auto f = rounded<DT>(ds, t);
+                const auto f = rounded<DT>(ds[sub], t);
 #pragma unroll
                 for (int j = 0; j < G::MS; ++j) dq[j] = mma(transposed<DT, G::LS>(ks, sub * 32 + 16 * t, 32 * j, lane), f, dq[j]);
             }
-        }
     }
     if (!there) return;
     const float by = a.scale * (E::kScaled ? scale.inverse() : 1.f);
@@ -342,15 +400,15 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Args p) {
 }
 
 // ---------------------------------------------------------------- dk and dv
-template <int DT, int DK>
-__global__ __launch_bounds__(kThreads) void dkv_kernel(const Args p) {
+template <int DT, int DK, int W>
+__global__ __launch_bounds__(kThreads, DK <= 64 ? 2 : 1) void dkv_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
     __shared__ __attribute__((aligned(16))) T qs[E::kRows * G::LS];
     __shared__ __attribute__((aligned(16))) T dos[E::kRows * G::LS];
     __shared__ __attribute__((aligned(16))) float off[E::kRows];    // kBias - log2 of the row's sum
-    __shared__ __attribute__((aligned(16))) float deltas[E::kRows];
+    __shared__ __attribute__((aligned(16))) float deltas[E::kRows];  // negative: what the products of dout and v start from
     const auto& a = p.a;
     const Block w = block_of(p);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
@@ -364,32 +422,49 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Args p) {
 
     typename E::Frag kf[G::KS], vf[G::KS];
     const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + (there ? key * a.kv_row : 0);
-    load_own<DT, DK>(kf, kv, there, a.d, half);
-    load_own<DT, DK>(vf, kv + a.kv_half, there, a.d, half);
-    const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.q_bg;
-    const T* dout = reinterpret_cast<const T*>(a.dout) + w.b * a.do_bg;
-    const auto at = [&](int r, const T*& x, const T*& y) {
-        const Row row = row_of(p, w.hk, r);
-        x = q + row.query * a.q_row + row.head * a.q_head;
-        y = dout + row.query * a.do_row + row.head * a.do_head;
-    };
+    load_own<DT, DK, W>(kf, kv, there, a.d, half);
+    load_own<DT, DK, W>(vf, kv + a.kv_half, there, a.d, half);
+    const T* q = reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + w.hk * p.group * a.q_head;
+    const T* dout = reinterpret_cast<const T*>(a.dout) + w.b * a.do_bg + w.hk * p.group * a.do_head;
+    const float* lse = a.lse + w.unit * p.rows;
+    const float* delta = p.delta + w.unit * p.rows;
+    // where a tile's first row is: head `at_head` of the unit's, query `at_query`
+    const int nq = (int)a.nq;
+    int at_head = begin < end ? begin / nq : 0, at_query = begin - at_head * nq;
 
     f32x16 dk[G::MS] = {}, dv[G::MS] = {};
     Scale scale;
-    Stage<DT, DK> stage;
+    Stage<DT, DK, W> stage;
+    stage.place(a.d, a.q_row, a.do_row);
     float next_off = 0.f, next_delta = 0.f;
-    const auto statistics = [&](int first) {
-        const int r = first + threadIdx.x;
+    const auto load = [&](int first) {
+        const int left = end - first;
+        const T* px = q + at_head * a.q_head + at_query * a.q_row;
+        const T* py = dout + at_head * a.do_head + at_query * a.do_row;
+        if (at_query + E::kRows <= nq || p.group == 1) {
+            stage.load(px, py, left);
+        } else if (nq >= E::kRows) {
+            stage.load_over(px, py, left, nq - at_query, (a.q_head - nq * a.q_row) * (int64_t)sizeof(T),
+                            (a.do_head - nq * a.do_row) * (int64_t)sizeof(T));
+        } else {
+            stage.load_each(left, [&](int row, const T*& x, const T*& y) {
+                const int h = (first + row) / nq, i = first + row - h * nq;
+                x = q + h * a.q_head + i * a.q_row;
+                y = dout + h * a.do_head + i * a.do_row;
+            });
+        }
+        at_query += E::kRows;
+        while (at_query >= nq) {
+            at_query -= nq;
+            ++at_head;
+        }
         if (threadIdx.x < E::kRows) {
-            const bool in = r < end;
-            next_off = in ? E::kBias - a.lse[w.unit * p.rows + r] * kLog2e : 0.f;
-            next_delta = in ? p.delta[w.unit * p.rows + r] : 0.f;
+            const bool in = (int)threadIdx.x < left;
+            next_off = in ? E::kBias - lse[first + threadIdx.x] * kLog2e : 0.f;
+            next_delta = in ? -delta[first + threadIdx.x] : 0.f;
         }
     };
-    if (begin < end) {
-        stage.load(begin, end, a.d, at);
-        statistics(begin);
-    }
+    if (begin < end) load(begin);
     for (int first = begin; first < end; first += E::kRows) {
         __syncthreads();
         stage.store(qs, dos);
@@ -398,39 +473,40 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Args p) {
             deltas[threadIdx.x] = next_delta;
         }
         __syncthreads();
-        if (first + E::kRows < end) {
-            stage.load(first + E::kRows, end, a.d, at);
-            statistics(first + E::kRows);
-        }
+        if (first + E::kRows < end) load(first + E::kRows);
 #pragma unroll
-        for (int sub = 0; sub < E::kRows / 32; ++sub) {
-            if (first + sub * 32 >= end) break;
-            f32x16 s = {}, dp = {};
+        for (int sub = 0; sub < G::NS; ++sub) {
+            f32x16 s = {}, dp;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(&deltas[sub * 32 + 2 * i + 4 * half]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dp[i + j] = d4[j];
+            }
 #pragma unroll
             for (int k = 0; k < G::KS; ++k) {
                 s = mma(direct<DT, DK>(qs, sub * 32 + (lane & 31), k, half), kf[k], s);
                 dp = mma(direct<DT, DK>(dos, sub * 32 + (lane & 31), k, half), vf[k], dp);
             }
-            float pr[16], ds[16];
+            float pr[16], ds[1][16];
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const f32x4 o4 = *reinterpret_cast<const f32x4*>(&off[sub * 32 + 2 * i + 4 * half]);
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(&deltas[sub * 32 + 2 * i + 4 * half]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     pr[i + j] = __builtin_amdgcn_exp2f(fmaf(s[i + j], p.c, o4[j]));
-                    ds[i + j] = pr[i + j] * (dp[i + j] - d4[j]);
+                    ds[0][i + j] = pr[i + j] * dp[i + j];
                 }
             }
-            if (first + sub * 32 + 32 > end) {  // rows that are not there: 0, also beside keys that are not finite
+            if (first + E::kRows > end) {  // rows that are not there: 0, also beside keys that are not finite
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) pr[i] = ds[i] = 0.f;
+                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) pr[i] = ds[0][i] = 0.f;
             }
             if constexpr (E::kScaled) scale.apply(ds, dk);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const auto pf = rounded<DT>(pr, t), f = rounded<DT>(ds, t);
+                const auto pf = rounded<DT>(pr, t), f = rounded<DT>(ds[0], t);
 #pragma unroll
                 for (int j = 0; j < G::MS; ++j) {
                     dv[j] = mma(transposed<DT, G::LS>(dos, sub * 32 + 16 * t, 32 * j, lane), pf, dv[j]);
@@ -466,25 +542,33 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Args p) {
         }
 }
 
-template <int DT, int DK>
+template <int DT, int DK, int W>
 int launch(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
     const dim3 grid((unsigned)blocks), threads(kThreads);
     switch (kind) {
-        case kForward: hipLaunchKernelGGL((forward_kernel<DT, DK>), grid, threads, 0, stream, p); break;
-        case kDq: hipLaunchKernelGGL((dq_kernel<DT, DK>), grid, threads, 0, stream, p); break;
-        case kDkv: hipLaunchKernelGGL((dkv_kernel<DT, DK>), grid, threads, 0, stream, p); break;
+        case kForward: hipLaunchKernelGGL((forward_kernel<DT, DK, W>), grid, threads, 0, stream, p); break;
+        case kDq: hipLaunchKernelGGL((dq_kernel<DT, DK, W>), grid, threads, 0, stream, p); break;
+        case kDkv: hipLaunchKernelGGL((dkv_kernel<DT, DK, W>), grid, threads, 0, stream, p); break;
     }
     return launch_status("attention_train");
 }
 
-template <int DT>
+template <int DT, int W>
 int launch_width(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
     const int d = p.a.d;
-    if (d <= 32) return launch<DT, 32>(kind, p, blocks, stream);
-    if (d <= 48) return launch<DT, 48>(kind, p, blocks, stream);
-    if (d <= 64) return launch<DT, 64>(kind, p, blocks, stream);
-    if (d <= 96) return launch<DT, 96>(kind, p, blocks, stream);
-    return launch<DT, 128>(kind, p, blocks, stream);
+    if (d <= 32) return launch<DT, 32, W>(kind, p, blocks, stream);
+    if (d <= 48) return launch<DT, 48, W>(kind, p, blocks, stream);
+    if (d <= 64) return launch<DT, 64, W>(kind, p, blocks, stream);
+    if (d <= 96) return launch<DT, 96, W>(kind, p, blocks, stream);
+    return launch<DT, 128, W>(kind, p, blocks, stream);
+}
+
+// Chunks of 16 bytes, where the host found everything aligned to them, or of 4 elements.
+template <int DT>
+int launch_chunks(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
+    if constexpr (DT != NORI_F32)
+        if (p.wide) return launch_width<DT, 8>(kind, p, blocks, stream);
+    return launch_width<DT, 4>(kind, p, blocks, stream);
 }
 
 }  // namespace attn_train

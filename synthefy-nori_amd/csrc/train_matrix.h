@@ -17,34 +17,44 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// An operand of 16 steps of a contraction: 8 elements a lane. Chunk: 4 elements. kRows: rows of an attention tile that
+// An operand of 16 steps of a contraction: 8 elements a lane.  kRows: rows of an attention tile that
 // passes; kPad: elements between the rows of a tile in LDS. kBias: the power of two on probabilities in their 16-bit form.
 template <int DT> struct El;
 template <> struct El<NORI_F16> {
     using T = uint16_t;
     using Frag = f16x8;
-    using Chunk = u32x2;
     static constexpr int kRows = 64, kPad = 8;
-    // p is below 2^-14, where float16 loses bits, for most keys of a long context: times 2^15 it keeps them to 2^-29
-    static constexpr float kBias = 15.f;
+    // p is below 2^-14, where float16 loses bits, for most keys of a long context: times 2^15 it keeps them to 2^-29,
+    // and beside a running maximum, which p may pass by 2^kSlack, times 2^kTop to 2^-22
+    static constexpr float kBias = 15.f, kTop = 8.f, kSlack = 7.f;
     static constexpr bool kScaled = true;
 };
 template <> struct El<NORI_BF16> {
     using T = uint16_t;
     using Frag = bf16x8;
-    using Chunk = u32x2;
     static constexpr int kRows = 64, kPad = 8;
-    static constexpr float kBias = 0.f;
+    static constexpr float kBias = 0.f, kTop = 0.f, kSlack = 8.f;
     static constexpr bool kScaled = false;
 };
 template <> struct El<NORI_F32> {
     using T = float;
     struct Frag { float v[8]; };
-    using Chunk = u32x4;
     static constexpr int kRows = 32, kPad = 4;
-    static constexpr float kBias = 0.f;
+    static constexpr float kBias = 0.f, kTop = 0.f, kSlack = 8.f;
     static constexpr bool kScaled = false;
 };
+
+// Element j of an operand.
+__device__ __forceinline__ float& at(El<NORI_F32>::Frag& f, int j) { return f.v[j]; }
+template <class V>
+struct Element {
+    V& f;
+    int j;
+    __device__ __forceinline__ operator float() const { return (float)f[j]; }
+    __device__ __forceinline__ void operator=(float v) { f[j] = (__typeof__(f[0] + f[0]))v; }
+};
+__device__ __forceinline__ Element<f16x8> at(f16x8& f, int j) { return {f, j}; }
+__device__ __forceinline__ Element<bf16x8> at(bf16x8& f, int j) { return {f, j}; }
 
 __device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }

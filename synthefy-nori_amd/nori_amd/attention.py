@@ -268,7 +268,8 @@ MAX_TRAIN_HEAD = 128  # NORI_ATTENTION_TRAIN_WIDTH
 def _in_fours(t: torch.Tensor) -> torch.Tensor:
     """t as the training kernels load it, 4 elements of a head at once: itself, or a contiguous copy."""
     if (t.stride(-1) == 1 and t.data_ptr() % (4 * t.element_size()) == 0
-            and all(n == 1 or s % 4 == 0 for n, s in zip(t.shape[:-1], t.stride()))):
+            and all(n == 1 or s % 4 == 0 for n, s in zip(t.shape[:-1], t.stride()))
+            and (t.shape[1] == 1 or t.stride(1) <= 2**24)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
