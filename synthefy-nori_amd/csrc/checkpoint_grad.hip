@@ -1,31 +1,26 @@
 // The gradients of a projection's weight and bias over rows kept in 8 bits: dw = dy^T x with x what the codes stand for, db = the
-// column sums of dy. A workgroup owns 128 x 128 of dw over a part of the rows; dy and x pass through LDS as they lie, both
+// column sums of dy. A workgroup owns 256 or 128 x 128 of dw over a part of the rows; dy and x pass through LDS as they lie, both
 // operands are transposed reads, the codes are widened on their way in. A k tile is one group: a scale a row.
 #include <algorithm>
 
-#include "layer_norm_train.h"
 #include "train_matrix.h"
 
 namespace {
 
 using namespace nori;
 using namespace nori::train;
-using nori_ln::fetch;
-using nori_ln::widen;
 
 constexpr int kThreads = 256;
-constexpr int kTile = 128;  // columns of dy and of x a workgroup; the latter a group of the codes
-static_assert(kTile == NORI_CHECKPOINT_GROUP, "a k tile has one scale a row");
-constexpr int kRows = 32;   // rows a step
-constexpr int64_t kLeast = 256;  // rows of a part
+constexpr int kGroup = NORI_CHECKPOINT_GROUP;  // columns of x a workgroup: one scale a row
+constexpr int64_t kLeast = 256;                // rows of a part
 
 struct Args {
     const void* dy; int64_t rows, dy_stride; int n, k;
     const int8_t* codes; const float* scales;
     int code_stride, groups;
-    int64_t per_split; int splits, n_tiles, k_tiles;
+    int64_t per_split; int splits, tile_n, n_tiles, k_tiles;
     void *dw, *db; int dw_dtype, db_dtype;
-    float *part_w, *part_b;  // sums of parts where splits > 1
+    float *part_w, *part_b;  // sums of parts where splits > 1; those of db are of the rows' steps that a k tile takes
 };
 
 // Eight elements of a row in the tile's type.
@@ -37,115 +32,160 @@ __device__ __forceinline__ void put(void* p, int dtype, int64_t i, float v) {
     else store_elem<DT == NORI_F32 ? NORI_F16 : DT>(p, i, v);
 }
 
+// The values of 8 codes. A code is one byte u less 128, (u - 128) s = u s - 128 s is rounded once: 128 s is exact.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void grad_kernel(const Args a) {
+__device__ __forceinline__ Eight<DT> values(uint32_t lo, uint32_t hi, float s) {
+    const uint32_t w[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
+    const float off = -128.0f * s;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fmaf((float)((w[i >> 2] >> (8 * (i & 3))) & 0xffu), s, off);
+    if constexpr (DT == NORI_F32) {
+        return __builtin_bit_cast(Eight<DT>, v);
+    } else {
+        typename El<DT>::Frag f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) at(f, i) = v[i];
+        return __builtin_bit_cast(Eight<DT>, f);
+    }
+}
+
+// TN columns of dy by 128 of x a workgroup, half of each a wavefront.
+template <int DT, int TN>
+__global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
     using E = El<DT>;
     using T = typename E::T;
-    constexpr int LS = kTile + E::kPad;
-    constexpr int kEights = kRows * kTile / 8 / kThreads;  // of dy and of x, a thread
-    __shared__ __attribute__((aligned(16))) T ys[kRows * LS];
-    __shared__ __attribute__((aligned(16))) T xs[kRows * LS];
-    __shared__ float sums[kThreads / (kTile / 8)][kTile];
-    int i = blockIdx.x;
-    const int kt = i % a.k_tiles;
-    i /= a.k_tiles;
-    const int nt = i % a.n_tiles, split = i / a.n_tiles;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = 64 * (wave & 1), wk = 64 * (wave >> 1);
+    constexpr int kRows = DT == NORI_F32 ? 32 : 64;  // rows a step
+    // transposed reads take 64 bytes of four rows at once: rows 16 banks apart (mod 64) meet no other's
+    constexpr int kPad = DT == NORI_F32 ? E::kPad : 32, YS = TN + kPad, XS = kGroup + kPad;
+    constexpr int MY = TN / 64, MX = 2;              // products of 32 columns a wavefront
+    constexpr int kPerRow = TN / 8, kYStep = kThreads / kPerRow, NY = kRows / kYStep;
+    constexpr int kXStep = kThreads / (kGroup / 16), NX = kRows / kXStep;
+    __shared__ __attribute__((aligned(16))) T ys[kRows * YS];
+    __shared__ __attribute__((aligned(16))) T xs[kRows * XS];
+    const int64_t i = blockIdx.x, eights = gridDim.x & ~7u;  // neighbours, which read the same rows, on one XCD
+    const int64_t work = i < eights ? (i & 7) * (eights >> 3) + (i >> 3) : i;
+    const int kt = (int)(work % a.k_tiles), nt = (int)(work / a.k_tiles % a.n_tiles), split = (int)(work / a.k_tiles / a.n_tiles);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = TN / 2 * (wave & 1), wk = kGroup / 2 * (wave >> 1);
     const int64_t begin = split * a.per_split, end = min(a.rows, begin + a.per_split);
-    const bool own_db = a.db && kt == 0;
-    // this thread's eight columns of either tile are the same in every row it takes
-    const int col = 8 * (threadIdx.x % (kTile / 8)), first_row = threadIdx.x / (kTile / 8);
-    constexpr int kStep = kThreads / (kTile / 8);
-    const int yc = nt * kTile + col, xc = kt * kTile + col;
+    // a thread's eight columns of dy and sixteen of x are the same in every row it takes
+    const int ycol = 8 * (threadIdx.x % kPerRow), yrow = threadIdx.x / kPerRow, yc = nt * TN + ycol;
+    const int xcol = 16 * (threadIdx.x % (kGroup / 16)), xrow = threadIdx.x / (kGroup / 16), xc = kt * kGroup + xcol;
+    // lanes past the last column read the first ones: their sums are not used
+    const int yat = yc < a.n ? yc : 0, xat = xc < a.code_stride ? xc : 0;
+    const uint32_t yoff = ((uint32_t)yrow * (uint32_t)a.dy_stride + yat) * sizeof(T), xoff = xrow * a.code_stride + xat;
 
-    Eight<DT> ye[kEights];
-    uint64_t xe[kEights];
-    float xsc[kEights];
+    Eight<DT> ye[NY];
+    uint4 xe[NX];
+    float xsc[NX];
+    // A step whose rows are all there, and not the last, whose eight columns past the row's end reach into the next row
+    const auto whole = [&](int64_t from) { return from + kRows <= end && from + kRows < a.rows && a.dy_stride >= 8; };
     const auto load = [&](int64_t from) {
+        const char* py = reinterpret_cast<const char*>(a.dy) + from * a.dy_stride * (int64_t)sizeof(T);
+        const int8_t* px = a.codes + from * a.code_stride;
+        const float* ps = a.scales + from * a.groups + kt;
 #pragma unroll
-        for (int j = 0; j < kEights; ++j) {
-            const int64_t r = from + first_row + j * kStep;
-            ye[j] = {};
-            xe[j] = 0;
-            xsc[j] = 0.f;
-            if (r >= end) continue;
-            const T* p = reinterpret_cast<const T*>(a.dy) + r * a.dy_stride;
-            if (yc + 8 <= a.n) {
-                __builtin_memcpy(&ye[j], p + yc, sizeof ye[j]);
-            } else {
+        for (int j = 0; j < NY; ++j) __builtin_memcpy(&ye[j], py + j * kYStep * a.dy_stride * (int64_t)sizeof(T) + yoff, sizeof ye[j]);
+        if (!a.dw) return;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (yc + e < a.n) ye[j].e[e] = p[yc + e];
-            }
-            if (a.dw && xc < a.code_stride) {
-                xe[j] = *reinterpret_cast<const uint64_t*>(a.codes + r * a.code_stride + xc);
-                xsc[j] = a.scales[r * a.groups + kt];
-            }
+        for (int j = 0; j < NX; ++j) {
+            xe[j] = *reinterpret_cast<const uint4*>(px + j * kXStep * a.code_stride + xoff);
+            xsc[j] = ps[j * kXStep * a.groups + xrow * a.groups];
         }
     };
     float colsum[8] = {};
-    f32x16 acc[2][2] = {};
-    load(begin);
+    const auto add = [&](const Eight<DT>& y) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (DT == NORI_F32) colsum[e] += y.e[e];
+            else colsum[e] += DT == NORI_F16 ? f16_to_f32(y.e[e]) : bf16_to_f32(y.e[e]);
+        }
+    };
+    f32x16 acc[MY][MX] = {};
+    int turn = a.db ? (a.splits > 1 ? kt : (kt == 0 ? 0 : -1)) : -1;  // steps until this k tile's next one of db
+    if (whole(begin)) load(begin);
     for (int64_t from = begin; from < end; from += kRows) {
         __syncthreads();
+        if (whole(from)) {
 #pragma unroll
-        for (int j = 0; j < kEights; ++j) {
-            const int at = (first_row + j * kStep) * LS + col;
-            *reinterpret_cast<Eight<DT>*>(&ys[at]) = ye[j];
-            if (own_db) {
+            for (int j = 0; j < NY; ++j) *reinterpret_cast<Eight<DT>*>(&ys[(yrow + j * kYStep) * YS + ycol]) = ye[j];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if constexpr (DT == NORI_F32) colsum[e] += ye[j].e[e];
-                    else colsum[e] += DT == NORI_F16 ? f16_to_f32(ye[j].e[e]) : bf16_to_f32(ye[j].e[e]);
+            for (int j = 0; j < NX; ++j) {
+                Eight<DT>* to = reinterpret_cast<Eight<DT>*>(&xs[(xrow + j * kXStep) * XS + xcol]);
+                to[0] = values<DT>(xe[j].x, xe[j].y, xsc[j]);
+                to[1] = values<DT>(xe[j].z, xe[j].w, xsc[j]);
+            }
+            if (turn == 0) {
+#pragma unroll
+                for (int j = 0; j < NY; ++j) add(ye[j]);
+            }
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < NY; ++j) {
+                const int64_t r = from + yrow + j * kYStep;
+                Eight<DT> y = {};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (r < end && yc + e < a.n) y.e[e] = reinterpret_cast<const T*>(a.dy)[r * a.dy_stride + yc + e];
+                *reinterpret_cast<Eight<DT>*>(&ys[(yrow + j * kYStep) * YS + ycol]) = y;
+                if (turn == 0) add(y);
+            }
+#pragma unroll 1
+            for (int j = 0; a.dw && j < NX; ++j) {
+                const int64_t r = from + xrow + j * kXStep;
+                uint4 x = {};
+                float sc = 0.f;
+                if (r < end) {
+                    x = *reinterpret_cast<const uint4*>(a.codes + r * a.code_stride + xat);
+                    sc = a.scales[r * a.groups + kt];
                 }
+                Eight<DT>* to = reinterpret_cast<Eight<DT>*>(&xs[(xrow + j * kXStep) * XS + xcol]);
+                to[0] = values<DT>(x.x, x.y, sc);
+                to[1] = values<DT>(x.z, x.w, sc);
             }
-            Eight<DT> x;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float v = (float)(int8_t)(xe[j] >> (8 * e)) * xsc[j];
-                if constexpr (DT == NORI_F32) x.e[e] = v;
-                else x.e[e] = DT == NORI_F16 ? f32_to_f16(v) : f32_to_bf16(v);
-            }
-            *reinterpret_cast<Eight<DT>*>(&xs[at]) = x;
         }
+        if (turn == 0) turn = a.splits > 1 ? a.k_tiles : 1;
+        if (turn > 0) --turn;
         __syncthreads();
-        if (from + kRows < end) load(from + kRows);
+        if (from + kRows < end && whole(from + kRows)) load(from + kRows);
         if (!a.dw) continue;
-#pragma unroll
+#pragma unroll 2
         for (int t = 0; t < kRows / 16; ++t) {
-            typename E::Frag y[2], x[2];
+            typename E::Frag y[MY], x[MX];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                y[j] = transposed<DT, LS>(ys, 16 * t, wn + 32 * j, lane);
-                x[j] = transposed<DT, LS>(xs, 16 * t, wk + 32 * j, lane);
-            }
+            for (int j = 0; j < MX; ++j) x[j] = transposed<DT, XS>(xs, 16 * t, wk + 32 * j, lane);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < MY; ++j) y[j] = transposed<DT, YS>(ys, 16 * t, wn + 32 * j, lane);
 #pragma unroll
-                for (int l = 0; l < 2; ++l) acc[j][l] = mma(y[j], x[l], acc[j][l]);
+            for (int j = 0; j < MY; ++j)
+#pragma unroll
+                for (int l = 0; l < MX; ++l) acc[j][l] = mma(y[j], x[l], acc[j][l]);
         }
     }
-    if (own_db) {
+    if (a.db && (a.splits > 1 || kt == 0)) {
+        float* sums = reinterpret_cast<float*>(ys);  // [kYStep][TN]
+        static_assert(kYStep * TN * 4 <= (int)sizeof(ys), "the column sums fit the tile");
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sums[first_row][col + e] = colsum[e];
+        for (int e = 0; e < 8; ++e) sums[yrow * TN + ycol + e] = colsum[e];
         __syncthreads();
         const int c = threadIdx.x;
-        if (c < kTile && nt * kTile + c < a.n) {
+        if (c < TN && nt * TN + c < a.n) {
             float s = 0.f;
-            for (int j = 0; j < kStep; ++j) s += sums[j][c];
-            if (a.splits > 1) a.part_b[(int64_t)split * a.n + nt * kTile + c] = s;
-            else put<DT>(a.db, a.db_dtype, nt * kTile + c, s);
+            for (int j = 0; j < kYStep; ++j) s += sums[j * TN + c];
+            if (a.splits > 1) a.part_b[((int64_t)split * a.k_tiles + kt) * a.n + nt * TN + c] = s;
+            else put<DT>(a.db, a.db_dtype, nt * TN + c, s);
         }
     }
     if (!a.dw) return;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < MY; ++j)
 #pragma unroll
-        for (int l = 0; l < 2; ++l)
+        for (int l = 0; l < MX; ++l)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int row = nt * kTile + wn + 32 * j + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-                const int c = kt * kTile + wk + 32 * l + (lane & 31);
+                const int row = nt * TN + wn + 32 * j + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
+                const int c = kt * kGroup + wk + 32 * l + (lane & 31);
                 if (row >= a.n || c >= a.k) continue;
                 const int64_t at = (int64_t)row * a.k + c;
                 if (a.splits > 1) a.part_w[(int64_t)split * a.n * a.k + at] = acc[j][l][e];
@@ -161,7 +201,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Args a) {
         const float* p = w ? a.part_w + i : a.part_b + (i - nk);
         const int64_t step = w ? nk : a.n;
         float s = 0.f;
-        for (int j = 0; j < a.splits; ++j) s += p[j * step];
+        const int parts = w ? a.splits : a.splits * a.k_tiles;
+#pragma unroll 8
+        for (int j = 0; j < parts; ++j) s += p[j * step];
         if (w) put<DT>(a.dw, a.dw_dtype, i, s);
         else put<DT>(a.db, a.db_dtype, i - nk, s);
     }
@@ -175,13 +217,14 @@ Args plan(int dtype, int64_t rows, int32_t n, int32_t k) {
     a.n = n;
     a.k = k;
     a.code_stride = (k + 15) / 16 * 16;
-    a.groups = (k + kTile - 1) / kTile;
-    a.n_tiles = (n + kTile - 1) / kTile;
+    a.groups = (k + kGroup - 1) / kGroup;
+    a.tile_n = dtype == NORI_F32 || (n + 127) / 128 % 2 ? 128 : 256;
+    a.n_tiles = (n + a.tile_n - 1) / a.tile_n;
     a.k_tiles = a.groups;
-    const int64_t tiles = (int64_t)a.n_tiles * a.k_tiles, want = 2 * device_cus();
-    int64_t splits = std::min<int64_t>((want + tiles - 1) / tiles, rows / kLeast);
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, 256));
-    a.per_split = std::max<int64_t>(kRows, ((rows + splits - 1) / splits + kRows - 1) / kRows * kRows);
+    // one round of the workgroups that the compute units hold
+    const int64_t tiles = (int64_t)a.n_tiles * a.k_tiles, hold = 2 * device_cus();
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(hold / tiles, rows / kLeast), 256));
+    a.per_split = std::max<int64_t>(64, ((rows + splits - 1) / splits + 63) / 64 * 64);
     a.splits = (int)std::max<int64_t>(1, (rows + a.per_split - 1) / a.per_split);
     return a;
 }
@@ -193,7 +236,7 @@ int64_t part_w_bytes(const Args& a) { return ((int64_t)a.splits * a.n * a.k * 4 
 extern "C" int64_t nori_checkpoint_grad_workspace_bytes(int dtype, int64_t rows, int32_t n, int32_t k) {
     if (rows < 0 || n < 1 || k < 1) return 0;
     const Args a = plan(dtype, rows, n, k);
-    return a.splits > 1 ? part_w_bytes(a) + (int64_t)a.splits * n * 4 : 0;
+    return a.splits > 1 ? part_w_bytes(a) + (int64_t)a.splits * a.k_tiles * n * 4 : 0;
 }
 
 extern "C" int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int32_t n, int64_t dy_row_stride, const void* codes,
@@ -208,6 +251,7 @@ extern "C" int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int
         return fail(NORI_ERR_UNSUPPORTED, "checkpoint_grad: gradients are of the rows' dtype or float32");
     if (dy_row_stride < 0 || (rows > 1 && dy_row_stride != 0 && dy_row_stride < n))
         return fail(NORI_ERR_INVALID, "checkpoint_grad: a row stride of %lld below rows of %d", (long long)dy_row_stride, n);
+    if (dy_row_stride > (1 << 24)) return fail(NORI_ERR_UNSUPPORTED, "checkpoint_grad: a row stride of %lld; up to 2^24 is taken", (long long)dy_row_stride);
     if (!dw && !db) return NORI_OK;
     if (rows > 0 && (!dy || (dw && (!codes || !scales || (uintptr_t)codes % 16))))
         return fail(NORI_ERR_INVALID, "checkpoint_grad: null or unaligned pointer");
@@ -232,7 +276,8 @@ extern "C" int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int
     }
     hipStream_t stream = (hipStream_t)stream_v;
     NORI_DISPATCH_FLOAT(dtype, DT, {
-        hipLaunchKernelGGL((grad_kernel<DT>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+        if (DT != NORI_F32 && a.tile_n == 256) hipLaunchKernelGGL((grad_kernel<DT, DT == NORI_F32 ? 128 : 256>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+        else hipLaunchKernelGGL((grad_kernel<DT, 128>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
         if (a.splits > 1) {
             const int64_t items = (dw ? (int64_t)n * k : 0) + (db ? n : 0);
             hipLaunchKernelGGL((join_kernel<DT>), dim3((unsigned)std::min<int64_t>((items + kThreads - 1) / kThreads, 16 * device_cus())),

@@ -69,6 +69,8 @@ class _CheckpointedLinear(torch.autograd.Function):
         if need_w or need_b:
             w_dtype, b_dtype = ctx.grad_dtypes
             dy, rows, stride = _rows_of(dy, n)
+            if stride > 2**24:
+                dy, stride = dy.contiguous(), n
             make = torch.empty if rows else torch.zeros
             dw = make((n, k), dtype=w_dtype, device=device) if need_w else None
             db = make((n,), dtype=b_dtype, device=device) if need_b else None
