@@ -21,15 +21,14 @@
 namespace nori {
 namespace attn_train {
 
-constexpr int kWaves = 4;               // wavefronts a workgroup
-constexpr int kThreads = kWaves * 64;
-constexpr int kOwn = kWaves * 32;       // rows or keys that stay, a workgroup
+constexpr int kFewWidth = 64;  // head widths to which workgroups of one and two wavefronts are built
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Args {
     nori_attention_train_args a;
     int group;            // query heads a key head
     int64_t rows;         // group * nq
+    int waves;            // of a workgroup, 32 rows or keys that stay each
     int64_t tiles;        // of the side that stays, a unit
     int64_t splits;       // parts of the side that passes
     int64_t per_split;    // its rows a part, whole tiles
@@ -56,10 +55,13 @@ __device__ __forceinline__ int64_t work_index(int64_t i, int64_t n) {
     return i < whole ? (i & 7) * (whole >> 3) + (i >> 3) : i;
 }
 
-// Threads a launch needs per output of the joining kernels, and the entry points of the typed translation units.
-enum Kind { kForward, kDq, kDkv };
+// What a launch does; kFew: the whole backward pass of units of few rows and keys. Launches of the typed translation units,
+// in chunks of 16 bytes or (narrow) of 4 elements.
+enum Kind { kForward, kDq, kDkv, kFew };
 int launch_f16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream);
+int launch_f16_narrow(Kind kind, const Args& p, int64_t blocks, hipStream_t stream);
 int launch_bf16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream);
+int launch_bf16_narrow(Kind kind, const Args& p, int64_t blocks, hipStream_t stream);
 int launch_f32(Kind kind, const Args& p, int64_t blocks, hipStream_t stream);
 
 }  // namespace attn_train

@@ -14,54 +14,75 @@ namespace {
 constexpr int64_t kTileRows = 64;      // a multiple of every type's tile
 constexpr int64_t kLeastRows = 256;    // of a part: below it, joining costs more than the idle units
 
-// out rows of a unit's rows from their parts: each part's result is normalised over its own keys.
-template <int DT>
-__global__ __launch_bounds__(256) void join_forward_kernel(const Args p) {
+// Element col of row `at` of a result: out or dq rows in a unit's order, or dk's and dv's (key, then K or V).
+template <bool KV>
+__device__ __forceinline__ int64_t place_of(const Args& p, int64_t at, int64_t col) {
     const auto& a = p.a;
-    const int64_t n = a.bg * a.kv_heads * p.rows, quads = a.d / 4;
-    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < n * quads; i += gridDim.x * 256LL) {
-        const int64_t at = i / quads, col = 4 * (i % quads);
-        float top = -INFINITY;
-        for (int64_t s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[s * n + at]);
-        f32x4 sum = {};
-        float total = 0.f;
-        const float base = top == -INFINITY ? 0.f : top;
-        for (int64_t s = 0; s < p.splits; ++s) {
-            const float l = p.part_lse[s * n + at];
-            if (l == -INFINITY) continue;  // no keys (or none that counts) in this part
-            const float w = __builtin_amdgcn_exp2f(l - base);
-            total += w;
-            sum += w * *reinterpret_cast<const f32x4*>(p.part + (s * n + at) * a.d + col);
-        }
-        const int64_t unit = at / p.rows, r = at % p.rows, b = unit / a.kv_heads;
-        if (total != 0.f) sum *= 1.f / total;
-        else if (length_of(a, b) > 0) sum = f32x4{} + NAN;  // every logit at -inf
-        const int64_t head = unit % a.kv_heads * p.group + r / a.nq, query = r % a.nq;
-        const int64_t to = ((b * a.nq + query) * a.heads + head) * a.d + col;
-        for (int j = 0; j < 4; ++j) store_elem<DT>(a.out, to + j, sum[j]);
-        if (col == 0 && a.lse) a.lse[at] = (base + __builtin_amdgcn_logf(total)) * kLn2;
+    if constexpr (KV) {
+        const int64_t unit = at / (2 * a.nk), row = at % (2 * a.nk);
+        return ((unit / a.kv_heads * 2 * a.nk + row) * a.kv_heads + unit % a.kv_heads) * a.d + col;
+    } else {
+        const int64_t unit = at / p.rows, r = at % p.rows;
+        const int64_t head = unit % a.kv_heads * p.group + r / a.nq;
+        return ((unit / a.kv_heads * a.nq + r % a.nq) * a.heads + head) * a.d + col;
     }
 }
 
-// The sums of dq's parts, or of dk's and dv's.
-template <int DT, bool KV>
-__global__ __launch_bounds__(256) void join_sums_kernel(const Args p) {
+// A row of a result from its parts by one workgroup: the parts are dealt to groups of d / 4 threads, whose sums are added in
+// order. Forward parts are normalised over their own keys and weighed by their shares of the row's sum.
+template <int DT, Kind KIND>
+__global__ __launch_bounds__(256) void join_kernel(const Args p) {
+    __shared__ float sums[256 * 4], totals[256], tops[4];
     const auto& a = p.a;
-    const int64_t n = a.bg * a.kv_heads * (KV ? 2 * a.nk : p.rows), quads = a.d / 4;
-    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < n * quads; i += gridDim.x * 256LL) {
-        const int64_t at = i / quads, col = 4 * (i % quads);
-        f32x4 sum = {};
-        for (int64_t s = 0; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4*>(p.part + (s * n + at) * a.d + col);
-        int64_t to;
-        if constexpr (KV) {
-            const int64_t unit = at / (2 * a.nk), row = at % (2 * a.nk);  // row: key, then K or V
-            to = ((unit / a.kv_heads * 2 * a.nk + row) * a.kv_heads + unit % a.kv_heads) * a.d + col;
-        } else {
-            const int64_t unit = at / p.rows, r = at % p.rows;
-            const int64_t head = unit % a.kv_heads * p.group + r / a.nq;
-            to = ((unit / a.kv_heads * a.nq + r % a.nq) * a.heads + head) * a.d + col;
+    const int64_t n = a.bg * a.kv_heads * (KIND == kDkv ? 2 * a.nk : p.rows);
+    const int quads = a.d / 4, groups = 256 / quads, group = threadIdx.x / quads, col = 4 * (threadIdx.x % quads);
+    for (int64_t at = blockIdx.x; at < n; at += gridDim.x) {
+        float base = 0.f;
+        if constexpr (KIND == kForward) {
+            float top = -INFINITY;
+            for (int64_t s = threadIdx.x; s < p.splits; s += 256) top = fmaxf(top, p.part_lse[s * n + at]);
+            for (int i = 32; i > 0; i /= 2) top = fmaxf(top, __shfl_xor(top, i));
+            if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+            __syncthreads();
+            top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            base = top == -INFINITY ? 0.f : top;
         }
-        for (int j = 0; j < 4; ++j) store_elem<DT>(KV ? a.dkv : a.dq, to + j, sum[j]);
+        f32x4 sum = {};
+        float total = 0.f;
+        if (group < groups) {
+#pragma unroll 4
+            for (int64_t s = group; s < p.splits; s += groups) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + (s * n + at) * a.d + col);
+                if constexpr (KIND == kForward) {
+                    const float l = p.part_lse[s * n + at];
+                    const float w = __builtin_amdgcn_exp2f(l - base);
+                    if (l != -INFINITY) {  // (no keys, or none that counts, in this part)
+                        total += w;
+                        sum += w * x;
+                    }
+                } else {
+                    sum += x;
+                }
+            }
+        }
+        *reinterpret_cast<f32x4*>(&sums[4 * threadIdx.x]) = sum;
+        totals[threadIdx.x] = total;
+        __syncthreads();
+        if (group == 0) {
+            for (int g = 1; g < groups && g < p.splits; ++g) {
+                sum += *reinterpret_cast<const f32x4*>(&sums[4 * (g * quads + threadIdx.x)]);
+                total += totals[g * quads];
+            }
+            if constexpr (KIND == kForward) {
+                if (total != 0.f) sum *= 1.f / total;
+                else if (length_of(a, at / p.rows / a.kv_heads) > 0) sum = f32x4{} + NAN;  // every logit at -inf
+                if (col == 0 && a.lse) a.lse[at] = (base + __builtin_amdgcn_logf(total)) * kLn2;
+            }
+            void* out = KIND == kForward ? a.out : (KIND == kDq ? a.dq : a.dkv);
+            const int64_t to = place_of<KIND == kDkv>(p, at, col);
+            for (int j = 0; j < 4; ++j) store_elem<DT>(out, to + j, sum[j]);
+        }
+        __syncthreads();
     }
 }
 
@@ -75,13 +96,19 @@ Args plan(const nori_attention_train_args& a, Kind kind) {
     p.rows = (int64_t)p.group * a.nq;
     p.c = a.scale * kLog2e;
     const int64_t stay = kind == kDkv ? a.nk : p.rows, pass = kind == kDkv ? p.rows : a.nk;
-    p.tiles = (stay + kOwn - 1) / kOwn;
-    const int64_t blocks = a.bg * a.kv_heads * p.tiles, want = 2 * device_cus();
+    p.waves = a.d > kFewWidth || stay > 64 ? 4 : (stay > 32 ? 2 : 1);
+    p.tiles = (stay + 32 * p.waves - 1) / (32 * p.waves);
+    const int64_t blocks = a.bg * a.kv_heads * p.tiles, want = 8 / p.waves * device_cus();
     int64_t splits = blocks > 0 && blocks < want ? (want + blocks - 1) / blocks : 1;
     splits = std::max<int64_t>(1, std::min(splits, pass / kLeastRows));
     p.per_split = std::max<int64_t>(kTileRows, ((pass + splits - 1) / splits + kTileRows - 1) / kTileRows * kTileRows);
     p.splits = std::max<int64_t>(1, (pass + p.per_split - 1) / p.per_split);
     return p;
+}
+
+// Units that one workgroup takes through the whole backward pass.
+bool few(const nori_attention_train_args& a) {
+    return a.dtype != NORI_F32 && a.d <= kFewWidth && a.dq && a.dkv && a.nk <= 64 && a.nq * (a.heads / a.kv_heads) <= 64;
 }
 
 int64_t part_bytes(const Args& p, Kind kind) { return p.splits > 1 ? p.splits * part_rows(p, kind) * p.a.d * 4 : 0; }
@@ -90,19 +117,18 @@ int64_t aligned16(int64_t n) { return (n + 15) / 16 * 16; }
 int launch_typed(Kind kind, const Args& p, hipStream_t stream) {
     const int64_t blocks = p.a.bg * p.a.kv_heads * p.tiles * p.splits;
     switch (p.a.dtype) {
-        case NORI_F16: return launch_f16(kind, p, blocks, stream);
-        case NORI_BF16: return launch_bf16(kind, p, blocks, stream);
+        case NORI_F16: return p.wide ? launch_f16(kind, p, blocks, stream) : launch_f16_narrow(kind, p, blocks, stream);
+        case NORI_BF16: return p.wide ? launch_bf16(kind, p, blocks, stream) : launch_bf16_narrow(kind, p, blocks, stream);
         default: return launch_f32(kind, p, blocks, stream);
     }
 }
 
 int join(Kind kind, const Args& p, hipStream_t stream) {
-    const int64_t items = part_rows(p, kind) * (p.a.d / 4);
-    const dim3 grid((unsigned)std::min<int64_t>((items + 255) / 256, 32 * device_cus())), threads(256);
+    const dim3 grid((unsigned)std::min<int64_t>(part_rows(p, kind), 32 * device_cus())), threads(256);
     NORI_DISPATCH_FLOAT(p.a.dtype, DT, {
-        if (kind == kForward) hipLaunchKernelGGL((join_forward_kernel<DT>), grid, threads, 0, stream, p);
-        else if (kind == kDq) hipLaunchKernelGGL((join_sums_kernel<DT, false>), grid, threads, 0, stream, p);
-        else hipLaunchKernelGGL((join_sums_kernel<DT, true>), grid, threads, 0, stream, p);
+        if (kind == kForward) hipLaunchKernelGGL((join_kernel<DT, kForward>), grid, threads, 0, stream, p);
+        else if (kind == kDq) hipLaunchKernelGGL((join_kernel<DT, kDq>), grid, threads, 0, stream, p);
+        else hipLaunchKernelGGL((join_kernel<DT, kDkv>), grid, threads, 0, stream, p);
     });
     return launch_status("attention_train join");
 }
@@ -156,7 +182,7 @@ int check(const nori_attention_train_args* a, bool backward) {
     const Kind kinds[3] = {kForward, kDq, kDkv};
     for (Kind k : kinds) {
         const Args p = plan(*a, k);
-        if (!one_launch(a->bg * a->kv_heads * p.tiles * p.splits, kThreads))
+        if (!one_launch(a->bg * a->kv_heads * p.tiles * p.splits, 64 * p.waves))
             return fail(NORI_ERR_UNSUPPORTED, "%s: more workgroups than one launch has", what);
     }
     return NORI_OK;
@@ -178,6 +204,7 @@ extern "C" int64_t nori_attention_train_workspace_bytes(const nori_attention_tra
         const Args p = plan(*a, kForward);
         return p.splits > 1 ? aligned16(part_bytes(p, kForward)) + aligned16(p.splits * part_rows(p, kForward) * 4) : 0;
     }
+    if (few(*a)) return 0;
     const Args q = plan(*a, kDq), kv = plan(*a, kDkv);
     return aligned16(part_rows(q, kDq) * 4) + std::max(a->dq ? part_bytes(q, kDq) : 0, a->dkv ? part_bytes(kv, kDkv) : 0);
 }
@@ -205,6 +232,11 @@ extern "C" int nori_attention_train_backward(const nori_attention_train_args* a,
     float* delta = reinterpret_cast<float*>(a->workspace);
     Args q = plan(*a, kDq);
     q.wide = wide(*a, true);
+    if (few(*a)) {
+        q.waves = std::max(q.waves, plan(*a, kDkv).waves);
+        q.tiles = q.splits = 1;
+        return launch_typed(kFew, q, stream);
+    }
     if (a->nq > 0) {
         if (!a->dq) q.splits = 1;  // the rows' sums alone
         q.delta = delta;

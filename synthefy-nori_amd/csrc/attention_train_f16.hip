@@ -1,10 +1,12 @@
-// Attention with gradients over float16 rows (attention_train_kernel.h).
+// Attention with gradients over float16 rows in 16-byte chunks (attention_train_kernel.h).
 #include "attention_train_kernel.h"
 
 namespace nori {
 namespace attn_train {
 
-int launch_f16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) { return launch_chunks<NORI_F16>(kind, p, blocks, stream); }
+int launch_f16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
+    return launch_width<NORI_F16, 8>(kind, p, blocks, stream);
+}
 
 }  // namespace attn_train
 }  // namespace nori

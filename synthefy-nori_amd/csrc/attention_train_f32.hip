@@ -4,7 +4,9 @@
 namespace nori {
 namespace attn_train {
 
-int launch_f32(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) { return launch_chunks<NORI_F32>(kind, p, blocks, stream); }
+int launch_f32(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
+    return launch_width<NORI_F32, 4>(kind, p, blocks, stream);
+}
 
 }  // namespace attn_train
 }  // namespace nori

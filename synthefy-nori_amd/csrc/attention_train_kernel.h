@@ -16,7 +16,7 @@ template <int DT, int DK> struct Geo {
     using T = typename E::T;
     static constexpr int DP = (DK + 31) / 32 * 32;
     static constexpr int LS = DP + E::kPad;      // elements from one row of a tile to the next
-    static constexpr int KS = DK / 16, MS = DP / 32, NS = E::kRows / 32;
+    static constexpr int KS = DK / 16, MS = DP / 32;
 };
 
 // Left operand: row `row` (lane % 32 of a step's 32) of a tile, its columns 16 k + 8 h .. + 7.
@@ -43,17 +43,28 @@ __device__ __forceinline__ void load_own(typename El<DT>::Frag (&f)[DK / 16], co
     }
 }
 
-// Writes 4 results, columns at .. at + 3 of a row.
-template <int DT>
-__device__ __forceinline__ void store4(typename El<DT>::T* p, const float (&x)[4]) {
-    if constexpr (DT == NORI_F32) {
-        *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
-    } else {
-        uint32_t w[4];
+// Writes a column of a result, `by` times, as the d elements of a row: in the type, or fp32 of a part.
+template <int DT, int MS, class Out>
+__device__ __forceinline__ void store_row(Out* out, const f32x16 (&x)[MS], float by, int d, int half) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = DT == NORI_F16 ? f32_to_f16(x[j]) : f32_to_bf16(x[j]);
-        *reinterpret_cast<u32x2*>(p) = u32x2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
-    }
+    for (int j = 0; j < MS; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int col = 32 * j + 2 * i + 4 * half;
+            if (col >= d) continue;
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = x[j][i + e] * by;
+            if constexpr (sizeof(Out) == 4) {
+                *reinterpret_cast<f32x4*>(out + col) = v;
+            } else if constexpr (DT == NORI_F16) {
+                typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<f16x4*>(out + col) = __builtin_convertvector(v, f16x4);
+            } else {
+                typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<bf16x4*>(out + col) = __builtin_convertvector(v, bf16x4);
+            }
+        }
 }
 
 // Query row r of a unit: head and query.
@@ -64,6 +75,11 @@ __device__ __forceinline__ Row row_of(const Args& p, int64_t unit_head, int r) {
     return {unit_head * p.group + h, r - h * (int)p.a.nq};
 }
 
+// Rows of a tile that passes a workgroup of NW wavefronts.
+template <int DT, int NW>
+constexpr int kTileOf = NW == 1 ? 32 : El<DT>::kRows;
+
+// The work of a workgroup: part `split` of what passes by tile `tile` of what stays, in a unit.
 struct Block { int64_t tile, split, unit, b, hk; };
 __device__ __forceinline__ Block block_of(const Args& p) {
     int64_t i = work_index(blockIdx.x, gridDim.x);
@@ -80,13 +96,13 @@ __device__ __forceinline__ Block block_of(const Args& p) {
 // A tile of two tensors on its way to LDS: chunks of W elements in registers, asked for while the tile before is worked on.
 // A thread's chunks are at the same places of every tile: 32-bit byte offsets from the tile's first row, which moves on
 // uniformly (the host keeps strides to what that takes).
-template <int DT, int DK, int W> struct Stage {
+template <int DT, int DK, int W, int TH, int ROWS> struct Stage {
     using G = Geo<DT, DK>;
     using E = El<DT>;
     using T = typename E::T;
     typedef uint32_t Chunk __attribute__((ext_vector_type(W * sizeof(T) / 4)));
     static constexpr int CH = DK / W;                                       // chunks a row
-    static constexpr int N = (E::kRows * CH + kThreads - 1) / kThreads;     // chunks a thread, a tile
+    static constexpr int N = (ROWS * CH + TH - 1) / TH;     // chunks a thread, a tile
     Chunk x[N], y[N];
     uint32_t ox[N], oy[N];
     int row[N];  // past every tile for chunks that no row has: they stay zero
@@ -94,8 +110,8 @@ template <int DT, int DK, int W> struct Stage {
     __device__ __forceinline__ void place(int d, int64_t x_stride, int64_t y_stride) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int idx = threadIdx.x + i * kThreads, r = idx / CH, col = W * (idx % CH);
-            row[i] = r < E::kRows && col < d ? r : 1 << 30;
+            const int idx = threadIdx.x + i * TH, r = idx / CH, col = W * (idx % CH);
+            row[i] = r < ROWS && col < d ? r : 1 << 30;
             ox[i] = (uint32_t)(r * (uint32_t)x_stride + col) * sizeof(T);
             oy[i] = (uint32_t)(r * (uint32_t)y_stride + col) * sizeof(T);
         }
@@ -135,7 +151,7 @@ template <int DT, int DK, int W> struct Stage {
             if (row[i] < left) {
                 const T *px, *py;
                 at(row[i], px, py);
-                const int col = W * ((threadIdx.x + i * kThreads) % CH);
+                const int col = W * ((threadIdx.x + i * TH) % CH);
                 x[i] = *reinterpret_cast<const Chunk*>(px + col);
                 y[i] = *reinterpret_cast<const Chunk*>(py + col);
             }
@@ -144,8 +160,8 @@ template <int DT, int DK, int W> struct Stage {
     __device__ __forceinline__ void store(T* tx, T* ty) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int idx = threadIdx.x + i * kThreads, to = idx / CH * G::LS + W * (idx % CH);
-            if (E::kRows * CH % kThreads == 0 || idx < E::kRows * CH) {
+            const int idx = threadIdx.x + i * TH, to = idx / CH * G::LS + W * (idx % CH);
+            if (ROWS * CH % TH == 0 || idx < ROWS * CH) {
                 *reinterpret_cast<Chunk*>(tx + to) = x[i];
                 *reinterpret_cast<Chunk*>(ty + to) = y[i];
             }
@@ -154,17 +170,71 @@ template <int DT, int DK, int W> struct Stage {
 };
 
 // ---------------------------------------------------------------- forward
-template <int DT, int DK, int W>
-__global__ __launch_bounds__(kThreads, DK <= 64 ? 3 : 2) void forward_kernel(const Args p) {
+// One tile's part of the forward pass: `left` of its keys are there.
+template <int DT, int DK, int NS>
+__device__ __forceinline__ void forward_step(const typename El<DT>::T* ks, const typename El<DT>::T* vs, int left,
+                                             const typename El<DT>::Frag (&qf)[DK / 16], f32x16 (&o)[Geo<DT, DK>::MS], float& m, float& l,
+                                             float c, int lane) {
+    using E = El<DT>;
+    using G = Geo<DT, DK>;
+    const int half = lane >> 5;
+    f32x16 s[NS];
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub) {
+        s[sub] = f32x16{};
+#pragma unroll
+        for (int k = 0; k < G::KS; ++k) s[sub] = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s[sub]);
+    }
+    if (left < 32 * NS) {
+#pragma unroll
+        for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (sub * 32 + 8 * (i / 4) + i % 4 >= left - 4 * half) s[sub][i] = -INFINITY;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 16 * NS; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+    top = fmaxf(top, other_half(top));
+    // the maximum that p is taken against moves when one passes it by 2^kSlack: rarely, after the first tiles
+    if (__any((top - m) * c > E::kSlack)) {
+        const float next = fmaxf(m, top);
+        const float shrink = next == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
+        m = next;
+        l *= shrink;
+#pragma unroll
+        for (int j = 0; j < 16 * G::MS; ++j) o[j / 16][j % 16] *= shrink;  // (whole vectors end up copied on every step)
+    }
+    const float off = E::kTop - (m == -INFINITY ? 0.f : m * c);  // (all keys so far at -inf: their p is 0)
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub) {
+        float e[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(fmaf(s[sub][i], c, off));
+            l += e[i];
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const auto pf = rounded<DT>(e, t);
+#pragma unroll
+            for (int j = 0; j < G::MS; ++j) o[j] = mma(transposed<DT, G::LS>(vs, sub * 32 + 16 * t, 32 * j, lane), pf, o[j]);
+        }
+    }
+}
+
+template <int DT, int DK, int W, int NW>
+__global__ __launch_bounds__(64 * NW, DK <= 64 && NW == 4 ? 3 : 2) void forward_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
-    __shared__ __attribute__((aligned(16))) T ks[E::kRows * G::LS];
-    __shared__ __attribute__((aligned(16))) T vs[E::kRows * G::LS];
+    constexpr int kRows = kTileOf<DT, NW>;
+    __shared__ __attribute__((aligned(16))) T ks[kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T vs[kRows * G::LS];
     const auto& a = p.a;
     const Block w = block_of(p);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int64_t r64 = w.tile * kOwn + wave * 32 + (lane & 31);
+    const int64_t r64 = w.tile * 32 * NW + wave * 32 + (lane & 31);
     const bool there = r64 < p.rows;
     const int r = (int)r64;
     const Row row = there ? row_of(p, w.hk, r) : Row{w.hk * p.group, 0};
@@ -174,7 +244,6 @@ __global__ __launch_bounds__(kThreads, DK <= 64 ? 3 : 2) void forward_kernel(con
 
     typename E::Frag qf[G::KS];
     load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
-    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + begin * a.kv_row;
     // the running maximum wants a positive factor: a negative one changes signs first, one of 0 makes the logits 0
     const float c = p.c == 0.f ? 1.f : fabsf(p.c);
     if (p.c <= 0.f) {
@@ -185,89 +254,42 @@ __global__ __launch_bounds__(kThreads, DK <= 64 ? 3 : 2) void forward_kernel(con
             for (int j = 0; j < 8; ++j) at(qf[k], j) = at(qf[k], j) * sign;
     }
 
-    float m = -INFINITY, l = 0.f;  // of this half-wave's keys
-    f32x16 o[G::MS] = {};
-    Stage<DT, DK, W> stage;
+    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + begin * a.kv_row;
+    Stage<DT, DK, W, 64 * NW, kRows> stage;
     stage.place(a.d, a.kv_row, a.kv_row);
     if (begin < end) stage.load(kv, kv + a.kv_half, end - begin);
-    for (int first = begin; first < end; first += E::kRows) {
+    float m = -INFINITY, l = 0.f;  // of this half-wave's keys
+    f32x16 o[G::MS] = {};
+    const auto finish = [&](const f32x16 (&x)[G::MS], float by, float lse2) {
+        if (p.splits > 1) {
+            const int64_t to = (w.split * a.bg * a.kv_heads + w.unit) * p.rows + r;
+            if (half == 0) p.part_lse[to] = lse2;
+            store_row<DT>(p.part + to * a.d, x, by, a.d, half);
+            return;
+        }
+        if (half == 0 && a.lse) a.lse[w.unit * p.rows + r] = lse2 * kLn2;
+        store_row<DT>(reinterpret_cast<T*>(a.out) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d, x, by, a.d, half);
+    };
+    if (begin >= end) {  // no keys: zeros. (On a path of its own: sums that the loop may skip would be copied on every step.)
+        if (there) finish(o, 0.f, -INFINITY);
+        return;
+    }
+    for (int first = begin; first < end; first += kRows) {
         __syncthreads();
         stage.store(ks, vs);
         __syncthreads();
-        kv += E::kRows * a.kv_row;
-        if (first + E::kRows < end) stage.load(kv, kv + a.kv_half, end - first - E::kRows);
-        f32x16 s[G::NS];
-#pragma unroll
-        for (int sub = 0; sub < G::NS; ++sub) {
-            s[sub] = f32x16{};
-#pragma unroll
-            for (int k = 0; k < G::KS; ++k) s[sub] = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s[sub]);
-        }
-        if (first + E::kRows > end) {
-#pragma unroll
-            for (int sub = 0; sub < G::NS; ++sub)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) s[sub][i] = -INFINITY;
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int i = 1; i < 16 * G::NS; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-        top = fmaxf(top, other_half(top));
-        // the maximum that p is taken against moves when one passes it by 2^kSlack: rarely, after the first tiles
-        if (__any((top - m) * c > E::kSlack)) {
-            const float next = fmaxf(m, top);
-            const float shrink = next == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
-            m = next;
-            l *= shrink;
-#pragma unroll
-            for (int j = 0; j < G::MS; ++j) o[j] *= shrink;
-        }
-        const float off = E::kTop - (m == -INFINITY ? 0.f : m * c);  // (all keys so far at -inf: their p is 0)
-#pragma unroll
-        for (int sub = 0; sub < G::NS; ++sub) {
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[i] = __builtin_amdgcn_exp2f(fmaf(s[sub][i], c, off));
-                l += x[i];
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const auto pf = rounded<DT>(x, t);
-#pragma unroll
-                for (int j = 0; j < G::MS; ++j) o[j] = mma(transposed<DT, G::LS>(vs, sub * 32 + 16 * t, 32 * j, lane), pf, o[j]);
-            }
-        }
+        kv += kRows * a.kv_row;
+        if (first + kRows < end) stage.load(kv, kv + a.kv_half, end - first - kRows);
+        forward_step<DT, DK, kRows / 32>(ks, vs, end - first, qf, o, m, l, c, lane);
     }
     if (!there) return;
     l += other_half(l);
-    const float inv = begin < end ? 1.f / l : 0.f;
-    const float lse2 = begin < end ? __builtin_amdgcn_logf(l) - E::kTop + m * c : -INFINITY;
-    if (p.splits > 1) {
-        const int64_t units = a.bg * a.kv_heads;
-        const int64_t to = (w.split * units + w.unit) * p.rows + r;
-        if (half == 0) p.part_lse[to] = lse2;
-#pragma unroll
-        for (int j = 0; j < G::MS; ++j)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int col = 32 * j + 2 * i + 4 * half;
-                if (col < a.d) *reinterpret_cast<f32x4*>(p.part + to * a.d + col) = f32x4{o[j][i] * inv, o[j][i + 1] * inv, o[j][i + 2] * inv, o[j][i + 3] * inv};
-            }
-        return;
-    }
-    if (half == 0 && a.lse) a.lse[w.unit * p.rows + r] = lse2 * kLn2;
-    T* out = reinterpret_cast<T*>(a.out) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d;
-#pragma unroll
-    for (int j = 0; j < G::MS; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int col = 32 * j + 2 * i + 4 * half;
-            const float x[4] = {o[j][i] * inv, o[j][i + 1] * inv, o[j][i + 2] * inv, o[j][i + 3] * inv};
-            if (col < a.d) store4<DT>(out + col, x);
-        }
+    finish(o, 1.f / l, __builtin_amdgcn_logf(l) - E::kTop + m * c);
 }
+
+// What takes kBias off again.
+template <int DT>
+constexpr float kUnbias = DT == NORI_F16 ? 0x1p-15f : 1.f;
 
 // ds in float16 carries a power of two a column (a query of dq, a key of dk): gradients of a mean over many rows lie below
 // float16's range, those under a loss scale above it. The power brings the first values to 2^8 and falls where a later
@@ -293,7 +315,7 @@ struct Scale {
             }
             const float by = f == 0.f ? 1.f : next / f;  // (nothing is summed while f is 0)
 #pragma unroll
-            for (int j = 0; j < MS; ++j) acc[j] *= by;
+            for (int j = 0; j < 16 * MS; ++j) acc[j / 16][j % 16] *= by;  // (whole vectors end up copied on every step)
             f = next;
         }
 #pragma unroll
@@ -303,17 +325,68 @@ struct Scale {
 };
 
 // ---------------------------------------------------------------- dq, and delta for dk and dv
-template <int DT, int DK, int W>
-__global__ __launch_bounds__(kThreads, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq_kernel(const Args p) {
+// The sum of a row's products of dout and out.
+template <int DT, int KS>
+__device__ __forceinline__ float row_sum(typename El<DT>::Frag (&x)[KS], typename El<DT>::Frag (&y)[KS]) {
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(at(x[k], j), at(y[k], j), sum);
+    return sum + other_half(sum);
+}
+
+// One tile's part of dq: `left` of its keys are there.
+template <int DT, int DK, int NS>
+__device__ __forceinline__ void dq_step(const typename El<DT>::T* ks, const typename El<DT>::T* vs, int left,
+                                        const typename El<DT>::Frag (&qf)[DK / 16], const typename El<DT>::Frag (&dof)[DK / 16],
+                                        f32x16 (&dq)[Geo<DT, DK>::MS], Scale& scale, float c, float lse2, float delta, int lane) {
+    using G = Geo<DT, DK>;
+    const int half = lane >> 5;
+    float ds[NS][16];
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub) {
+        f32x16 s = {}, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] = -delta;
+#pragma unroll
+        for (int k = 0; k < G::KS; ++k) {
+            s = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s);
+            dp = mma(direct<DT, DK>(vs, sub * 32 + (lane & 31), k, half), dof[k], dp);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[sub][i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) * dp[i];
+    }
+    if (left < 32 * NS) {
+#pragma unroll
+        for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (sub * 32 + 8 * (i / 4) + i % 4 >= left - 4 * half) ds[sub][i] = 0.f;
+    }
+    if constexpr (El<DT>::kScaled) scale.apply(ds, dq);
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const auto f = rounded<DT>(ds[sub], t);
+#pragma unroll
+            for (int j = 0; j < G::MS; ++j) dq[j] = mma(transposed<DT, G::LS>(ks, sub * 32 + 16 * t, 32 * j, lane), f, dq[j]);
+        }
+}
+
+template <int DT, int DK, int W, int NW>
+__global__ __launch_bounds__(64 * NW, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
-    __shared__ __attribute__((aligned(16))) T ks[E::kRows * G::LS];
-    __shared__ __attribute__((aligned(16))) T vs[E::kRows * G::LS];
+    constexpr int kRows = kTileOf<DT, NW>;
+    __shared__ __attribute__((aligned(16))) T ks[kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T vs[kRows * G::LS];
     const auto& a = p.a;
     const Block w = block_of(p);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int64_t r64 = w.tile * kOwn + wave * 32 + (lane & 31);
+    const int64_t r64 = w.tile * 32 * NW + wave * 32 + (lane & 31);
     const bool there = r64 < p.rows;
     const int r = (int)r64;
     const Row row = there ? row_of(p, w.hk, r) : Row{w.hk * p.group, 0};
@@ -325,100 +398,103 @@ __global__ __launch_bounds__(kThreads, DT == NORI_F32 && DK > 96 ? 1 : 2) void d
     typename E::Frag dof[G::KS], qf[G::KS];
     load_own<DT, DK, W>(dof, reinterpret_cast<const T*>(a.dout) + w.b * a.do_bg + row.query * a.do_row + row.head * a.do_head, there, a.d, half);
     load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.out) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d, there, a.d, half);
-    float delta = 0.f;
-#pragma unroll
-    for (int k = 0; k < G::KS; ++k) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (DT == NORI_F32) delta = fmaf(dof[k].v[j], qf[k].v[j], delta);
-            else delta = fmaf((float)dof[k][j], (float)qf[k][j], delta);
-        }
-    }
-    delta += other_half(delta);
+    const float delta = row_sum<DT>(dof, qf);
     if (there && half == 0 && w.split == 0) p.delta[unit_row] = delta;
     if (!a.dq) return;
     load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
     const float lse2 = there ? a.lse[unit_row] * kLog2e : 0.f;
-    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + begin * a.kv_row;
 
-    f32x16 dq[G::MS] = {};
-    Scale scale;
-    Stage<DT, DK, W> stage;
+    const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + begin * a.kv_row;
+    Stage<DT, DK, W, 64 * NW, kRows> stage;
     stage.place(a.d, a.kv_row, a.kv_row);
     if (begin < end) stage.load(kv, kv + a.kv_half, end - begin);
-    for (int first = begin; first < end; first += E::kRows) {
+    f32x16 dq[G::MS] = {};
+    Scale scale;
+    for (int first = begin; first < end; first += kRows) {
         __syncthreads();
         stage.store(ks, vs);
         __syncthreads();
-        kv += E::kRows * a.kv_row;
-        if (first + E::kRows < end) stage.load(kv, kv + a.kv_half, end - first - E::kRows);
-        float ds[G::NS][16];
-#pragma unroll
-        for (int sub = 0; sub < G::NS; ++sub) {
-            f32x16 s = {}, dp;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dp[i] = -delta;
-#pragma unroll
-            for (int k = 0; k < G::KS; ++k) {
-                s = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s);
-                dp = mma(direct<DT, DK>(vs, sub * 32 + (lane & 31), k, half), dof[k], dp);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ds[sub][i] = __builtin_amdgcn_exp2f(fmaf(s[i], p.c, -lse2)) * dp[i];
-        }
-        if (first + E::kRows > end) {
-#pragma unroll
-            for (int sub = 0; sub < G::NS; ++sub)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) ds[sub][i] = 0.f;
-        }
-        if constexpr (E::kScaled) scale.apply(ds, dq);
-#pragma unroll
-        for (int sub = 0; sub < G::NS; ++sub)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const auto f = rounded<DT>(ds[sub], t);
-#pragma unroll
-                for (int j = 0; j < G::MS; ++j) dq[j] = mma(transposed<DT, G::LS>(ks, sub * 32 + 16 * t, 32 * j, lane), f, dq[j]);
-            }
+        kv += kRows * a.kv_row;
+        if (first + kRows < end) stage.load(kv, kv + a.kv_half, end - first - kRows);
+        dq_step<DT, DK, kRows / 32>(ks, vs, end - first, qf, dof, dq, scale, p.c, lse2, delta, lane);
     }
     if (!there) return;
     const float by = a.scale * (E::kScaled ? scale.inverse() : 1.f);
-    T* out = reinterpret_cast<T*>(a.dq) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d;
-    float* part = p.part + (w.split * a.bg * a.kv_heads * p.rows + unit_row) * a.d;
-#pragma unroll
-    for (int j = 0; j < G::MS; ++j)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int col = 32 * j + 2 * i + 4 * half;
-            const float x[4] = {dq[j][i] * by, dq[j][i + 1] * by, dq[j][i + 2] * by, dq[j][i + 3] * by};
-            if (col >= a.d) continue;
-            if (p.splits > 1) *reinterpret_cast<f32x4*>(part + col) = f32x4{x[0], x[1], x[2], x[3]};
-            else store4<DT>(out + col, x);
-        }
+    if (p.splits > 1) store_row<DT>(p.part + (w.split * a.bg * a.kv_heads * p.rows + unit_row) * a.d, dq, by, a.d, half);
+    else store_row<DT>(reinterpret_cast<T*>(a.dq) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d, dq, by, a.d, half);
 }
 
 // ---------------------------------------------------------------- dk and dv
-template <int DT, int DK, int W>
-__global__ __launch_bounds__(kThreads, DK <= 64 ? 2 : 1) void dkv_kernel(const Args p) {
+// One tile's part of dk and dv: `left` of its rows are there. off: kBias - log2 of a row's sum, deltas: its -delta, what the
+// products of dout and v start from.
+template <int DT, int DK, int NS>
+__device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typename El<DT>::T* dos, const float* off, const float* deltas,
+                                         int left, const typename El<DT>::Frag (&kf)[DK / 16], const typename El<DT>::Frag (&vf)[DK / 16],
+                                         f32x16 (&dk)[Geo<DT, DK>::MS], f32x16 (&dv)[Geo<DT, DK>::MS], Scale& scale, float c, int lane) {
+    using G = Geo<DT, DK>;
+    const int half = lane >> 5;
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub) {
+        f32x16 s = {}, dp;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(&deltas[sub * 32 + 2 * i + 4 * half]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dp[i + j] = d4[j];
+        }
+#pragma unroll
+        for (int k = 0; k < G::KS; ++k) {
+            s = mma(direct<DT, DK>(qs, sub * 32 + (lane & 31), k, half), kf[k], s);
+            dp = mma(direct<DT, DK>(dos, sub * 32 + (lane & 31), k, half), vf[k], dp);
+        }
+        float pr[16], ds[1][16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const f32x4 o4 = *reinterpret_cast<const f32x4*>(&off[sub * 32 + 2 * i + 4 * half]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                pr[i + j] = __builtin_amdgcn_exp2f(fmaf(s[i + j], c, o4[j]));
+                ds[0][i + j] = pr[i + j] * dp[i + j];
+            }
+        }
+        if (left < 32 * NS) {  // rows that are not there: 0, also beside keys that are not finite
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (sub * 32 + 8 * (i / 4) + i % 4 >= left - 4 * half) pr[i] = ds[0][i] = 0.f;
+        }
+        if constexpr (El<DT>::kScaled) scale.apply(ds, dk);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const auto pf = rounded<DT>(pr, t), f = rounded<DT>(ds[0], t);
+#pragma unroll
+            for (int j = 0; j < G::MS; ++j) {
+                dv[j] = mma(transposed<DT, G::LS>(dos, sub * 32 + 16 * t, 32 * j, lane), pf, dv[j]);
+                dk[j] = mma(transposed<DT, G::LS>(qs, sub * 32 + 16 * t, 32 * j, lane), f, dk[j]);
+            }
+        }
+    }
+}
+
+template <int DT, int DK, int W, int NW>
+__global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
-    __shared__ __attribute__((aligned(16))) T qs[E::kRows * G::LS];
-    __shared__ __attribute__((aligned(16))) T dos[E::kRows * G::LS];
-    __shared__ __attribute__((aligned(16))) float off[E::kRows];    // kBias - log2 of the row's sum
-    __shared__ __attribute__((aligned(16))) float deltas[E::kRows];  // negative: what the products of dout and v start from
+    constexpr int kRows = kTileOf<DT, NW>;
+    __shared__ __attribute__((aligned(16))) T qs[kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T dos[kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) float off[kRows];
+    __shared__ __attribute__((aligned(16))) float deltas[kRows];
     const auto& a = p.a;
     const Block w = block_of(p);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
-    const int64_t key64 = w.tile * kOwn + wave * 32 + (lane & 31);
+    const int64_t key64 = w.tile * 32 * NW + wave * 32 + (lane & 31);
     const int length = length_of(a, w.b);
     const bool there = key64 < length;
     const int key = (int)key64;
     const int begin = (int)(w.split * p.per_split);
     // (a tile behind the length has no products, its gradients are zeros)
-    const int end = w.tile * kOwn < length ? (int)min(p.rows, w.split * p.per_split + p.per_split) : begin;
+    const int end = w.tile * 32 * NW < length ? (int)min(p.rows, w.split * p.per_split + p.per_split) : begin;
 
     typename E::Frag kf[G::KS], vf[G::KS];
     const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + (there ? key * a.kv_row : 0);
@@ -434,16 +510,16 @@ __global__ __launch_bounds__(kThreads, DK <= 64 ? 2 : 1) void dkv_kernel(const A
 
     f32x16 dk[G::MS] = {}, dv[G::MS] = {};
     Scale scale;
-    Stage<DT, DK, W> stage;
+    Stage<DT, DK, W, 64 * NW, kRows> stage;
     stage.place(a.d, a.q_row, a.do_row);
     float next_off = 0.f, next_delta = 0.f;
     const auto load = [&](int first) {
         const int left = end - first;
         const T* px = q + at_head * a.q_head + at_query * a.q_row;
         const T* py = dout + at_head * a.do_head + at_query * a.do_row;
-        if (at_query + E::kRows <= nq || p.group == 1) {
+        if (at_query + kRows <= nq || p.group == 1) {
             stage.load(px, py, left);
-        } else if (nq >= E::kRows) {
+        } else if (nq >= kRows) {
             stage.load_over(px, py, left, nq - at_query, (a.q_head - nq * a.q_row) * (int64_t)sizeof(T),
                             (a.do_head - nq * a.do_row) * (int64_t)sizeof(T));
         } else {
@@ -453,122 +529,149 @@ __global__ __launch_bounds__(kThreads, DK <= 64 ? 2 : 1) void dkv_kernel(const A
                 y = dout + h * a.do_head + i * a.do_row;
             });
         }
-        at_query += E::kRows;
+        at_query += kRows;
         while (at_query >= nq) {
             at_query -= nq;
             ++at_head;
         }
-        if (threadIdx.x < E::kRows) {
+        if (threadIdx.x < kRows) {
             const bool in = (int)threadIdx.x < left;
             next_off = in ? E::kBias - lse[first + threadIdx.x] * kLog2e : 0.f;
             next_delta = in ? -delta[first + threadIdx.x] : 0.f;
         }
     };
     if (begin < end) load(begin);
-    for (int first = begin; first < end; first += E::kRows) {
+    for (int first = begin; first < end; first += kRows) {
         __syncthreads();
         stage.store(qs, dos);
-        if (threadIdx.x < E::kRows) {
+        if (threadIdx.x < kRows) {
             off[threadIdx.x] = next_off;
             deltas[threadIdx.x] = next_delta;
         }
         __syncthreads();
-        if (first + E::kRows < end) load(first + E::kRows);
-#pragma unroll
-        for (int sub = 0; sub < G::NS; ++sub) {
-            f32x16 s = {}, dp;
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(&deltas[sub * 32 + 2 * i + 4 * half]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) dp[i + j] = d4[j];
-            }
-#pragma unroll
-            for (int k = 0; k < G::KS; ++k) {
-                s = mma(direct<DT, DK>(qs, sub * 32 + (lane & 31), k, half), kf[k], s);
-                dp = mma(direct<DT, DK>(dos, sub * 32 + (lane & 31), k, half), vf[k], dp);
-            }
-            float pr[16], ds[1][16];
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const f32x4 o4 = *reinterpret_cast<const f32x4*>(&off[sub * 32 + 2 * i + 4 * half]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    pr[i + j] = __builtin_amdgcn_exp2f(fmaf(s[i + j], p.c, o4[j]));
-                    ds[0][i + j] = pr[i + j] * dp[i + j];
-                }
-            }
-            if (first + E::kRows > end) {  // rows that are not there: 0, also beside keys that are not finite
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (first + sub * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) pr[i] = ds[0][i] = 0.f;
-            }
-            if constexpr (E::kScaled) scale.apply(ds, dk);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const auto pf = rounded<DT>(pr, t), f = rounded<DT>(ds[0], t);
-#pragma unroll
-                for (int j = 0; j < G::MS; ++j) {
-                    dv[j] = mma(transposed<DT, G::LS>(dos, sub * 32 + 16 * t, 32 * j, lane), pf, dv[j]);
-                    dk[j] = mma(transposed<DT, G::LS>(qs, sub * 32 + 16 * t, 32 * j, lane), f, dk[j]);
-                }
-            }
-        }
+        if (first + kRows < end) load(first + kRows);
+dkv_step<DT, DK, kRows / 32>(qs, dos, off, deltas, end - first, kf, vf, dk, dv, scale, p.c, lane);
     }
     if (key64 >= a.nk) return;
-    constexpr float unbias = DT == NORI_F16 ? 0x1p-15f : 1.f;
-    const float byk = there ? a.scale * unbias * (E::kScaled ? scale.inverse() : 1.f) : 0.f, byv = unbias;
-    T* out = reinterpret_cast<T*>(a.dkv) + (((w.b * a.nk + key) * 2) * a.kv_heads + w.hk) * a.d;
-    float* part = p.part + ((w.split * a.bg * a.kv_heads + w.unit) * a.nk + key) * 2 * a.d;
+    if (!there) {  // past the length
 #pragma unroll
-    for (int j = 0; j < G::MS; ++j)
+        for (int j = 0; j < G::MS; ++j) dk[j] = dv[j] = f32x16{};
+    }
+    const float byk = a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f);
+    if (p.splits > 1) {
+        float* part = p.part + ((w.split * a.bg * a.kv_heads + w.unit) * a.nk + key) * 2 * a.d;
+        store_row<DT>(part, dk, byk, a.d, half);
+        store_row<DT>(part + a.d, dv, kUnbias<DT>, a.d, half);
+    } else {
+        T* out = reinterpret_cast<T*>(a.dkv) + (((w.b * a.nk + key) * 2) * a.kv_heads + w.hk) * a.d;
+        store_row<DT>(out, dk, byk, a.d, half);
+        store_row<DT>(out + (int64_t)a.kv_heads * a.d, dv, kUnbias<DT>, a.d, half);
+    }
+}
+
+// ---------------------------------------------------------------- few rows and few keys
+// The whole backward pass of a unit of up to 32 NW rows and keys: both sides in LDS, read from memory once, where the kernels
+// above read them twice and the row sums pass through memory.
+template <int DT, int DK, int W, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) {
+    using E = El<DT>;
+    using G = Geo<DT, DK>;
+    using T = typename E::T;
+    constexpr int kTile = 32 * NW * G::LS;
+    __shared__ __attribute__((aligned(16))) T tiles[4 * kTile];
+    __shared__ __attribute__((aligned(16))) float off[32 * NW];
+    __shared__ __attribute__((aligned(16))) float deltas[32 * NW];
+    T *ks = tiles, *vs = tiles + kTile, *qs = tiles + 2 * kTile, *dos = tiles + 3 * kTile;
+    const auto& a = p.a;
+    const int64_t unit = work_index(blockIdx.x, gridDim.x), b = unit / a.kv_heads, hk = unit % a.kv_heads;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, own = wave * 32 + (lane & 31);
+    const int length = length_of(a, b), rows = (int)p.rows, nq = (int)a.nq;
+
+    const T* kv = reinterpret_cast<const T*>(a.kv) + b * a.kv_bg + hk * a.kv_head;
+    const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_bg + hk * p.group * a.q_head;
+    const T* dout = reinterpret_cast<const T*>(a.dout) + b * a.do_bg + hk * p.group * a.do_head;
+    Stage<DT, DK, W, 64 * NW, 32 * NW> keys, queries;
+    keys.place(a.d, a.kv_row, a.kv_row);
+    keys.load(kv, kv + a.kv_half, length);
+    queries.place(a.d, a.q_row, a.do_row);
+    if (p.group == 1) queries.load(q, dout, rows);
+    else queries.load_each(rows, [&](int r, const T*& x, const T*& y) {
+        const int h = r / nq, i = r - h * nq;
+        x = q + h * a.q_head + i * a.q_row;
+        y = dout + h * a.do_head + i * a.do_row;
+    });
+    const bool there = own < rows;
+    const Row row = there ? row_of(p, hk, own) : Row{hk * p.group, 0};
+    const int64_t out_row = ((b * a.nq + row.query) * a.heads + row.head) * a.d;
+    typename E::Frag x[G::KS], y[G::KS];
+    load_own<DT, DK, W>(x, reinterpret_cast<const T*>(a.out) + out_row, there, a.d, half);
+    const float lse2 = there ? a.lse[unit * p.rows + own] * kLog2e : 0.f;
+    keys.store(ks, vs);
+    queries.store(qs, dos);
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int col = 32 * j + 2 * i + 4 * half;
-            float x[4], y[4];
+    for (int k = 0; k < G::KS; ++k) y[k] = direct<DT, DK>(dos, own, k, half);
+    const float delta = row_sum<DT>(y, x);
+    if (half == 0) {
+        off[own] = there ? E::kBias - lse2 : 0.f;
+        deltas[own] = there ? -delta : 0.f;
+    }
+    {
+        f32x16 dq[G::MS] = {};
+        Scale scale;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = there ? dk[j][i + e] * byk : 0.f;
-                y[e] = there ? dv[j][i + e] * byv : 0.f;
-            }
-            if (col >= a.d) continue;
-            if (p.splits > 1) {
-                *reinterpret_cast<f32x4*>(part + col) = f32x4{x[0], x[1], x[2], x[3]};
-                *reinterpret_cast<f32x4*>(part + a.d + col) = f32x4{y[0], y[1], y[2], y[3]};
-            } else {
-                store4<DT>(out + col, x);
-                store4<DT>(out + (int64_t)a.kv_heads * a.d + col, y);
-            }
-        }
+        for (int k = 0; k < G::KS; ++k) x[k] = direct<DT, DK>(qs, own, k, half);
+        if (length > 0) dq_step<DT, DK, NW>(ks, vs, length, x, y, dq, scale, p.c, lse2, delta, lane);
+        if (there) store_row<DT>(reinterpret_cast<T*>(a.dq) + out_row, dq, a.scale * (E::kScaled ? scale.inverse() : 1.f), a.d, half);
+    }
+    __syncthreads();
+    f32x16 dk[G::MS] = {}, dv[G::MS] = {};
+    Scale scale;
+#pragma unroll
+    for (int k = 0; k < G::KS; ++k) {
+        x[k] = direct<DT, DK>(ks, own, k, half);
+        y[k] = direct<DT, DK>(vs, own, k, half);
+    }
+    if (length > 0 && rows > 0) dkv_step<DT, DK, NW>(qs, dos, off, deltas, rows, x, y, dk, dv, scale, p.c, lane);
+    if (own >= a.nk) return;
+    if (own >= length) {
+#pragma unroll
+        for (int j = 0; j < G::MS; ++j) dk[j] = dv[j] = f32x16{};
+    }
+    T* out = reinterpret_cast<T*>(a.dkv) + (((b * a.nk + own) * 2) * a.kv_heads + hk) * a.d;
+    store_row<DT>(out, dk, a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f), a.d, half);
+    store_row<DT>(out + (int64_t)a.kv_heads * a.d, dv, kUnbias<DT>, a.d, half);
+}
+
+// ---------------------------------------------------------------- launches
+template <int DT, int DK, int W, int NW>
+void launch_one(Kind kind, const Args& p, dim3 grid, hipStream_t stream) {
+    const dim3 threads(64 * NW);
+    if (kind == kForward) hipLaunchKernelGGL((forward_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
+    else if (kind == kDq) hipLaunchKernelGGL((dq_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
+    else if (kind == kDkv) hipLaunchKernelGGL((dkv_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
+    else if constexpr (DT != NORI_F32 && DK <= kFewWidth && NW <= 2) hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
 }
 
 template <int DT, int DK, int W>
-int launch(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
-    const dim3 grid((unsigned)blocks), threads(kThreads);
-    switch (kind) {
-        case kForward: hipLaunchKernelGGL((forward_kernel<DT, DK, W>), grid, threads, 0, stream, p); break;
-        case kDq: hipLaunchKernelGGL((dq_kernel<DT, DK, W>), grid, threads, 0, stream, p); break;
-        case kDkv: hipLaunchKernelGGL((dkv_kernel<DT, DK, W>), grid, threads, 0, stream, p); break;
+void launch_waves(Kind kind, const Args& p, dim3 grid, hipStream_t stream) {
+    if constexpr (DK <= kFewWidth) {
+        if (p.waves == 1) return launch_one<DT, DK, W, 1>(kind, p, grid, stream);
+        if (p.waves == 2) return launch_one<DT, DK, W, 2>(kind, p, grid, stream);
     }
-    return launch_status("attention_train");
+    launch_one<DT, DK, W, 4>(kind, p, grid, stream);
 }
 
 template <int DT, int W>
 int launch_width(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
     const int d = p.a.d;
-    if (d <= 32) return launch<DT, 32, W>(kind, p, blocks, stream);
-    if (d <= 48) return launch<DT, 48, W>(kind, p, blocks, stream);
-    if (d <= 64) return launch<DT, 64, W>(kind, p, blocks, stream);
-    if (d <= 96) return launch<DT, 96, W>(kind, p, blocks, stream);
-    return launch<DT, 128, W>(kind, p, blocks, stream);
-}
-
-// Chunks of 16 bytes, where the host found everything aligned to them, or of 4 elements.
-template <int DT>
-int launch_chunks(Kind kind, const Args& p, int64_t blocks, hipStream_t stream) {
-    if constexpr (DT != NORI_F32)
-        if (p.wide) return launch_width<DT, 8>(kind, p, blocks, stream);
-    return launch_width<DT, 4>(kind, p, blocks, stream);
+    const dim3 grid((unsigned)blocks);
+    if (d <= 32) launch_waves<DT, 32, W>(kind, p, grid, stream);
+    else if (d <= 48) launch_waves<DT, 48, W>(kind, p, grid, stream);
+    else if (d <= 64) launch_waves<DT, 64, W>(kind, p, grid, stream);
+    else if (d <= 96) launch_waves<DT, 96, W>(kind, p, grid, stream);
+    else launch_waves<DT, 128, W>(kind, p, grid, stream);
+    return launch_status("attention_train");
 }
 
 }  // namespace attn_train

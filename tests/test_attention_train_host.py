@@ -106,11 +106,14 @@ def test_calls_of_the_library_are_refused(changes, status):
 
 def test_the_backward_call_needs_its_own():
     lib = nat.lib()
-    need = lib.nori_attention_train_workspace_bytes(arguments(), True)
-    assert need >= 2 * 4 * 3 * 4
+    need = lib.nori_attention_train_workspace_bytes(arguments(nq=300), True)
+    assert need >= 2 * 4 * 300 * 4
+    assert lib.nori_attention_train_workspace_bytes(arguments(), True) == 0  # few rows and keys
     for changes in (dict(lse=None), dict(dout=None), dict(workspace=None, workspace_bytes=need), dict(workspace=1 << 20, workspace_bytes=need - 1),
                     dict(workspace=(1 << 20) + 4, workspace_bytes=need)):
-        assert lib.nori_attention_train_backward(arguments(**changes), None) == nat.NORI_ERR_INVALID
+        assert lib.nori_attention_train_backward(arguments(nq=300, **changes), None) == nat.NORI_ERR_INVALID
+    for changes in (dict(q_row=(1 << 24) + 4), dict(kv_row=-32), dict(do_row=1 << 25)):
+        assert lib.nori_attention_train_backward(arguments(**changes), None) == nat.NORI_ERR_UNSUPPORTED
     assert lib.nori_attention_train_backward(arguments(do_row=34), None) == nat.NORI_ERR_UNSUPPORTED
     assert lib.nori_attention_train_forward(None, None) == nat.NORI_ERR_INVALID
     assert lib.nori_attention_train_backward(arguments(dq=None, dkv=None), None) == nat.NORI_OK
