@@ -2,7 +2,7 @@
 // gradient over gate and up kept so. One pass each, HBM-bound: 16 lanes hold a group, 8 elements each, in registers
 // between the largest magnitude (DPP) and the codes.
 //
-// The code of x is the whole number nearest to x / s, ties to even, exactly: k = rint(x * (1 / s)) may be one off beside a
+// The code of x is the whole number nearest to x / s, ties to even, exactly: k, the nearest to x (1 / s), may be one off beside a
 // half, and the remainder x - k s, which one fma gives without error there, says so. (Both terms are multiples of half
 // the last place of s, and their difference is not above s: it has 24 bits.)
 #include <math.h>
@@ -20,29 +20,68 @@ constexpr int kThreads = 256;
 constexpr int kGroup = NORI_CHECKPOINT_GROUP, kLanes = 16, kEach = kGroup / kLanes;
 constexpr int kItems = kThreads / kLanes;  // groups a workgroup
 
-// 8 elements from column c of a row of cols, zeros past its end.
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t row, int c, int cols, float (&v)[kEach]) {
-    if (c + kEach <= cols) {
-        widen<DT, kEach>(fetch<DT, kEach>(p, row + c), v);
-    } else {
+using Raw8 = nori_ln::Raw<DT, kEach>;
+
+// 8 elements from column c of a row of cols as they lie in memory, zeros past its end: at most three accesses there.
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load8(const void* p, int64_t row, int c, int cols) {
+    if (c + kEach <= cols) return fetch<DT, kEach>(p, row + c);
+    Raw8<DT> r = {};
+    const int n = cols - c;
+    if (n <= 0) return r;
+    if (n & 4) {
+        const auto x = fetch<DT, 4>(p, row + c);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) v[i] = c + i < cols ? load_elem<DT>(p, row + c + i) : 0.f;
+        for (int i = 0; i < 4; ++i) r.e[i] = x.e[i];
     }
+    if (n & 2) {
+        const auto x = fetch<DT, 2>(p, row + c + (n & 4));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) (n & 4 ? r.e[4 + i] : r.e[i]) = x.e[i];
+    }
+    if (n & 1) {
+        const auto x = fetch<DT, 1>(p, row + c + (n & 6)).e[0];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            if ((n & 6) == i) r.e[i] = x;
+    }
+    return r;
 }
 
 template <int DT>
 __device__ __forceinline__ void store8(void* p, int64_t row, int c, int cols, const float (&v)[kEach]) {
-    if (c + kEach <= cols) {
-        store<DT, kEach>(p, row + c, v);
-    } else {
+    const int n = cols - c;
+    if (n <= 0) return;
+    if (n >= kEach) return store<DT, kEach>(p, row + c, v);
+    if (n & 4) store<DT, 4>(p, row + c, {v[0], v[1], v[2], v[3]});
+    if (n & 2) {
+        if (n & 4) store<DT, 2>(p, row + c + 4, {v[4], v[5]});
+        else store<DT, 2>(p, row + c, {v[0], v[1]});
+    }
+    if (n & 1) store_elem<DT>(p, row + c + (n & 6), n & 4 ? (n & 2 ? v[6] : v[4]) : (n & 2 ? v[2] : v[0]));
+}
+
+// The largest magnitude of 8 elements as a whole number, NaN on top: of their own bits, two at a time in the 16-bit types.
+template <int DT>
+__device__ __forceinline__ uint32_t magnitude(const Raw8<DT>& r) {
+    if constexpr (DT == NORI_F32) {
+        uint32_t key = 0;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            if (c + i < cols) store_elem<DT>(p, row + c + i, v[i]);
+        for (int i = 0; i < kEach; ++i) key = max(key, r.e[i] & 0x7fffffffu);
+        return key;
+    } else {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 w[4];
+        __builtin_memcpy(w, r.e, sizeof w);
+        u16x2 key = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) key = __builtin_elementwise_max(key, w[i] & (uint16_t)0x7fff);
+        return max((uint32_t)key[0], (uint32_t)key[1]);
     }
 }
 
-// The largest of a value over 16 lanes (whole numbers: float magnitudes, NaN on top).
+// The largest of a value over 16 lanes.
 __device__ __forceinline__ uint32_t max16(uint32_t v) {
     v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // row_ror:8
     v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
@@ -50,44 +89,67 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
 }
 
-// The group's scale and this lane's codes.
-__device__ __forceinline__ float quantize8(const float (&v)[kEach], uint64_t& codes) {
-    uint32_t key = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) key = max(key, __float_as_uint(v[i]) & 0x7fffffffu);
-    key = max16(key);
-    const float s = key < 0x7f800000u ? __uint_as_float(key) / 127.0f : NAN;  // an infinity or NaN: NaN throughout
+// The group's scale and this lane's codes of elements r, v widened. A scale that is a normal number: k in one fma with a number
+// whose last place is 1, the code in its low byte; it is looked at again only where a lane of the wavefront has a remainder of
+// half a scale. (Quotients stay below 127.5: no code passes 127.)
+template <int DT>
+__device__ __forceinline__ float quantize8(const Raw8<DT>& r, const float (&v)[kEach], uint64_t& codes) {
+    constexpr float kOnes = 12582912.0f;  // 3 * 2^22
+    const uint32_t key = max16(magnitude<DT>(r));
+    const float amax = DT == NORI_F32 ? __uint_as_float(key) : (DT == NORI_F16 ? f16_to_f32((uint16_t)key) : bf16_to_f32((uint16_t)key));
+    const float s = amax <= 3.402823466e38f ? amax / 127.0f : NAN;  // an infinity or NaN: NaN throughout
     const bool normal = s >= 0x1p-126f;
     const float y = normal ? 1.0f / s : 0.0f;
-    uint32_t w[2] = {0, 0};
+    float k[kEach], most = 0.f;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        float k = rintf(v[i] * y);
-        if (normal) {
-            const float rest = fmaf(-k, s, v[i]), twice = 2.0f * fabsf(rest);
-            if (twice > s || (twice == s && ((int)k & 1))) k += copysignf(1.0f, rest);
-        } else if (s > 0.0f) {
-            k = rintf(v[i] / s);  // a scale of few bits: quotients up to 190
+        k[i] = fmaf(v[i], y, kOnes);
+        most = fmaxf(most, fabsf(fmaf(kOnes - k[i], s, v[i])));
+    }
+    if (__any(normal ? 2.0f * most >= s : s > 0.0f)) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            float c = k[i] - kOnes;
+            if (normal) {
+                const float rest = fmaf(-c, s, v[i]), twice = 2.0f * fabsf(rest);
+                if (twice > s || (twice == s && ((int)c & 1))) c += copysignf(1.0f, rest);
+            } else if (s > 0.0f) {
+                c = fminf(fmaxf(rintf(v[i] / s), -127.0f), 127.0f);  // a scale of few bits: quotients up to 190
+            }
+            k[i] = c + kOnes;
         }
-        k = fminf(fmaxf(k, -127.0f), 127.0f);
-        w[i >> 2] |= ((uint32_t)(int)k & 0xffu) << (8 * (i & 3));
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(k[4 * j + 1]), __float_as_uint(k[4 * j]), 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(k[4 * j + 3]), __float_as_uint(k[4 * j + 2]), 0x04000c0cu);
+        w[j] = lo | hi;
     }
     codes = (uint64_t)w[1] << 32 | w[0];
     return s;
 }
 
+// What codes stand for, rounded once: a code is one byte u less 128, and 128 s is exact.
 __device__ __forceinline__ void restore8(const uint64_t codes, float s, float (&v)[kEach]) {
+    const uint32_t w[2] = {(uint32_t)codes ^ 0x80808080u, (uint32_t)(codes >> 32) ^ 0x80808080u};
+    const float off = -128.0f * s;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) v[i] = (float)(int8_t)(codes >> (8 * i)) * s;
+    for (int i = 0; i < kEach; ++i) v[i] = fmaf((float)((w[i >> 2] >> (8 * (i & 3))) & 0xffu), s, off);
 }
 
-// Where a thread works: group `group` of row `row`, its 8 columns from `col`.
+// 1 / (1 + exp(-g)), to about 2^-22 of itself and |g| 2^-24.
+__device__ __forceinline__ float sigmoid(float g) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
+}
+
+// Where a thread works: group `group` of row `row`, its 8 columns from `col`. (A launch has fewer than 2^28 groups.)
 struct Item { int64_t row; int group, col; bool there; };
 __device__ __forceinline__ Item item_of(int64_t rows, int groups) {
-    const int64_t i = (int64_t)blockIdx.x * kItems + threadIdx.x / kLanes;
+    const uint32_t i = blockIdx.x * kItems + threadIdx.x / kLanes, row = i / (uint32_t)groups;
     Item it;
-    it.row = i / groups;
-    it.group = (int)(i - it.row * groups);
+    it.row = row;
+    it.group = (int)(i - row * (uint32_t)groups);
     it.col = it.group * kGroup + (threadIdx.x % kLanes) * kEach;
     it.there = it.row < rows;
     return it;
@@ -101,10 +163,11 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const void* x, int64
                                                             uint8_t* codes, float* scales) {
     const Item it = item_of(rows, groups);
     if (!it.there) return;  // (16 lanes alike)
+    const auto r = load8<DT>(x, it.row * stride, it.col, cols);
     float v[kEach];
-    load8<DT>(x, it.row * stride, it.col, cols, v);
+    widen<DT, kEach>(r, v);
     uint64_t w;
-    const float s = quantize8(v, w);
+    const float s = quantize8<DT>(r, v, w);
     const int to = code_stride(cols);
     if (it.col < to) *reinterpret_cast<uint64_t*>(codes + it.row * to + it.col) = w;
     if (threadIdx.x % kLanes == 0) scales[it.row * groups + it.group] = s;
@@ -116,15 +179,17 @@ __global__ __launch_bounds__(kThreads) void silu_mul_forward_kernel(const void* 
     const Item it = item_of(rows, groups);
     if (!it.there) return;
     float g[kEach], u[kEach], o[kEach];
-    load8<DT>(gu, it.row * stride, it.col, hidden, g);
-    load8<DT>(gu, it.row * stride + hidden, it.col, hidden, u);
+    const auto rg = load8<DT>(gu, it.row * stride, it.col, hidden);
+    const auto ru = load8<DT>(gu, it.row * stride + hidden, it.col, hidden);
+    widen<DT, kEach>(rg, g);
+    widen<DT, kEach>(ru, u);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) o[i] = g[i] / (1.0f + expf(-g[i])) * u[i];
+    for (int i = 0; i < kEach; ++i) o[i] = g[i] * sigmoid(g[i]) * u[i];
     store8<DT>(y, it.row * hidden, it.col, hidden, o);
     if constexpr (KEEP) {
         const int to = code_stride(hidden);
         uint64_t w[2];
-        const float s[2] = {quantize8(g, w[0]), quantize8(u, w[1])};
+        const float s[2] = {quantize8<DT>(rg, g, w[0]), quantize8<DT>(ru, u, w[1])};
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int64_t at = j * rows + it.row;
@@ -143,10 +208,10 @@ __global__ __launch_bounds__(kThreads) void silu_mul_backward_kernel(const uint8
     float g[kEach], u[kEach], d[kEach];
     restore8(*reinterpret_cast<const uint64_t*>(codes + it.row * to + it.col), scales[it.row * groups + it.group], g);
     restore8(*reinterpret_cast<const uint64_t*>(codes + (rows + it.row) * to + it.col), scales[(rows + it.row) * groups + it.group], u);
-    load8<DT>(dy, it.row * stride, it.col, hidden, d);
+    widen<DT, kEach>(load8<DT>(dy, it.row * stride, it.col, hidden), d);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        const float sig = 1.0f / (1.0f + expf(-g[i]));
+        const float sig = sigmoid(g[i]);
         const float du = d[i] * g[i] * sig;
         g[i] = d[i] * u[i] * (sig * (1.0f + g[i] * (1.0f - sig)));
         u[i] = du;
