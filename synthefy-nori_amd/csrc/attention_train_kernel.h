@@ -19,6 +19,22 @@ template <int DT, int DK> struct Geo {
     static constexpr int KS = DK / 16, MS = DP / 32;
 };
 
+// The order in which the compiler lays out `products` products, each with `reads` reads of its operand from LDS: the operands of
+// `ahead` products first, then a product and the next operand's reads in turn. Left to itself it reads an operand right
+// before its product, a latency every time.
+template <int DT, int products, int reads, int ahead, int before = 0>
+__device__ __forceinline__ void interleave() {
+    if constexpr (DT != NORI_F32) {
+        __builtin_amdgcn_sched_group_barrier(0x100, before + ahead * reads, 0);
+#pragma unroll
+        for (int i = 0; i < products - ahead; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, ahead, 0);
+    }
+}
+
 // Left operand: row `row` (lane % 32 of a step's 32) of a tile, its columns 16 k + 8 h .. + 7.
 template <int DT, int DK>
 __device__ __forceinline__ typename El<DT>::Frag direct(const typename El<DT>::T* tile, int row, int k, int half) {
@@ -354,6 +370,7 @@ __device__ __forceinline__ void dq_step(const typename El<DT>::T* ks, const type
             s = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s);
             dp = mma(direct<DT, DK>(vs, sub * 32 + (lane & 31), k, half), dof[k], dp);
         }
+        interleave<DT, 2 * G::KS, 1, 4>();
 #pragma unroll
         for (int i = 0; i < 16; ++i) ds[sub][i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) * dp[i];
     }
@@ -447,6 +464,7 @@ __device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typ
             s = mma(direct<DT, DK>(qs, sub * 32 + (lane & 31), k, half), kf[k], s);
             dp = mma(direct<DT, DK>(dos, sub * 32 + (lane & 31), k, half), vf[k], dp);
         }
+        interleave<DT, 2 * G::KS, 1, 4, 4>();
         float pr[16], ds[1][16];
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
@@ -472,6 +490,7 @@ __device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typ
                 dk[j] = mma(transposed<DT, G::LS>(qs, sub * 32 + 16 * t, 32 * j, lane), f, dk[j]);
             }
         }
+        interleave<DT, 4 * G::MS, 2, 2>();
     }
 }
 
