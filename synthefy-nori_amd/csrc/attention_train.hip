@@ -107,9 +107,10 @@ Args plan(const nori_attention_train_args& a, Kind kind) {
 }
 
 // Units that one workgroup takes through the whole backward pass.
-bool few(const nori_attention_train_args& a) {
-    return a.dtype != NORI_F32 && a.d <= kFewWidth && a.dq && a.dkv && a.nk <= 64 && a.nq * (a.heads / a.kv_heads) <= 64;
+bool few(const nori_attention_train_args& a, bool backward) {
+    return a.dtype != NORI_F32 && a.d <= kFewWidth && a.nk <= 64 && a.nq * (a.heads / a.kv_heads) <= 64 && (!backward || (a.dq && a.dkv));
 }
+
 
 int64_t part_bytes(const Args& p, Kind kind) { return p.splits > 1 ? p.splits * part_rows(p, kind) * p.a.d * 4 : 0; }
 int64_t aligned16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -121,6 +122,13 @@ int launch_typed(Kind kind, const Args& p, hipStream_t stream) {
         case NORI_BF16: return p.wide ? launch_bf16(kind, p, blocks, stream) : launch_bf16_narrow(kind, p, blocks, stream);
         default: return launch_f32(kind, p, blocks, stream);
     }
+}
+
+// One workgroup a unit, of wavefronts for its rows and for its keys.
+int launch_few(Kind kind, Args p, hipStream_t stream) {
+    p.waves = p.a.nk > 32 || p.rows > 32 ? 2 : 1;
+    p.tiles = p.splits = 1;
+    return launch_typed(kind, p, stream);
 }
 
 int join(Kind kind, const Args& p, hipStream_t stream) {
@@ -204,7 +212,7 @@ extern "C" int64_t nori_attention_train_workspace_bytes(const nori_attention_tra
         const Args p = plan(*a, kForward);
         return p.splits > 1 ? aligned16(part_bytes(p, kForward)) + aligned16(p.splits * part_rows(p, kForward) * 4) : 0;
     }
-    if (few(*a)) return 0;
+    if (few(*a, true)) return 0;
     const Args q = plan(*a, kDq), kv = plan(*a, kDkv);
     return aligned16(part_rows(q, kDq) * 4) + std::max(a->dq ? part_bytes(q, kDq) : 0, a->dkv ? part_bytes(kv, kDkv) : 0);
 }
@@ -217,6 +225,7 @@ extern "C" int nori_attention_train_forward(const nori_attention_train_args* a, 
     hipStream_t stream = (hipStream_t)stream_v;
     Args p = plan(*a, kForward);
     p.wide = wide(*a, false);
+    if (few(*a, false)) return launch_few(kFewForward, p, stream);
     p.part = reinterpret_cast<float*>(a->workspace);
     p.part_lse = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + aligned16(part_bytes(p, kForward)));
     if (int rc = launch_typed(kForward, p, stream)) return rc;
@@ -232,11 +241,7 @@ extern "C" int nori_attention_train_backward(const nori_attention_train_args* a,
     float* delta = reinterpret_cast<float*>(a->workspace);
     Args q = plan(*a, kDq);
     q.wide = wide(*a, true);
-    if (few(*a)) {
-        q.waves = std::max(q.waves, plan(*a, kDkv).waves);
-        q.tiles = q.splits = 1;
-        return launch_typed(kFew, q, stream);
-    }
+    if (few(*a, true)) return launch_few(kFew, q, stream);
     if (a->nq > 0) {
         if (!a->dq) q.splits = 1;  // the rows' sums alone
         q.delta = delta;

@@ -83,6 +83,24 @@ __device__ __forceinline__ void store_row(Out* out, const f32x16 (&x)[MS], float
         }
 }
 
+// The same for the 32 rows of a wavefront's columns by way of LDS (its own 32 rows there): a lane's columns are apart in memory, 32
+// lines an access, which the address units bound short scans by; from LDS rows go out side by side. to(row): where it begins.
+template <int DT, int DK, int W, int LS, int MS, class To>
+__device__ __forceinline__ void store_rows(typename El<DT>::T* lds, const f32x16 (&x)[MS], float by, int d, int lane, int rows, To to) {
+    using T = typename El<DT>::T;
+    typedef uint32_t Chunk __attribute__((ext_vector_type(W * sizeof(T) / 4)));
+    constexpr int CH = DK / W;
+    store_row<DT>(lds + (lane & 31) * LS, x, by, d, lane >> 5);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < (32 * CH + 63) / 64; ++i) {
+        const int idx = lane + 64 * i, row = idx / CH, col = W * (idx % CH);
+        if (row < rows && col < d) *reinterpret_cast<Chunk*>(to(row) + col) = *reinterpret_cast<const Chunk*>(lds + row * LS + col);
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Query row r of a unit: head and query.
 struct Row { int64_t head, query; };
 __device__ __forceinline__ Row row_of(const Args& p, int64_t unit_head, int r) {
@@ -239,6 +257,20 @@ __device__ __forceinline__ void forward_step(const typename El<DT>::T* ks, const
     }
 }
 
+// The magnitude of the logits' factor: the running maximum wants it positive, so a negative one changes the queries' signs, and one
+// of 0 makes them 0 beside a factor of 1.
+template <int DT, int KS>
+__device__ __forceinline__ float positive(float c, typename El<DT>::Frag (&q)[KS]) {
+    if (c <= 0.f) {
+        const float sign = c < 0.f ? -1.f : 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) at(q[k], j) = at(q[k], j) * sign;
+    }
+    return c == 0.f ? 1.f : fabsf(c);
+}
+
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, DK <= 64 && NW == 4 ? 3 : 2) void forward_kernel(const Args p) {
     using E = El<DT>;
@@ -260,15 +292,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && NW == 4 ? 3 : 2) void forward_
 
     typename E::Frag qf[G::KS];
     load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
-    // the running maximum wants a positive factor: a negative one changes signs first, one of 0 makes the logits 0
-    const float c = p.c == 0.f ? 1.f : fabsf(p.c);
-    if (p.c <= 0.f) {
-        const float sign = p.c < 0.f ? -1.f : 0.f;
-#pragma unroll
-        for (int k = 0; k < G::KS; ++k)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) at(qf[k], j) = at(qf[k], j) * sign;
-    }
+    const float c = positive<DT>(p.c, qf);
 
     const T* kv = reinterpret_cast<const T*>(a.kv) + w.b * a.kv_bg + w.hk * a.kv_head + begin * a.kv_row;
     Stage<DT, DK, W, 64 * NW, kRows> stage;
@@ -589,8 +613,48 @@ dkv_step<DT, DK, kRows / 32>(qs, dos, off, deltas, end - first, kf, vf, dk, dv, 
 }
 
 // ---------------------------------------------------------------- few rows and few keys
-// The whole backward pass of a unit of up to 32 NW rows and keys: both sides in LDS, read from memory once, where the kernels
-// above read them twice and the row sums pass through memory.
+// The forward pass of a unit of up to 32 NW rows and keys. One tile and no loop: half the registers of forward_kernel, so twice the
+// wavefronts, which is what units this short go by.
+template <int DT, int DK, int W, int NW>
+__global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
+    using E = El<DT>;
+    using G = Geo<DT, DK>;
+    using T = typename E::T;
+    __shared__ __attribute__((aligned(16))) T ks[32 * NW * G::LS];
+    __shared__ __attribute__((aligned(16))) T vs[32 * NW * G::LS];
+    const auto& a = p.a;
+    const int64_t unit = work_index(blockIdx.x, gridDim.x), b = unit / a.kv_heads, hk = unit % a.kv_heads;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, own = wave * 32 + (lane & 31);
+    const int length = length_of(a, b), rows = (int)p.rows;
+    const T* kv = reinterpret_cast<const T*>(a.kv) + b * a.kv_bg + hk * a.kv_head;
+    const bool there = own < rows;
+    const Row row = there ? row_of(p, hk, own) : Row{hk * p.group, 0};
+    typename E::Frag qf[G::KS];
+    {
+        Stage<DT, DK, W, 64 * NW, 32 * NW> keys;
+        keys.place(a.d, a.kv_row, a.kv_row);
+        keys.load(kv, kv + a.kv_half, length);
+        load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.q) + b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
+        keys.store(ks, vs);
+    }
+    const float c = positive<DT>(p.c, qf);
+    __syncthreads();
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[G::MS] = {};
+    if (length > 0) forward_step<DT, DK, NW>(ks, vs, length, qf, o, m, l, c, lane);
+    l += other_half(l);
+    if (there && half == 0 && a.lse) a.lse[unit * p.rows + own] = length > 0 ? (__builtin_amdgcn_logf(l) - E::kTop + m * c) * kLn2 : -INFINITY;
+    T* out = reinterpret_cast<T*>(a.out) + b * a.nq * a.heads * a.d;
+    __syncthreads();  // the tile is everyone's until here
+    store_rows<DT, DK, W, G::LS>(ks + wave * 32 * G::LS, o, length > 0 ? 1.f / l : 0.f, a.d, lane, rows - wave * 32, [&](int i) {
+        const Row to = row_of(p, hk, wave * 32 + i);
+        return out + (to.query * a.heads + to.head) * a.d;
+    });
+}
+
+// The whole backward pass of such a unit: both sides in LDS, read from memory once, where the kernels above read them twice and the
+// rows' sums pass through memory. (Keys first and queries in their place later take half the LDS and a wavefront a SIMD more, but
+// read the queries twice: 8,192 x 8 units of 33 x 33 of 44, fp16, 656 us so, 557 this way.)
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) {
     using E = El<DT>;
@@ -669,7 +733,10 @@ void launch_one(Kind kind, const Args& p, dim3 grid, hipStream_t stream) {
     if (kind == kForward) hipLaunchKernelGGL((forward_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
     else if (kind == kDq) hipLaunchKernelGGL((dq_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
     else if (kind == kDkv) hipLaunchKernelGGL((dkv_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
-    else if constexpr (DT != NORI_F32 && DK <= kFewWidth && NW <= 2) hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
+    else if constexpr (DT != NORI_F32 && DK <= kFewWidth && NW <= 2) {
+        if (kind == kFewForward) hipLaunchKernelGGL((forward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
+        else hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
+    }
 }
 
 template <int DT, int DK, int W>
