@@ -416,6 +416,48 @@ __device__ __forceinline__ void dq_step(const typename El<DT>::T* ks, const type
         }
 }
 
+// The same of rows whose keys are all in this tile, which takes delta = sum of p (dout v) from them: with few keys ds is a small
+// difference, and delta of the result as it was rounded would be off by as much.
+template <int DT, int DK, int NS>
+__device__ __forceinline__ void dq_whole(const typename El<DT>::T* ks, const typename El<DT>::T* vs, int left,
+                                         const typename El<DT>::Frag (&qf)[DK / 16], const typename El<DT>::Frag (&dof)[DK / 16],
+                                         f32x16 (&dq)[Geo<DT, DK>::MS], Scale& scale, float c, float lse2, float& delta, int lane) {
+    using G = Geo<DT, DK>;
+    const int half = lane >> 5;
+    float pr[NS][16], ds[NS][16];
+    delta = 0.f;
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub) {
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int k = 0; k < G::KS; ++k) {
+            s = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s);
+            dp = mma(direct<DT, DK>(vs, sub * 32 + (lane & 31), k, half), dof[k], dp);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bool in = sub * 32 + 8 * (i / 4) + i % 4 < left - 4 * half;
+            pr[sub][i] = in ? __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) : 0.f;
+            ds[sub][i] = in ? dp[i] : 0.f;
+            delta = fmaf(pr[sub][i], ds[sub][i], delta);
+        }
+    }
+    delta += other_half(delta);
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[sub][i] = pr[sub][i] * (ds[sub][i] - delta);
+    if constexpr (El<DT>::kScaled) scale.apply(ds, dq);
+#pragma unroll
+    for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const auto f = rounded<DT>(ds[sub], t);
+#pragma unroll
+            for (int j = 0; j < G::MS; ++j) dq[j] = mma(transposed<DT, G::LS>(ks, sub * 32 + 16 * t, 32 * j, lane), f, dq[j]);
+        }
+}
+
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq_kernel(const Args p) {
     using E = El<DT>;
@@ -434,14 +476,15 @@ __global__ __launch_bounds__(64 * NW, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq
     const int64_t unit_row = w.unit * p.rows + r;
     const int length = length_of(a, w.b);
     const int begin = (int)(w.split * p.per_split);
-    const int end = a.dq ? (int)min((int64_t)length, w.split * p.per_split + p.per_split) : begin;
+    const bool whole = length <= kRows;  // all keys in the first part's first tile
+    const int end = a.dq || whole ? (int)min((int64_t)length, w.split * p.per_split + p.per_split) : begin;
 
     typename E::Frag dof[G::KS], qf[G::KS];
     load_own<DT, DK, W>(dof, reinterpret_cast<const T*>(a.dout) + w.b * a.do_bg + row.query * a.do_row + row.head * a.do_head, there, a.d, half);
     load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.out) + ((w.b * a.nq + row.query) * a.heads + row.head) * a.d, there, a.d, half);
-    const float delta = row_sum<DT>(dof, qf);
-    if (there && half == 0 && w.split == 0) p.delta[unit_row] = delta;
-    if (!a.dq) return;
+    float delta = row_sum<DT>(dof, qf);
+    if (there && half == 0 && w.split == 0 && !whole) p.delta[unit_row] = delta;
+    if (begin >= end && !a.dq) return;
     load_own<DT, DK, W>(qf, reinterpret_cast<const T*>(a.q) + w.b * a.q_bg + row.query * a.q_row + row.head * a.q_head, there, a.d, half);
     const float lse2 = there ? a.lse[unit_row] * kLog2e : 0.f;
 
@@ -451,7 +494,14 @@ __global__ __launch_bounds__(64 * NW, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq
     if (begin < end) stage.load(kv, kv + a.kv_half, end - begin);
     f32x16 dq[G::MS] = {};
     Scale scale;
-    for (int first = begin; first < end; first += kRows) {
+    if (whole && begin < end) {
+        stage.store(ks, vs);
+        __syncthreads();
+        dq_whole<DT, DK, kRows / 32>(ks, vs, length, qf, dof, dq, scale, p.c, lse2, delta, lane);
+        if (there && half == 0) p.delta[unit_row] = delta;
+        if (!a.dq) return;
+    }
+    for (int first = whole ? end : begin; first < end; first += kRows) {
         __syncthreads();
         stage.store(ks, vs);
         __syncthreads();
@@ -687,24 +737,24 @@ __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) 
     const Row row = there ? row_of(p, hk, own) : Row{hk * p.group, 0};
     const int64_t out_row = ((b * a.nq + row.query) * a.heads + row.head) * a.d;
     typename E::Frag x[G::KS], y[G::KS];
-    load_own<DT, DK, W>(x, reinterpret_cast<const T*>(a.out) + out_row, there, a.d, half);
     const float lse2 = there ? a.lse[unit * p.rows + own] * kLog2e : 0.f;
     keys.store(ks, vs);
     queries.store(qs, dos);
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < G::KS; ++k) y[k] = direct<DT, DK>(dos, own, k, half);
-    const float delta = row_sum<DT>(y, x);
-    if (half == 0) {
-        off[own] = there ? E::kBias - lse2 : 0.f;
-        deltas[own] = there ? -delta : 0.f;
-    }
     {
         f32x16 dq[G::MS] = {};
         Scale scale;
+        float delta = 0.f;
 #pragma unroll
-        for (int k = 0; k < G::KS; ++k) x[k] = direct<DT, DK>(qs, own, k, half);
-        if (length > 0) dq_step<DT, DK, NW>(ks, vs, length, x, y, dq, scale, p.c, lse2, delta, lane);
+        for (int k = 0; k < G::KS; ++k) {
+            x[k] = direct<DT, DK>(qs, own, k, half);
+            y[k] = direct<DT, DK>(dos, own, k, half);
+        }
+        if (length > 0) dq_whole<DT, DK, NW>(ks, vs, length, x, y, dq, scale, p.c, lse2, delta, lane);
+        if (half == 0) {
+            off[own] = there ? E::kBias - lse2 : 0.f;
+            deltas[own] = there ? -delta : 0.f;
+        }
         if (there) store_row<DT>(reinterpret_cast<T*>(a.dq) + out_row, dq, a.scale * (E::kScaled ? scale.inverse() : 1.f), a.d, half);
     }
     __syncthreads();

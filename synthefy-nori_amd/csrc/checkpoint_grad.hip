@@ -50,19 +50,37 @@ __device__ __forceinline__ Eight<DT> values(uint32_t lo, uint32_t hi, float s) {
     }
 }
 
-// TN columns of dy by 128 of x a workgroup, half of each a wavefront.
-template <int DT, int TN>
+// dy s in two bfloat16 pieces, to 2^-17 of itself, beside codes that are whole numbers: what an fp32 gradient of 16-bit rows takes. x
+// rounded to the rows' type would leave 2^-12 (float16) or 2^-9 of every term, above what the gradient's type can tell.
+template <int DT>
+__device__ __forceinline__ void pieces(const Eight<DT>& y, float s, Eight<NORI_BF16>& hi, Eight<NORI_BF16>& lo) {
+    bf16x8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float v = (DT == NORI_F16 ? f16_to_f32(y.e[e]) : bf16_to_f32(y.e[e])) * s;
+        h[e] = (__bf16)v;
+        const float w = (float)h[e];
+        l[e] = (__bf16)(fabsf(w) == INFINITY ? 0.f : v - w);
+    }
+    hi = __builtin_bit_cast(Eight<NORI_BF16>, h);
+    lo = __builtin_bit_cast(Eight<NORI_BF16>, l);
+}
+
+// TN columns of dy by 128 of x a workgroup, half of each a wavefront. FINE: dw in fp32 of 16-bit rows, two products a pair.
+template <int DT, int TN, bool FINE>
 __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
-    using E = El<DT>;
-    using T = typename E::T;
+    constexpr int MT = FINE ? NORI_BF16 : DT;  // the products' type
+    using E = El<MT>;
+    using T = typename El<DT>::T;
     constexpr int kRows = DT == NORI_F32 ? 32 : 64;  // rows a step
     // transposed reads take 64 bytes of four rows at once: rows 16 banks apart (mod 64) meet no other's
-    constexpr int kPad = DT == NORI_F32 ? E::kPad : 32, YS = TN + kPad, XS = kGroup + kPad;
+    constexpr int kPad = DT == NORI_F32 ? El<DT>::kPad : 32, YS = TN + kPad, XS = kGroup + kPad;
     constexpr int MY = TN / 64, MX = 2;              // products of 32 columns a wavefront
     constexpr int kPerRow = TN / 8, kYStep = kThreads / kPerRow, NY = kRows / kYStep;
     constexpr int kXStep = kThreads / (kGroup / 16), NX = kRows / kXStep;
     __shared__ __attribute__((aligned(16))) T ys[kRows * YS];
     __shared__ __attribute__((aligned(16))) T xs[kRows * XS];
+    __shared__ __attribute__((aligned(16))) T ls[FINE ? kRows * YS : 8];  // dy's low pieces
     const int64_t i = blockIdx.x, eights = gridDim.x & ~7u;  // neighbours, which read the same rows, on one XCD
     const int64_t work = i < eights ? (i & 7) * (eights >> 3) + (i >> 3) : i;
     const int kt = (int)(work % a.k_tiles), nt = (int)(work / a.k_tiles % a.n_tiles), split = (int)(work / a.k_tiles / a.n_tiles);
@@ -77,7 +95,7 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
 
     Eight<DT> ye[NY];
     uint4 xe[NX];
-    float xsc[NX];
+    float xsc[FINE ? 1 : NX], ysc[FINE ? NY : 1];
     // A step whose rows are all there, and not the last, whose eight columns past the row's end reach into the next row
     const auto whole = [&](int64_t from) { return from + kRows <= end && from + kRows < a.rows && a.dy_stride >= 8; };
     const auto load = [&](int64_t from) {
@@ -90,8 +108,22 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
             xe[j] = *reinterpret_cast<const uint4*>(px + j * kXStep * a.code_stride + xoff);
-            xsc[j] = ps[j * kXStep * a.groups + xrow * a.groups];
+            if constexpr (!FINE) xsc[j] = ps[j * kXStep * a.groups + xrow * a.groups];
         }
+        if constexpr (FINE) {
+#pragma unroll
+            for (int j = 0; j < NY; ++j) ysc[j] = ps[j * kYStep * a.groups + yrow * a.groups];
+        }
+    };
+    const auto put_y = [&](int j, const Eight<DT>& y, float s) {
+        const int at = (yrow + j * kYStep) * YS + ycol;
+        if constexpr (FINE) pieces<DT>(y, s, *reinterpret_cast<Eight<NORI_BF16>*>(&ys[at]), *reinterpret_cast<Eight<NORI_BF16>*>(&ls[at]));
+        else *reinterpret_cast<Eight<DT>*>(&ys[at]) = y;
+    };
+    const auto put_x = [&](int j, uint4 x, float s) {
+        Eight<MT>* to = reinterpret_cast<Eight<MT>*>(&xs[(xrow + j * kXStep) * XS + xcol]);
+        to[0] = values<MT>(x.x, x.y, s);
+        to[1] = values<MT>(x.z, x.w, s);
     };
     float colsum[8] = {};
     const auto add = [&](const Eight<DT>& y) {
@@ -108,13 +140,9 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
         __syncthreads();
         if (whole(from)) {
 #pragma unroll
-            for (int j = 0; j < NY; ++j) *reinterpret_cast<Eight<DT>*>(&ys[(yrow + j * kYStep) * YS + ycol]) = ye[j];
+            for (int j = 0; j < NY; ++j) put_y(j, ye[j], FINE ? ysc[FINE ? j : 0] : 1.f);
 #pragma unroll
-            for (int j = 0; j < NX; ++j) {
-                Eight<DT>* to = reinterpret_cast<Eight<DT>*>(&xs[(xrow + j * kXStep) * XS + xcol]);
-                to[0] = values<DT>(xe[j].x, xe[j].y, xsc[j]);
-                to[1] = values<DT>(xe[j].z, xe[j].w, xsc[j]);
-            }
+            for (int j = 0; j < NX; ++j) put_x(j, xe[j], FINE ? 1.f : xsc[FINE ? 0 : j]);
             if (turn == 0) {
 #pragma unroll
                 for (int j = 0; j < NY; ++j) add(ye[j]);
@@ -127,7 +155,7 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (r < end && yc + e < a.n) y.e[e] = reinterpret_cast<const T*>(a.dy)[r * a.dy_stride + yc + e];
-                *reinterpret_cast<Eight<DT>*>(&ys[(yrow + j * kYStep) * YS + ycol]) = y;
+                put_y(j, y, FINE && a.dw && r < end ? a.scales[r * a.groups + kt] : 1.f);
                 if (turn == 0) add(y);
             }
 #pragma unroll 1
@@ -137,11 +165,9 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
                 float sc = 0.f;
                 if (r < end) {
                     x = *reinterpret_cast<const uint4*>(a.codes + r * a.code_stride + xat);
-                    sc = a.scales[r * a.groups + kt];
+                    sc = FINE ? 1.f : a.scales[r * a.groups + kt];
                 }
-                Eight<DT>* to = reinterpret_cast<Eight<DT>*>(&xs[(xrow + j * kXStep) * XS + xcol]);
-                to[0] = values<DT>(x.x, x.y, sc);
-                to[1] = values<DT>(x.z, x.w, sc);
+                put_x(j, x, sc);
             }
         }
         if (turn == 0) turn = a.splits > 1 ? a.k_tiles : 1;
@@ -153,13 +179,21 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
         for (int t = 0; t < kRows / 16; ++t) {
             typename E::Frag y[MY], x[MX];
 #pragma unroll
-            for (int j = 0; j < MX; ++j) x[j] = transposed<DT, XS>(xs, 16 * t, wk + 32 * j, lane);
+            for (int j = 0; j < MX; ++j) x[j] = transposed<MT, XS>(xs, 16 * t, wk + 32 * j, lane);
 #pragma unroll
-            for (int j = 0; j < MY; ++j) y[j] = transposed<DT, YS>(ys, 16 * t, wn + 32 * j, lane);
+            for (int j = 0; j < MY; ++j) y[j] = transposed<MT, YS>(ys, 16 * t, wn + 32 * j, lane);
 #pragma unroll
             for (int j = 0; j < MY; ++j)
 #pragma unroll
                 for (int l = 0; l < MX; ++l) acc[j][l] = mma(y[j], x[l], acc[j][l]);
+            if constexpr (FINE) {
+#pragma unroll
+                for (int j = 0; j < MY; ++j) y[j] = transposed<MT, YS>(ls, 16 * t, wn + 32 * j, lane);
+#pragma unroll
+                for (int j = 0; j < MY; ++j)
+#pragma unroll
+                    for (int l = 0; l < MX; ++l) acc[j][l] = mma(y[j], x[l], acc[j][l]);
+            }
         }
     }
     if (a.db && (a.splits > 1 || kt == 0)) {
@@ -211,14 +245,15 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Args a) {
 
 constexpr int kMost = 1 << 20;  // columns
 
-Args plan(int dtype, int64_t rows, int32_t n, int32_t k) {
+// fine: dw in fp32 of 16-bit rows
+Args plan(int dtype, bool fine, int64_t rows, int32_t n, int32_t k) {
     Args a{};
     a.rows = rows;
     a.n = n;
     a.k = k;
     a.code_stride = (k + 15) / 16 * 16;
     a.groups = (k + kGroup - 1) / kGroup;
-    a.tile_n = dtype == NORI_F32 || (n + 127) / 128 % 2 ? 128 : 256;
+    a.tile_n = dtype == NORI_F32 || fine || (n + 127) / 128 % 2 ? 128 : 256;
     a.n_tiles = (n + a.tile_n - 1) / a.tile_n;
     a.k_tiles = a.groups;
     // one round of the workgroups that the compute units hold
@@ -233,9 +268,9 @@ int64_t part_w_bytes(const Args& a) { return ((int64_t)a.splits * a.n * a.k * 4 
 
 }  // namespace
 
-extern "C" int64_t nori_checkpoint_grad_workspace_bytes(int dtype, int64_t rows, int32_t n, int32_t k) {
+extern "C" int64_t nori_checkpoint_grad_workspace_bytes(int dtype, int dw_dtype, int64_t rows, int32_t n, int32_t k) {
     if (rows < 0 || n < 1 || k < 1) return 0;
-    const Args a = plan(dtype, rows, n, k);
+    const Args a = plan(dtype, dw_dtype != dtype, rows, n, k);
     return a.splits > 1 ? part_w_bytes(a) + (int64_t)a.splits * a.k_tiles * n * 4 : 0;
 }
 
@@ -255,7 +290,8 @@ extern "C" int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int
     if (!dw && !db) return NORI_OK;
     if (rows > 0 && (!dy || (dw && (!codes || !scales || (uintptr_t)codes % 16))))
         return fail(NORI_ERR_INVALID, "checkpoint_grad: null or unaligned pointer");
-    Args a = plan(dtype, rows, n, k);
+    const bool fine = dw && dw_dtype != dtype;
+    Args a = plan(dtype, fine, rows, n, k);
     a.dy = dy;
     a.dy_stride = dy_row_stride;
     a.codes = (const int8_t*)codes;
@@ -268,7 +304,7 @@ extern "C" int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int
     const int64_t blocks = (int64_t)a.n_tiles * a.k_tiles * a.splits;
     if (!one_launch(blocks, kThreads)) return fail(NORI_ERR_UNSUPPORTED, "checkpoint_grad: more workgroups than one launch has");
     if (a.splits > 1) {
-        const int64_t need = nori_checkpoint_grad_workspace_bytes(dtype, rows, n, k);
+        const int64_t need = nori_checkpoint_grad_workspace_bytes(dtype, dw ? dw_dtype : dtype, rows, n, k);
         if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
             return fail(NORI_ERR_INVALID, "checkpoint_grad: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
         a.part_w = (float*)workspace;
@@ -276,8 +312,14 @@ extern "C" int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int
     }
     hipStream_t stream = (hipStream_t)stream_v;
     NORI_DISPATCH_FLOAT(dtype, DT, {
-        if (DT != NORI_F32 && a.tile_n == 256) hipLaunchKernelGGL((grad_kernel<DT, DT == NORI_F32 ? 128 : 256>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
-        else hipLaunchKernelGGL((grad_kernel<DT, 128>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+        const dim3 grid((unsigned)blocks), threads(kThreads);
+        if constexpr (DT == NORI_F32) {
+            hipLaunchKernelGGL((grad_kernel<DT, 128, false>), grid, threads, 0, stream, a);
+        } else {
+            if (fine) hipLaunchKernelGGL((grad_kernel<DT, 128, true>), grid, threads, 0, stream, a);
+            else if (a.tile_n == 256) hipLaunchKernelGGL((grad_kernel<DT, 256, false>), grid, threads, 0, stream, a);
+            else hipLaunchKernelGGL((grad_kernel<DT, 128, false>), grid, threads, 0, stream, a);
+        }
         if (a.splits > 1) {
             const int64_t items = (dw ? (int64_t)n * k : 0) + (db ? n : 0);
             hipLaunchKernelGGL((join_kernel<DT>), dim3((unsigned)std::min<int64_t>((items + kThreads - 1) / kThreads, 16 * device_cus())),

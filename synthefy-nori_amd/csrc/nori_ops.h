@@ -196,10 +196,10 @@ int nori_checkpoint_silu_mul_backward(const void* codes, const float* scales, in
                                       int64_t dy_row_stride, void* dgu, void* stream);
 
 // The gradients of a projection's weight and bias over rows kept in 8 bits (checkpoint_grad.hip): dw [n, k] = sum over rows of
-// dy^T x, x what the codes stand for rounded to dy's dtype, db [n] = sum of dy; each NULL where it is not asked for, of its own
-// dtype (dy's or fp32), contiguous. The workspace, of nori_checkpoint_grad_workspace_bytes and 16-byte aligned, takes the sums
+// dy^T x, x what the codes stand for (rounded to dy's dtype where dw is of it; beside an fp32 dw of 16-bit rows each term is held to
+// 2^-17), db [n] = sum of dy; each NULL where it is not asked for, of its own dtype (dy's or fp32), contiguous. The workspace, of nori_checkpoint_grad_workspace_bytes and 16-byte aligned, takes the sums
 // of parts of the rows, which are joined in order. Sums are fp32. No rows: zeros.
-int64_t nori_checkpoint_grad_workspace_bytes(int dtype, int64_t rows, int32_t n, int32_t k);
+int64_t nori_checkpoint_grad_workspace_bytes(int dtype, int dw_dtype, int64_t rows, int32_t n, int32_t k);
 int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int32_t n, int64_t dy_row_stride, const void* codes,
                          const float* scales, int32_t k, void* dw, int dw_dtype, void* db, int db_dtype, void* workspace,
                          int64_t workspace_bytes, void* stream);

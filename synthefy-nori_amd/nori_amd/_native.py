@@ -193,7 +193,7 @@ OPS: dict[str, tuple[object, list]] = {
     "nori_checkpoint_quantize": (ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _vp]),
     "nori_checkpoint_silu_mul": (ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _vp, _vp]),
     "nori_checkpoint_silu_mul_backward": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _i64, _vp, _vp]),
-    "nori_checkpoint_grad_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32]),
+    "nori_checkpoint_grad_workspace_bytes": (_i64, [_i32, _i32, _i64, _i32, _i32]),
     "nori_checkpoint_grad": (
         ctypes.c_int, [_vp, _i32, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i64, _vp],
     ),

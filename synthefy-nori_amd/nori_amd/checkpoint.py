@@ -77,7 +77,7 @@ class _CheckpointedLinear(torch.autograd.Function):
             if rows:
                 lib, dtype = nat.lib(), nat.dtype_code(dy.dtype)
                 with nat.on(device):
-                    size = lib.nori_checkpoint_grad_workspace_bytes(dtype, rows, n, k)
+                    size = lib.nori_checkpoint_grad_workspace_bytes(dtype, nat.dtype_code(w_dtype) if need_w else dtype, rows, n, k)
                     workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
                     nat.check(
                         lib.nori_checkpoint_grad(

@@ -83,8 +83,8 @@ def test_the_library_refuses():
     assert g(p, f16, 2, 8, 7, p, p, 8, p, f32, p, f32, None, 0, None) == bad
     assert g(p, f16, 2, 8, 8, None, p, 8, p, f32, p, f32, None, 0, None) == bad
     assert g(p, f16, 2, (1 << 20) + 1, 1 << 21, p, p, 8, p, f32, p, f32, None, 0, None) == no
-    need = lib.nori_checkpoint_grad_workspace_bytes(f16, 100000, 64, 64)
-    assert need > 0 and lib.nori_checkpoint_grad_workspace_bytes(f16, 100, 64, 64) == 0
+    need = lib.nori_checkpoint_grad_workspace_bytes(f16, f32, 100000, 64, 64)
+    assert need > 0 and lib.nori_checkpoint_grad_workspace_bytes(f16, f32, 100, 64, 64) == 0
     assert g(p, f16, 100000, 64, 64, p, p, 64, p, f32, p, f32, p, need - 1, None) == bad
     assert g(p, f16, 100000, 64, 64, p, p, 64, p, f32, p, f32, p + 8, need, None) == bad
     assert g(p, f16, 2, 8, 8, p, p, 8, None, f32, None, f32, None, 0, None) == ok

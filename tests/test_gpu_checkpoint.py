@@ -95,9 +95,10 @@ def test_linear(cuda, rows, k, n, wide, dtype):
     w16, _, xh = w.to(dtype).double(), None, kept(x)[2]
     near("dx", dx, dy.double() @ w16, (n * U + h) * (dy.double().abs() @ w16.abs()) + least(dtype))
     a = dy.double().t().abs() @ xh.abs()
-    # kept values below the type's normal range are rounded to its subnormal step
-    rounding = 0.0 if dtype == torch.float32 else h
-    sub = dy.double().abs().sum(0)[:, None] * least(dtype)
+    # kept values are rounded to the rows' type, below its normal range to its subnormal step, or held to 2^-17 for an fp32 gradient
+    fine = wt == torch.float32 and dtype != torch.float32
+    rounding = 2.0**-17 if fine else (0.0 if dtype == torch.float32 else h)
+    sub = 0.0 if fine else dy.double().abs().sum(0)[:, None] * least(dtype)
     near("dw", dw, dy.double().t() @ xh, (rows * U + rounding + half(wt)) * a + sub + least(wt))
     near("db", db, dy.double().sum(0), (rows * U + half(wt)) * dy.double().abs().sum(0) + least(wt))
 
