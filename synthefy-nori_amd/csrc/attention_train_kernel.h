@@ -623,9 +623,10 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Ar
             });
         }
         at_query += kRows;
-        while (at_query >= nq) {
-            at_query -= nq;
-            ++at_head;
+        if (p.group > 1) {
+            const int heads = at_query / nq;
+            at_head += heads;
+            at_query -= heads * nq;
         }
         if (threadIdx.x < kRows) {
             const bool in = (int)threadIdx.x < left;

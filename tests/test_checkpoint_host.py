@@ -58,7 +58,6 @@ def test_the_library_refuses():
     assert q(p, nat.NORI_I8, 2, 8, 8, p, p, None) == no
     assert q(p, nat.NORI_F16, -1, 8, 8, p, p, None) == bad
     assert q(p, nat.NORI_F16, 2, 0, 8, p, p, None) == bad
-    assert q(p, nat.NORI_F16, 2, 8, 7, p, p, None) == bad
     assert q(p, nat.NORI_F16, 2, 8, -8, p, p, None) == bad
     assert q(p, nat.NORI_F16, 1 << 40, 8, 8, p, p, None) == no
     assert q(p, nat.NORI_F16, 1 << 33, 8, 8, p, p, None) == no  # more workgroups than one launch has
@@ -66,12 +65,12 @@ def test_the_library_refuses():
     assert q(p, nat.NORI_F16, 2, 8, 8, p + 8, p, None) == bad
     assert q(None, nat.NORI_F16, 0, 8, 8, None, None, None) == ok
     s = lib.nori_checkpoint_silu_mul
-    assert s(p, nat.NORI_F16, 2, 8, 15, p, p, p, None) == bad
+    assert s(p, nat.NORI_F16, 2, 8, -16, p, p, p, None) == bad
     assert s(p, nat.NORI_F16, 2, 8, 16, p, p, None, None) == bad
     assert s(p, nat.NORI_F16, 2, 8, 16, None, p, p, None) == bad
     assert s(p, nat.NORI_I8, 2, 8, 16, p, p, p, None) == no
     t = lib.nori_checkpoint_silu_mul_backward
-    assert t(p, p, nat.NORI_F16, 2, 8, p, 7, p, None) == bad
+    assert t(p, p, nat.NORI_F16, 2, 8, p, -8, p, None) == bad
     assert t(p, None, nat.NORI_F16, 2, 8, p, 8, p, None) == bad
     assert t(None, None, nat.NORI_F16, 0, 8, None, 8, None, None) == ok
     g = lib.nori_checkpoint_grad
@@ -80,7 +79,8 @@ def test_the_library_refuses():
     assert g(p, f16, 2, 8, 8, p, p, 8, p, nat.NORI_BF16, p, f32, None, 0, None) == no
     assert g(p, f32, 2, 8, 8, p, p, 8, p, f16, p, f32, None, 0, None) == no
     assert g(p, f16, 2, 0, 8, p, p, 8, p, f32, p, f32, None, 0, None) == bad
-    assert g(p, f16, 2, 8, 7, p, p, 8, p, f32, p, f32, None, 0, None) == bad
+    assert g(p, f16, 2, 8, -8, p, p, 8, p, f32, p, f32, None, 0, None) == bad
+    assert g(p, f16, 2, 8, (1 << 24) + 1, p, p, 8, p, f32, p, f32, None, 0, None) == no
     assert g(p, f16, 2, 8, 8, None, p, 8, p, f32, p, f32, None, 0, None) == bad
     assert g(p, f16, 2, (1 << 20) + 1, 1 << 21, p, p, 8, p, f32, p, f32, None, 0, None) == no
     need = lib.nori_checkpoint_grad_workspace_bytes(f16, f32, 100000, 64, 64)

@@ -220,3 +220,53 @@ def test_other_stream_and_captured(cuda):
         torch.cuda.synchronize()
         got = [t.clone() for t in kept]
         assert all(torch.equal(a, b) for a, b in zip(got, eager()))
+
+
+def test_rows_whose_offsets_pass_32_bits(cuda):
+    """A context whose rows lie 2^16 elements apart, 70,000 of them: the contiguous call's bits."""
+    g = torch.Generator().manual_seed(13)
+    far = torch.empty(70000 * 65536, dtype=torch.float16, device="cuda").as_strided((1, 70000, 2, 1, 16), (70000 * 65536, 65536, 16, 16, 1))
+    kv = torch.randn(1, 70000, 2, 1, 16, generator=g).half()
+    far.copy_(kv)
+    q, dout = torch.randn(1, 3, 2, 16, generator=g).half(), torch.randn(1, 3, 2, 16, generator=g).half()
+
+    def grads(t):
+        a, b = q.cuda().requires_grad_(True), t.detach().requires_grad_(True)
+        out = nori_amd.trainable_attention(a, b)
+        return (out, *torch.autograd.grad(out, (a, b), dout.cuda()))
+
+    assert all(torch.equal(x, y) for x, y in zip(grads(far), grads(kv.cuda())))
+
+
+def test_few_keys_keep_small_differences(cuda):
+    """Two keys: ds is a difference of nearly equal products, which delta of a rounded result would swamp."""
+    for dtype in (torch.float16, torch.bfloat16):
+        for nq in (5, 300):  # both backward passes
+            q, kv, dout = inputs(8, nq, 2, 2, 2, 64, dtype, seed=14)
+            kv[:, 1] = kv[:, 0]
+            kv[:, 1, 1, :, ::7] += 0.5
+            kv[:, 0, 1] += 4
+            kv[:, 1, 1] += 4
+            out, dq, dkv = run(q, kv, None, dout)
+            expected, _ = reference(q, kv, None, dout)
+            # p is 1/2 and ds exact but for its own rounding, p's, and the fp32 sums beside products of up to 64 x 4.5 x 0.5:
+            # 2^-23 x 144 x 64 at most of terms that are 0.05 in the mean
+            h = torch.finfo(dtype).eps / 2
+            assert (dkv[:, :, 0].double().cpu() - expected[3][:, :, 0]).norm() <= 4 * h * expected[3][:, :, 0].norm()
+
+
+def test_shared_and_broadcast_contexts(cuda):
+    """One context expanded over the batch: its gradient is the sum over the batch."""
+    q, kv, dout = (t.cuda() for t in inputs(3, 40, 50, 4, 2, 24, torch.float32, seed=15))
+    one = kv[:1].clone().requires_grad_(True)
+    d = torch.autograd.grad(nori_amd.trainable_attention(q, one.expand(3, -1, -1, -1, -1)), one, dout)[0]
+    whole = kv[:1].repeat(3, 1, 1, 1, 1).requires_grad_(True)
+    each = torch.autograd.grad(nori_amd.trainable_attention(q, whole), whole, dout)[0]
+    assert torch.equal(d, each.sum(0, keepdim=True))
+
+
+def test_second_derivatives_are_refused(cuda):
+    q, kv, _ = (t.cuda().requires_grad_(True) for t in inputs(1, 3, 4, 1, 1, 8, torch.float32))
+    dq = torch.autograd.grad(nori_amd.trainable_attention(q, kv).square().sum(), q, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.sum(), kv)

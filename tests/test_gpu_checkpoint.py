@@ -225,3 +225,33 @@ def test_the_same_bits_again_and_captured(cuda):
         torch.cuda.synchronize()
         got = [t.clone() for t in held]
         assert all(torch.equal(a, b) for a, b in zip(got, eager()))
+
+
+def test_overlapping_and_distant_rows(cuda):
+    """Windows that share elements, and rows whose offsets pass 2^32 elements: what contiguous copies of them give."""
+    g = torch.Generator().manual_seed(6)
+    line = torch.randn(4000, generator=g).half().cuda()
+    windows = line.unfold(0, 40, 9)[:400]
+    w = torch.randn(24, 40, generator=g).half().cuda().requires_grad_(True)
+    slopes = line.unfold(0, 24, 9)[:400]
+
+    def grads(x, dy):
+        return torch.autograd.grad(nori_amd.checkpointed_linear(x, w), w, dy)[0]
+
+    assert torch.equal(grads(windows, slopes), grads(windows.contiguous(), slopes.contiguous()))
+    far = torch.empty(70000 * 65536, dtype=torch.float16, device="cuda").view(70000, 65536)[:, :40]
+    x = torch.randn(70000, 40, generator=g).half().cuda()
+    far.copy_(x)
+    dy = torch.randn(70000, 24, generator=g).half().cuda()
+    assert torch.equal(grads(far, dy), grads(x, dy))
+
+
+def test_second_derivatives_are_refused(cuda):
+    x, w = torch.randn(5, 8, device="cuda", requires_grad=True), torch.randn(3, 8, device="cuda", requires_grad=True)
+    dx = torch.autograd.grad(nori_amd.checkpointed_linear(x, w).square().sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), w)
+    gu = torch.randn(5, 8, device="cuda", requires_grad=True)
+    d = torch.autograd.grad(nori_amd.checkpointed_silu_mul(gu, 4).square().sum(), gu, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(d.sum(), gu)
