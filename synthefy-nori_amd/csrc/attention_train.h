@@ -22,6 +22,8 @@ namespace nori {
 namespace attn_train {
 
 constexpr int kFewWidth = 64;  // head widths to which workgroups of one and two wavefronts are built
+// Whether both sides of a unit of 32 `waves` rows and keys fit a workgroup's LDS.
+constexpr bool few_fits(bool f32, int d, int waves) { return waves <= 2 && d <= kFewWidth && (!f32 || waves == 1 || d <= 32); }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Args {

@@ -106,11 +106,11 @@ Args plan(const nori_attention_train_args& a, Kind kind) {
     return p;
 }
 
-// Units that one workgroup takes through the whole backward pass.
+// Wavefronts for a unit's rows and for its keys, where one workgroup takes it through a whole pass.
+int few_waves(const nori_attention_train_args& a) { return (int)((std::max(a.nk, a.nq * (a.heads / a.kv_heads)) + 31) / 32); }
 bool few(const nori_attention_train_args& a, bool backward) {
-    return a.dtype != NORI_F32 && a.d <= kFewWidth && a.nk <= 64 && a.nq * (a.heads / a.kv_heads) <= 64 && (!backward || (a.dq && a.dkv));
+    return a.nk <= 64 && a.nq * (a.heads / a.kv_heads) <= 64 && few_fits(a.dtype == NORI_F32, a.d, few_waves(a)) && (!backward || (a.dq && a.dkv));
 }
-
 
 int64_t part_bytes(const Args& p, Kind kind) { return p.splits > 1 ? p.splits * part_rows(p, kind) * p.a.d * 4 : 0; }
 int64_t aligned16(int64_t n) { return (n + 15) / 16 * 16; }
@@ -124,9 +124,8 @@ int launch_typed(Kind kind, const Args& p, hipStream_t stream) {
     }
 }
 
-// One workgroup a unit, of wavefronts for its rows and for its keys.
 int launch_few(Kind kind, Args p, hipStream_t stream) {
-    p.waves = p.a.nk > 32 || p.rows > 32 ? 2 : 1;
+    p.waves = std::max(1, few_waves(p.a));
     p.tiles = p.splits = 1;
     return launch_typed(kind, p, stream);
 }

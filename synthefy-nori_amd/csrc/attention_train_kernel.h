@@ -646,20 +646,30 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Ar
         if (first + kRows < end) load(first + kRows);
 dkv_step<DT, DK, kRows / 32>(qs, dos, off, deltas, end - first, kf, vf, dk, dv, scale, p.c, lane);
     }
-    if (key64 >= a.nk) return;
     if (!there) {  // past the length
 #pragma unroll
         for (int j = 0; j < G::MS; ++j) dk[j] = dv[j] = f32x16{};
     }
     const float byk = a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f);
     if (p.splits > 1) {
+        if (key64 >= a.nk) return;
         float* part = p.part + ((w.split * a.bg * a.kv_heads + w.unit) * a.nk + key) * 2 * a.d;
         store_row<DT>(part, dk, byk, a.d, half);
         store_row<DT>(part + a.d, dv, kUnbias<DT>, a.d, half);
-    } else {
-        T* out = reinterpret_cast<T*>(a.dkv) + (((w.b * a.nk + key) * 2) * a.kv_heads + w.hk) * a.d;
-        store_row<DT>(out, dk, byk, a.d, half);
-        store_row<DT>(out + (int64_t)a.kv_heads * a.d, dv, kUnbias<DT>, a.d, half);
+        return;
+    }
+    // the tiles hold 32 rows for each of two wavefronts (one in float32) at a time
+    constexpr int kAtOnce = kRows / 32;
+    const int64_t from = w.tile * 32 * NW + wave * 32;
+    T* to = reinterpret_cast<T*>(a.dkv) + ((w.b * a.nk + from) * 2 * a.kv_heads + w.hk) * a.d;
+    const int left = (int)min((int64_t)32, a.nk - from);
+#pragma unroll
+    for (int turn = 0; turn < NW / kAtOnce; ++turn) {
+        __syncthreads();
+        if (wave / kAtOnce != turn) continue;
+        const int mine = wave % kAtOnce * 32 * G::LS;
+        store_rows<DT, DK, W, G::LS>(qs + mine, dk, byk, a.d, lane, left, [&](int i) { return to + (int64_t)i * 2 * a.kv_heads * a.d; });
+        store_rows<DT, DK, W, G::LS>(dos + mine, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
     }
 }
 
@@ -735,46 +745,49 @@ __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) 
         y = dout + h * a.do_head + i * a.do_row;
     });
     const bool there = own < rows;
-    const Row row = there ? row_of(p, hk, own) : Row{hk * p.group, 0};
-    const int64_t out_row = ((b * a.nq + row.query) * a.heads + row.head) * a.d;
     typename E::Frag x[G::KS], y[G::KS];
     const float lse2 = there ? a.lse[unit * p.rows + own] * kLog2e : 0.f;
     keys.store(ks, vs);
     queries.store(qs, dos);
     __syncthreads();
-    {
-        f32x16 dq[G::MS] = {};
-        Scale scale;
-        float delta = 0.f;
+    f32x16 dq[G::MS] = {};
+    Scale qscale;
+    float delta = 0.f;
 #pragma unroll
-        for (int k = 0; k < G::KS; ++k) {
-            x[k] = direct<DT, DK>(qs, own, k, half);
-            y[k] = direct<DT, DK>(dos, own, k, half);
-        }
-        if (length > 0) dq_whole<DT, DK, NW>(ks, vs, length, x, y, dq, scale, p.c, lse2, delta, lane);
-        if (half == 0) {
-            off[own] = there ? E::kBias - lse2 : 0.f;
-            deltas[own] = there ? -delta : 0.f;
-        }
-        if (there) store_row<DT>(reinterpret_cast<T*>(a.dq) + out_row, dq, a.scale * (E::kScaled ? scale.inverse() : 1.f), a.d, half);
+    for (int k = 0; k < G::KS; ++k) {
+        x[k] = direct<DT, DK>(qs, own, k, half);
+        y[k] = direct<DT, DK>(dos, own, k, half);
+    }
+    if (length > 0) dq_whole<DT, DK, NW>(ks, vs, length, x, y, dq, qscale, p.c, lse2, delta, lane);
+    if (half == 0) {
+        off[own] = there ? E::kBias - lse2 : 0.f;
+        deltas[own] = there ? -delta : 0.f;
     }
     __syncthreads();
-    f32x16 dk[G::MS] = {}, dv[G::MS] = {};
-    Scale scale;
+    // from here on a wavefront's 32 rows of ks and vs are its own
 #pragma unroll
     for (int k = 0; k < G::KS; ++k) {
         x[k] = direct<DT, DK>(ks, own, k, half);
         y[k] = direct<DT, DK>(vs, own, k, half);
     }
+    T *lk = ks + wave * 32 * G::LS, *lv = vs + wave * 32 * G::LS;
+    T* to_q = reinterpret_cast<T*>(a.dq) + b * a.nq * a.heads * a.d;
+    store_rows<DT, DK, W, G::LS>(lk, dq, a.scale * (E::kScaled ? qscale.inverse() : 1.f), a.d, lane, rows - wave * 32, [&](int i) {
+        const Row to = row_of(p, hk, wave * 32 + i);
+        return to_q + (to.query * a.heads + to.head) * a.d;
+    });
+    f32x16 dk[G::MS] = {}, dv[G::MS] = {};
+    Scale scale;
     if (length > 0 && rows > 0) dkv_step<DT, DK, NW>(qs, dos, off, deltas, rows, x, y, dk, dv, scale, p.c, lane);
-    if (own >= a.nk) return;
     if (own >= length) {
 #pragma unroll
         for (int j = 0; j < G::MS; ++j) dk[j] = dv[j] = f32x16{};
     }
-    T* out = reinterpret_cast<T*>(a.dkv) + (((b * a.nk + own) * 2) * a.kv_heads + hk) * a.d;
-    store_row<DT>(out, dk, a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f), a.d, half);
-    store_row<DT>(out + (int64_t)a.kv_heads * a.d, dv, kUnbias<DT>, a.d, half);
+    T* to_k = reinterpret_cast<T*>(a.dkv) + ((b * a.nk + wave * 32) * 2 * a.kv_heads + hk) * a.d;
+    const int left = (int)a.nk - wave * 32;
+    store_rows<DT, DK, W, G::LS>(lk, dk, a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f), a.d, lane, left,
+                                 [&](int i) { return to_k + (int64_t)i * 2 * a.kv_heads * a.d; });
+    store_rows<DT, DK, W, G::LS>(lv, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to_k + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
 }
 
 // ---------------------------------------------------------------- launches
@@ -784,7 +797,7 @@ void launch_one(Kind kind, const Args& p, dim3 grid, hipStream_t stream) {
     if (kind == kForward) hipLaunchKernelGGL((forward_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
     else if (kind == kDq) hipLaunchKernelGGL((dq_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
     else if (kind == kDkv) hipLaunchKernelGGL((dkv_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
-    else if constexpr (DT != NORI_F32 && DK <= kFewWidth && NW <= 2) {
+    else if constexpr (few_fits(DT == NORI_F32, DK, NW)) {
         if (kind == kFewForward) hipLaunchKernelGGL((forward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
         else hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
     }
