@@ -38,7 +38,10 @@ __device__ __forceinline__ Raw8<DT> load8(const void* p, int64_t row, int c, int
     if (n & 2) {
         const auto x = fetch<DT, 2>(p, row + c + (n & 4));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) (n & 4 ? r.e[4 + i] : r.e[i]) = x.e[i];
+        for (int i = 0; i < 2; ++i) {
+            r.e[i] = n & 4 ? +r.e[i] : +x.e[i];
+            if (n & 4) r.e[4 + i] = x.e[i];
+        }
     }
     if (n & 1) {
         const auto x = fetch<DT, 1>(p, row + c + (n & 6)).e[0];
@@ -54,12 +57,13 @@ __device__ __forceinline__ void store8(void* p, int64_t row, int c, int cols, co
     const int n = cols - c;
     if (n <= 0) return;
     if (n >= kEach) return store<DT, kEach>(p, row + c, v);
-    if (n & 4) store<DT, 4>(p, row + c, {v[0], v[1], v[2], v[3]});
-    if (n & 2) {
-        if (n & 4) store<DT, 2>(p, row + c + 4, {v[4], v[5]});
-        else store<DT, 2>(p, row + c, {v[0], v[1]});
-    }
-    if (n & 1) store_elem<DT>(p, row + c + (n & 6), n & 4 ? (n & 2 ? v[6] : v[4]) : (n & 2 ? v[2] : v[0]));
+    // (taken out before the choices: a choice between places would put v into memory)
+    const float v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3], v4 = v[4], v5 = v[5], v6 = v[6];
+    if (n & 4) store<DT, 4>(p, row + c, {v0, v1, v2, v3});
+    const float pair[2] = {n & 4 ? v4 : v0, n & 4 ? v5 : v1};
+    if (n & 2) store<DT, 2>(p, row + c + (n & 4), pair);
+    const float low = n & 2 ? v2 : v0, high = n & 2 ? v6 : v4;
+    if (n & 1) store_elem<DT>(p, row + c + (n & 6), n & 4 ? high : low);
 }
 
 // The largest magnitude of 8 elements as a whole number, NaN on top: of their own bits, two at a time in the 16-bit types.
@@ -100,24 +104,26 @@ __device__ __forceinline__ float quantize8(const Raw8<DT>& r, const float (&v)[k
     const float s = amax <= 3.402823466e38f ? amax / 127.0f : NAN;  // an infinity or NaN: NaN throughout
     const bool normal = s >= 0x1p-126f;
     const float y = normal ? 1.0f / s : 0.0f;
-    float k[kEach], most = 0.f;
+    float k[kEach], rest[kEach], most = 0.f;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         k[i] = fmaf(v[i], y, kOnes);
-        most = fmaxf(most, fabsf(fmaf(kOnes - k[i], s, v[i])));
+        rest[i] = fmaf(kOnes - k[i], s, v[i]);
+        most = fmaxf(most, fabsf(rest[i]));
     }
-    if (__any(normal ? 2.0f * most >= s : s > 0.0f)) {
+    const float half = 0.5f * s;
+    if (__any(normal && most >= half)) {  // (bfloat16's halves are not rare: amax / 2 is one)
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            float c = k[i] - kOnes;
-            if (normal) {
-                const float rest = fmaf(-c, s, v[i]), twice = 2.0f * fabsf(rest);
-                if (twice > s || (twice == s && ((int)c & 1))) c += copysignf(1.0f, rest);
-            } else if (s > 0.0f) {
-                c = fminf(fmaxf(rintf(v[i] / s), -127.0f), 127.0f);  // a scale of few bits: quotients up to 190
-            }
-            k[i] = c + kOnes;
+            const float far = fabsf(rest[i]);
+            const bool up = far > half || (far == half && (__float_as_uint(k[i]) & 1u));
+            k[i] += up ? copysignf(1.0f, rest[i]) : 0.0f;
         }
+    }
+    if (__any(s > 0.0f && !normal)) {  // a scale of few bits: quotients up to 190
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (s > 0.0f && !normal) k[i] = fminf(fmaxf(rintf(v[i] / s), -127.0f), 127.0f) + kOnes;
     }
     uint32_t w[2];
 #pragma unroll
