@@ -84,12 +84,18 @@ __device__ __forceinline__ void store_row(Out* out, const f32x16 (&x)[MS], float
 }
 
 // The same for the 32 rows of a wavefront's columns by way of LDS (its own 32 rows there): a lane's columns are apart in memory, 32
-// lines an access, which the address units bound short scans by; from LDS rows go out side by side. to(row): where it begins.
-template <int DT, int DK, int W, int LS, int MS, class To>
+// lines an access, which the address units bound short scans by; from LDS rows go out side by side. to(row): where it begins. DIRECT:
+// without LDS, for the backward passes in 8-byte chunks, which gain nothing by it (8,192 x 8 units of 33 x 33 of 44, fp16: forward
+// 250 us direct, 196 so, backward 527 and 553; x 10 of 51 x 51 of 56 in 16-byte chunks: backward 951 and 859).
+template <int DT, int DK, int W, int LS, bool DIRECT, int MS, class To>
 __device__ __forceinline__ void store_rows(typename El<DT>::T* lds, const f32x16 (&x)[MS], float by, int d, int lane, int rows, To to) {
     using T = typename El<DT>::T;
     typedef uint32_t Chunk __attribute__((ext_vector_type(W * sizeof(T) / 4)));
     constexpr int CH = DK / W;
+    if constexpr (DIRECT) {
+        if ((lane & 31) < rows) store_row<DT>(to(lane & 31), x, by, d, lane >> 5);
+        return;
+    }
     store_row<DT>(lds + (lane & 31) * LS, x, by, d, lane >> 5);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -668,8 +674,8 @@ dkv_step<DT, DK, kRows / 32>(qs, dos, off, deltas, end - first, kf, vf, dk, dv, 
         __syncthreads();
         if (wave / kAtOnce != turn) continue;
         const int mine = wave % kAtOnce * 32 * G::LS;
-        store_rows<DT, DK, W, G::LS>(qs + mine, dk, byk, a.d, lane, left, [&](int i) { return to + (int64_t)i * 2 * a.kv_heads * a.d; });
-        store_rows<DT, DK, W, G::LS>(dos + mine, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
+        store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(qs + mine, dk, byk, a.d, lane, left, [&](int i) { return to + (int64_t)i * 2 * a.kv_heads * a.d; });
+        store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(dos + mine, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
     }
 }
 
@@ -707,7 +713,7 @@ __global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
     if (there && half == 0 && a.lse) a.lse[unit * p.rows + own] = length > 0 ? (__builtin_amdgcn_logf(l) - E::kTop + m * c) * kLn2 : -INFINITY;
     T* out = reinterpret_cast<T*>(a.out) + b * a.nq * a.heads * a.d;
     __syncthreads();  // the tile is everyone's until here
-    store_rows<DT, DK, W, G::LS>(ks + wave * 32 * G::LS, o, length > 0 ? 1.f / l : 0.f, a.d, lane, rows - wave * 32, [&](int i) {
+    store_rows<DT, DK, W, G::LS, false>(ks + wave * 32 * G::LS, o, length > 0 ? 1.f / l : 0.f, a.d, lane, rows - wave * 32, [&](int i) {
         const Row to = row_of(p, hk, wave * 32 + i);
         return out + (to.query * a.heads + to.head) * a.d;
     });
@@ -772,7 +778,7 @@ __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) 
     }
     T *lk = ks + wave * 32 * G::LS, *lv = vs + wave * 32 * G::LS;
     T* to_q = reinterpret_cast<T*>(a.dq) + b * a.nq * a.heads * a.d;
-    store_rows<DT, DK, W, G::LS>(lk, dq, a.scale * (E::kScaled ? qscale.inverse() : 1.f), a.d, lane, rows - wave * 32, [&](int i) {
+    store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(lk, dq, a.scale * (E::kScaled ? qscale.inverse() : 1.f), a.d, lane, rows - wave * 32, [&](int i) {
         const Row to = row_of(p, hk, wave * 32 + i);
         return to_q + (to.query * a.heads + to.head) * a.d;
     });
@@ -785,9 +791,9 @@ __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) 
     }
     T* to_k = reinterpret_cast<T*>(a.dkv) + ((b * a.nk + wave * 32) * 2 * a.kv_heads + hk) * a.d;
     const int left = (int)a.nk - wave * 32;
-    store_rows<DT, DK, W, G::LS>(lk, dk, a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f), a.d, lane, left,
+    store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(lk, dk, a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f), a.d, lane, left,
                                  [&](int i) { return to_k + (int64_t)i * 2 * a.kv_heads * a.d; });
-    store_rows<DT, DK, W, G::LS>(lv, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to_k + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
+    store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(lv, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to_k + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
 }
 
 // ---------------------------------------------------------------- launches
