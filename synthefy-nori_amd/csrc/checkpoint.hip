@@ -101,7 +101,7 @@ __device__ __forceinline__ float quantize8(const Raw8<DT>& r, const float (&v)[k
     constexpr float kOnes = 12582912.0f;  // 3 * 2^22
     const uint32_t key = max16(magnitude<DT>(r));
     const float amax = DT == NORI_F32 ? __uint_as_float(key) : (DT == NORI_F16 ? f16_to_f32((uint16_t)key) : bf16_to_f32((uint16_t)key));
-    const float s = amax <= 3.402823466e38f ? amax / 127.0f : NAN;  // an infinity or NaN: NaN throughout
+    const float s = amax <= 3.402823466e38f ? amax * (1.0f / 127.0f) : NAN;  // an infinity or NaN: NaN throughout
     const bool normal = s >= 0x1p-126f;
     const float y = normal ? 1.0f / s : 0.0f;
     float k[kEach], rest[kEach], most = 0.f;

@@ -50,26 +50,33 @@ __device__ __forceinline__ Eight<DT> values(uint32_t lo, uint32_t hi, float s) {
     }
 }
 
-// dy s in two bfloat16 pieces, to 2^-17 of itself, beside codes that are whole numbers: what an fp32 gradient of 16-bit rows takes. x
+// dy s in two float16 pieces, to 2^-22 of itself, beside codes that are whole numbers: what an fp32 gradient of 16-bit rows takes. x
 // rounded to the rows' type would leave 2^-12 (float16) or 2^-9 of every term, above what the gradient's type can tell.
 template <int DT>
-__device__ __forceinline__ void pieces(const Eight<DT>& y, float s, Eight<NORI_BF16>& hi, Eight<NORI_BF16>& lo) {
-    bf16x8 h, l;
+__device__ __forceinline__ float wide(const Eight<DT>& y, int e) {
+    if constexpr (DT == NORI_F32) return y.e[e];
+    else return DT == NORI_F16 ? f16_to_f32(y.e[e]) : bf16_to_f32(y.e[e]);
+}
+template <int DT>
+__device__ __forceinline__ void pieces(const Eight<DT>& y, float s, Eight<NORI_F16>& hi, Eight<NORI_F16>& lo) {
+    f16x8 h, l;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float v = (DT == NORI_F16 ? f16_to_f32(y.e[e]) : bf16_to_f32(y.e[e])) * s;
-        h[e] = (__bf16)v;
+        float v = wide<DT>(y, e) * s;
+        // one value for both pieces: a product folded into one of its roundings to float16, and not into the other, rounds otherwise
+        asm("" : "+v"(v));
+        h[e] = (_Float16)v;
         const float w = (float)h[e];
-        l[e] = (__bf16)(fabsf(w) == INFINITY ? 0.f : v - w);
+        l[e] = (_Float16)(fabsf(w) == INFINITY ? 0.f : v - w);
     }
-    hi = __builtin_bit_cast(Eight<NORI_BF16>, h);
-    lo = __builtin_bit_cast(Eight<NORI_BF16>, l);
+    hi = __builtin_bit_cast(Eight<NORI_F16>, h);
+    lo = __builtin_bit_cast(Eight<NORI_F16>, l);
 }
 
 // TN columns of dy by 128 of x a workgroup, half of each a wavefront. FINE: dw in fp32 of 16-bit rows, two products a pair.
 template <int DT, int TN, bool FINE>
 __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
-    constexpr int MT = FINE ? NORI_BF16 : DT;  // the products' type
+    constexpr int MT = FINE ? NORI_F16 : DT;  // the products' type
     using E = El<MT>;
     using T = typename El<DT>::T;
     constexpr int kRows = DT == NORI_F32 ? 32 : 64;  // rows a step
@@ -115,9 +122,17 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
             for (int j = 0; j < NY; ++j) ysc[j] = ps[j * kYStep * a.groups + yrow * a.groups];
         }
     };
+    // of a row at the end of the rows or of the columns
+    const auto partial = [&](int64_t r) {
+        Eight<DT> y = {};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (r < end && yc + e < a.n) y.e[e] = reinterpret_cast<const T*>(a.dy)[r * a.dy_stride + yc + e];
+        return y;
+    };
     const auto put_y = [&](int j, const Eight<DT>& y, float s) {
         const int at = (yrow + j * kYStep) * YS + ycol;
-        if constexpr (FINE) pieces<DT>(y, s, *reinterpret_cast<Eight<NORI_BF16>*>(&ys[at]), *reinterpret_cast<Eight<NORI_BF16>*>(&ls[at]));
+        if constexpr (FINE) pieces<DT>(y, s, *reinterpret_cast<Eight<NORI_F16>*>(&ys[at]), *reinterpret_cast<Eight<NORI_F16>*>(&ls[at]));
         else *reinterpret_cast<Eight<DT>*>(&ys[at]) = y;
     };
     const auto put_x = [&](int j, uint4 x, float s) {
@@ -128,19 +143,58 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
     float colsum[8] = {};
     const auto add = [&](const Eight<DT>& y) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if constexpr (DT == NORI_F32) colsum[e] += y.e[e];
-            else colsum[e] += DT == NORI_F16 ? f16_to_f32(y.e[e]) : bf16_to_f32(y.e[e]);
-        }
+        for (int e = 0; e < 8; ++e) colsum[e] += wide<DT>(y, e);
     };
     f32x16 acc[MY][MX] = {};
+    // FINE: a power of two on dy s, which float16 has no range for. It brings the first step's largest to 2^8 and falls where a later
+    // one would pass 2^15; the sums are brought along.
+    __shared__ float tops[kThreads / 64];
+    float power = 0.f, top = 0.f;
+    const int live = yc < a.n ? min(8, a.n - yc) : 8;  // past the row's end anything may lie
+    const auto look = [&](const Eight<DT>& y, float s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = fabsf(wide<DT>(y, e)) * s;
+            top = fmaxf(top, e < live && v < INFINITY ? v : 0.f);
+        }
+    };
+    const auto share = [&] {
+        for (int i = 32; i > 0; i /= 2) top = fmaxf(top, __shfl_xor(top, i));
+        if (lane == 0) tops[wave] = top;
+    };
+    const auto agree = [&] {
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        if (power == 0.f ? top > 0.f : top * power > 32768.f) {
+            int e = 8 + 127 - (int)(__float_as_uint(top) >> 23);
+            e = e > 120 ? 120 : (e < -120 ? -120 : e);
+            const float next = __uint_as_float((uint32_t)(e + 127) << 23), by = power == 0.f ? 1.f : next / power;
+#pragma unroll
+            for (int i = 0; i < 16 * MY * MX; ++i) acc[i / 16 / MX][i / 16 % MX][i % 16] *= by;
+            power = next;
+        }
+        top = 0.f;
+    };
     int turn = a.db ? (a.splits > 1 ? kt : (kt == 0 ? 0 : -1)) : -1;  // steps until this k tile's next one of db
     if (whole(begin)) load(begin);
     for (int64_t from = begin; from < end; from += kRows) {
+        if constexpr (FINE) {
+            if (whole(from)) {
+#pragma unroll
+                for (int j = 0; j < NY; ++j) look(ye[j], ysc[j]);
+            } else if (a.dw) {
+#pragma unroll 1
+                for (int j = 0; j < NY; ++j) {
+                    const int64_t r = from + yrow + j * kYStep;
+                    look(partial(r), r < end ? a.scales[r * a.groups + kt] : 0.f);
+                }
+            }
+            share();
+        }
         __syncthreads();
+        if constexpr (FINE) agree();
         if (whole(from)) {
 #pragma unroll
-            for (int j = 0; j < NY; ++j) put_y(j, ye[j], FINE ? ysc[FINE ? j : 0] : 1.f);
+            for (int j = 0; j < NY; ++j) put_y(j, ye[j], FINE ? ysc[FINE ? j : 0] * power : 1.f);
 #pragma unroll
             for (int j = 0; j < NX; ++j) put_x(j, xe[j], FINE ? 1.f : xsc[FINE ? 0 : j]);
             if (turn == 0) {
@@ -151,11 +205,8 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
 #pragma unroll 1
             for (int j = 0; j < NY; ++j) {
                 const int64_t r = from + yrow + j * kYStep;
-                Eight<DT> y = {};
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (r < end && yc + e < a.n) y.e[e] = reinterpret_cast<const T*>(a.dy)[r * a.dy_stride + yc + e];
-                put_y(j, y, FINE && a.dw && r < end ? a.scales[r * a.groups + kt] : 1.f);
+                const Eight<DT> y = partial(r);
+                put_y(j, y, FINE && a.dw && r < end ? a.scales[r * a.groups + kt] * power : 1.f);
                 if (turn == 0) add(y);
             }
 #pragma unroll 1
@@ -212,6 +263,7 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
         }
     }
     if (!a.dw) return;
+    const float by = FINE && power != 0.f ? 1.f / power : 1.f;
 #pragma unroll
     for (int j = 0; j < MY; ++j)
 #pragma unroll
@@ -222,8 +274,8 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
                 const int c = kt * kGroup + wk + 32 * l + (lane & 31);
                 if (row >= a.n || c >= a.k) continue;
                 const int64_t at = (int64_t)row * a.k + c;
-                if (a.splits > 1) a.part_w[(int64_t)split * a.n * a.k + at] = acc[j][l][e];
-                else put<DT>(a.dw, a.dw_dtype, at, acc[j][l][e]);
+                if (a.splits > 1) a.part_w[(int64_t)split * a.n * a.k + at] = acc[j][l][e] * by;
+                else put<DT>(a.dw, a.dw_dtype, at, acc[j][l][e] * by);
             }
 }
 

@@ -96,7 +96,7 @@ def checkpointed_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     keep their own dtype). in and out up to 2^20. Where autocast is on x, and 16-bit weights, are cast to its dtype.
 
     The result and the gradients of x and bias are ``F.linear``'s. The weight's is dy^T x with x the values that the codes stand
-    for (``code * scale``, scale = fp32(amax / 127) of 128 columns of a row, nearest codes, ties to even), rounded to x's dtype
+    for (``code * scale``, scale = amax times fp32(1/127) of 128 columns of a row, nearest codes, ties to even), rounded to x's dtype
     for the product; a group of columns that holds an infinity or NaN stands for NaN. First derivatives, in reverse mode; sums
     have a fixed order, so the same inputs give the same bits. Without a gradient of the weight nothing is kept of x."""
     if weight.dim() != 2 or min(weight.shape) == 0:

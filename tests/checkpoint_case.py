@@ -6,7 +6,7 @@ GROUP = 128
 
 
 def kept(x):
-    """(codes, scales, the values in float64) of x [rows, cols] on the CPU: fp32(amax / 127) of each 128 columns, nearest codes with
+    """(codes, scales, the values in float64) of x [rows, cols] on the CPU: amax fp32(1/127), rounded, of each 128 columns, nearest codes with
     ties to even. The quotient of two fp32 values in 64 bits is exact enough to tell a half from its neighbours: one that
     is not a half is at least 2^-25 of itself away from it."""
     x = x.detach().double().cpu()
@@ -16,7 +16,7 @@ def kept(x):
     wide[:, :cols] = x
     wide = wide.view(rows, groups, GROUP)
     amax = wide.abs().amax(-1, keepdim=True)
-    scales = (amax / 127).float().double()
+    scales = (amax.float() * torch.tensor(1 / 127, dtype=torch.float32)).double()
     codes = torch.where(scales > 0, (wide / torch.where(scales > 0, scales, 1.0)).round().clamp(-127, 127), 0.0)
     bad = ~torch.isfinite(amax)
     scales = torch.where(bad, torch.nan, scales)

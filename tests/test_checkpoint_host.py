@@ -96,7 +96,7 @@ def test_what_the_codes_stand_for():
     assert codes.abs().max() == 127 and torch.equal(codes, codes.round())
     step = scales.repeat_interleave(128, 1)[:, :300]
     assert ((values - x.double()).abs() <= step * (0.5 + 2.0**-20)).all()
-    assert torch.equal(codes[2, 1:100], (torch.arange(1, 100) + 0.5).double().round())  # halves, to even
+    assert torch.equal(codes[2, 1:100], (torch.arange(1, 100) + 0.5).double().round())
 
 
 def test_the_gate_against_differences():

@@ -49,7 +49,7 @@ def test_codes_beside_halves(cuda):
     """fp32 rows of values one step from the halves between two codes, under scales of every last digit."""
     g = torch.Generator().manual_seed(0)
     amax = (1 + torch.rand(500, generator=g)) * 2.0 ** torch.randint(-60, 60, (500,), generator=g)
-    s = (amax.double() / 127).float()
+    s = amax * torch.tensor(1 / 127, dtype=torch.float32)
     x = ((torch.arange(128) - 63.5) * s[:, None].double()).float()
     for step in (-1, 0, 1):
         y = x if step == 0 else torch.nextafter(x, x + step * x.abs())
@@ -95,10 +95,11 @@ def test_linear(cuda, rows, k, n, wide, dtype):
     w16, _, xh = w.to(dtype).double(), None, kept(x)[2]
     near("dx", dx, dy.double() @ w16, (n * U + h) * (dy.double().abs() @ w16.abs()) + least(dtype))
     a = dy.double().t().abs() @ xh.abs()
-    # kept values are rounded to the rows' type, below its normal range to its subnormal step, or held to 2^-17 for an fp32 gradient
+    # kept values are rounded to the rows' type, below its normal range to its subnormal step, or held to 2^-22 (and 2^-33 of the largest
+    # of any) for an fp32 gradient
     fine = wt == torch.float32 and dtype != torch.float32
-    rounding = 2.0**-17 if fine else (0.0 if dtype == torch.float32 else h)
-    sub = 0.0 if fine else dy.double().abs().sum(0)[:, None] * least(dtype)
+    rounding = 2.0**-22 if fine else (0.0 if dtype == torch.float32 else h)
+    sub = 2.0**-33 * rows * dy.double().abs().max() * xh.abs().max() if fine else dy.double().abs().sum(0)[:, None] * least(dtype)
     near("dw", dw, dy.double().t() @ xh, (rows * U + rounding + half(wt)) * a + sub + least(wt))
     near("db", db, dy.double().sum(0), (rows * U + half(wt)) * dy.double().abs().sum(0) + least(wt))
 
@@ -255,3 +256,24 @@ def test_second_derivatives_are_refused(cuda):
     d = torch.autograd.grad(nori_amd.checkpointed_silu_mul(gu, 4).square().sum(), gu, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         torch.autograd.grad(d.sum(), gu)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_fp32_gradients_of_slopes_of_any_size(cuda, dtype):
+    """Slopes that grow by 2^24 from row to row's end, beside infinities in other columns and in the memory between rows: each weight's
+    gradient to 2^-22 of its terms and 2^-33 of the largest of any."""
+    g = torch.Generator().manual_seed(7)
+    rows, k, n = 700, 40, 21
+    x = torch.randn(rows, k, generator=g).to(dtype)
+    buffer = torch.full((rows, n + 3), math.inf, dtype=dtype)
+    buffer[:, :n] = torch.randn(rows, n, generator=g) * 2.0 ** torch.linspace(-12, 12, rows)[:, None]
+    buffer[3, 5] = math.inf
+    dy = buffer.cuda()[:, :n]
+    w = torch.randn(n, k, generator=g).cuda().requires_grad_(True)
+    dw = torch.autograd.grad(nori_amd.checkpointed_linear(x.cuda(), w), w, dy)[0].double().cpu()
+    d, xh = buffer[:, :n].double(), kept(x)[2]
+    others = [i for i in range(n) if i != 5]
+    assert not torch.isfinite(dw[5]).any()
+    d = d[:, others]
+    bound = (rows * U + 2.0**-22) * (d.t().abs() @ xh.abs()) + 2.0**-33 * rows * d.abs().max() * xh.abs().max()
+    near("dw", dw[others], d.t() @ xh, bound)
