@@ -277,6 +277,9 @@ __device__ __forceinline__ float positive(float c, typename El<DT>::Frag (&q)[KS
     return c == 0.f ? 1.f : fabsf(c);
 }
 
+// Bound by the matrix instructions and the exponentials between them over many rows, by HBM over few. 9 x 2 heads of 64, 8,192 x
+// 8,192, bf16: 411-445 us (700 TFLOP/s); four wavefronts a SIMD spill. One row over 65,536 keys: 52 us (5.8 TB/s) and 10 for the
+// parts.
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, DK <= 64 && NW == 4 ? 3 : 2) void forward_kernel(const Args p) {
     using E = El<DT>;
@@ -464,6 +467,8 @@ __device__ __forceinline__ void dq_whole(const typename El<DT>::T* ks, const typ
         }
 }
 
+// Three products of the pairs, bound as the forward pass over many rows: 9 x 2 heads of 64, 8,192 x 8,192, bf16:
+// 527-536 us (880 TFLOP/s). Three wavefronts a SIMD spill.
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq_kernel(const Args p) {
     using E = El<DT>;
@@ -574,6 +579,8 @@ __device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typ
     }
 }
 
+// Four products of the pairs; keys stay, so two sums of 32 x D a wavefront take the registers that a third wavefront would need. The
+// same rows: 740-758 us (835 TFLOP/s).
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Args p) {
     using E = El<DT>;
@@ -681,7 +688,7 @@ dkv_step<DT, DK, kRows / 32>(qs, dos, off, deltas, end - first, kf, vf, dk, dv, 
 
 // ---------------------------------------------------------------- few rows and few keys
 // The forward pass of a unit of up to 32 NW rows and keys. One tile and no loop: half the registers of forward_kernel, so twice the
-// wavefronts, which is what units this short go by.
+// wavefronts, which is what units this short go by: 8,192 x 8 units of 33 x 33 of 44, fp16, 196 us (3.9 TB/s).
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
     using E = El<DT>;
@@ -721,7 +728,8 @@ __global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
 
 // The whole backward pass of such a unit: both sides in LDS, read from memory once, where the kernels above read them twice and the
 // rows' sums pass through memory. (Keys first and queries in their place later take half the LDS and a wavefront a SIMD more, but
-// read the queries twice: 8,192 x 8 units of 33 x 33 of 44, fp16, 656 us so, 557 this way.)
+// read the queries twice: 8,192 x 8 units of 33 x 33 of 44, fp16, 656 us so, 557 this way.) The same units now: 527 us (2.5 TB/s),
+// by the instructions of tiles that are half empty.
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) {
     using E = El<DT>;

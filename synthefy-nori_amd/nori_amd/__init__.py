@@ -9,7 +9,9 @@ and cached apply built on them (``layer``), and the context-cache API around the
 stack -- ``FeaturesTransformer.build_context_cache`` / ``apply_context_cache`` with the
 input encoders (``transformer``, ``encoders``). Its quantile decoder can be fitted to single
 tables and served for many of them at once: LayerNorm with its gradients (``norm``) and
-low-rank adapters beside its projections (``adapters``).
+low-rank adapters beside its projections (``adapters``). A training step through an encoder
+block has its operators beside them: attention with its gradients (``attention``), projections
+and SwiGLU gates that keep their inputs in 8 bits (``checkpoint``).
 """
 
 from . import _native, encoders, layer, transformer
