@@ -168,7 +168,8 @@ int check(const nori_attention_train_args* a, bool backward) {
         return fail(NORI_ERR_UNSUPPORTED, "%s: up to 2^30 keys, and queries of heads that share one, are taken", what);
     if (a->bg > (1LL << 40) / ((int64_t)a->heads * std::max<int64_t>(1, std::max(a->nq, a->nk))))
         return fail(NORI_ERR_UNSUPPORTED, "%s: too many rows", what);
-    if (!(a->scale - a->scale == 0.f)) return fail(NORI_ERR_INVALID, "%s: the scale must be finite", what);
+    const float c = a->scale * kLog2e;
+    if (!(c - c == 0.f)) return fail(NORI_ERR_INVALID, "%s: the scale must be finite, times log2(e) too", what);
     if (a->lengths && (a->length_group < 1)) return fail(NORI_ERR_INVALID, "%s: lengths of %lld entries each", what, (long long)a->length_group);
     const int size = dtype_size(a->dtype);
     if (a->bg * a->nq > 0) {

@@ -137,12 +137,11 @@ __device__ __forceinline__ float quantize8(const Raw8<DT>& r, const float (&v)[k
     return s;
 }
 
-// What codes stand for, rounded once: a code is one byte u less 128, and 128 s is exact.
+// What codes stand for, rounded once.
 __device__ __forceinline__ void restore8(const uint64_t codes, float s, float (&v)[kEach]) {
-    const uint32_t w[2] = {(uint32_t)codes ^ 0x80808080u, (uint32_t)(codes >> 32) ^ 0x80808080u};
-    const float off = -128.0f * s;
+    const uint32_t w[2] = {(uint32_t)codes, (uint32_t)(codes >> 32)};
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) v[i] = fmaf((float)((w[i >> 2] >> (8 * (i & 3))) & 0xffu), s, off);
+    for (int i = 0; i < kEach; ++i) v[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * s;
 }
 
 // 1 / (1 + exp(-g)), to about 2^-22 of itself and |g| 2^-24.

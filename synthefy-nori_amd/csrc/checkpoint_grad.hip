@@ -36,14 +36,13 @@ __device__ __forceinline__ void put(void* p, int dtype, int64_t i, float v) {
     else store_elem<DT == NORI_F32 ? NORI_F16 : DT>(p, i, v);
 }
 
-// The values of 8 codes. A code is one byte u less 128, (u - 128) s = u s - 128 s is rounded once: 128 s is exact.
+// The values of 8 codes.
 template <int DT>
 __device__ __forceinline__ Eight<DT> values(uint32_t lo, uint32_t hi, float s) {
-    const uint32_t w[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
-    const float off = -128.0f * s;
+    const uint32_t w[2] = {lo, hi};
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fmaf((float)((w[i >> 2] >> (8 * (i & 3))) & 0xffu), s, off);
+    for (int i = 0; i < 8; ++i) v[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * s;
     if constexpr (DT == NORI_F32) {
         return __builtin_bit_cast(Eight<DT>, v);
     } else {
@@ -62,11 +61,11 @@ __device__ __forceinline__ float wide(const Eight<DT>& y, int e) {
     else return DT == NORI_F16 ? f16_to_f32(y.e[e]) : bf16_to_f32(y.e[e]);
 }
 template <int DT>
-__device__ __forceinline__ void pieces(const Eight<DT>& y, float s, Eight<NORI_F16>& hi, Eight<NORI_F16>& lo) {
+__device__ __forceinline__ void pieces(const Eight<DT>& y, float s, float power, Eight<NORI_F16>& hi, Eight<NORI_F16>& lo) {
     f16x8 h, l;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        float v = wide<DT>(y, e) * s;
+        float v = wide<DT>(y, e) * s * power;
         // one value for both pieces: a product folded into one of its roundings to float16, and not into the other, rounds otherwise
         asm("" : "+v"(v));
         h[e] = (_Float16)v;
@@ -134,9 +133,9 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
             if (r < end && yc + e < a.n) y.e[e] = reinterpret_cast<const T*>(a.dy)[r * a.dy_stride + yc + e];
         return y;
     };
-    const auto put_y = [&](int j, const Eight<DT>& y, float s) {
+    const auto put_y = [&](int j, const Eight<DT>& y, float s, float power) {
         const int at = (yrow + j * kYStep) * YS + ycol;
-        if constexpr (FINE) pieces<DT>(y, s, *reinterpret_cast<Eight<NORI_F16>*>(&ys[at]), *reinterpret_cast<Eight<NORI_F16>*>(&ls[at]));
+        if constexpr (FINE) pieces<DT>(y, s, power, *reinterpret_cast<Eight<NORI_F16>*>(&ys[at]), *reinterpret_cast<Eight<NORI_F16>*>(&ls[at]));
         else *reinterpret_cast<Eight<DT>*>(&ys[at]) = y;
     };
     const auto put_x = [&](int j, uint4 x, float s) {
@@ -198,7 +197,7 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
         if constexpr (FINE) agree();
         if (whole(from)) {
 #pragma unroll
-            for (int j = 0; j < NY; ++j) put_y(j, ye[j], FINE ? ysc[FINE ? j : 0] * power : 1.f);
+            for (int j = 0; j < NY; ++j) put_y(j, ye[j], FINE ? ysc[FINE ? j : 0] : 1.f, power);
 #pragma unroll
             for (int j = 0; j < NX; ++j) put_x(j, xe[j], FINE ? 1.f : xsc[FINE ? 0 : j]);
             if (turn == 0) {
@@ -210,7 +209,7 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
             for (int j = 0; j < NY; ++j) {
                 const int64_t r = from + yrow + j * kYStep;
                 const Eight<DT> y = partial(r);
-                put_y(j, y, FINE && a.dw && r < end ? a.scales[r * a.groups + kt] * power : 1.f);
+                put_y(j, y, FINE && a.dw && r < end ? a.scales[r * a.groups + kt] : 1.f, power);
                 if (turn == 0) add(y);
             }
 #pragma unroll 1

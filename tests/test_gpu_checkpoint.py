@@ -277,3 +277,38 @@ def test_fp32_gradients_of_slopes_of_any_size(cuda, dtype):
     d = d[:, others]
     bound = (rows * U + 2.0**-22) * (d.t().abs() @ xh.abs()) + 2.0**-33 * rows * d.abs().max() * xh.abs().max()
     near("dw", dw[others], d.t() @ xh, bound)
+
+
+@pytest.mark.parametrize("dtype, weight", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16)],
+                         ids=str)
+def test_values_at_the_top_of_the_range(cuda, dtype, weight):
+    """Rows up to the type's largest number beside slopes down to 2^-100: 128 scales are past fp32, a scale times a power of two too."""
+    x = activations(70, 130, torch.float32).to(dtype)
+    x[5] *= 2.0**100
+    x[40, 129] = torch.finfo(dtype).max
+    dy = (torch.randn(70, 9, generator=torch.Generator().manual_seed(3)) * 2.0**-100).to(dtype)
+    w = torch.zeros(9, 130, dtype=weight, device="cuda", requires_grad=True)
+    dw = torch.autograd.grad(nori_amd.checkpointed_linear(x.cuda(), w), w, dy.cuda())[0].double().cpu()
+    xh, d = kept(x)[2], dy.double()
+    assert torch.isfinite(xh).all()
+    # x to the rows' type, the result to the weight's, sums in fp32; float32 weights take two pieces of the slopes instead
+    fine = weight != dtype
+    each = 2.0**-22 if fine else torch.finfo(dtype).eps / 2
+    bound = (71 * U + each) * (d.t().abs() @ xh.abs()) + torch.finfo(weight).eps / 2 * (d.t() @ xh).abs()
+    if fine:
+        bound[:, :128] += 2.0**-33 * 70 * (d.abs().amax(1) * xh[:, :128].abs().amax(1)).max()
+        bound[:, 128:] += 2.0**-33 * 70 * (d.abs().amax(1) * xh[:, 128:].abs().amax(1)).max()
+    near("dw", dw, d.t() @ xh, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_gates_at_the_top_of_the_range(cuda, dtype):
+    gu = torch.ones(3, 260, dtype=dtype)
+    gu[1, 130:] = torch.finfo(dtype).max
+    dy = torch.full((3, 130), 2.0**-100, dtype=dtype)
+    gu = gu.cuda().requires_grad_(True)
+    dgu = torch.autograd.grad(nori_amd.checkpointed_silu_mul(gu, 130), gu, dy.cuda())[0].double().cpu()
+    g, u = torch.ones(3, 130).double(), kept(gu[:, 130:])[2]
+    s = torch.sigmoid(g)
+    expected = torch.cat([dy.double() * u * s * (1 + g * (1 - s)), dy.double() * g * s], 1)
+    near("dgu", dgu, expected, expected.abs() * (torch.finfo(dtype).eps / 2 + 64 * U))
