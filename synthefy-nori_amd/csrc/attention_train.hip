@@ -146,11 +146,11 @@ bool loads(const void* p, int size, std::initializer_list<int64_t> strides, int 
     return std::all_of(strides.begin(), strides.end(), [n](int64_t s) { return s % n == 0; });
 }
 
-// Whether everything that is read lies in 16-byte chunks of a 16-bit type.
+// Whether everything that is read or written lies in 16-byte chunks of a 16-bit type.
 bool wide(const nori_attention_train_args& a, bool backward) {
     return a.dtype != NORI_F32 && a.d % 8 == 0 && loads(a.q, 2, {a.q_bg, a.q_row, a.q_head}, 8) &&
            loads(a.kv, 2, {a.kv_bg, a.kv_row, a.kv_half, a.kv_head}, 8) && loads(a.out, 2, {}, 8) &&
-           (!backward || loads(a.dout, 2, {a.do_bg, a.do_row, a.do_head}, 8));
+           (!backward || (loads(a.dout, 2, {a.do_bg, a.do_row, a.do_head}, 8) && loads(a.dq, 2, {}, 8) && loads(a.dkv, 2, {}, 8)));
 }
 
 int check(const nori_attention_train_args* a, bool backward) {

@@ -43,14 +43,22 @@ def _quantized(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return codes, scales
 
 
+def _linear(x, weight, bias):
+    """(x weight^T + bias, the weight as it entered the product)."""
+    w = weight if weight.dtype == x.dtype else weight.to(x.dtype)
+    b = bias if bias is None or bias.dtype == x.dtype else bias.to(x.dtype)
+    with torch.autocast("cuda", enabled=False):
+        if x.dim() == 2:
+            return F.linear(x, w, b), w
+        # (one product: rows that do not fold would be a batch of them)
+        return F.linear(x.reshape(-1, x.shape[-1]), w, b).view(*x.shape[:-1], w.shape[0]), w
+
+
 class _CheckpointedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         ctx.grad_dtypes = weight.dtype, None if bias is None else bias.dtype
-        w = weight if weight.dtype == x.dtype else weight.to(x.dtype)
-        b = bias if bias is None or bias.dtype == x.dtype else bias.to(x.dtype)
-        with torch.autocast("cuda", enabled=False):
-            y = F.linear(x, w, b)
+        y, w = _linear(x, weight, bias)
         kept = _quantized(x) if ctx.needs_input_grad[1] else (None, None)
         ctx.save_for_backward(w if ctx.needs_input_grad[0] else None, *kept)
         ctx.cols = int(x.shape[-1])
@@ -120,7 +128,9 @@ def checkpointed_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and t.dtype not in (x.dtype, torch.float32):
             raise ValueError(f"checkpointed_linear: {name} is {t.dtype}, x {x.dtype}")
-    return _CheckpointedLinear.apply(x, weight, bias)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _CheckpointedLinear.apply(x, weight, bias)
+    return _linear(x, weight, bias)[0]
 
 
 class _CheckpointedSiluMul(torch.autograd.Function):

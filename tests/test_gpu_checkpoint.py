@@ -312,3 +312,39 @@ def test_gates_at_the_top_of_the_range(cuda, dtype):
     s = torch.sigmoid(g)
     expected = torch.cat([dy.double() * u * s * (1 + g * (1 - s)), dy.double() * g * s], 1)
     near("dgu", dgu, expected, expected.abs() * (torch.finfo(dtype).eps / 2 + 64 * U))
+
+
+def test_nothing_is_kept_where_nothing_is_trained(cuda, monkeypatch):
+    x = activations(37, 130, torch.float16).cuda()
+    w = torch.randn(9, 130, device="cuda", dtype=torch.float16, requires_grad=True)
+    expected = F.linear(x, w.detach())
+
+    def kept_anyway(x):
+        raise AssertionError("the input was quantised")
+
+    monkeypatch.setattr(cp, "_quantized", kept_anyway)
+    with torch.no_grad():
+        assert torch.equal(nori_amd.checkpointed_linear(x, w), expected)
+    assert torch.equal(nori_amd.checkpointed_linear(x, w.detach()), expected)
+    leaf = x.clone().requires_grad_(True)
+    y = nori_amd.checkpointed_linear(leaf, w.detach())
+    assert torch.equal(y, expected)
+    assert torch.equal(torch.autograd.grad(y, leaf, torch.ones_like(y))[0], torch.ones_like(y) @ w.detach())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_rows_that_do_not_fold(cuda, dtype):
+    """A batch of rows cut out of a larger one, and rows of a single dimension: what their contiguous copies give, bit for bit."""
+    big = activations(6 * 11, 48, dtype).view(6, 11, 48).cuda()
+    w = torch.randn(20, 32, device="cuda").to(dtype).requires_grad_(True)
+    b = torch.randn(20, device="cuda").to(dtype).requires_grad_(True)
+    for cut in (big[1:5, 2:9, 8:40], big[1, 2, 8:40]):
+        dy = torch.randn(*cut.shape[:-1], 20, device="cuda").to(dtype)
+        got = []
+        for x in (cut, cut.contiguous()):
+            x = x.detach().requires_grad_(True)
+            y = nori_amd.checkpointed_linear(x, w, b)
+            assert y.shape == dy.shape
+            got.append((y, *torch.autograd.grad(y, (x, w, b), dy)))
+        for one, other in zip(*got):
+            assert torch.equal(one, other)
