@@ -15,7 +15,8 @@ template <int DT, int DK> struct Geo {
     using E = El<DT>;
     using T = typename E::T;
     static constexpr int DP = (DK + 31) / 32 * 32;
-    static constexpr int LS = DP + E::kPad;      // elements from one row of a tile to the next
+    static constexpr int LS = DK + E::kPad;      // elements from one row of a tile to the next
+    static constexpr int kTail = DP - DK;        // behind a tile: what the last products' columns past DK reach of its last row
     static constexpr int KS = DK / 16, MS = DP / 32;
 };
 
@@ -40,6 +41,13 @@ template <int DT, int DK>
 __device__ __forceinline__ typename El<DT>::Frag direct(const typename El<DT>::T* tile, int row, int k, int half) {
     const auto* p = tile + row * Geo<DT, DK>::LS + 16 * k + 8 * half;
     return *reinterpret_cast<const typename El<DT>::Frag*>(p);
+}
+
+// Lane's row of a tile's 32-row step `sub`, of T16 sixteens: past them the last one, whose products are not used.
+template <int T16>
+__device__ __forceinline__ int row_in(int sub, int lane) {
+    const int row = sub * 32 + (lane & 31);
+    return 32 * sub + 32 > 16 * T16 ? min(row, 16 * T16 - 1) : row;
 }
 
 // The operands that stay: columns 16 k + 8 h .. + 7 of the row at p, zeros past d or where the row is not there.
@@ -84,19 +92,14 @@ __device__ __forceinline__ void store_row(Out* out, const f32x16 (&x)[MS], float
 }
 
 // The same for the 32 rows of a wavefront's columns by way of LDS (its own 32 rows there): a lane's columns are apart in memory, 32
-// lines an access, which the address units bound short scans by; from LDS rows go out side by side. to(row): where it begins. DIRECT:
-// without LDS, for the backward passes in 8-byte chunks, which gain nothing by it (8,192 x 8 units of 33 x 33 of 44, fp16: forward
-// 250 us direct, 196 so, backward 527 and 553; x 10 of 51 x 51 of 56 in 16-byte chunks: backward 951 and 859).
-template <int DT, int DK, int W, int LS, bool DIRECT, int MS, class To>
+// lines an access, which the address units bound short scans by; from LDS rows go out side by side. to(row): where it begins.
+// (Units of 33 x 33 of 44, fp16, 8,192 x 8: backward 487 us without, 404 so; x 10 of 51 x 51 of 56: 951 and 859.)
+template <int DT, int DK, int W, int LS, int MS, class To>
 __device__ __forceinline__ void store_rows(typename El<DT>::T* lds, const f32x16 (&x)[MS], float by, int d, int lane, int rows, To to) {
     using T = typename El<DT>::T;
     typedef uint32_t Chunk __attribute__((ext_vector_type(W * sizeof(T) / 4)));
     constexpr int CH = DK / W;
-    if constexpr (DIRECT) {
-        if ((lane & 31) < rows) store_row<DT>(to(lane & 31), x, by, d, lane >> 5);
-        return;
-    }
-    store_row<DT>(lds + (lane & 31) * LS, x, by, d, lane >> 5);
+    if ((lane & 31) < rows) store_row<DT>(lds + (lane & 31) * LS, x, by, d, lane >> 5);  // (past them another's may begin)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -286,8 +289,8 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && NW == 4 ? 3 : 2) void forward_
     using G = Geo<DT, DK>;
     using T = typename E::T;
     constexpr int kRows = kTileOf<DT, NW>;
-    __shared__ __attribute__((aligned(16))) T ks[kRows * G::LS];
-    __shared__ __attribute__((aligned(16))) T vs[kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T ks[kRows * G::LS + G::kTail];
+    __shared__ __attribute__((aligned(16))) T vs[kRows * G::LS + G::kTail];
     const auto& a = p.a;
     const Block w = block_of(p);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
@@ -427,7 +430,8 @@ __device__ __forceinline__ void dq_step(const typename El<DT>::T* ks, const type
 
 // The same of rows whose keys are all in this tile, which takes delta = sum of p (dout v) from them: with few keys ds is a small
 // difference, and delta of the result as it was rounded would be off by as much.
-template <int DT, int DK, int NS>
+// T16: the sixteens of rows that the tile has.
+template <int DT, int DK, int NS, int T16 = 2 * NS>
 __device__ __forceinline__ void dq_whole(const typename El<DT>::T* ks, const typename El<DT>::T* vs, int left,
                                          const typename El<DT>::Frag (&qf)[DK / 16], const typename El<DT>::Frag (&dof)[DK / 16],
                                          f32x16 (&dq)[Geo<DT, DK>::MS], Scale& scale, float c, float lse2, float& delta, int lane) {
@@ -440,12 +444,12 @@ __device__ __forceinline__ void dq_whole(const typename El<DT>::T* ks, const typ
         f32x16 s = {}, dp = {};
 #pragma unroll
         for (int k = 0; k < G::KS; ++k) {
-            s = mma(direct<DT, DK>(ks, sub * 32 + (lane & 31), k, half), qf[k], s);
-            dp = mma(direct<DT, DK>(vs, sub * 32 + (lane & 31), k, half), dof[k], dp);
+            s = mma(direct<DT, DK>(ks, row_in<T16>(sub, lane), k, half), qf[k], s);
+            dp = mma(direct<DT, DK>(vs, row_in<T16>(sub, lane), k, half), dof[k], dp);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const bool in = sub * 32 + 8 * (i / 4) + i % 4 < left - 4 * half;
+            const bool in = 2 * sub + i / 8 < T16 && sub * 32 + 8 * (i / 4) + i % 4 < left - 4 * half;
             pr[sub][i] = in ? __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) : 0.f;
             ds[sub][i] = in ? dp[i] : 0.f;
             delta = fmaf(pr[sub][i], ds[sub][i], delta);
@@ -461,6 +465,7 @@ __device__ __forceinline__ void dq_whole(const typename El<DT>::T* ks, const typ
     for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            if (2 * sub + t >= T16) continue;
             const auto f = rounded<DT>(ds[sub], t);
 #pragma unroll
             for (int j = 0; j < G::MS; ++j) dq[j] = mma(transposed<DT, G::LS>(ks, sub * 32 + 16 * t, 32 * j, lane), f, dq[j]);
@@ -475,8 +480,8 @@ __global__ __launch_bounds__(64 * NW, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq
     using G = Geo<DT, DK>;
     using T = typename E::T;
     constexpr int kRows = kTileOf<DT, NW>;
-    __shared__ __attribute__((aligned(16))) T ks[kRows * G::LS];
-    __shared__ __attribute__((aligned(16))) T vs[kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T ks[kRows * G::LS + G::kTail];
+    __shared__ __attribute__((aligned(16))) T vs[kRows * G::LS + G::kTail];
     const auto& a = p.a;
     const Block w = block_of(p);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
@@ -529,7 +534,7 @@ __global__ __launch_bounds__(64 * NW, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq
 // ---------------------------------------------------------------- dk and dv
 // One tile's part of dk and dv: `left` of its rows are there. off: kBias - log2 of a row's sum, deltas: its -delta, what the
 // products of dout and v start from.
-template <int DT, int DK, int NS>
+template <int DT, int DK, int NS, int T16 = 2 * NS>
 __device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typename El<DT>::T* dos, const float* off, const float* deltas,
                                          int left, const typename El<DT>::Frag (&kf)[DK / 16], const typename El<DT>::Frag (&vf)[DK / 16],
                                          f32x16 (&dk)[Geo<DT, DK>::MS], f32x16 (&dv)[Geo<DT, DK>::MS], Scale& scale, float c, int lane) {
@@ -546,8 +551,8 @@ __device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typ
         }
 #pragma unroll
         for (int k = 0; k < G::KS; ++k) {
-            s = mma(direct<DT, DK>(qs, sub * 32 + (lane & 31), k, half), kf[k], s);
-            dp = mma(direct<DT, DK>(dos, sub * 32 + (lane & 31), k, half), vf[k], dp);
+            s = mma(direct<DT, DK>(qs, row_in<T16>(sub, lane), k, half), kf[k], s);
+            dp = mma(direct<DT, DK>(dos, row_in<T16>(sub, lane), k, half), vf[k], dp);
         }
         interleave<DT, 2 * G::KS, 1, 4, 4>();
         float pr[16], ds[1][16];
@@ -563,11 +568,12 @@ __device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typ
         if (left < 32 * NS) {  // rows that are not there: 0, also beside keys that are not finite
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (sub * 32 + 8 * (i / 4) + i % 4 >= left - 4 * half) pr[i] = ds[0][i] = 0.f;
+                if (2 * sub + i / 8 >= T16 || sub * 32 + 8 * (i / 4) + i % 4 >= left - 4 * half) pr[i] = ds[0][i] = 0.f;
         }
         if constexpr (El<DT>::kScaled) scale.apply(ds, dk);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            if (2 * sub + t >= T16) continue;
             const auto pf = rounded<DT>(pr, t), f = rounded<DT>(ds[0], t);
 #pragma unroll
             for (int j = 0; j < G::MS; ++j) {
@@ -587,8 +593,8 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Ar
     using G = Geo<DT, DK>;
     using T = typename E::T;
     constexpr int kRows = kTileOf<DT, NW>;
-    __shared__ __attribute__((aligned(16))) T qs[kRows * G::LS];
-    __shared__ __attribute__((aligned(16))) T dos[kRows * G::LS];
+    __shared__ __attribute__((aligned(16))) T qs[kRows * G::LS + G::kTail];
+    __shared__ __attribute__((aligned(16))) T dos[kRows * G::LS + G::kTail];
     __shared__ __attribute__((aligned(16))) float off[kRows];
     __shared__ __attribute__((aligned(16))) float deltas[kRows];
     const auto& a = p.a;
@@ -657,7 +663,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Ar
         }
         __syncthreads();
         if (first + kRows < end) load(first + kRows);
-dkv_step<DT, DK, kRows / 32>(qs, dos, off, deltas, end - first, kf, vf, dk, dv, scale, p.c, lane);
+        dkv_step<DT, DK, kRows / 32>(qs, dos, off, deltas, end - first, kf, vf, dk, dv, scale, p.c, lane);
     }
     if (!there) {  // past the length
 #pragma unroll
@@ -681,8 +687,8 @@ dkv_step<DT, DK, kRows / 32>(qs, dos, off, deltas, end - first, kf, vf, dk, dv, 
         __syncthreads();
         if (wave / kAtOnce != turn) continue;
         const int mine = wave % kAtOnce * 32 * G::LS;
-        store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(qs + mine, dk, byk, a.d, lane, left, [&](int i) { return to + (int64_t)i * 2 * a.kv_heads * a.d; });
-        store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(dos + mine, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
+        store_rows<DT, DK, W, G::LS>(qs + mine, dk, byk, a.d, lane, left, [&](int i) { return to + (int64_t)i * 2 * a.kv_heads * a.d; });
+        store_rows<DT, DK, W, G::LS>(dos + mine, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
     }
 }
 
@@ -694,8 +700,8 @@ __global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
-    __shared__ __attribute__((aligned(16))) T ks[32 * NW * G::LS];
-    __shared__ __attribute__((aligned(16))) T vs[32 * NW * G::LS];
+    __shared__ __attribute__((aligned(16))) T ks[32 * NW * G::LS + G::kTail];
+    __shared__ __attribute__((aligned(16))) T vs[32 * NW * G::LS + G::kTail];
     const auto& a = p.a;
     const int64_t unit = work_index(blockIdx.x, gridDim.x), b = unit / a.kv_heads, hk = unit % a.kv_heads;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, own = wave * 32 + (lane & 31);
@@ -720,7 +726,7 @@ __global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
     if (there && half == 0 && a.lse) a.lse[unit * p.rows + own] = length > 0 ? (__builtin_amdgcn_logf(l) - E::kTop + m * c) * kLn2 : -INFINITY;
     T* out = reinterpret_cast<T*>(a.out) + b * a.nq * a.heads * a.d;
     __syncthreads();  // the tile is everyone's until here
-    store_rows<DT, DK, W, G::LS, false>(ks + wave * 32 * G::LS, o, length > 0 ? 1.f / l : 0.f, a.d, lane, rows - wave * 32, [&](int i) {
+    store_rows<DT, DK, W, G::LS>(ks + wave * 32 * G::LS, o, length > 0 ? 1.f / l : 0.f, a.d, lane, rows - wave * 32, [&](int i) {
         const Row to = row_of(p, hk, wave * 32 + i);
         return out + (to.query * a.heads + to.head) * a.d;
     });
@@ -728,27 +734,28 @@ __global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
 
 // The whole backward pass of such a unit: both sides in LDS, read from memory once, where the kernels above read them twice and the
 // rows' sums pass through memory. (Keys first and queries in their place later take half the LDS and a wavefront a SIMD more, but
-// read the queries twice: 8,192 x 8 units of 33 x 33 of 44, fp16, 656 us so, 557 this way.) The same units now: 527 us (2.5 TB/s),
-// by the instructions of tiles that are half empty.
-template <int DT, int DK, int W, int NW>
+// read the queries twice: 8,192 x 8 units of 33 x 33 of 44, fp16, 656 us so, 557 this way.) ROWS is 48 where that holds both sides, for LDS
+// that lets a wavefront a SIMD more in and a quarter less work: the same units 529 us with 64, 499 with 48. Now: 404 us (3.3 TB/s), bound
+// by the instructions that tiles half empty take.
+template <int DT, int DK, int W, int NW, int ROWS>
 __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
-    constexpr int kTile = 32 * NW * G::LS;
-    __shared__ __attribute__((aligned(16))) T tiles[4 * kTile];
+    constexpr int kTile = ROWS * G::LS;
+    __shared__ __attribute__((aligned(16))) T tiles[4 * kTile + G::kTail];
     __shared__ __attribute__((aligned(16))) float off[32 * NW];
     __shared__ __attribute__((aligned(16))) float deltas[32 * NW];
     T *ks = tiles, *vs = tiles + kTile, *qs = tiles + 2 * kTile, *dos = tiles + 3 * kTile;
     const auto& a = p.a;
     const int64_t unit = work_index(blockIdx.x, gridDim.x), b = unit / a.kv_heads, hk = unit % a.kv_heads;
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, own = wave * 32 + (lane & 31);
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6, own = wave * 32 + (lane & 31), mine = row_in<ROWS / 16>(wave, lane);
     const int length = length_of(a, b), rows = (int)p.rows, nq = (int)a.nq;
 
     const T* kv = reinterpret_cast<const T*>(a.kv) + b * a.kv_bg + hk * a.kv_head;
     const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_bg + hk * p.group * a.q_head;
     const T* dout = reinterpret_cast<const T*>(a.dout) + b * a.do_bg + hk * p.group * a.do_head;
-    Stage<DT, DK, W, 64 * NW, 32 * NW> keys, queries;
+    Stage<DT, DK, W, 64 * NW, ROWS> keys, queries;
     keys.place(a.d, a.kv_row, a.kv_row);
     keys.load(kv, kv + a.kv_half, length);
     queries.place(a.d, a.q_row, a.do_row);
@@ -769,10 +776,10 @@ __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) 
     float delta = 0.f;
 #pragma unroll
     for (int k = 0; k < G::KS; ++k) {
-        x[k] = direct<DT, DK>(qs, own, k, half);
-        y[k] = direct<DT, DK>(dos, own, k, half);
+        x[k] = direct<DT, DK>(qs, mine, k, half);
+        y[k] = direct<DT, DK>(dos, mine, k, half);
     }
-    if (length > 0) dq_whole<DT, DK, NW>(ks, vs, length, x, y, dq, qscale, p.c, lse2, delta, lane);
+    if (length > 0) dq_whole<DT, DK, NW, ROWS / 16>(ks, vs, length, x, y, dq, qscale, p.c, lse2, delta, lane);
     if (half == 0) {
         off[own] = there ? E::kBias - lse2 : 0.f;
         deltas[own] = there ? -delta : 0.f;
@@ -781,27 +788,27 @@ __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) 
     // from here on a wavefront's 32 rows of ks and vs are its own
 #pragma unroll
     for (int k = 0; k < G::KS; ++k) {
-        x[k] = direct<DT, DK>(ks, own, k, half);
-        y[k] = direct<DT, DK>(vs, own, k, half);
+        x[k] = direct<DT, DK>(ks, mine, k, half);
+        y[k] = direct<DT, DK>(vs, mine, k, half);
     }
     T *lk = ks + wave * 32 * G::LS, *lv = vs + wave * 32 * G::LS;
     T* to_q = reinterpret_cast<T*>(a.dq) + b * a.nq * a.heads * a.d;
-    store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(lk, dq, a.scale * (E::kScaled ? qscale.inverse() : 1.f), a.d, lane, rows - wave * 32, [&](int i) {
+    store_rows<DT, DK, W, G::LS>(lk, dq, a.scale * (E::kScaled ? qscale.inverse() : 1.f), a.d, lane, rows - wave * 32, [&](int i) {
         const Row to = row_of(p, hk, wave * 32 + i);
         return to_q + (to.query * a.heads + to.head) * a.d;
     });
     f32x16 dk[G::MS] = {}, dv[G::MS] = {};
     Scale scale;
-    if (length > 0 && rows > 0) dkv_step<DT, DK, NW>(qs, dos, off, deltas, rows, x, y, dk, dv, scale, p.c, lane);
+    if (length > 0 && rows > 0) dkv_step<DT, DK, NW, ROWS / 16>(qs, dos, off, deltas, rows, x, y, dk, dv, scale, p.c, lane);
     if (own >= length) {
 #pragma unroll
         for (int j = 0; j < G::MS; ++j) dk[j] = dv[j] = f32x16{};
     }
     T* to_k = reinterpret_cast<T*>(a.dkv) + ((b * a.nk + wave * 32) * 2 * a.kv_heads + hk) * a.d;
     const int left = (int)a.nk - wave * 32;
-    store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(lk, dk, a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f), a.d, lane, left,
+    store_rows<DT, DK, W, G::LS>(lk, dk, a.scale * kUnbias<DT> * (E::kScaled ? scale.inverse() : 1.f), a.d, lane, left,
                                  [&](int i) { return to_k + (int64_t)i * 2 * a.kv_heads * a.d; });
-    store_rows<DT, DK, W, G::LS, (W * sizeof(T) < 16)>(lv, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to_k + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
+    store_rows<DT, DK, W, G::LS>(lv, dv, kUnbias<DT>, a.d, lane, left, [&](int i) { return to_k + ((int64_t)i * 2 + 1) * a.kv_heads * a.d; });
 }
 
 // ---------------------------------------------------------------- launches
@@ -813,7 +820,8 @@ void launch_one(Kind kind, const Args& p, dim3 grid, hipStream_t stream) {
     else if (kind == kDkv) hipLaunchKernelGGL((dkv_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
     else if constexpr (few_fits(DT == NORI_F32, DK, NW)) {
         if (kind == kFewForward) hipLaunchKernelGGL((forward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
-        else hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
+        else if (NW == 2 && p.rows <= 48 && p.a.nk <= 48) hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW, NW == 2 ? 48 : 32>), grid, threads, 0, stream, p);
+        else hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW, 32 * NW>), grid, threads, 0, stream, p);
     }
 }
 

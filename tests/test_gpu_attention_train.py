@@ -270,3 +270,27 @@ def test_second_derivatives_are_refused(cuda):
     dq = torch.autograd.grad(nori_amd.trainable_attention(q, kv).square().sum(), q, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dq.sum(), kv)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [
+    (3, 48, 48, 2, 2, 44, [48, 0, 47]),
+    (3, 47, 33, 1, 1, 64, [33, 16, 32]),
+    (2, 24, 41, 4, 2, 56, None),        # 48 rows of two heads that share a key head
+    (2, 49, 48, 2, 2, 44, [48, 17]),
+    (2, 48, 49, 2, 1, 32, [49, 48]),
+    (5, 1, 48, 1, 1, 48, None),
+    (5, 48, 1, 1, 1, 40, None),
+    (70, 33, 33, 3, 3, 12, None),
+], ids=lambda s: "x".join(map(str, s[:6])))
+def test_units_of_about_48_rows_and_keys(cuda, shape, dtype):
+    """Rows and keys at and beside the ends of the tiles' halves, NaN and infinities behind the lengths among them."""
+    *sizes, lengths = shape
+    q, kv, dout = inputs(*sizes, dtype, seed=9)
+    expected, bounds = reference(q, kv, lengths, dout)
+    if lengths is not None:
+        for i, n in enumerate(lengths * (len(kv) // len(lengths))):
+            kv[i, n:] = (math.nan, math.inf, -math.inf)[i % 3]
+    out, dq, dkv = run(q, kv, lengths, dout)
+    for name, got, i in (("out", out, 0), ("dq", dq, 2), ("dkv", dkv, 3)):
+        assert_near(name, got, expected[i], bounds[i])
