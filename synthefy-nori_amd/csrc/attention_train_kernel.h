@@ -123,10 +123,21 @@ template <int DT, int NW>
 constexpr int kTileOf = NW == 1 ? 32 : El<DT>::kRows;
 
 // The work of a workgroup: part `split` of what passes by tile `tile` of what stays, in a unit.
+// heads: the heads of one tile are neighbours and not the tiles of one head.
 struct Block { int64_t tile, split, unit, b, hk; };
-__device__ __forceinline__ Block block_of(const Args& p) {
+__device__ __forceinline__ Block block_of(const Args& p, bool heads = false) {
     int64_t i = work_index(blockIdx.x, gridDim.x);
     Block w;
+    if (heads) {
+        w.hk = i % p.a.kv_heads;
+        i /= p.a.kv_heads;
+        w.tile = i % p.tiles;
+        i /= p.tiles;
+        w.split = i % p.splits;
+        w.b = i / p.splits;
+        w.unit = w.b * p.a.kv_heads + w.hk;
+        return w;
+    }
     w.tile = i % p.tiles;
     i /= p.tiles;
     w.split = i % p.splits;
@@ -451,6 +462,7 @@ __device__ __forceinline__ void dq_whole(const typename El<DT>::T* ks, const typ
         for (int i = 0; i < 16; ++i) {
             const bool in = 2 * sub + i / 8 < T16 && sub * 32 + 8 * (i / 4) + i % 4 < left - 4 * half;
             pr[sub][i] = in ? __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) : 0.f;
+            if (sub == 0 && i == 0 && left == 1 && half == 0) pr[0][0] = fmaf(pr[0][0], 0.f, 1.f);  // one key: 1, so that ds is 0
             ds[sub][i] = in ? dp[i] : 0.f;
             delta = fmaf(pr[sub][i], ds[sub][i], delta);
         }
@@ -587,18 +599,24 @@ __device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typ
 
 // Four products of the pairs; keys stay, so two sums of 32 x D a wavefront take the registers that a third wavefront would need. The
 // same rows: 740-758 us (835 TFLOP/s).
-template <int DT, int DK, int W, int NW>
+// kRows: of the tile that passes. Up to 32 rows in all take one tile of 32; the time goes to keys in and out then, so every
+// wavefront's results have room in LDS at once, and heads whose rows share lines of memory are neighbours. One row of 8 heads over 8,192
+// keys, 64 times, dq, dk and dv together: bf16 heads of 64 703 us (4.6 TB/s; results by turns 790, neighbouring heads 752), fp16 of 44
+// 768 (869 in tiles of 64 rows, 891 with a head's tiles as neighbours).
+template <int DT, int DK, int W, int NW, int kRows>
 __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Args p) {
     using E = El<DT>;
     using G = Geo<DT, DK>;
     using T = typename E::T;
-    constexpr int kRows = kTileOf<DT, NW>;
-    __shared__ __attribute__((aligned(16))) T qs[kRows * G::LS + G::kTail];
-    __shared__ __attribute__((aligned(16))) T dos[kRows * G::LS + G::kTail];
+    constexpr bool kFewRows = kRows != kTileOf<DT, NW>;
+    // rows of the tiles, or of the results on their way out
+    constexpr int kRoom = !kFewRows ? kRows : (sizeof(T) == 2 && DK <= 64 ? 32 * NW : kTileOf<DT, NW>);
+    __shared__ __attribute__((aligned(16))) T qs[kRoom * G::LS + G::kTail];
+    __shared__ __attribute__((aligned(16))) T dos[kRoom * G::LS + G::kTail];
     __shared__ __attribute__((aligned(16))) float off[kRows];
     __shared__ __attribute__((aligned(16))) float deltas[kRows];
     const auto& a = p.a;
-    const Block w = block_of(p);
+    const Block w = block_of(p, kFewRows && a.d * sizeof(T) % 128 != 0);
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = threadIdx.x >> 6;
     const int64_t key64 = w.tile * 32 * NW + wave * 32 + (lane & 31);
     const int length = length_of(a, w.b);
@@ -677,8 +695,8 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Ar
         store_row<DT>(part + a.d, dv, kUnbias<DT>, a.d, half);
         return;
     }
-    // the tiles hold 32 rows for each of two wavefronts (one in float32) at a time
-    constexpr int kAtOnce = kRows / 32;
+    // there is room for 32 rows of each of so many wavefronts at a time
+    constexpr int kAtOnce = kRoom / 32;
     const int64_t from = w.tile * 32 * NW + wave * 32;
     T* to = reinterpret_cast<T*>(a.dkv) + ((w.b * a.nk + from) * 2 * a.kv_heads + w.hk) * a.d;
     const int left = (int)min((int64_t)32, a.nk - from);
@@ -817,7 +835,8 @@ void launch_one(Kind kind, const Args& p, dim3 grid, hipStream_t stream) {
     const dim3 threads(64 * NW);
     if (kind == kForward) hipLaunchKernelGGL((forward_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
     else if (kind == kDq) hipLaunchKernelGGL((dq_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
-    else if (kind == kDkv) hipLaunchKernelGGL((dkv_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
+    else if (kind == kDkv && p.rows <= 32) hipLaunchKernelGGL((dkv_kernel<DT, DK, W, NW, 32>), grid, threads, 0, stream, p);
+    else if (kind == kDkv) hipLaunchKernelGGL((dkv_kernel<DT, DK, W, NW, kTileOf<DT, NW>>), grid, threads, 0, stream, p);
     else if constexpr (few_fits(DT == NORI_F32, DK, NW)) {
         if (kind == kFewForward) hipLaunchKernelGGL((forward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
         else if (NW == 2 && p.rows <= 48 && p.a.nk <= 48) hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW, NW == 2 ? 48 : 32>), grid, threads, 0, stream, p);

@@ -294,3 +294,13 @@ def test_units_of_about_48_rows_and_keys(cuda, shape, dtype):
     out, dq, dkv = run(q, kv, lengths, dout)
     for name, got, i in (("out", out, 0), ("dq", dq, 2), ("dkv", dkv, 3)):
         assert_near(name, got, expected[i], bounds[i])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("queries", [1, 33, 300])
+def test_one_key_takes_no_gradient_of_queries(cuda, queries, dtype):
+    q, kv, dout = inputs(3, queries, 5, 2, 1, 36, dtype, seed=10)
+    _, dq, _ = run(q, kv[:, :1], None, dout)
+    assert not dq.any()
+    _, dq, _ = run(q, kv, [1, 0, 1], dout)
+    assert not dq.any()
