@@ -57,8 +57,8 @@ __device__ __forceinline__ int64_t work_index(int64_t i, int64_t n) {
     return i < whole ? (i & 7) * (whole >> 3) + (i >> 3) : i;
 }
 
-// What a launch does; kFewForward, kFew: the forward and the whole backward pass of units of few rows and keys. Launches of the typed translation units,
-// in chunks of 16 bytes or (narrow) of 4 elements.
+// What a launch does; kFewForward, kFew: the forward and the whole backward pass of units of few rows and keys. Launches of the
+// typed translation units, in chunks of 16 bytes or (narrow) of 4 elements.
 enum Kind { kForward, kDq, kDkv, kFewForward, kFew };
 int launch_f16(Kind kind, const Args& p, int64_t blocks, hipStream_t stream);
 int launch_f16_narrow(Kind kind, const Args& p, int64_t blocks, hipStream_t stream);

@@ -839,7 +839,8 @@ void launch_one(Kind kind, const Args& p, dim3 grid, hipStream_t stream) {
     else if (kind == kDkv) hipLaunchKernelGGL((dkv_kernel<DT, DK, W, NW, kTileOf<DT, NW>>), grid, threads, 0, stream, p);
     else if constexpr (few_fits(DT == NORI_F32, DK, NW)) {
         if (kind == kFewForward) hipLaunchKernelGGL((forward_few_kernel<DT, DK, W, NW>), grid, threads, 0, stream, p);
-        else if (NW == 2 && p.rows <= 48 && p.a.nk <= 48) hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW, NW == 2 ? 48 : 32>), grid, threads, 0, stream, p);
+        else if (NW == 2 && p.rows <= 48 && p.a.nk <= 48)
+            hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW, NW == 2 ? 48 : 32>), grid, threads, 0, stream, p);
         else hipLaunchKernelGGL((backward_few_kernel<DT, DK, W, NW, 32 * NW>), grid, threads, 0, stream, p);
     }
 }

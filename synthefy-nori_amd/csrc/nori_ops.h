@@ -179,8 +179,8 @@ int nori_attention_train_forward(const nori_attention_train_args* args, void* st
 int nori_attention_train_backward(const nori_attention_train_args* args, void* stream);
 
 // Activations kept in 8 bits (checkpoint.hip). Of every NORI_CHECKPOINT_GROUP columns of a row (the last group may be shorter): a
-// scale, amax times fp32(1/127) (as torch divides by a number on the device), and int8 codes, the nearest whole number to x / scale (ties to even, -127 .. 127; 0 where the
-// scale is 0); a code stands for code * scale. A group with an infinity or NaN stands for NaN throughout. codes
+// scale, amax times fp32(1/127) (as torch divides by a number on the device), and int8 codes, the nearest whole number to
+// x / scale (ties to even, -127 .. 127; 0 where the scale is 0); a code stands for code * scale. A group with an infinity or NaN stands for NaN throughout. codes
 // [rows, code_stride] with code_stride cols rounded up to 16, the columns past cols 0; scales [rows, groups]; codes 16-byte
 // aligned. x rows at x_row_stride, any alignment.
 #define NORI_CHECKPOINT_GROUP 128
@@ -197,8 +197,9 @@ int nori_checkpoint_silu_mul_backward(const void* codes, const float* scales, in
 
 // The gradients of a projection's weight and bias over rows kept in 8 bits (checkpoint_grad.hip): dw [n, k] = sum over rows of
 // dy^T x, x what the codes stand for (rounded to dy's dtype where dw is of it; beside an fp32 dw of 16-bit rows each term is held to
-// 2^-22 of itself and 2^-33 of the largest), db [n] = sum of dy; each NULL where it is not asked for, of its own dtype (dy's or fp32), contiguous. The workspace, of nori_checkpoint_grad_workspace_bytes and 16-byte aligned, takes the sums
-// of parts of the rows, which are joined in order. Sums are fp32. No rows: zeros.
+// 2^-22 of itself and 2^-33 of the largest), db [n] = sum of dy; each NULL where it is not asked for, of its own dtype (dy's or
+// fp32), contiguous. The workspace, of nori_checkpoint_grad_workspace_bytes and 16-byte aligned, takes the sums of parts of the
+// rows, which are joined in order. Sums are fp32. No rows: zeros.
 int64_t nori_checkpoint_grad_workspace_bytes(int dtype, int dw_dtype, int64_t rows, int32_t n, int32_t k);
 int nori_checkpoint_grad(const void* dy, int dtype, int64_t rows, int32_t n, int64_t dy_row_stride, const void* codes,
                          const float* scales, int32_t k, void* dw, int dw_dtype, void* db, int db_dtype, void* workspace,
