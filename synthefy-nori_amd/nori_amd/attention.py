@@ -279,6 +279,7 @@ def _steps(t: torch.Tensor, *dims: int) -> tuple[int, ...]:
 
 
 def _train_args(q, kv, lengths, scale, out, lse) -> nat.AttentionTrainArgs:
+    """The arguments of a call on these tensors, which hold them: their addresses are good as long as the arguments live."""
     bg, nq, heads, d = q.shape
     args = nat.AttentionTrainArgs(bg=bg, nq=nq, nk=kv.shape[1], dtype=nat.dtype_code(q.dtype), heads=heads, kv_heads=kv.shape[3], d=d,
                                   q=q.data_ptr(), kv=kv.data_ptr(), scale=scale, out=out.data_ptr(), lse=nat.ptr(lse))
@@ -286,6 +287,7 @@ def _train_args(q, kv, lengths, scale, out, lse) -> nat.AttentionTrainArgs:
     args.kv_bg, args.kv_row, args.kv_half, args.kv_head = _steps(kv, 0, 1, 2, 3)
     if lengths is not None:
         args.lengths, args.length_group, args.lengths_i64 = lengths.data_ptr(), bg // lengths.shape[0], lengths.dtype == torch.int64
+    args.held = (q, kv, lengths, out, lse)
     return args
 
 
@@ -327,6 +329,7 @@ class _TrainableAttention(torch.autograd.Function):
             q, kv, dout = _in_fours(q), _in_fours(kv), _in_fours(dout)
             args = _train_args(q, kv, lengths, ctx.scale, out, lse)
             args.dout, args.dq, args.dkv = dout.data_ptr(), nat.ptr(dq), nat.ptr(dkv)
+            args.held += (dout, dq, dkv)
             args.do_bg, args.do_row, args.do_head = _steps(dout, 0, 1, 2)
             _train_call("nori_attention_train_backward", args, True, q.device)
         return dq, dkv, None, None

@@ -1,7 +1,9 @@
 """trainable_attention's refusals, and its formulas in 64 bits against differences (no GPU needed)."""
 
 import ctypes
+import gc
 import math
+import weakref
 
 import pytest
 import torch
@@ -140,3 +142,38 @@ def test_the_formulas_against_differences():
     value = lambda s: (reference(q + s * a, kv + s * b, lengths, dout)[0][0] * dout).sum().item()
     along = ((dq * a).sum() + (dkv * b).sum()).item()
     assert abs((value(t) - value(-t)) / (2 * t) - along) <= 1e-5 * dout.abs().sum().item()
+
+
+def test_copies_live_until_the_kernels_are_launched(monkeypatch):
+    """Operands that are not aligned go in as copies, to whose memory the arguments point: what the call allocates for its workspace
+    must not be theirs, in serving, in training or in the backward pass."""
+    from nori_amd import attention
+
+    copies, launches = [], []
+    in_fours = attention._in_fours
+
+    def copied(t):
+        c = in_fours(t)
+        assert c is not t
+        copies.append(weakref.ref(c))
+        return c
+
+    def launch(name, args, backward, device):
+        gc.collect()
+        at = {c().data_ptr() for c in copies if c() is not None}
+        launches.append(name)
+        assert len(at) == len(copies), "a copy is gone before the launch"
+        assert {args.q, args.kv} | ({args.dout} if backward else set()) <= at
+        copies.clear()
+
+    monkeypatch.setattr(attention, "_in_fours", copied)
+    monkeypatch.setattr(attention, "_train_call", launch)
+    monkeypatch.setattr(nat, "require_device", lambda *t: None)
+    q = torch.randn(2 * 3 * 4 * 8 + 1, requires_grad=True)
+    kv = torch.randn(2 * 5 * 2 * 2 * 8 + 1, requires_grad=True)
+    odd = lambda: (q[1:].view(2, 3, 4, 8), kv[1:].view(2, 5, 2, 2, 8))
+    with torch.no_grad():
+        nori_amd.trainable_attention(*odd())
+    out = nori_amd.trainable_attention(*odd())
+    torch.autograd.grad(out, (q, kv), torch.randn(out.numel() + 1)[1:].view(out.shape))
+    assert launches == ["nori_attention_train_forward"] * 2 + ["nori_attention_train_backward"]

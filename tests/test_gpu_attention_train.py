@@ -304,3 +304,23 @@ def test_one_key_takes_no_gradient_of_queries(cuda, queries, dtype):
     assert not dq.any()
     _, dq, _ = run(q, kv, [1, 0, 1], dout)
     assert not dq.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("queries, keys", [(1, 3001), (5, 3001), (1, 65536), (3, 20000)])
+def test_copied_operands_beside_a_workspace(cuda, queries, keys, dtype):
+    """Few rows over many keys, in parts whose results lie in a workspace, with q and kv at odd offsets and with their heads' elements
+    apart, which go in as copies: the contiguous call's bits, served and trained."""
+    q, kv, dout = (t.cuda() for t in inputs(2, queries, keys, 2, 2, 64, dtype, seed=16))
+    apart = lambda t: t.movedim(-1, 0).contiguous().movedim(0, -1)
+    odd = lambda t: torch.empty(t.numel() + 1, dtype=dtype, device="cuda")[1:].view(t.shape).copy_(t)
+    lengths = torch.tensor([keys, keys - 7], device="cuda")
+    with torch.no_grad():
+        served = nori_amd.trainable_attention(q, kv, lengths)
+    trained = run(q, kv, [keys, keys - 7], dout)
+    assert torch.equal(served, trained[0])
+    for change in (odd, apart):
+        for x, y in ((change(q), change(kv)), (change(q), kv), (q, change(kv))):
+            with torch.no_grad():
+                assert torch.equal(nori_amd.trainable_attention(x, y, lengths), served)
+            assert all(torch.equal(a, b) for a, b in zip(trained, run(x, y, [keys, keys - 7], change(dout))))
