@@ -550,11 +550,11 @@ def swiglu_mlp_residual_norm(x: torch.Tensor, gate_up: torch.Tensor, down: torch
     if layout is None or layout[0] != groups or out.data_ptr() % 8:
         return None
     _, group, gstride, rstride = layout
+    gate_up, down = gate_up.contiguous(), down.contiguous()
     nat.check(
         nat.lib().nori_swiglu_mlp_residual_rms_norm(
-            x2.data_ptr(), nat.NORI_F16, rows, width, x2.stride(0), gate_up.contiguous().data_ptr(),
-            down.contiguous().data_ptr(), hidden, float(alpha), stream.data_ptr(), width, norm_width, float(eps),
-            out.data_ptr(), group, gstride, rstride, nat.stream_of(x.device),
+            x2.data_ptr(), nat.NORI_F16, rows, width, x2.stride(0), gate_up.data_ptr(), down.data_ptr(), hidden,
+            float(alpha), stream.data_ptr(), width, norm_width, float(eps), out.data_ptr(), group, gstride, rstride, nat.stream_of(x.device),
         ),
         "swiglu_mlp_residual_rms_norm",
     )
@@ -574,9 +574,10 @@ def swiglu_mlp_residual(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tens
     x2 = x.reshape(-1, width)
     if x2.stride(-1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16 or stream.data_ptr() % 16:
         return False
+    gate_up, down = gate_up.contiguous(), down.contiguous()
     nat.check(
         nat.lib().nori_swiglu_mlp_residual(
-            x2.data_ptr(), x2.shape[0], width, x2.stride(0), gate_up.contiguous().data_ptr(), down.contiguous().data_ptr(),
+            x2.data_ptr(), x2.shape[0], width, x2.stride(0), gate_up.data_ptr(), down.data_ptr(),
             hidden, float(alpha), stream.data_ptr(), width, nat.stream_of(x.device),
         ),
         "swiglu_mlp_residual",

@@ -241,3 +241,21 @@ def test_residual_without_a_norm_equals_the_separate_passes(width, hidden, rows)
 def test_residual_epilogues_around_the_split_rule(rows):
     test_residual_norm_epilogue_equals_the_separate_kernels(128, 128, 256, rows)
     test_residual_without_a_norm_equals_the_separate_passes(128, 256, rows)
+
+
+def test_residual_epilogues_of_transposed_weights():
+    # weights that are copied for the call: the contiguous call's bits
+    from nori_amd.norm import swiglu_mlp_residual, swiglu_mlp_residual_norm
+
+    gate_up, down, hp = _weights(256, 128, seed=6)
+    across = [w.t().contiguous().t() for w in (gate_up, down)]
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(500, 256, generator=g).half().to(DEV)
+    stream = torch.randn(500, 256, generator=g).to(DEV)
+    results = []
+    for w in ((gate_up, down), across):
+        plain, normed = stream.clone(), stream.clone()
+        assert swiglu_mlp_residual(x, *w, hp, plain, ALPHA)
+        y = swiglu_mlp_residual_norm(x, *w, hp, normed, ALPHA, 1e-5, 256)
+        results.append((plain, normed, y))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
