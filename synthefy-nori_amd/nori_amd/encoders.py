@@ -498,11 +498,12 @@ class MaskEmbEncoder(nn.Module):
         ln_w = None if rbf.norm.weight is None else rbf.norm.weight.float().contiguous()
         ln_b = None if rbf.norm.bias is None else rbf.norm.bias.float().contiguous()
         mask = None if self.nan_to_zero else self.mask_embedding.float().contiguous()
+        centers, sigma = rbf.centers.float().contiguous(), rbf.sigma.float().reshape(1)
         h = torch.empty((b, s, g, f * self.embedding_dim), dtype=torch.float16, device=dev)
         ptr = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
         nat.check(
             nat.lib().nori_cell_tokens(
-                ptr(x), b, s, g, f, rbf.n_kernels, ptr(rbf.centers.float().contiguous()), ptr(rbf.sigma.float().reshape(1)),
+                ptr(x), b, s, g, f, rbf.n_kernels, ptr(centers), ptr(sigma),
                 ptr(table), ptr(ln_w), ptr(ln_b), float(rbf.norm.eps), ptr(w16), ptr(b16), 96, ptr(edges), 32, ptr(mask),
                 ptr(h), nat.stream_of(dev),
             ),

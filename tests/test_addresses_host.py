@@ -50,3 +50,22 @@ def test_residual_epilogues_of_transposed_weights(library):
     assert norm.swiglu_mlp_residual(x, *weights, 256, stream, 0.5)
     assert norm.swiglu_mlp_residual_norm(x, *weights, 256, stream, 0.5, 1e-5, 128) is not None
     assert library.calls == [("nori_swiglu_mlp_residual", []), ("nori_swiglu_mlp_residual_rms_norm", [])]
+
+
+def test_cell_tokens_of_double_centers(library):
+    encoder = encoders.MaskEmbEncoder(
+        num_features=2, emsize=128, mask_embedding_size=128, numeric_embed_type="RBF",
+        RBF_config=dict(token_embed_dim=8, n_kernels=16, sigma=0.5, use_learn_sigma=False, use_learn_embeddings=False,
+                        use_original_features=False),
+        prompt_quantile_ple_bins=32)
+    encoder.numeric_mlp.centers = encoder.numeric_mlp.centers.double()
+    encoder.numeric_mlp.sigma = encoder.numeric_mlp.sigma.double()
+    x = torch.randn(2, 5, 3, 2)
+    key = encoders.PromptQuantilePLEEncoder.reference_key
+    torch.set_autocast_enabled("cuda", True)
+    try:
+        with torch.no_grad():
+            assert encoder._tokens_on_device(x, {key: {"edges": torch.randn(2, 3, 2, 33)}}) is not None
+    finally:
+        torch.set_autocast_enabled("cuda", False)
+    assert [name for name, _ in library.calls] == ["nori_cell_tokens"] and not library.calls[0][1]

@@ -130,6 +130,19 @@ def test_encoder_output_with_and_without_the_kernel(cuda, n_kernels, monkeypatch
     assert float((outs[0] - outs[1]).abs().max()) <= 2e-3 * float(outs[1].abs().max())
 
 
+def test_centers_and_width_in_double(cuda):
+    enc = make_encoder(16, cuda)
+    x, reference = make_cells(cuda)
+    inp = {"data": x, encoders.PromptQuantilePLEEncoder.reference_key: reference}
+    tokens = []
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16):
+        for dtype in (torch.float32, torch.float64):
+            rbf = enc.numeric_mlp
+            rbf.centers, rbf.sigma = rbf.centers.to(dtype), rbf.sigma.to(dtype)
+            tokens.append(enc._tokens_on_device(x, inp))
+    assert torch.equal(*tokens)
+
+
 def test_fp32_and_unsupported_configurations_take_the_torch_ops(cuda):
     enc = make_encoder(16, cuda)
     x, reference = make_cells(cuda)
