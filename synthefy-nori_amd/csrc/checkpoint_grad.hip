@@ -153,7 +153,7 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
     // one would pass 2^15; the sums are brought along.
     __shared__ float tops[kThreads / 64];
     float power = 0.f, top = 0.f;
-    const int live = yc < a.n ? min(8, a.n - yc) : 8;  // past the row's end anything may lie
+    const int live = min(8, a.n - yat);  // past the row's end anything may lie
     const auto look = [&](const Eight<DT>& y, float s) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {

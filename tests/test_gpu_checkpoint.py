@@ -348,3 +348,21 @@ def test_rows_that_do_not_fold(cuda, dtype):
             got.append((y, *torch.autograd.grad(y, (x, w, b), dy)))
         for one, other in zip(*got):
             assert torch.equal(one, other)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("n", [1, 3, 5, 7, 8, 9, 130])
+def test_slopes_cut_out_of_a_wider_buffer(cuda, n, dtype):
+    """Columns beside the slopes, finite and far larger, are not looked at: the contiguous slopes' bits, in fp32 and in the type."""
+    g = torch.Generator().manual_seed(n)
+    rows, k = 700, 150
+    x = torch.randn(rows, k, generator=g).to(dtype).cuda()
+    buffer = torch.full((rows, n + 14), torch.finfo(dtype).max, dtype=dtype)
+    buffer[:, 2 : 2 + n] = (torch.randn(rows, n, generator=g) * 1e-3).to(dtype)
+    dy = buffer.cuda()[:, 2 : 2 + n]
+    for wt in (torch.float32, dtype):
+        w, b = (torch.randn(s, generator=g).to(wt).cuda().requires_grad_(True) for s in ((n, k), (n,)))
+        got = torch.autograd.grad(nori_amd.checkpointed_linear(x, w, b), (w, b), dy)
+        expected = torch.autograd.grad(nori_amd.checkpointed_linear(x, w, b), (w, b), dy.contiguous())
+        assert all(torch.equal(a, c) for a, c in zip(got, expected))
+        assert got[0].any(1).all()
