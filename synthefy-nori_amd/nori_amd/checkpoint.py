@@ -13,7 +13,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _native as nat
-from .norm import _FLOATS, _first_derivative, _refuse_tangents, _rows_of
+from .norm import _FLOATS, _first_derivative, _refuse_tangents, _rows_of, unviewed
 
 __all__ = ["checkpointed_linear", "checkpointed_silu_mul"]
 
@@ -51,7 +51,7 @@ def _linear(x, weight, bias):
         if x.dim() == 2:
             return F.linear(x, w, b), w
         # (one product: rows that do not fold would be a batch of them)
-        return F.linear(x.reshape(-1, x.shape[-1]), w, b).view(*x.shape[:-1], w.shape[0]), w
+        return unviewed(F.linear(x.reshape(-1, x.shape[-1]), w, b), (*x.shape[:-1], w.shape[0])), w
 
 
 class _CheckpointedLinear(torch.autograd.Function):

@@ -437,6 +437,12 @@ def _first_derivative(backward):
     return run
 
 
+def unviewed(t: torch.Tensor, shape: tuple[int, ...]) -> torch.Tensor:
+    """``t.view(shape)`` of a t that is used no more, as a tensor of its own: torch refuses changes in place of a view that a
+    Function returns, or that was made under no_grad."""
+    return torch.ops.aten._unsafe_view.default(t, shape)
+
+
 class _TrainableLayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype):

@@ -106,3 +106,26 @@ def test_the_gate_against_differences():
     sig = torch.sigmoid(a)
     along = (d * b * sig * (1 + a * (1 - sig)) * va + d * a * sig * vb).sum()
     assert abs((value(1e-4) - value(-1e-4)) / 2e-4 - along) <= 1e-6
+
+
+@pytest.mark.parametrize("shape", [(8,), (3, 8), (2, 3, 8), (2, 2, 3, 8)], ids=str)
+@pytest.mark.parametrize("biased", [False, True])
+def test_results_are_changed_in_place(monkeypatch, shape, biased):
+    """What F.linear's result takes: sums and activations in place, of rows of any number of dimensions."""
+    monkeypatch.setattr(nat, "require_device", lambda *t: None)
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(shape, generator=g).requires_grad_(True), torch.randn(5, 8, generator=g)
+    b = torch.randn(5, generator=g) if biased else None
+    residual = torch.randn(*shape[:-1], 5, generator=g).requires_grad_(True)
+    slope = torch.randn(*shape[:-1], 5, generator=g)
+    y = torch.relu(nori_amd.checkpointed_linear(x, w, b) + residual)
+    expected = torch.autograd.grad(y, (x, residual), slope)
+    z = nori_amd.checkpointed_linear(x, w, b)
+    z += residual
+    z = torch.relu_(z)
+    assert torch.equal(z, y)
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(z, (x, residual), slope), expected))
+    with torch.no_grad():
+        z = nori_amd.checkpointed_linear(x, w, b)
+    z += residual
+    assert torch.equal(torch.autograd.grad(z, residual, slope)[0], slope)

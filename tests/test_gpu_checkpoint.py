@@ -366,3 +366,28 @@ def test_slopes_cut_out_of_a_wider_buffer(cuda, n, dtype):
         expected = torch.autograd.grad(nori_amd.checkpointed_linear(x, w, b), (w, b), dy.contiguous())
         assert all(torch.equal(a, c) for a, c in zip(got, expected))
         assert got[0].any(1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("biased", [False, True])
+def test_results_are_changed_in_place(cuda, biased, dtype):
+    """A residual is added to the result, which goes through a gate, in place: what the same out of place gives."""
+    g = torch.Generator().manual_seed(8)
+    make = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda().requires_grad_(True)
+    for lead in ((), (3,), (3, 5), (2, 3, 5)):
+        x, w, b, r = make(*lead, 24), make(20, 24), make(20) if biased else None, make(*lead, 20)
+        leaves = [t for t in (x, w, b, r) if t is not None]
+        slope = torch.randn(*lead, 20, generator=g).to(dtype).cuda()
+        y = torch.relu(nori_amd.checkpointed_linear(x, w, b) + r)
+        z = nori_amd.checkpointed_linear(x, w, b)
+        z += r
+        z = F.relu(z, inplace=True)
+        assert torch.equal(y, z)
+        pairs = zip(torch.autograd.grad(y, leaves, slope), torch.autograd.grad(z, leaves, slope))
+        assert all(torch.equal(a, c) for a, c in pairs)
+        gu = make(*lead, 40)
+        h = nori_amd.checkpointed_silu_mul(gu, 20) + r
+        v = nori_amd.checkpointed_silu_mul(gu, 20)
+        v += r
+        pairs = zip(torch.autograd.grad(h, (gu, r), slope), torch.autograd.grad(v, (gu, r), slope))
+        assert torch.equal(h, v) and all(torch.equal(a, c) for a, c in pairs)
