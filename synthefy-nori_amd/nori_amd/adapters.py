@@ -21,7 +21,7 @@ from torch.nn.modules import module as _module_base
 
 from . import _native as nat
 from .layer import _hooked
-from .norm import _FLOATS, _first_derivative, _refuse_tangents, _rows_of, _strided_rows, trainable_layer_norm
+from .norm import _FLOATS, _first_derivative, _refuse_tangents, _rows_of, _strided_rows, trainable_layer_norm, unviewed
 
 __all__ = ["AdapterPlan", "LowRankAdapters", "ReadoutAdapters", "adapted_linear", "low_rank_update"]
 
@@ -216,6 +216,8 @@ def _projected(x, weight, bias, a, b, plan, scales, keep):
         y = F.linear(x, weight, bias)
     if _strided_rows(y, int(y.shape[-1])) is None:
         y = y.contiguous()
+    elif y._is_view():  # (of some x of other than two dimensions)
+        y = unviewed(y, y.shape)
     return y, _update(x, y, a, b, plan, scales, y, keep)
 
 

@@ -5,7 +5,7 @@ import pickle
 import pytest
 import torch
 
-from nori_amd import AdapterPlan, low_rank_update
+from nori_amd import AdapterPlan, adapted_linear, low_rank_update
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,23 @@ def test_a_plan_may_go_while_another_stream_still_reads_it():
     assert all(t.data_ptr() != at for t in taken)
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_adapted_results_are_changed_in_place():
+    # with a bias, rows of any number of dimensions: a sum in place is what the sum out of place is, also of a result of no_grad
+    g = torch.Generator().manual_seed(1)
+    for lead in ((6,), (2, 3), (1, 2, 3)):
+        plan = AdapterPlan([1, -1, 0], [2, 1, 3], device=DEV)
+        x, r = (torch.randn(*lead, n, generator=g).to(DEV).requires_grad_(True) for n in (24, 40))
+        _, _, a, b = _make(6, 24, 40, 4, 2)
+        w, bias = torch.randn(40, 24, generator=g).to(DEV), torch.randn(40, generator=g).to(DEV)
+        y = adapted_linear(x, w, bias, a, b, plan) + r
+        z = adapted_linear(x, w, bias, a, b, plan)
+        z += r
+        slope = torch.randn(*lead, 40, generator=g).to(DEV)
+        assert torch.equal(y, z)
+        assert all(torch.equal(p, q) for p, q in zip(*(torch.autograd.grad(t, (x, r), slope) for t in (y, z))))
+        with torch.no_grad():
+            z = adapted_linear(x, w, bias, a, b, plan)
+        z += r
+        assert torch.equal(y, z) and torch.equal(torch.autograd.grad(z, r, slope)[0], slope)
