@@ -195,9 +195,10 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
         }
         __syncthreads();
         if constexpr (FINE) agree();
+        const float factor = power == 0.f ? 1.f : power;  // (nothing but zeros so far, or infinities, which stay)
         if (whole(from)) {
 #pragma unroll
-            for (int j = 0; j < NY; ++j) put_y(j, ye[j], FINE ? ysc[FINE ? j : 0] : 1.f, power);
+            for (int j = 0; j < NY; ++j) put_y(j, ye[j], FINE ? ysc[FINE ? j : 0] : 1.f, factor);
 #pragma unroll
             for (int j = 0; j < NX; ++j) put_x(j, xe[j], FINE ? 1.f : xsc[FINE ? 0 : j]);
             if (turn == 0) {
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(kThreads, 2) void grad_kernel(const Args a) {
             for (int j = 0; j < NY; ++j) {
                 const int64_t r = from + yrow + j * kYStep;
                 const Eight<DT> y = partial(r);
-                put_y(j, y, FINE && a.dw && r < end ? a.scales[r * a.groups + kt] : 1.f, power);
+                put_y(j, y, FINE && a.dw && r < end ? a.scales[r * a.groups + kt] : 1.f, factor);
                 if (turn == 0) add(y);
             }
 #pragma unroll 1

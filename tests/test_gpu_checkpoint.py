@@ -391,3 +391,19 @@ def test_results_are_changed_in_place(cuda, biased, dtype):
         v += r
         pairs = zip(torch.autograd.grad(h, (gu, r), slope), torch.autograd.grad(v, (gu, r), slope))
         assert torch.equal(h, v) and all(torch.equal(a, c) for a, c in pairs)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows", [5, 300])
+def test_an_infinite_slope_among_zeros(cuda, rows, dtype):
+    """The fp32 gradient is what the formula gives: infinite where the row's kept value is not zero, NaN where it is."""
+    x = activations(rows, 150, dtype, seed=1)
+    x[4, 7] = 0
+    dy = torch.zeros(rows, 9, dtype=dtype)
+    dy[4, 2] = math.inf
+    w = torch.zeros(9, 150, device="cuda", requires_grad=True)
+    dw = torch.autograd.grad(nori_amd.checkpointed_linear(x.cuda(), w), w, dy.cuda())[0].double().cpu()
+    xh = kept(x)[2]
+    expected = torch.zeros(9, 150).double()
+    expected[2] = math.inf * xh[4]
+    assert torch.equal(dw.nan_to_num(nan=1.0), expected.nan_to_num(nan=1.0))
