@@ -324,3 +324,32 @@ def test_copied_operands_beside_a_workspace(cuda, queries, keys, dtype):
             with torch.no_grad():
                 assert torch.equal(nori_amd.trainable_attention(x, y, lengths), served)
             assert all(torch.equal(a, b) for a, b in zip(trained, run(x, y, [keys, keys - 7], change(dout))))
+
+
+@pytest.mark.parametrize("queries, keys", [(1, 30000), (3, 3000), (200, 3000), (40, 64)])
+def test_float16_probabilities_far_below_the_largest(cuda, queries, keys):
+    """One key 2^23 to 2^30 above all others, whose values are the larger ones. The forward pass holds a probability in float16 beside
+    the largest so far (of a part of the keys), under 2^8: normal down to 2^-22 of it, and off by at most half of float16's
+    subnormal step, 2^-25 / 2^8 = 2^-33 of the row's largest, below. The other bounds are those of every shape."""
+    g = torch.Generator().manual_seed(17)
+    q, kv, dout = inputs(2, queries, keys, 2, 1, 32, torch.float16, seed=17)
+    q[..., 0], q[..., 1:] = 4, q[..., 1:] * 2.0**-6
+    kv[:, :, 0] *= 2.0**-6
+    kv[:, :, 0, :, 0] = (22 - math.log(2) * (23 + 7 * torch.rand(2, keys, 1, generator=g))) / 4
+    kv[:, :, 1] = kv[:, :, 1].abs() * 256
+    at = torch.randint(keys, (2,), generator=g).tolist()
+    for i in range(2):
+        kv[i, at[i], 0, :, 0] = 5.5
+        kv[i, at[i], 1] *= 2.0**-12
+    out, dq, dkv = run(q, kv, None, dout, 1.0)
+    expected, bounds = reference(q, kv, None, dout, 1.0)
+    low = 2.0**-33 * kv[:, :, 1].double().abs().sum(1)[:, None]  # one key head
+    assert_near("out", out, expected[0], bounds[0] + low)
+    # delta of a result that is off by as much, in each ds = p (dout v - delta)
+    off = (dout.double().abs() * low).sum(-1)  # [BG, Q, H]
+    p = torch.softmax(torch.einsum("bqhd,bkd->bqhk", q.double(), kv[:, :, 0, 0].double()), -1) * off[..., None]
+    k = kv[:, :, 0, 0].double().abs()
+    assert_near("dq", dq, expected[2], bounds[2] + torch.einsum("bqhk,bkd->bqhd", p, k))
+    more = torch.zeros_like(expected[3])
+    more[:, :, 0, 0] = torch.einsum("bqhk,bqhd->bkd", p, q.double().abs())
+    assert_near("dkv", dkv, expected[3], bounds[3] + more)
