@@ -292,8 +292,8 @@ __device__ __forceinline__ float positive(float c, typename El<DT>::Frag (&q)[KS
 }
 
 // Bound by the matrix instructions and the exponentials between them over many rows, by HBM over few. 9 x 2 heads of 64, 8,192 x
-// 8,192, bf16: 411-445 us (700 TFLOP/s); four wavefronts a SIMD spill. One row over 65,536 keys: 52 us (5.8 TB/s) and 10 for the
-// parts.
+// 8,192, bf16: 398 us (777 TFLOP/s; the card settled, as all figures here); four wavefronts a SIMD spill. One row over 65,536 keys: 49 us
+// (6.2 TB/s, keys in part still in the cache) and 10 for the parts.
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, DK <= 64 && NW == 4 ? 3 : 2) void forward_kernel(const Args p) {
     using E = El<DT>;
@@ -485,7 +485,7 @@ __device__ __forceinline__ void dq_whole(const typename El<DT>::T* ks, const typ
 }
 
 // Three products of the pairs, bound as the forward pass over many rows: 9 x 2 heads of 64, 8,192 x 8,192, bf16:
-// 527-536 us (880 TFLOP/s). Three wavefronts a SIMD spill.
+// 487 us (952 TFLOP/s). Three wavefronts a SIMD spill.
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, DT == NORI_F32 && DK > 96 ? 1 : 2) void dq_kernel(const Args p) {
     using E = El<DT>;
@@ -598,11 +598,11 @@ __device__ __forceinline__ void dkv_step(const typename El<DT>::T* qs, const typ
 }
 
 // Four products of the pairs; keys stay, so two sums of 32 x D a wavefront take the registers that a third wavefront would need. The
-// same rows: 740-758 us (835 TFLOP/s).
+// same rows: 685 us (903 TFLOP/s).
 // kRows: of the tile that passes. Up to 32 rows in all take one tile of 32; the time goes to keys in and out then, so every
 // wavefront's results have room in LDS at once, and heads whose rows share lines of memory are neighbours. One row of 8 heads over 8,192
-// keys, 64 times, dq, dk and dv together: bf16 heads of 64 703 us (4.6 TB/s; results by turns 790, neighbouring heads 752), fp16 of 44
-// 768 (869 in tiles of 64 rows, 891 with a head's tiles as neighbours).
+// keys, 64 times, dq, dk and dv together: bf16 heads of 64 700 us (4.6 TB/s; results by turns 790, neighbouring heads 752), fp16 of 44
+// 757 (869 in tiles of 64 rows, 891 with a head's tiles as neighbours).
 template <int DT, int DK, int W, int NW, int kRows>
 __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Args p) {
     using E = El<DT>;
@@ -712,7 +712,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 ? 2 : 1) void dkv_kernel(const Ar
 
 // ---------------------------------------------------------------- few rows and few keys
 // The forward pass of a unit of up to 32 NW rows and keys. One tile and no loop: half the registers of forward_kernel, so twice the
-// wavefronts, which is what units this short go by: 8,192 x 8 units of 33 x 33 of 44, fp16, 196 us (3.9 TB/s).
+// wavefronts, which is what units this short go by: 8,192 x 8 units of 33 x 33 of 44, fp16, 188 us (4.0 TB/s).
 template <int DT, int DK, int W, int NW>
 __global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
     using E = El<DT>;
@@ -753,7 +753,7 @@ __global__ __launch_bounds__(64 * NW, 4) void forward_few_kernel(const Args p) {
 // The whole backward pass of such a unit: both sides in LDS, read from memory once, where the kernels above read them twice and the
 // rows' sums pass through memory. (Keys first and queries in their place later take half the LDS and a wavefront a SIMD more, but
 // read the queries twice: 8,192 x 8 units of 33 x 33 of 44, fp16, 656 us so, 557 this way.) ROWS is 48 where that holds both sides, for LDS
-// that lets a wavefront a SIMD more in and a quarter less work: the same units 529 us with 64, 499 with 48. Now: 404 us (3.3 TB/s), bound
+// that lets a wavefront a SIMD more in and a quarter less work: the same units 529 us with 64, 499 with 48. Now: 401 us (3.3 TB/s), bound
 // by the instructions that tiles half empty take.
 template <int DT, int DK, int W, int NW, int ROWS>
 __global__ __launch_bounds__(64 * NW, 2) void backward_few_kernel(const Args p) {

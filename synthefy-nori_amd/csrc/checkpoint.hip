@@ -1,7 +1,7 @@
 // Activations kept in 8 bits for the backward pass: rows quantised in groups of 128 columns, and the SwiGLU gate with its
 // gradient over gate and up kept so. One pass each, HBM-bound: 16 lanes hold a group, 8 elements each, in registers
-// between the largest magnitude (DPP) and the codes. 131,072 x 560 bf16 quantised: 44-47 us (4.9 TB/s); gate of 938, bf16: 199 us
-// with its codes, 183 for its gradient (4.9 and 5.4 TB/s).
+// between the largest magnitude (DPP) and the codes. 131,072 x 560 bf16 quantised: 44-47 us (4.9 TB/s); gate of 938, bf16: 186 us
+// with its codes, 177 for its gradient (5.3 and 5.6 TB/s).
 //
 // The code of x is the whole number nearest to x / s, ties to even, exactly: k, the nearest to x (1 / s), may be one off beside a
 // half, and the remainder x - k s, which one fma gives without error there, says so. (Both terms are multiples of half

@@ -3,7 +3,7 @@
 // operands are transposed reads, the codes are widened on their way in. A k tile is one group: a scale a row.
 //
 // Bound by the matrix instructions and what stands between them (reads of both operands, codes to values): 131,072 rows 560 -> 2,240
-// bf16, 494-524 us (640 TFLOP/s; a library product of these sizes with both operands as it wants them: 367-508). 256 columns of dy a
+// bf16, 437 us (753 TFLOP/s; a library product of these sizes with both operands as it wants them: 331-488). 256 columns of dy a
 // workgroup halve the reads of x's tile a product; where n fills no pair of 128s, or dy takes two pieces or 4 bytes, it is 128.
 #include <algorithm>
 

@@ -197,7 +197,7 @@ int nori_checkpoint_silu_mul_backward(const void* codes, const float* scales, in
 
 // The gradients of a projection's weight and bias over rows kept in 8 bits (checkpoint_grad.hip): dw [n, k] = sum over rows of
 // dy^T x, x what the codes stand for (rounded to dy's dtype where dw is of it; beside an fp32 dw of 16-bit rows each term is held to
-// 2^-22 of itself and 2^-33 of the largest), db [n] = sum of dy; each NULL where it is not asked for, of its own dtype (dy's or
+// 2^-22 of itself and 2^-33 of the largest of a workgroup's part of the rows and 128 columns of dy), db [n] = sum of dy; each NULL where it is not asked for, of its own dtype (dy's or
 // fp32), contiguous. The workspace, of nori_checkpoint_grad_workspace_bytes and 16-byte aligned, takes the sums of parts of the
 // rows, which are joined in order. Sums are fp32. No rows: zeros.
 int64_t nori_checkpoint_grad_workspace_bytes(int dtype, int dw_dtype, int64_t rows, int32_t n, int32_t k);

@@ -348,7 +348,7 @@ def trainable_attention(q: torch.Tensor, kv: torch.Tensor, key_lengths: torch.Te
     Differentiable in q and kv (first derivatives, in reverse mode). The backward pass keeps q, kv, the result and a float32
     log-sum-exp a row, and recomputes the probabilities. Products are summed in fp32, statistics are fp32; probabilities and
     their gradients enter the second products rounded to the inputs' dtype, in float16 under powers of two that keep
-    small ones their bits. Sums have a fixed order: the same inputs give the same bits. Strides are taken as they
+    small ones their bits (probabilities down to 2^-22 of a row's largest in the result). Sums have a fixed order: the same inputs give the same bits. Strides are taken as they
     are where 4 elements of a head are aligned together, else through a contiguous copy."""
     if q.dim() != 4:
         raise ValueError(f"query must be [BG, Q, H, D], got {tuple(q.shape)}")

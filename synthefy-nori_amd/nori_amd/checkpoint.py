@@ -104,9 +104,14 @@ def checkpointed_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tenso
     keep their own dtype). in and out up to 2^20. Where autocast is on x, and 16-bit weights, are cast to its dtype.
 
     The result and the gradients of x and bias are ``F.linear``'s. The weight's is dy^T x with x the values that the codes stand
-    for (``code * scale``, scale = amax times fp32(1/127) of 128 columns of a row, nearest codes, ties to even), rounded to x's dtype
-    for the product; a group of columns that holds an infinity or NaN stands for NaN. First derivatives, in reverse mode; sums
-    have a fixed order, so the same inputs give the same bits. Without a gradient of the weight nothing is kept of x."""
+    for (``code * scale``, scale = amax times fp32(1/127) of 128 columns of a row, nearest codes, ties to even); a group of columns that
+    holds an infinity or NaN stands for NaN. A weight of x's dtype has these values rounded to it for the product. A float32 weight beside
+    16-bit x, as under autocast, has them whole, and each term dy * x to 2^-22 of itself and 2^-33 of the largest among 128 neighbouring
+    outputs: an output whose slopes are far below its neighbours' keeps fewer bits. Such a weight is cast on each call, and the cast
+    kept where x asks for a gradient.
+
+    First derivatives, in reverse mode; sums have a fixed order, so the same inputs give the same bits. Without a gradient of the
+    weight nothing is kept of x."""
     if weight.dim() != 2 or min(weight.shape) == 0:
         raise ValueError(f"weight must be [out, in], got {tuple(weight.shape)}")
     n, k = (int(s) for s in weight.shape)
