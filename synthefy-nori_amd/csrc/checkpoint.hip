@@ -4,7 +4,7 @@
 // with its codes, 177 for its gradient (5.3 and 5.6 TB/s).
 //
 // The code of x is the whole number nearest to x / s, ties to even, exactly: k, the nearest to x (1 / s), may be one off beside a
-// half, and the remainder x - k s, which one fma gives without error there, says so. (Both terms are multiples of half
+// half, and the remainder x - k s, which one fma gives without error there, says so. (Both terms are multiples of 2^-149 or half
 // the last place of s, and their difference is not above s: it has 24 bits.)
 #include <math.h>
 
@@ -95,8 +95,8 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
 }
 
 // The group's scale and this lane's codes of elements r, v widened. A scale that is a normal number: k in one fma with a number
-// whose last place is 1, the code in its low byte; it is looked at again only where a lane of the wavefront has a remainder of
-// half a scale. (Quotients stay below 127.5: no code passes 127.)
+// whose last place is 1, the code in its low byte (quotients stay below 127.5: no code passes 127); of few bits: by division. Looked at again
+// only where a lane of the wavefront has a remainder of half a scale.
 template <int DT>
 __device__ __forceinline__ float quantize8(const Raw8<DT>& r, const float (&v)[kEach], uint64_t& codes) {
     constexpr float kOnes = 12582912.0f;  // 3 * 2^22
@@ -107,24 +107,26 @@ __device__ __forceinline__ float quantize8(const Raw8<DT>& r, const float (&v)[k
     const float y = normal ? 1.0f / s : 0.0f;
     float k[kEach], rest[kEach], most = 0.f;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        k[i] = fmaf(v[i], y, kOnes);
-        rest[i] = fmaf(kOnes - k[i], s, v[i]);
-        most = fmaxf(most, fabsf(rest[i]));
-    }
-    const float half = 0.5f * s;
-    if (__any(normal && most >= half)) {  // (bfloat16's halves are not rare: amax / 2 is one)
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const float far = fabsf(rest[i]);
-            const bool up = far > half || (far == half && (__float_as_uint(k[i]) & 1u));
-            k[i] += up ? copysignf(1.0f, rest[i]) : 0.0f;
-        }
-    }
+    for (int i = 0; i < kEach; ++i) k[i] = fmaf(v[i], y, kOnes);
     if (__any(s > 0.0f && !normal)) {  // a scale of few bits: quotients up to 190
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             if (s > 0.0f && !normal) k[i] = fminf(fmaxf(rintf(v[i] / s), -127.0f), 127.0f) + kOnes;
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        rest[i] = fmaf(kOnes - k[i], s, v[i]);
+        most = fmaxf(most, fabsf(rest[i]));
+    }
+    // twice a remainder against s: half of s may be no number. (bfloat16's halves are not rare: amax / 2 is one)
+    if (__any(s > 0.0f && 2.0f * most >= s)) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const float far = 2.0f * fabsf(rest[i]);
+            const bool up = s > 0.0f && (far > s || (far == s && (__float_as_uint(k[i]) & 1u)));
+            const float next = fminf(fmaxf(k[i] + copysignf(1.0f, rest[i]), kOnes - 127.0f), kOnes + 127.0f);
+            k[i] = up ? next : k[i];
+        }
     }
     uint32_t w[2];
 #pragma unroll

@@ -407,3 +407,22 @@ def test_an_infinite_slope_among_zeros(cuda, rows, dtype):
     expected = torch.zeros(9, 150).double()
     expected[2] = math.inf * xh[4]
     assert torch.equal(dw.nan_to_num(nan=1.0), expected.nan_to_num(nan=1.0))
+
+
+def test_codes_beside_halves_of_the_smallest_scales(cuda):
+    """fp32 rows whose scales lie about and below the least normal number, values at and one step from the halves between two codes:
+    where half a scale is no number, a quotient next to a half rounds to it."""
+    g = torch.Generator().manual_seed(9)
+    step = 2.0**-149
+    scale = torch.cat([torch.randint(2**21, 2**25, (400,), generator=g), torch.randint(1, 2**10, (100,), generator=g),
+                       torch.tensor([2**23 - 1, 2**23, 2**23 + 1, 2**24 - 1, 2**24, 2**24 + 1])]).double() * step
+    amax = (scale * 127).float()
+    s = (amax * torch.tensor(1 / 127, dtype=torch.float32)).double()
+    middle = (torch.arange(128) - 63.5) * s[:, None]
+    for way in (torch.floor, torch.ceil):
+        for beside in (-1, 0, 1):
+            x = ((way(middle / step) + beside) * step).float()
+            x[:, 0] = amax
+            codes, scales, _ = kept(x)
+            got, sc = cp._quantized(x.cuda())
+            assert torch.equal(sc.double().cpu(), scales) and torch.equal(got.double().cpu(), codes)
